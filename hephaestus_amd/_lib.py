@@ -1,5 +1,5 @@
-"""ctypes binding of libhephfp8.so (the C ABI declared in include/hephfp8.h
-and include/hephdecode.h).
+"""ctypes binding of libhephfp8.so (the C ABI declared in include/hephfp8.h,
+include/hephdecode.h and include/hephserve.h).
 
 The library is built in-tree by hephaestus_amd/build.py. There is no
 fallback: if the shared object is missing, loading raises.
@@ -12,7 +12,7 @@ import re
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libhephfp8.so")
 _INCLUDE = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include")
-HEADERS = [os.path.join(_INCLUDE, "hephfp8.h"), os.path.join(_INCLUDE, "hephdecode.h")]
+HEADERS = [os.path.join(_INCLUDE, h) for h in ("hephfp8.h", "hephdecode.h", "hephserve.h")]
 
 _lib = None
 
@@ -53,6 +53,7 @@ class LaunchOverrides(ctypes.Structure):
 _vp = ctypes.c_void_p
 _i = ctypes.c_int
 _sz = ctypes.c_size_t
+_i64 = ctypes.c_int64
 
 SIGNATURES = {
     "heph_fp8_quant_act": (_i, [_vp, _vp, _vp, _i, _i, _i, _vp]),
@@ -90,9 +91,25 @@ SIGNATURES = {
     "heph_silu_mul": (_i, [_vp, _vp, _vp, _i, _vp]),
     "heph_argmax_ws_bytes": (_sz, [_i]),
     "heph_argmax_bf16": (_i, [_vp, _vp, _i, _vp, _sz, _vp]),
+    # hephserve.h
+    "heph_rope_table_f32": (_i, [_vp, _i, _i, ctypes.c_double, _vp]),
+    "heph_qk_norm_rope_pages": (_i, [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _i, _vp, _vp, _i,
+                                     _vp, _vp, _i, _i, _i, _i, ctypes.c_float, _vp]),
+    "heph_pages_attention_plan_bytes": (_sz, [_i, _i, _i, _i, _i]),
+    "heph_pages_attention_ws_bytes": (_sz, [_i, _i, _i, _i, _i]),
+    "heph_pages_attention_plan": (_i, [_vp, _sz, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp]),
+    "heph_pages_attention": (_i, [_vp, _vp, _i64, _vp, _vp, _i, _vp, _vp, _i, _vp, _sz, _vp, _sz,
+                                  _i, _i, _i, _i, _i, _i, _vp]),
+    "heph_copy_pages": (_i, [_vp, _vp, _i, _i, _i, _vp, _vp, _i, _vp]),
+    "heph_lora_plan_bytes": (_sz, [_i, _i]),
+    "heph_lora_ws_bytes": (_sz, [_i, _i, _i, _i]),
+    "heph_lora_plan": (_i, [_vp, _sz, _vp, _i, _i, _vp]),
+    "heph_lora_add": (_i, [_vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp, _sz, _i, _i, _i, _i,
+                           _i, _vp]),
 }
 
 ATTN_MAX_KEYS = 262144
+PAGE_KEYS = 64
 # HEPH_ABI_VERSION of include/hephfp8.h that these signatures follow
 ABI_VERSION = 6
 
@@ -123,7 +140,7 @@ def lib():
 
 
 def header_functions() -> list[str]:
-    """Names of the functions include/hephfp8.h and hephdecode.h declare."""
+    """Names of the functions the headers declare."""
     names = set()
     for h in HEADERS:
         text = re.sub(r"/\*.*?\*/", "", open(h).read(), flags=re.S)

@@ -1,0 +1,80 @@
+// pages_copy.hip - copies of pages within the pools of the paged KV cache.
+#include <algorithm>
+#include <new>
+#include <vector>
+
+#include "pages.h"
+
+namespace heph {
+namespace {
+
+// The pairs travel in the launch's arguments: no upload, and a captured launch
+// keeps them.
+constexpr int kPairs = 256;
+struct CopyArgs {
+    uint8_t* pool[2];
+    size_t page_bytes, layer_bytes;
+    int n;
+    int src[kPairs], dst[kPairs];
+};
+
+// One workgroup moves 16 KB of one page: 4 KB pieces, 16 bytes a thread.
+constexpr int kPiece = 8192;
+__global__ __launch_bounds__(256) void copy_pages_kernel(CopyArgs a)
+{
+    const int pieces = (int)(a.page_bytes / kPiece);
+    const int piece = blockIdx.x % pieces, pair = blockIdx.x / pieces;
+    uint8_t* pool = a.pool[blockIdx.z] + (size_t)blockIdx.y * a.layer_bytes + (size_t)piece * kPiece;
+    const uint8_t* from = pool + (size_t)a.src[pair] * a.page_bytes;
+    uint8_t* to = pool + (size_t)a.dst[pair] * a.page_bytes;
+    const int o = threadIdx.x * 16;
+    const uint4 x = ldg16u(from + o), y = ldg16u(from + o + 4096);
+    *reinterpret_cast<uint4*>(to + o) = x;
+    *reinterpret_cast<uint4*>(to + o + 4096) = y;
+}
+
+}  // namespace
+}  // namespace heph
+
+using namespace heph;
+
+extern "C" int heph_copy_pages(uint8_t* k_pages, uint8_t* v_pages, int n_layers, int n_pages,
+                               int n_kv_heads, const int32_t* src, const int32_t* dst, int n,
+                               void* stream)
+{
+    if (!k_pages || !v_pages || (n > 0 && (!src || !dst))) return HEPH_ERR_NULL;
+    if (n_layers < 1 || n_layers > 65535 || n_pages < 1 || n_kv_heads < 1 || n_kv_heads > 4096 ||
+        n < 0 || n > n_pages)
+        return HEPH_ERR_SHAPE;
+    if (!aligned(k_pages, 16) || !aligned(v_pages, 16)) return HEPH_ERR_ALIGN;
+    if (n == 0) return HEPH_OK;
+    try {
+        // destinations that repeat or are read by another pair would race
+        std::vector<int32_t> to(dst, dst + n);
+        std::sort(to.begin(), to.end());
+        if (to.front() < 0 || to.back() >= n_pages ||
+            std::adjacent_find(to.begin(), to.end()) != to.end())
+            return HEPH_ERR_SHAPE;
+        for (int i = 0; i < n; ++i)
+            if (src[i] < 0 || src[i] >= n_pages ||
+                std::binary_search(to.begin(), to.end(), src[i]))
+                return HEPH_ERR_SHAPE;
+    } catch (const std::bad_alloc&) {
+        return HEPH_ERR_SCRATCH;
+    }
+    if (int st = check_device()) return st;
+    CopyArgs a;
+    a.pool[0] = k_pages;
+    a.pool[1] = v_pages;
+    a.page_bytes = (size_t)n_kv_heads * kPageBytes;
+    a.layer_bytes = (size_t)n_pages * a.page_bytes;
+    for (int i = 0; i < n; i += kPairs) {
+        a.n = std::min(kPairs, n - i);
+        std::copy(src + i, src + i + a.n, a.src);
+        std::copy(dst + i, dst + i + a.n, a.dst);
+        const unsigned pieces = (unsigned)(a.page_bytes / kPiece);
+        copy_pages_kernel<<<dim3(pieces * a.n, n_layers, 2), 256, 0, static_cast<hipStream_t>(stream)>>>(a);
+        if (hipGetLastError() != hipSuccess) return HEPH_ERR_LAUNCH;
+    }
+    return HEPH_OK;
+}

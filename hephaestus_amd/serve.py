@@ -1,0 +1,489 @@
+"""A batched serving step of a Qwen3 model around the W8A8 linears: the paged
+E4M3 KV cache, the ops of include/hephserve.h and a batch decoder on them.
+
+    per layer, T tokens of S sequences:
+        qkv = rmsnorm(x, attn_norm) @ Wqkv^T             heph_rmsnorm_quant_fp8, heph_fp8_linear
+              (+ adapters)                               heph_lora_add
+        q, k, v: per-head q/k norm, rotation, k/v pages  heph_qk_norm_rope_pages
+        att = attention over each sequence's pages,      heph_pages_attention
+              shared prefixes once for all
+        x  += att @ Wo^T                                 heph_fp8_linear + ADD_RESIDUAL
+        act = silu(gate) * up of rmsnorm(x) @ Wgu^T      heph_silu_mul_quant_fp8
+        x  += act @ Wdown^T
+
+The step is the batched form of the reference's forward_fp8_batched_decode
+(src/hephaestus/forward.mojo:618-871), which keeps one contiguous cache per
+sequence and calls attention per sequence.
+"""
+from __future__ import annotations
+
+import heapq
+
+import numpy as np
+import torch
+
+from . import _lib as L
+from . import decode as DEC
+from . import kernels as HK
+from .kernels import HephError
+from .loader import Fp8Weight, Qwen3Config, Qwen3Fp8Weights
+
+PAGE = L.PAGE_KEYS
+_U8 = (torch.uint8, torch.float8_e4m3fn)
+_I32, _BF16, _F32 = (torch.int32,), (torch.bfloat16,), (torch.float32,)
+
+
+def _dev(t, name: str, dtypes, numel: int | None = None) -> int:
+    """Pointer of a contiguous tensor on the current device with at least
+    numel elements."""
+    p = HK._dev(t, name, dtypes)
+    if t.device.index != torch.cuda.current_device():
+        raise ValueError(f"{name} is on {t.device}, not on the current device")
+    if numel is not None and t.numel() < numel:
+        raise ValueError(f"{name} has {t.numel()} elements, {numel} are needed")
+    return p
+
+
+def _rows(t, name: str, n: int, width: int) -> tuple[int, int]:
+    """Pointer and row stride (elements) of n rows of width bf16 values; the
+    rows may lie apart (a slice of a wider buffer)."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch tensor")
+    if t.device.type != "cuda" or t.device.index != torch.cuda.current_device():
+        raise ValueError(f"{name} must be in the current device's memory (got {t.device})")
+    if t.dtype != torch.bfloat16:
+        raise TypeError(f"{name} has dtype {t.dtype}, expected torch.bfloat16")
+    if t.dim() < 2 or t.shape[0] < n or t[0].numel() != width or not t[0].is_contiguous():
+        raise ValueError(f"{name} of shape {tuple(t.shape)} is not {n} rows of {width} "
+                         "consecutive values")
+    return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else max(width, t.stride(0))
+
+
+def _call(name: str, *args) -> None:
+    HK._check(getattr(L.lib(), name)(*args), name)
+
+
+def v_place(j: int) -> int:
+    """Where a page's V rows hold key j (0..63)."""
+    return j // 4 % 4 * 16 + j // 32 * 8 + j // 16 % 2 * 4 + j % 4
+
+
+# ------------------------------------------------------------- the ops ----
+
+def rope_table_f32(n_pos: int, theta: float = 1e6, device="cuda", ctx=None) -> torch.Tensor:
+    """(cos, sin) in f32 of the 64 pairs of a 128-wide head at positions
+    0..n_pos-1, [n_pos, 64, 2], the angles in double."""
+    t = torch.empty(n_pos, 64, 2, dtype=torch.float32, device=device)
+    _call("heph_rope_table_f32", _dev(t, "table", _F32), n_pos, 128, theta, HK._stream(ctx))
+    return t
+
+
+def _pools(k_pages, v_pages, n_kv: int) -> tuple[int, int, int]:
+    if k_pages.dim() < 5 or tuple(k_pages.shape[-4:]) != (n_kv, 2, PAGE, 64) or \
+            tuple(v_pages.shape) != tuple(k_pages.shape[:-3]) + (128, PAGE):
+        raise ValueError(f"pools of shapes {tuple(k_pages.shape)} and {tuple(v_pages.shape)} are "
+                         f"not [n_pages, {n_kv}, 2, 64, 64] and [n_pages, {n_kv}, 128, 64]")
+    return _dev(k_pages, "k_pages", _U8), _dev(v_pages, "v_pages", _U8), k_pages.shape[-5]
+
+
+def qk_norm_rope_pages(q_out, qkv, q_gamma, k_gamma, k_pages, v_pages, kv_inv, rope, positions,
+                       slots, eps: float = 1e-6, ctx=None) -> None:
+    """For each token: per-head RMSNorm of q and k, rotation by rope's row
+    positions[t], q [n_tok, n_heads, 128] to q_out, k and v as E4M3 codes into
+    slots[t] (page * 64 + key) of k_pages [n_pages, n_kv, 2, 64, 64] and
+    v_pages [n_pages, n_kv, 128, 64]. qkv: [n_tok, n_heads + 2 n_kv, 128], its
+    rows may lie apart; q_out may be qkv[:, :n_heads]. A position outside
+    rope skips the token, a slot outside the pools the cache write."""
+    n_tok, n_heads = q_out.shape[0], q_out[0].numel() // 128
+    n_kv = k_pages.shape[-4]
+    qp, qs = _rows(q_out, "q_out", n_tok, n_heads * 128)
+    xp, xs = _rows(qkv, "qkv", n_tok, (n_heads + 2 * n_kv) * 128)
+    kp, vp, n_pages = _pools(k_pages, v_pages, n_kv)
+    if rope.dim() != 3 or tuple(rope.shape[1:]) != (64, 2):
+        raise ValueError(f"rope of shape {tuple(rope.shape)} is not [n_pos, 64, 2]")
+    _call("heph_qk_norm_rope_pages", qp, qs, xp, xs, _dev(q_gamma, "q_gamma", _BF16, 128),
+          _dev(k_gamma, "k_gamma", _BF16, 128), kp, vp, n_pages,
+          _dev(kv_inv, "kv_inv", _F32, 2 * n_kv), _dev(rope, "rope", _F32), rope.shape[0],
+          _dev(positions, "positions", _I32, n_tok), _dev(slots, "slots", _I32, n_tok), n_tok,
+          n_heads, n_kv, 128, eps, HK._stream(ctx))
+
+
+class AttentionPlan:
+    """The layout of one step's attention and its workspace: update() it from
+    the step's lengths in device memory, then call attention_pages for every
+    layer. All sizes are fixed, so a captured step can be replayed with other
+    lengths."""
+
+    def __init__(self, n_seqs: int, n_tok: int, n_heads: int, n_kv: int, table_pages: int,
+                 n_groups: int = 0, device="cuda"):
+        self.n_seqs, self.n_tok, self.n_groups = n_seqs, n_tok, n_groups
+        self.n_heads, self.n_kv, self.table_pages = n_heads, n_kv, table_pages
+        sizes = (n_tok, n_seqs, n_groups, n_heads, n_kv)
+        nb = L.lib().heph_pages_attention_plan_bytes(*sizes)
+        if nb == 0:
+            raise HephError(L.HEPH_ERR_SHAPE, "AttentionPlan")
+        # (zeros: no plan until the first update)
+        self.plan = torch.zeros(nb, dtype=torch.uint8, device=device)
+        self.ws = torch.empty(max(16, L.lib().heph_pages_attention_ws_bytes(*sizes)),
+                              dtype=torch.uint8, device=device)
+
+    def update(self, q_start, kv_len, group_start=None, shared_pages=None, ctx=None) -> None:
+        """q_start int32 [n_seqs + 1], kv_len int32 [n_seqs]; with groups
+        group_start int32 [n_groups + 1], shared_pages int32 [n_groups]."""
+        g = self.n_groups > 0
+        if g != (group_start is not None) or g != (shared_pages is not None):
+            raise ValueError(f"a plan of {self.n_groups} groups "
+                             + ("needs" if g else "takes no") + " group_start and shared_pages")
+        _call("heph_pages_attention_plan", _dev(self.plan, "plan", _U8), self.plan.numel(),
+              _dev(q_start, "q_start", _I32, self.n_seqs + 1),
+              _dev(kv_len, "kv_len", _I32, self.n_seqs),
+              _dev(group_start, "group_start", _I32, self.n_groups + 1) if g else None,
+              _dev(shared_pages, "shared_pages", _I32, self.n_groups) if g else None,
+              self.n_tok, self.n_seqs, self.n_groups, self.table_pages, self.n_heads, self.n_kv,
+              HK._stream(ctx))
+
+
+def attention_pages(out, q, k_pages, v_pages, kv_scale, page_table, plan: AttentionPlan,
+                    ctx=None) -> None:
+    """out[t] = attention of token t over its sequence's keys in the pages,
+    laid out by plan (updated with this step's lengths). q [n_tok, n_heads,
+    128] (rows may lie apart), out contiguous; page_table int32 [n_seqs,
+    table_pages]."""
+    p = plan
+    if tuple(page_table.shape) != (p.n_seqs, p.table_pages):
+        raise ValueError(f"page_table of shape {tuple(page_table.shape)} is not "
+                         f"[{p.n_seqs}, {p.table_pages}] as planned")
+    qp, qs = _rows(q, "q", p.n_tok, p.n_heads * 128)
+    kp, vp, n_pages = _pools(k_pages, v_pages, p.n_kv)
+    _call("heph_pages_attention", _dev(out, "out", _BF16, p.n_tok * p.n_heads * 128), qp, qs, kp,
+          vp, n_pages, _dev(kv_scale, "kv_scale", _F32, 2 * p.n_kv),
+          _dev(page_table, "page_table", _I32), p.table_pages, _dev(p.plan, "plan", _U8),
+          p.plan.numel(), _dev(p.ws, "ws", _U8), p.ws.numel(), p.n_tok, p.n_seqs, p.n_groups,
+          p.n_heads, p.n_kv, 128, HK._stream(ctx))
+
+
+def copy_pages(k_pools, v_pools, src, dst, ctx=None) -> None:
+    """Page src[i] of every layer copied to page dst[i] in both pools
+    [n_layers, n_pages, ...]; src and dst are host lists. A destination may
+    neither repeat nor be a source."""
+    if k_pools.dim() != 6:
+        raise ValueError(f"k_pools of shape {tuple(k_pools.shape)} has no layers")
+    kp, vp, n_pages = _pools(k_pools, v_pools, k_pools.shape[2])
+    s, d = np.asarray(src, dtype=np.int32).reshape(-1), np.asarray(dst, dtype=np.int32).reshape(-1)
+    if s.size != d.size:
+        raise ValueError(f"{s.size} sources and {d.size} destinations")
+    _call("heph_copy_pages", kp, vp, k_pools.shape[0], n_pages, k_pools.shape[2], s.ctypes.data,
+          d.ctypes.data, int(s.size), HK._stream(ctx))
+
+
+class LoraPlan:
+    """The rows of a step grouped by adapter, and the workspace of lora_add for
+    projections of up to rank x k -> n: update() it from the rows' adapter ids
+    in device memory (an id outside [0, n_adapters): no adapter)."""
+
+    def __init__(self, m: int, n_adapters: int, rank: int, k: int, n: int | None = None,
+                 device="cuda"):
+        self.m, self.n_adapters = m, n_adapters
+        nb = L.lib().heph_lora_plan_bytes(m, n_adapters)
+        wb = L.lib().heph_lora_ws_bytes(m, n_adapters, k, rank)
+        if nb == 0 or wb == 0:
+            raise HephError(L.HEPH_ERR_SHAPE, "LoraPlan")
+        self.plan = torch.zeros(nb, dtype=torch.uint8, device=device)
+        self.ws = torch.empty(max(16, wb), dtype=torch.uint8, device=device)
+
+    def update(self, ids, ctx=None) -> None:
+        _call("heph_lora_plan", _dev(self.plan, "plan", _U8), self.plan.numel(),
+              _dev(ids, "ids", _I32, self.m), self.m, self.n_adapters, HK._stream(ctx))
+
+
+def lora_add(c, base, x, a, b, scale, plan: LoraPlan, ctx=None) -> None:
+    """c = base + scale[i] * (x @ a[i]^T) @ b[i]^T per row with the adapter i
+    that plan holds for it (c may be base, the projection's own output).
+    a [n_adapters, rank, k], b [n_adapters, n, rank], x [m, k] bf16; c and base
+    [m, n] bf16 or f32."""
+    if a.dim() != 3 or b.dim() != 3 or a.shape[0] != b.shape[0] or a.shape[1] != b.shape[2]:
+        raise ValueError(f"a {tuple(a.shape)} and b {tuple(b.shape)} are not [adapters, rank, k] "
+                         "and [adapters, n, rank]")
+    if a.shape[0] != plan.n_adapters:
+        raise ValueError(f"{a.shape[0]} adapters, planned for {plan.n_adapters}")
+    rank, k, n, m = a.shape[1], a.shape[2], b.shape[1], plan.m
+    if c.dtype not in HK._OUT or base.dtype != c.dtype:
+        raise TypeError(f"lora_add: c {c.dtype} and base {base.dtype} not supported")
+    dt = (c.dtype,)
+    _call("heph_lora_add", _dev(c, "c", dt, m * n), HK._OUT[c.dtype],
+          _dev(base, "base", dt, m * n), _dev(x, "x", _BF16, m * k), _dev(a, "a", _BF16),
+          _dev(b, "b", _BF16), _dev(scale, "scale", _F32, plan.n_adapters),
+          _dev(plan.plan, "plan", _U8), plan.plan.numel(), _dev(plan.ws, "ws", _U8),
+          plan.ws.numel(), m, n, k, rank, plan.n_adapters, HK._stream(ctx))
+
+
+# --------------------------------------------------------------- the cache ----
+
+class Sequence:
+    """A sequence's pages (ids, in key order) and its number of keys."""
+
+    def __init__(self):
+        self.pages: list[int] = []
+        self.length = 0
+
+
+class PagedKVCache:
+    """K and V pools of all layers with E4M3 codes, k [n_layers, n_pages, n_kv,
+    2, 64, 64] and v [n_layers, n_pages, n_kv, 128, 64], f32 scales [n_layers,
+    2*n_kv] and their reciprocals, and which sequence holds which page. A page
+    may belong to several sequences (a shared prefix): it is freed with the
+    last of them."""
+
+    def __init__(self, cfg: Qwen3Config, n_pages: int, device="cuda"):
+        if cfg.head_dim != 128:
+            raise ValueError("head_dim must be 128")
+        if n_pages < 1:
+            raise ValueError(f"a cache of {n_pages} pages")
+        self.cfg, self.n_pages = cfg, n_pages
+        shape = (cfg.n_layers, n_pages, cfg.n_kv_heads)
+        self.k = torch.zeros(*shape, 2, PAGE, 64, dtype=torch.uint8, device=device)
+        self.v = torch.zeros(*shape, 128, PAGE, dtype=torch.uint8, device=device)
+        self.scale = torch.ones(cfg.n_layers, 2 * cfg.n_kv_heads, dtype=torch.float32,
+                                device=device)
+        self.inv = torch.ones_like(self.scale)
+        self._free = list(range(n_pages))          # a heap: the lowest page first
+        self._users = [0] * n_pages
+        self._seqs: list[Sequence] = []
+
+    @property
+    def free_pages(self) -> int:
+        return len(self._free)
+
+    def _take(self, n: int) -> list[int]:
+        if n > len(self._free):
+            raise MemoryError(f"{n} pages wanted, {len(self._free)} free")
+        got = [heapq.heappop(self._free) for _ in range(n)]
+        for p in got:
+            self._users[p] = 1
+        return got
+
+    def _drop(self, page: int) -> None:
+        self._users[page] -= 1
+        if self._users[page] == 0:
+            heapq.heappush(self._free, page)
+
+    def _own(self, seq: Sequence) -> Sequence:
+        if not any(s is seq for s in self._seqs):
+            raise ValueError("the sequence is not in this cache")
+        return seq
+
+    def new(self) -> Sequence:
+        """An empty sequence."""
+        self._seqs.append(Sequence())
+        return self._seqs[-1]
+
+    def extend(self, seq: Sequence, n: int) -> list[int]:
+        """Room for n more keys; their slots. Nothing changes if the pages do
+        not suffice."""
+        if n < 0:
+            raise ValueError(f"{n} keys")
+        self._own(seq)
+        if seq.length + n > L.ATTN_MAX_KEYS:
+            raise ValueError(f"{seq.length + n} keys > {L.ATTN_MAX_KEYS}")
+        seq.pages += self._take(-(-(seq.length + n) // PAGE) - len(seq.pages))
+        keys = range(seq.length, seq.length + n)
+        seq.length += n
+        return [seq.pages[j // PAGE] * PAGE + j % PAGE for j in keys]
+
+    def fork(self, seq: Sequence, n: int = 1, ctx=None) -> list[Sequence]:
+        """n sequences with seq's keys: its full pages are shared, its partly
+        filled last page is copied for each (on the current stream)."""
+        self._own(seq)
+        if n < 0:
+            raise ValueError(f"{n} forks")
+        full = seq.length // PAGE
+        tails = self._take(n if seq.length % PAGE else 0)
+        made = []
+        for i in range(n):
+            s = self.new()
+            s.pages, s.length = seq.pages[:full] + tails[i:i + 1], seq.length
+            for p in seq.pages[:full]:
+                self._users[p] += 1
+            made.append(s)
+        if tails:
+            copy_pages(self.k, self.v, [seq.pages[full]] * n, tails, ctx)
+        return made
+
+    def free(self, seq: Sequence) -> None:
+        """The sequence leaves the cache; pages that no other one holds are free."""
+        self._own(seq)
+        for p in seq.pages:
+            self._drop(p)
+        self._seqs = [s for s in self._seqs if s is not seq]
+        seq.pages, seq.length = [], 0
+
+    def compact(self, ctx=None) -> int:
+        """Live pages move down into the lowest ids, so that the pages from the
+        number of live ones on are free; returns how many moved. Page tables
+        made before are stale."""
+        live = self.n_pages - len(self._free)
+        dst = sorted(p for p in self._free if p < live)
+        src = [p for p in range(live, self.n_pages) if self._users[p]]
+        copy_pages(self.k, self.v, src, dst, ctx)
+        to = dict(zip(src, dst))
+        for s in self._seqs:
+            s.pages = [to.get(p, p) for p in s.pages]
+        for a, b in to.items():
+            self._users[b], self._users[a] = self._users[a], 0
+        self._free = list(range(live, self.n_pages))
+        return len(src)
+
+
+# ------------------------------------------------------------- the decoder ----
+
+class LoraWeights:
+    """Adapters of one model: per layer and projection ("qkv", "o", "gate_up",
+    "down"; those absent have none) the pair (a [n_adapters, rank, k], b
+    [n_adapters, n, rank]), and scale f32 [n_adapters]."""
+
+    def __init__(self, scale: torch.Tensor, layers: list[dict]):
+        self.scale, self.layers = scale, layers
+        self.n_adapters = scale.numel()
+        pairs = [p for d in layers for p in d.values()]
+        self.max_rank = max((a.shape[1] for a, _ in pairs), default=8)
+        self.max_k = max((a.shape[2] for a, _ in pairs), default=128)
+
+
+def _groups(seqs: list[Sequence]) -> tuple[list[int], list[int]]:
+    """Runs of neighbouring sequences that share their first pages:
+    group_start and shared_pages. A run grows while its common prefix keeps
+    at least half of the pages its first two share."""
+    start, shared = [0], []
+    n = None
+    for i in range(1, len(seqs) + 1):
+        if i < len(seqs):
+            a, b = seqs[start[-1]].pages, seqs[i].pages
+            m = 0
+            while m < min(len(a), len(b)) and a[m] == b[m]:
+                m += 1
+            if n is None:
+                if m > 0:
+                    n = m
+                    continue
+            elif 2 * min(n, m) >= n:
+                n = min(n, m)
+                continue
+        shared.append(n or 0)
+        start.append(i)
+        n = None
+    return start, shared
+
+
+class Qwen3BatchDecoder:
+    """A step of many sequences: prompts or single tokens, behind whatever
+    their caches hold."""
+
+    def __init__(self, weights: Qwen3Fp8Weights, kv: PagedKVCache, n_pos: int = 40960,
+                 lora: LoraWeights | None = None):
+        if not weights.embed.block:
+            raise ValueError("the decoder takes 128x128 block-scaled weights")
+        if lora is not None and len(lora.layers) != weights.cfg.n_layers:
+            raise ValueError(f"adapters of {len(lora.layers)} layers, "
+                             f"{weights.cfg.n_layers} in the model")
+        self.w, self.kv, self.lora = weights, kv, lora
+        self.n_pos = min(n_pos, L.ATTN_MAX_KEYS)
+        self.rope = rope_table_f32(self.n_pos, weights.cfg.theta, device=weights.embed.w.device)
+
+    def _linear(self, c, x, fw: Fp8Weight, K: int, ws, residual: bool = False,
+                quantized: bool = False) -> None:
+        fn = HK.linear_add_residual_fp8 if residual else HK.linear_fp8
+        fn(c, x, fw.w, fw.scale, ws[0], ws[1], c.shape[0], fw.N, K, do_quantize=not quantized)
+
+    def step(self, tokens: list[list[int]], seqs: list[Sequence],
+             adapters: list[int] | None = None) -> torch.Tensor:
+        """tokens[i] (one or more) enter sequence seqs[i], with adapter
+        adapters[i] (-1: none). Returns the f32 logits [len(seqs), vocab] after
+        each sequence's last token."""
+        cfg, w, kv = self.w.cfg, self.w, self.kv
+        if len(tokens) != len(seqs) or not seqs or any(len(t) < 1 for t in tokens):
+            raise ValueError("every sequence brings one token or more")
+        if len({id(s) for s in seqs}) != len(seqs):
+            raise ValueError("a sequence appears twice")
+        if adapters is not None and (self.lora is None or len(adapters) != len(seqs)):
+            raise ValueError("adapters without weights, or not one a sequence")
+        need = 0
+        for t, s in zip(tokens, seqs):
+            kv._own(s)
+            if s.length + len(t) > self.n_pos:
+                raise ValueError(f"position {s.length + len(t) - 1} outside the rotation table "
+                                 f"of {self.n_pos}")
+            need += -(-(s.length + len(t)) // PAGE) - len(s.pages)
+        if need > kv.free_pages:
+            raise MemoryError(f"{need} pages wanted, {kv.free_pages} free")
+        flat = [i for t in tokens for i in t]
+        positions = [s.length + i for t, s in zip(tokens, seqs) for i in range(len(t))]
+        slots = [i for t, s in zip(tokens, seqs) for i in kv.extend(s, len(t))]
+        q_start = np.concatenate([[0], np.cumsum([len(t) for t in tokens])])
+        group_start, shared = _groups(seqs)
+        T, S, G = len(flat), len(seqs), len(shared)
+        width = max(len(s.pages) for s in seqs)
+        ids = [-1] * T if adapters is None else [a for t, a in zip(tokens, adapters) for _ in t]
+        table = [s.pages + [-1] * (width - len(s.pages)) for s in seqs]
+        parts = [flat, positions, slots, q_start, [s.length for s in seqs], group_start, shared,
+                 ids, sum(table, [])]
+        # one upload for everything the step's ops read
+        meta = torch.from_numpy(np.concatenate(parts).astype(np.int32)).to(w.embed.w.device)
+        (tok, pos, slot, q_start, kv_len, group_start, shared, ids,
+         table) = meta.split([len(p) for p in parts])
+
+        H, I, Q, KV = cfg.hidden, cfg.inter, cfg.q_out, cfg.kv_out
+        dev = w.embed.w.device
+        bf = dict(dtype=torch.bfloat16, device=dev)
+        x, xn = torch.empty(T, H, **bf), torch.empty(T, H, **bf)
+        qkv, att = torch.empty(T, Q + 2 * KV, **bf), torch.empty(T, Q, **bf)
+        gu, act = torch.empty(T, 2 * I, **bf), torch.empty(T, I, **bf)
+        q_bytes = max(L.lib().heph_fp8_linear_ws_bytes(T, n, k) for n, k in
+                      ((Q + 2 * KV, H), (H, Q), (2 * I, H), (H, I)))
+        ws = (torch.empty(q_bytes, dtype=torch.uint8, device=dev),
+              torch.empty(T * max(H, Q, I) // 128, dtype=torch.float32, device=dev))
+        plan = AttentionPlan(S, T, cfg.n_heads, cfg.n_kv_heads, width, n_groups=G, device=dev)
+        plan.update(q_start, kv_len, group_start, shared)
+        table = table.view(S, width)
+        lora = self.lora if adapters is not None else None
+        if lora is not None:
+            lplan = LoraPlan(T, lora.n_adapters, lora.max_rank, lora.max_k, device=dev)
+            lplan.update(ids)
+
+        def adapt(li, op, c, a):
+            if lora is not None and op in lora.layers[li]:
+                lora_add(c, c, a, *lora.layers[li][op], lora.scale, lplan)
+
+        def norm_linear(li, op, c, gamma, fw):
+            if lora is not None and op in lora.layers[li]:
+                # the adapter takes the normalized row too
+                DEC.rmsnorm(xn, x, gamma, cfg.eps)
+                self._linear(c, xn, fw, H, ws)
+                adapt(li, op, c, xn)
+            else:
+                HK.rmsnorm_quant_fp8(ws[0], ws[1], x, gamma, T, H, cfg.eps)
+                self._linear(c, None, fw, H, ws, quantized=True)
+
+        DEC.embed_fp8(x, w.embed.w, w.embed.scale, tok)
+        q = att.view(T, cfg.n_heads, 128)
+        qs = qkv.view(T, -1, 128)[:, :cfg.n_heads]
+        for li, lw in enumerate(w.layers):
+            norm_linear(li, "qkv", qkv, lw.attn_norm, lw.qkv)
+            qk_norm_rope_pages(qs, qkv.view(T, -1, 128), lw.q_norm, lw.k_norm, kv.k[li], kv.v[li],
+                               kv.inv[li], self.rope, pos, slot, cfg.eps)
+            attention_pages(q, qs, kv.k[li], kv.v[li], kv.scale[li], table, plan)
+            self._linear(x, att, lw.o, Q, ws, residual=True)
+            adapt(li, "o", x, att)
+            norm_linear(li, "gate_up", gu, lw.ffn_norm, lw.gate_up)
+            if lora is not None and "down" in lora.layers[li]:
+                # (the op takes gate and up each in one piece)
+                DEC.silu_mul(act, gu[:, :I].contiguous(), gu[:, I:].contiguous(), T * I)
+                self._linear(x, act, lw.down, I, ws, residual=True)
+                adapt(li, "down", x, act)
+            else:
+                HK.silu_mul_quant_fp8(ws[0], ws[1], gu, gu[:, I:], T, I, 2 * I)
+                self._linear(x, None, lw.down, I, ws, residual=True, quantized=True)
+        last = x[q_start[1:].long() - 1]
+        logits = torch.empty(S, cfg.vocab, dtype=torch.float32, device=dev)
+        HK.rmsnorm_quant_fp8(ws[0], ws[1], last, w.final_norm, S, H, cfg.eps)
+        self._linear(logits, None, w.embed, H, ws, quantized=True)
+        return logits

@@ -1,0 +1,328 @@
+"""The serving ops' argument checks and the page bookkeeping, without a GPU."""
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+from hephaestus_amd import _lib as L
+from hephaestus_amd import serve as S
+from hephaestus_amd.loader import Qwen3Config
+
+FAKE, ODD = 0x10000, 0x10008        # never dereferenced by validation
+CFG = Qwen3Config(vocab=512, hidden=256, n_layers=2, n_heads=8, n_kv_heads=2, inter=384)
+
+
+@pytest.fixture(scope="module")
+def lib():
+    return L.lib()
+
+
+def qk(lib, **kw):
+    a = dict(q=FAKE, qs=4096, x=FAKE * 2, xs=6144, qg=FAKE, kg=FAKE, k=FAKE, v=FAKE, np=4, inv=FAKE,
+             rope=FAKE, nr=10, pos=FAKE, slot=FAKE, T=3, H=32, KV=8, D=128)
+    a.update(kw)
+    return lib.heph_qk_norm_rope_pages(a["q"], a["qs"], a["x"], a["xs"], a["qg"], a["kg"], a["k"],
+                                       a["v"], a["np"], a["inv"], a["rope"], a["nr"], a["pos"],
+                                       a["slot"], a["T"], a["H"], a["KV"], a["D"], 1e-6, None)
+
+
+@pytest.mark.parametrize("kw,status", [
+    *[({f: None}, L.HEPH_ERR_NULL) for f in ("q", "x", "qg", "kg", "k", "v", "inv", "rope", "pos",
+                                             "slot")],
+    *[({f: ODD}, L.HEPH_ERR_ALIGN) for f in ("q", "x", "qg", "kg", "k", "v", "rope")],
+    (dict(qs=4088), L.HEPH_ERR_SHAPE), (dict(xs=6136), L.HEPH_ERR_SHAPE),
+    (dict(qs=4100), L.HEPH_ERR_ALIGN), (dict(xs=6150), L.HEPH_ERR_ALIGN),
+    (dict(T=0), L.HEPH_ERR_SHAPE), (dict(np=0), L.HEPH_ERR_SHAPE), (dict(nr=0), L.HEPH_ERR_SHAPE),
+    (dict(D=64), L.HEPH_ERR_SHAPE), (dict(H=30), L.HEPH_ERR_SHAPE), (dict(KV=0), L.HEPH_ERR_SHAPE),
+    (dict(H=130, KV=2, qs=1 << 20, xs=1 << 20), L.HEPH_ERR_SHAPE),
+    (dict(q=FAKE * 2), L.HEPH_ERR_SHAPE),                       # in place with another stride
+])
+def test_qk_rejects(lib, kw, status):
+    assert qk(lib, **kw) == status
+
+
+def attn(lib, **kw):
+    sizes = dict(T=3, S=2, G=0, H=32, KV=8)
+    sizes.update({f: kw[f] for f in sizes if f in kw})
+    a = dict(out=FAKE, q=FAKE * 4, qs=4096, k=FAKE, v=FAKE, np=4, sc=FAKE, table=FAKE, tp=5, plan=FAKE,
+             pb=1 << 40, ws=FAKE, wb=1 << 40, D=128, **sizes)
+    a.update(kw)
+    return lib.heph_pages_attention(a["out"], a["q"], a["qs"], a["k"], a["v"], a["np"], a["sc"],
+                                    a["table"], a["tp"], a["plan"], a["pb"], a["ws"], a["wb"],
+                                    a["T"], a["S"], a["G"], a["H"], a["KV"], a["D"], None)
+
+
+@pytest.mark.parametrize("kw,status", [
+    *[({f: None}, L.HEPH_ERR_NULL) for f in ("out", "q", "k", "v", "sc", "table", "plan", "ws")],
+    *[({f: ODD}, L.HEPH_ERR_ALIGN) for f in ("out", "q", "k", "v", "plan", "ws")],
+    (dict(qs=4088), L.HEPH_ERR_SHAPE), (dict(qs=4100), L.HEPH_ERR_ALIGN),
+    (dict(T=0), L.HEPH_ERR_SHAPE), (dict(S=0), L.HEPH_ERR_SHAPE), (dict(G=3), L.HEPH_ERR_SHAPE),
+    (dict(G=-1), L.HEPH_ERR_SHAPE), (dict(np=0), L.HEPH_ERR_SHAPE), (dict(tp=0), L.HEPH_ERR_SHAPE),
+    (dict(tp=4097), L.HEPH_ERR_SHAPE), (dict(D=64), L.HEPH_ERR_SHAPE), (dict(H=36), L.HEPH_ERR_SHAPE),
+    (dict(H=65, KV=1, qs=1 << 20), L.HEPH_ERR_SHAPE),
+    (dict(pb=16), L.HEPH_ERR_WORKSPACE), (dict(wb=8), L.HEPH_ERR_WORKSPACE),
+])
+def test_attention_rejects(lib, kw, status):
+    assert attn(lib, **kw) == status
+
+
+def test_attention_plan_rejects(lib):
+    def plan(p=FAKE, pb=1 << 40, qs=FAKE, kl=FAKE, gs=None, sh=None, T=3, S_=2, G=0, tp=5, H=32, KV=8):
+        return lib.heph_pages_attention_plan(p, pb, qs, kl, gs, sh, T, S_, G, tp, H, KV, None)
+    assert plan(p=None) == plan(qs=None) == plan(kl=None) == plan(G=1) == L.HEPH_ERR_NULL
+    assert plan(G=1, gs=FAKE) == L.HEPH_ERR_NULL
+    assert plan(p=ODD) == L.HEPH_ERR_ALIGN
+    assert plan(pb=8) == L.HEPH_ERR_WORKSPACE
+    for kw in (dict(T=0), dict(S_=0), dict(G=3, gs=FAKE, sh=FAKE), dict(tp=0), dict(H=33), dict(T=1 << 30)):
+        assert plan(**kw) == L.HEPH_ERR_SHAPE, kw
+    assert lib.heph_pages_attention_plan_bytes(0, 1, 0, 32, 8) == 0
+    assert lib.heph_pages_attention_ws_bytes(1, 0, 0, 32, 8) == 0
+
+
+def copy(lib, src, dst, k=FAKE, v=FAKE, layers=2, pages=8, kv=4, n=None):
+    s, d = np.array(src, np.int32), np.array(dst, np.int32)
+    return lib.heph_copy_pages(k, v, layers, pages, kv, s.ctypes.data, d.ctypes.data,
+                               len(src) if n is None else n, None)
+
+
+def test_copy_pages_rejects(lib):
+    for src, dst in (([0], [0]), ([0, 1], [2, 2]), ([0, 1], [1, 2]), ([-1], [0]), ([0], [8]),
+                     ([8], [0]), ([0], [-1]), ([0, 1, 2], [4, 5, 0])):
+        assert copy(lib, src, dst) == L.HEPH_ERR_SHAPE, (src, dst)
+    assert copy(lib, [0], [1], k=None) == L.HEPH_ERR_NULL
+    assert lib.heph_copy_pages(FAKE, FAKE, 1, 8, 4, None, FAKE, 1, None) == L.HEPH_ERR_NULL
+    assert copy(lib, [0], [1], v=ODD) == L.HEPH_ERR_ALIGN
+    for kw in (dict(layers=0), dict(pages=0), dict(kv=0), dict(n=-1)):
+        assert copy(lib, [0], [1], **kw) == L.HEPH_ERR_SHAPE, kw
+    assert copy(lib, [], []) == L.HEPH_OK
+
+
+def lora(lib, **kw):
+    a = dict(c=FAKE, dt=0, base=FAKE, x=FAKE, a=FAKE, b=FAKE, sc=FAKE, plan=FAKE, pb=1 << 40, ws=FAKE,
+             wb=1 << 40, M=4, N=96, K=256, r=16, A=3)
+    a.update(kw)
+    return lib.heph_lora_add(a["c"], a["dt"], a["base"], a["x"], a["a"], a["b"], a["sc"], a["plan"],
+                             a["pb"], a["ws"], a["wb"], a["M"], a["N"], a["K"], a["r"], a["A"], None)
+
+
+@pytest.mark.parametrize("kw,status", [
+    *[({f: None}, L.HEPH_ERR_NULL) for f in ("c", "base", "x", "a", "b", "sc", "plan", "ws")],
+    *[({f: ODD}, L.HEPH_ERR_ALIGN) for f in ("c", "base", "x", "a", "b", "plan", "ws")],
+    (dict(dt=2), L.HEPH_ERR_DTYPE), (dict(M=0), L.HEPH_ERR_SHAPE), (dict(N=40), L.HEPH_ERR_SHAPE),
+    (dict(K=24), L.HEPH_ERR_SHAPE), (dict(r=12), L.HEPH_ERR_SHAPE), (dict(r=136), L.HEPH_ERR_SHAPE),
+    (dict(r=0), L.HEPH_ERR_SHAPE), (dict(A=0), L.HEPH_ERR_SHAPE),
+    (dict(pb=8), L.HEPH_ERR_WORKSPACE), (dict(wb=8), L.HEPH_ERR_WORKSPACE),
+])
+def test_lora_rejects(lib, kw, status):
+    assert lora(lib, **kw) == status
+
+
+def test_lora_plan_rejects(lib):
+    assert lib.heph_lora_plan(None, 1 << 20, FAKE, 4, 3, None) == L.HEPH_ERR_NULL
+    assert lib.heph_lora_plan(FAKE, 1 << 20, None, 4, 3, None) == L.HEPH_ERR_NULL
+    assert lib.heph_lora_plan(ODD, 1 << 20, FAKE, 4, 3, None) == L.HEPH_ERR_ALIGN
+    assert lib.heph_lora_plan(FAKE, 8, FAKE, 4, 3, None) == L.HEPH_ERR_WORKSPACE
+    assert lib.heph_lora_plan(FAKE, 1 << 20, FAKE, 0, 3, None) == L.HEPH_ERR_SHAPE
+    assert lib.heph_lora_plan_bytes(0, 3) == 0 and lib.heph_lora_ws_bytes(4, 3, 256, 12) == 0
+
+
+def test_rope_table_rejects(lib):
+    assert lib.heph_rope_table_f32(None, 4, 128, 1e6, None) == L.HEPH_ERR_NULL
+    assert lib.heph_rope_table_f32(ODD, 4, 128, 1e6, None) == L.HEPH_ERR_ALIGN
+    for n, d, th in ((0, 128, 1e6), (262145, 128, 1e6), (4, 64, 1e6), (4, 128, 0.0), (4, 128, float("nan"))):
+        assert lib.heph_rope_table_f32(FAKE, n, d, th, None) == L.HEPH_ERR_SHAPE
+
+
+def test_valid_calls_without_a_gpu_report_the_device(lib):
+    if torch.cuda.is_available():
+        pytest.skip("a GPU is present")
+    assert qk(lib) == attn(lib) == lora(lib) == copy(lib, [0, 0], [1, 2]) == L.HEPH_ERR_DEVICE
+    assert lib.heph_lora_plan(FAKE, 1 << 20, FAKE, 4, 3, None) == L.HEPH_ERR_DEVICE
+
+
+def test_python_rejects_host_tensors():
+    t = torch.zeros(2, 8, 128, dtype=torch.bfloat16)
+    k, v = torch.zeros(4, 2, 2, 64, 64, dtype=torch.uint8), torch.zeros(4, 2, 128, 64, dtype=torch.uint8)
+    i = torch.zeros(2, dtype=torch.int32)
+    with pytest.raises(ValueError):
+        S.qk_norm_rope_pages(t, torch.zeros(2, 12, 128, dtype=torch.bfloat16), t[0, 0], t[0, 0], k, v,
+                             torch.ones(4), torch.zeros(4, 64, 2), i, i)
+    with pytest.raises(ValueError):
+        S.copy_pages(k[None], v[None], [0], [1])
+    with pytest.raises(ValueError):
+        S.lora_add(t[0], t[0], t[0], t, t, i, None)
+
+
+def test_v_place_is_a_permutation_that_keeps_runs_of_four():
+    p = [S.v_place(j) for j in range(64)]
+    assert sorted(p) == list(range(64))
+    assert all(p[j] == p[j - j % 4] + j % 4 for j in range(64))
+
+
+# ---------------------------------------------------------- page bookkeeping ----
+
+@pytest.fixture
+def cache(monkeypatch):
+    """A cache on the host whose page copies are torch's."""
+    c = S.PagedKVCache(CFG, 12, device="cpu")
+    c.copies = []
+
+    def copy_pages(k, v, src, dst, ctx=None):
+        assert not set(src) & set(dst) and len(set(dst)) == len(dst)
+        c.copies.append((list(src), list(dst)))
+        k[:, dst], v[:, dst] = k[:, src], v[:, src]
+    monkeypatch.setattr(S, "copy_pages", copy_pages)
+    return c
+
+
+def check_counts(c):
+    users = [0] * c.n_pages
+    for s in c._seqs:
+        assert len(s.pages) == -(-s.length // 64) and len(set(s.pages)) == len(s.pages)
+        for p in s.pages:
+            users[p] += 1
+    assert users == c._users
+    assert sorted(c._free) == [p for p in range(c.n_pages) if not users[p]]
+
+
+def write(c, slots, value):
+    for s in slots:
+        c.k[:, s // 64, :, :, s % 64] = value
+        c.v[:, s // 64, :, :, S.v_place(s % 64)] = value
+
+
+def read(c, seq):
+    k = [int(c.k[0, seq.pages[j // 64], 0, 0, j % 64, 0]) for j in range(seq.length)]
+    v = [int(c.v[1, seq.pages[j // 64], 1, 5, S.v_place(j % 64)]) for j in range(seq.length)]
+    assert k == v
+    return k
+
+
+def test_extend_fork_free_compact(cache):
+    c = cache
+    a = c.new()
+    slots = c.extend(a, 100)
+    assert slots == list(range(100)) and c.free_pages == 10
+    write(c, slots, 1)
+    b, d = c.fork(a, 2)
+    assert c.copies == [([1, 1], [2, 3])] and b.pages == [0, 2] and d.pages == [0, 3]
+    check_counts(c)
+    write(c, c.extend(b, 30), 2)
+    write(c, c.extend(d, 60), 3)
+    write(c, c.extend(a, 1), 4)
+    assert read(c, a) == [1] * 100 + [4]
+    assert read(c, b) == [1] * 100 + [2] * 30 and read(c, d) == [1] * 100 + [3] * 60
+    c.free(a)
+    check_counts(c)
+    assert c.free_pages == 12 - 6 + 1 and 0 not in c._free         # page 0 is still shared
+    c.free(b)
+    moved = c.compact()
+    check_counts(c)
+    assert moved == 2 and sorted(d.pages) == [0, 1, 2] and read(c, d) == [1] * 100 + [3] * 60
+    assert c.compact() == 0
+    c.free(d)
+    assert c.free_pages == 12
+
+
+def test_fork_of_full_pages_and_of_nothing(cache):
+    c = cache
+    a = c.new()
+    e, = c.fork(a)
+    assert e.pages == [] and c.copies == []
+    c.extend(a, 128)
+    f, g = c.fork(a, 2)
+    assert f.pages == a.pages == g.pages and c.copies == []
+    assert c.fork(a, 0) == []
+    c.extend(f, 1)
+    assert f.pages[:2] == a.pages and len(f.pages) == 3
+    check_counts(c)
+
+
+def test_bookkeeping_refusals(cache):
+    c = cache
+    a = c.new()
+    with pytest.raises(MemoryError):
+        c.extend(a, 12 * 64 + 1)
+    assert a.length == 0 and a.pages == []
+    c.extend(a, 11 * 64 + 5)
+    with pytest.raises(MemoryError):
+        c.fork(a)
+    check_counts(c)
+    with pytest.raises(ValueError):
+        c.extend(a, -1)
+    with pytest.raises(ValueError):
+        c.fork(a, -1)
+    c.free(a)
+    for f in (c.free, c.fork, lambda s: c.extend(s, 1)):
+        with pytest.raises(ValueError):
+            f(a)
+    with pytest.raises(ValueError):
+        S.PagedKVCache(CFG, 0, device="cpu")
+
+
+def test_random_use_keeps_every_sequence(cache):
+    c, rng, want = cache, np.random.default_rng(0), {}
+    value = 0
+    for step in range(300):
+        what, seqs = rng.integers(0, 5), list(c._seqs)
+        if what == 0 or not seqs:
+            s = c.new()
+            want[id(s)] = []
+            continue
+        s = seqs[rng.integers(len(seqs))]
+        try:
+            if what == 1:
+                n = int(rng.integers(0, 90))
+                value = value % 100 + 1
+                write(c, c.extend(s, n), value)
+                want[id(s)] = want[id(s)] + [value] * n
+            elif what == 2:
+                for f in c.fork(s, int(rng.integers(0, 3))):
+                    want[id(f)] = list(want[id(s)])
+            elif what == 3:
+                c.free(s)
+                # (keep the object: ids are not reused)
+                want[id(s)], want[("kept", step)] = [], s
+            else:
+                c.compact()
+        except MemoryError:
+            pass
+        check_counts(c)
+        for t in c._seqs:
+            assert read(c, t) == want[id(t)]
+
+
+def test_groups_of_sequences():
+    def seq(*pages):
+        s = S.Sequence()
+        s.pages = list(pages)
+        return s
+    assert S._groups([seq(1)]) == ([0, 1], [0])
+    assert S._groups([seq(1, 2, 3), seq(1, 2, 4), seq(1, 2, 5, 6)]) == ([0, 3], [2])
+    assert S._groups([seq(1, 2), seq(3, 4), seq(3, 5), seq()]) == ([0, 1, 3, 4], [0, 1, 0])
+    # a long common prefix is not given up for a member that shares little of it
+    assert S._groups([seq(*range(9)), seq(*range(9)), seq(0, 20)]) == ([0, 2, 3], [9, 0])
+
+
+def test_group_lists_fit_the_plan():
+    rng = np.random.default_rng(1)
+    for _ in range(50):
+        seqs = []
+        for _ in range(int(rng.integers(1, 12))):
+            s = S.Sequence()
+            s.pages = [int(rng.integers(0, 2)) * 100 + j for j in range(int(rng.integers(0, 6)))]
+            seqs.append(s)
+        start, shared = S._groups(seqs)
+        assert start[0] == 0 and start[-1] == len(seqs) and len(shared) == len(start) - 1 <= len(seqs)
+        for g, n in enumerate(shared):
+            rows = [s.pages[:n] for s in seqs[start[g]:start[g + 1]]]
+            assert all(r == rows[0] and len(r) == n for r in rows)
+
+
+def test_ctypes_signatures_of_the_serving_ops():
+    for name, nargs in (("heph_qk_norm_rope_pages", 20), ("heph_pages_attention", 20),
+                        ("heph_pages_attention_plan", 13), ("heph_copy_pages", 9),
+                        ("heph_lora_add", 17)):
+        assert len(L.SIGNATURES[name][1]) == nargs
+        assert getattr(L.lib(), name).restype is ctypes.c_int
