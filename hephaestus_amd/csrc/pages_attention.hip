@@ -19,6 +19,8 @@
 // together, everything else of one sequence's rows. The plan kernel lays the
 // units out from the lengths in device memory; units of the same row meet in
 // the workspace and merge_kernel joins them.
+#include <algorithm>
+
 #include "pages.h"
 
 namespace heph {
@@ -30,6 +32,7 @@ constexpr int kPlanThreads = 1024;
 
 struct PlanHeader {
     int magic, n_tok, n_seqs, n_groups, table_pages, n_heads, n_kv, n_units;
+    int merges, pad[3];            // whether any row has other than one unit
 };
 // Rows row0 .. row0+rows-1 (row = token * G + head of the group, from token
 // tok0 on) over pages page0 .. page0+pages-1 of table row seq. part: the
@@ -73,9 +76,8 @@ __host__ __device__ inline Unit* plan_units(PlanHeader* p, int n_tok)
 
 __device__ __forceinline__ int clampi(int v, int lo, int hi) { return min(max(v, lo), hi); }
 
-// Query rows of a unit by how many there are: 16, 32, 64 or 128. Four waves
-// share its pages (16 and 32 rows), pairs of waves do, or each wave takes 32
-// rows over all pages.
+// Query rows of a unit by how many there are: 16, 32 or 64 (attend_narrow: a
+// wave takes 16 rows, waves left over split the pages) or 128 (attend_wide).
 __device__ __forceinline__ int tile_rows(int rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128; }
 
 struct Source {
@@ -154,22 +156,24 @@ __device__ int scan_block(int v, int* red, int& total)
     return before + x - v;
 }
 
-// How a source is cut: row tiles, and pages a unit so that a unit's time (in
-// quarters of one wave's page of 16 rows: 32 rows cost twice, and with more
-// rows fewer waves share the pages) is about tau.
+// How a source is cut: row tiles, and pages a unit so that its time is about tau
+// (a page of a narrow unit costs the stream of its 16 KB, one of a wide unit
+// twice that in matrix work), but not so few that writing and joining 128 rows'
+// results outweighs their pages.
 struct Cut {
     int tile, tiles, per, chunks;
 };
+__device__ __forceinline__ int page_cost(int tile) { return tile == 128 ? 2 : 1; }
+__device__ __forceinline__ int min_pages(int tile) { return tile == 128 ? 8 : 4; }
 __device__ Cut cut_source(const Source& x, int G, long tau, int cap)
 {
     Cut c;
     const int rows = x.n_tok * G;
     c.tile = tile_rows(rows);
     c.tiles = (rows + c.tile - 1) / c.tile;
-    const int w = c.tile / 16;
-    const long per = (tau + w - 1) / w;
+    const int w = page_cost(c.tile);
+    const long per = max((tau + w - 1) / w, (long)min_pages(c.tile));
     c.per = max((int)min(per, (long)max(x.pages, 1)), (x.pages + cap - 1) / cap);
-    c.per = max(c.per, 1);
     c.chunks = (x.pages + c.per - 1) / c.per;
     if (c.chunks > 0) c.per = (x.pages + c.chunks - 1) / c.chunks;     // even
     if (c.chunks > 0) c.chunks = (x.pages + c.per - 1) / c.per;
@@ -185,13 +189,30 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanArgs a)
 {
     __shared__ long red_l[kPlanThreads / 64];
     __shared__ int red_i[kPlanThreads / 64];
+    __shared__ int32_t in_lds[4][kPlanThreads + 1];
+    __shared__ int merges;
     const int t = threadIdx.x, G = a.s.group(), n_src = a.s.n_groups + a.s.n_seqs;
     const int cap = a.s.parts(), cap_prefix = a.s.n_groups ? cap / 2 : 0, cap_own = cap - cap_prefix;
     const long max_units = a.s.max_units();
     Token* tokens = plan_tokens(a.plan);
     Unit* units = plan_units(a.plan, a.s.n_tok);
+    // The lengths, all on their way at once: what follows reads them in chains.
+    if (a.s.n_seqs <= kPlanThreads) {
+        if (t < a.s.n_seqs) in_lds[1][t] = a.kv_len[t];
+        for (int i = t; i <= a.s.n_seqs; i += kPlanThreads) in_lds[0][i] = a.q_start[i];
+        if (a.s.n_groups) {
+            if (t < a.s.n_groups) in_lds[3][t] = a.shared[t];
+            for (int i = t; i <= a.s.n_groups; i += kPlanThreads) in_lds[2][i] = a.group_start[i];
+        }
+        a.q_start = in_lds[0];
+        a.kv_len = in_lds[1];
+        a.group_start = in_lds[2];
+        a.shared = in_lds[3];
+    }
+    if (t == 0) merges = 0;
     // rows of no sequence
     for (int i = t; i < a.s.n_tok; i += kPlanThreads) tokens[i] = Token{-1, 0, 0, 0};
+    __syncthreads();
     auto source = [&](int j, int& kv) {
         kv = 0;
         return j < a.s.n_groups ? group_source(a, j) : seq_source(a, j - a.s.n_groups, kv);
@@ -201,10 +222,10 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanArgs a)
         int kv;
         const Source x = source(j, kv);
         const int rows = x.n_tok * G, tile = tile_rows(rows);
-        cost += (long)((rows + tile - 1) / tile) * x.pages * (tile / 16);
+        cost += (long)((rows + tile - 1) / tile) * x.pages * page_cost(tile);
     }
     cost = sum_block(cost, red_l) * a.s.n_kv;
-    const long tau = max(4L, (cost + kTargetUnits - 1) / kTargetUnits);
+    const long tau = (cost + kTargetUnits - 1) / kTargetUnits;
     int base = 0;
     for (int j0 = 0; j0 < n_src; j0 += kPlanThreads) {
         const int j = j0 + t;
@@ -236,7 +257,9 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanArgs a)
         }
         auto token = [&](int i, int tok0, int n_tok, int kv_, int page0, const Cut& p, const Cut& o) {
             const int limit = max(kv_ - n_tok + i + 1, 0);
-            tokens[tok0 + i] = Token{limit, parts_seen(limit, p), parts_seen(limit - page0 * kPage, o), 0};
+            const int np = parts_seen(limit, p), no = parts_seen(limit - page0 * kPage, o);
+            tokens[tok0 + i] = Token{limit, np, no, 0};
+            if (np + no != 1) merges = 1;
         };
         const int mine = j < n_src && !prefix ? x.n_tok : 0;
         if (mine <= 4)
@@ -254,7 +277,7 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanArgs a)
     __syncthreads();
     if (t == 0)
         *a.plan = PlanHeader{kMagic, a.s.n_tok, a.s.n_seqs, a.s.n_groups, a.table_pages, a.s.n_heads,
-                             a.s.n_kv, (int)min((long)base, max_units)};
+                             a.s.n_kv, (int)min((long)base, max_units), merges, {}};
 }
 
 // -------------------------------------------------------------- attention ----
@@ -298,7 +321,7 @@ __device__ __forceinline__ bf16x8 bf16_of_codes(int lo, int hi)
     return r.v;
 }
 
-// Max / sum over the four lanes l, l^16, l^32, l^48, in each of them.
+// Max over the four lanes l, l^16, l^32, l^48, in each of them.
 __device__ __forceinline__ float rows4_max(float v)
 {
     auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
@@ -306,18 +329,18 @@ __device__ __forceinline__ float rows4_max(float v)
     r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
-__device__ __forceinline__ float rows4_sum(float v)
-{
-    auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
-    r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
-}
 
-// Bytes of w that are NaN codes (0x7F, 0xFF), as 0x80 in their place.
-__device__ __forceinline__ uint32_t nan_bytes(uint32_t w)
+// Takes the NaN codes (0x7F, 0xFF) out of 16 codes, 0 in their place; whether there were any.
+__device__ __forceinline__ bool clear_nan(i32x4& w)
 {
-    return ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
+    uint32_t any = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t n = (((uint32_t)w[i] & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
+        w[i] &= (int)~(n | (n - (n >> 7)));
+        any |= n;
+    }
+    return any != 0;
 }
 
 // exp2(x - m) of a maximum that may be -inf (nothing seen): 0, not NaN.
@@ -326,9 +349,9 @@ __device__ __forceinline__ float weight(float x, float m)
     return __builtin_amdgcn_exp2f(x - (m == -INFINITY ? 0.0f : m));
 }
 
-// Bit 4 d + i of hit[r]: this lane's row of tile r sees a NaN code in V at dim
-// 16 d + 4 (lane / 16) + i of the page at vp: the product of the NaN codes with
-// the seen keys, both as 0 and 1. A rare path: V is read again, a dim tile at a time.
+// Bit 4 d + i of hit[r]: this lane's row of tile r sees a NaN in V at dim 16 d + 4
+// (lane / 16) + i of the page whose codes this lane reads at vp: the product of the NaN
+// codes with the seen keys, both as 0 and 1. A rare path: V is read again.
 template <int RT>
 __device__ __forceinline__ void nan_seen(const uint8_t* vp, int key0, const int (&limit)[RT],
                                          uint32_t (&hit)[RT])
@@ -346,8 +369,8 @@ __device__ __forceinline__ void nan_seen(const uint8_t* vp, int key0, const int 
                 bf16x8 is_nan, seen;
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    const uint32_t b = nan_bytes((uint32_t)w[2 * h + i / 4]) >> (i % 4 * 8) & 0x80u;
-                    is_nan[i] = (__bf16)(b ? 1.0f : 0.0f);
+                    const uint32_t b = (uint32_t)w[2 * h + i / 4] >> (i % 4 * 8) & 0x7Fu;
+                    is_nan[i] = (__bf16)(b == 0x7F ? 1.0f : 0.0f);
                     seen[i] = (__bf16)(key0 + h * 32 + i / 4 * 16 + i % 4 < limit[r] ? 1.0f : 0.0f);
                 }
                 n = mfma_bf16(is_nan, seen, n);
@@ -358,286 +381,428 @@ __device__ __forceinline__ void nan_seen(const uint8_t* vp, int key0, const int 
     }
 }
 
-// RT 16-row tiles a wave; kw of KW waves on the same rows take every KW-th page.
+// One wave's query rows: RT tiles of 16, column c of each in lane c, c+16, c+32, c+48.
 template <int RT>
-__device__ __forceinline__ void attend(const AttnArgs& a, const Unit& u, int head, int wave_rows,
-                                       int kw, int KW, f32x4* lds_o, float2* lds_ml)
-{
-    const int l = threadIdx.x & 63, wave = threadIdx.x >> 6, c = l & 15, g4 = l >> 4;
-    const int G = a.s.group(), H = a.s.n_heads, n_kv = a.s.n_kv;
-    const Token* tokens = plan_tokens(a.plan);
-    // this lane's rows: column c of each tile
+struct Rows {
     int tok[RT], hd[RT], limit[RT];
-    int lo = INT32_MAX, hi = 0;
+    int lo, hi;              // wave-uniform: smallest and largest limit of the rows
     bf16x8 q[RT][4];
-#pragma unroll
-    for (int r = 0; r < RT; ++r) {
-        const int row = wave_rows + r * 16 + c;
-        const bool live = row < u.rows;
-        const int at = u.row0 + (live ? row : 0);
-        tok[r] = live ? u.tok0 + at / G : -1;
-        hd[r] = head * G + at % G;
-        limit[r] = live ? tokens[tok[r]].limit : 0;
-        if (live) {
-            lo = min(lo, limit[r]);
-            hi = max(hi, limit[r]);
-        }
-        const uint16_t* p = a.q + (size_t)(live ? tok[r] : u.tok0) * a.q_stride + (size_t)hd[r] * kHeadDim;
-#pragma unroll
-        for (int f = 0; f < 4; ++f) {
-            const i32x4 w = ldg16(p + f / 2 * 64 + g4 * 16 + f % 2 * 8);
-            q[r][f] = __builtin_bit_cast(bf16x8, w);
-        }
-    }
-    // wave-uniform: pages below `full` need no mask, those from `end` on hold no key of ours
-#pragma unroll
-    for (int o = 1; o < 16; o <<= 1) {
-        lo = min(lo, __shfl_xor(lo, o));
-        hi = max(hi, __shfl_xor(hi, o));
-    }
-    lo = __builtin_amdgcn_readfirstlane(lo);
-    hi = __builtin_amdgcn_readfirstlane(hi);
-    const int first = u.page0, end = min(u.page0 + u.pages, (hi + kPage - 1) / kPage);
-
-    const float sc = a.kv_scale[head] * (0.08838834764831845f * 1.4426950408889634f);
     f32x4 o[8][RT];
-    float m[RT], sum[RT];
+    float m[RT];
+    f32x4 sum[RT];           // four times the same value
+
+    __device__ __forceinline__ void init(const AttnArgs& a, const Unit& u, int head, int wave_rows)
+    {
+        const int l = threadIdx.x & 63, c = l & 15, g4 = l >> 4, G = a.s.group();
+        const Token* tokens = plan_tokens(a.plan);
+        lo = INT32_MAX;
+        hi = 0;
 #pragma unroll
-    for (int r = 0; r < RT; ++r) {
-        m[r] = -INFINITY;
-        sum[r] = 0.0f;
+        for (int r = 0; r < RT; ++r) {
+            const int row = wave_rows + r * 16 + c;
+            const bool live = row < u.rows;
+            const int at = u.row0 + (live ? row : 0);
+            tok[r] = live ? u.tok0 + at / G : -1;
+            hd[r] = head * G + at % G;
+            limit[r] = live ? tokens[tok[r]].limit : 0;
+            if (live) {
+                lo = min(lo, limit[r]);
+                hi = max(hi, limit[r]);
+            }
+            const uint16_t* p = a.q + (size_t)(live ? tok[r] : u.tok0) * a.q_stride + (size_t)hd[r] * kHeadDim;
 #pragma unroll
-        for (int d = 0; d < 8; ++d) o[d][r] = f32x4{0, 0, 0, 0};
-    }
-    const int32_t* table = a.table + (size_t)u.seq * a.table_pages;
-    int ids_at = first, ids = first + l < a.table_pages ? table[first + l] : -1;
-    auto page_id = [&](int p) {
-        if (p >= ids_at + 64) {
-            ids_at = p;
-            ids = p + l < a.table_pages ? table[p + l] : -1;
+            for (int f = 0; f < 4; ++f)
+                q[r][f] = __builtin_bit_cast(bf16x8, ldg16(p + f / 2 * 64 + g4 * 16 + f % 2 * 8));
+            m[r] = -INFINITY;
+            sum[r] = f32x4{0, 0, 0, 0};
+#pragma unroll
+            for (int d = 0; d < 8; ++d) o[d][r] = f32x4{0, 0, 0, 0};
         }
-        return __builtin_amdgcn_readlane(ids, p - ids_at);
-    };
-    auto page_at = [&](const uint8_t* pool, int id) {
-        // (a page that is not there is not used: any address in the pool)
-        const int at = id >= 0 && id < a.n_pages ? id : 0;
-        return pool + ((size_t)at * n_kv + head) * kPageBytes + c * 64 + g4 * 16;
-    };
-    i32x4 k[8], v[8];
-    int p = first + kw, id = 0;
-    if (p < end) {
-        id = page_id(p);
-        const uint8_t* kp = page_at(a.k_pages, id);
-        const uint8_t* vp = page_at(a.v_pages, id);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) k[i] = ldg16(kp + i * 1024);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = ldg16(vp + i * 1024);
+        for (int o_ = 1; o_ < 16; o_ <<= 1) {
+            lo = min(lo, __shfl_xor(lo, o_));
+            hi = max(hi, __shfl_xor(hi, o_));
+        }
+        lo = __builtin_amdgcn_readfirstlane(lo);
+        hi = __builtin_amdgcn_readfirstlane(hi);
     }
-    while (p < end) {
-        const int next = p + KW;
-        const bool ok = id >= 0 && id < a.n_pages;
+
+    // The keys of one page. k(i, h) and v(i, h) give this lane's operands from the
+    // i-th 1 KB of the page's K (half i/4, keys 16 (i%4) ..; dims 8 h .. of the
+    // lane's 16) and V (dims 16 i ..; the lane's keys of the page's half h). page: its
+    // number in the sequence. Where some row does not see all of it, clear() takes the
+    // NaN out of what v gives and says whether there was any: a NaN must reach the rows
+    // that see its key and no other, and 0 * NaN is NaN; vp reads V's codes again for
+    // them. AHEAD: operands come from LDS, eight of them a step ahead of their products.
+    template <bool AHEAD, class K, class V, class C>
+    __device__ __forceinline__ void page(int page, float sc, K k, V v, C clear, const uint8_t* vp)
+    {
+        const int g4 = (threadIdx.x & 63) >> 4;
         f32x4 s[4][RT];
+        bf16x8 w0[8], w1[8];
+        auto k8 = [&](bf16x8 (&w)[8], int g) {
 #pragma unroll
-        for (int kt = 0; kt < 4; ++kt) {
+            for (int i = 0; i < 8; ++i) w[i] = k(i % 4 / 2 * 4 + 2 * g + i / 4, i % 2);
+        };
+        auto v8 = [&](bf16x8 (&w)[8], int g) {
 #pragma unroll
-            for (int r = 0; r < RT; ++r) s[kt][r] = f32x4{0, 0, 0, 0};
+            for (int i = 0; i < 8; ++i) w[i] = v(4 * g + i / 2, i % 2);
+        };
+        auto scores8 = [&](const bf16x8 (&w)[8], int g) {
 #pragma unroll
-            for (int f = 0; f < 2; ++f) {
-                const i32x4 w = k[f * 4 + kt];
-                const bf16x8 k0 = bf16_of_codes(w[0], w[1]), k1 = bf16_of_codes(w[2], w[3]);
+            for (int i = 0; i < 8; ++i)
 #pragma unroll
                 for (int r = 0; r < RT; ++r) {
-                    s[kt][r] = mfma_bf16(k0, q[r][2 * f], s[kt][r]);
-                    s[kt][r] = mfma_bf16(k1, q[r][2 * f + 1], s[kt][r]);
+                    const f32x4 zero = {0, 0, 0, 0};
+                    f32x4& x = s[2 * g + i / 4][r];
+                    x = mfma_bf16(w[i], q[r][i % 4], i % 4 ? x : zero);
                 }
-            }
-        }
-        const int id_next = next < end ? page_id(next) : -1;
-        const uint8_t* vp = page_at(a.v_pages, id_next);
-        if (next < end) {
-            const uint8_t* kp = page_at(a.k_pages, id_next);
+        };
+        auto step = [] { if constexpr (AHEAD) __builtin_amdgcn_sched_barrier(0); };
+        k8(w0, 0);
+        step();
+        if constexpr (AHEAD) k8(w1, 1);
+        step();
+        scores8(w0, 0);
+        step();
+        if constexpr (AHEAD) v8(w0, 0);
+        else k8(w1, 1);
+        step();
+        scores8(w1, 1);
+        step();
+        if ((page + 1) * kPage > lo) {
+            const int key0 = page * kPage + g4 * 4;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) k[i] = ldg16(kp + i * 1024);
-        }
-        if (ok) {
-            const bool masked = (p + 1) * kPage > lo;
-            if (masked) {
+            for (int r = 0; r < RT; ++r)
 #pragma unroll
-                for (int r = 0; r < RT; ++r)
+                for (int kt = 0; kt < 4; ++kt)
 #pragma unroll
-                    for (int kt = 0; kt < 4; ++kt)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            if (p * kPage + kt * 16 + g4 * 4 + i >= limit[r]) s[kt][r][i] = -INFINITY;
-                // A NaN code in V must reach the rows that see its key and no other, and
-                // 0 * NaN is NaN: such codes leave V, and where a row sees one its sum is
-                // set to NaN.
-                uint32_t any = 0;
+                    for (int i = 0; i < 4; ++i)
+                        if (key0 + kt * 16 + i >= limit[r]) s[kt][r][i] = -INFINITY;
+            if (clear()) {
+                uint32_t hit[RT];
+                nan_seen<RT>(vp, key0, limit, hit);
 #pragma unroll
                 for (int d = 0; d < 8; ++d)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) any |= nan_bytes((uint32_t)v[d][i]);
-                if (__any(any != 0)) {
-                    uint32_t hit[RT];
-                    nan_seen<RT>(page_at(a.v_pages, id), p * kPage + g4 * 4, limit, hit);
+                    for (int r = 0; r < RT; ++r)
 #pragma unroll
-                    for (int d = 0; d < 8; ++d)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const uint32_t w = nan_bytes((uint32_t)v[d][i]);
-                            v[d][i] &= (int)~(w | (w - (w >> 7)));
-#pragma unroll
-                            for (int r = 0; r < RT; ++r)
-                                if (hit[r] >> (4 * d + i) & 1) o[d][r][i] = NAN;
-                        }
-                }
+                        for (int i = 0; i < 4; ++i)
+                            if (hit[r] >> (4 * d + i) & 1) o[d][r][i] = NAN;
             }
-            bf16x8 prob[RT][2];
+        }
+        float top[RT];
+        bool moves = false;
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+            float x = -INFINITY;
+#pragma unroll
+            for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x = fmaxf(x, s[kt][r][i]);
+            // sc > 0: the largest score has the largest scaled one
+            top[r] = rows4_max(x * sc);
+            moves |= top[r] > m[r] + 8.0f;
+        }
+        // The maximum moves only by 2^8 or more: probabilities stay below 2^8, sums
+        // far from f32's range, and most pages scale nothing.
+        if (__any(moves)) {
 #pragma unroll
             for (int r = 0; r < RT; ++r) {
-                float top = -INFINITY;
+                const float now = fmaxf(m[r], top[r]), f = weight(m[r], now);
+                m[r] = now;
+                sum[r] *= f;
 #pragma unroll
-                for (int kt = 0; kt < 4; ++kt)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) top = fmaxf(top, s[kt][r][i]);
-                // sc >= 0: the largest score has the largest scaled one
-                top = rows4_max(top * sc);
-                // The maximum moves only by 2^8 or more: probabilities stay below
-                // 2^8, sums far from f32's range, and most pages scale nothing.
-                if (__any(top > m[r] + 8.0f)) {
-                    const float now = fmaxf(m[r], top), f = weight(m[r], now);
-                    m[r] = now;
-                    sum[r] *= f;
-#pragma unroll
-                    for (int d = 0; d < 8; ++d) o[d][r] *= f;
-                }
-                const float base = m[r] == -INFINITY ? 0.0f : m[r];
-                union {
-                    bf16x2 p[8];
-                    bf16x8 v[2];
-                } w;
-                float part = 0.0f;
-#pragma unroll
-                for (int kt = 0; kt < 4; ++kt)
-#pragma unroll
-                    for (int i = 0; i < 4; i += 2) {
-                        const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kt][r][i], sc, -base));
-                        const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kt][r][i + 1], sc, -base));
-                        part += e0 + e1;
-                        w.p[kt * 2 + i / 2] = __builtin_convertvector((f32x2){e0, e1}, bf16x2);
-                    }
-                sum[r] += part;
-                prob[r][0] = w.v[0];
-                prob[r][1] = w.v[1];
+                for (int d = 0; d < 8; ++d) o[d][r] *= f;
             }
+        }
+        bf16x8 prob[RT][2];
 #pragma unroll
-            for (int d = 0; d < 8; ++d)
+        for (int r = 0; r < RT; ++r) {
+            const float base = m[r] == -INFINITY ? 0.0f : m[r];
+            union {
+                bf16x2 p[8];
+                bf16x8 v[2];
+            } w;
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const bf16x8 w = bf16_of_codes(v[d][2 * h], v[d][2 * h + 1]);
+            for (int kt = 0; kt < 4; ++kt)
 #pragma unroll
-                    for (int r = 0; r < RT; ++r) o[d][r] = mfma_bf16(w, prob[r][h], o[d][r]);
+                for (int i = 0; i < 4; i += 2) {
+                    const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kt][r][i], sc, -base));
+                    const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kt][r][i + 1], sc, -base));
+                    w.p[kt * 2 + i / 2] = __builtin_convertvector((f32x2){e0, e1}, bf16x2);
                 }
+            prob[r][0] = w.v[0];
+            prob[r][1] = w.v[1];
         }
-        if (next < end) {
+        auto add8 = [&](const bf16x8 (&w)[8], int g) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = ldg16(vp + i * 1024);
-        }
-        p = next;
-        id = id_next;
+            for (int i = 0; i < 8; ++i)
+#pragma unroll
+                for (int r = 0; r < RT; ++r)
+                    o[4 * g + i / 2][r] = mfma_bf16(w[i], prob[r][i % 2], o[4 * g + i / 2][r]);
+        };
+        step();
+        if constexpr (AHEAD) v8(w1, 1);
+        else v8(w0, 0);
+        step();
+        // The sum of the rounded probabilities, as the product with a row of ones: it
+        // takes what the numerators take, and the matrix cores have the time.
+        const bf16x8 one = {1.0f, 1.0f, 1.0f, 1.0f, 1.0f, 1.0f, 1.0f, 1.0f};
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int r = 0; r < RT; ++r) sum[r] = mfma_bf16(one, prob[r][h], sum[r]);
+        add8(w0, 0);
+        step();
+        if constexpr (!AHEAD) v8(w1, 1);
+        add8(w1, 1);
     }
+
+    // The rows' results over dim tiles d0 .. d0+nd-1, held in o[0 .. nd): to out
+    // where the unit is the row's only one, else to its slot in the workspace.
+    __device__ __forceinline__ void store(const AttnArgs& a, const Unit& u, int head, int d0, int nd)
+    {
+        const int g4 = (threadIdx.x & 63) >> 4;
+        const Token* tokens = plan_tokens(a.plan);
+        const float sv = a.kv_scale[a.s.n_kv + head];
 #pragma unroll
-    for (int r = 0; r < RT; ++r) sum[r] = rows4_sum(sum[r]);
+        for (int r = 0; r < RT; ++r) {
+            if (tok[r] < 0) continue;
+            const Token tk = tokens[tok[r]];
+            if (u.part >= (u.prefix ? tk.n_prefix : tk.n_own)) continue;    // none of its keys here
+            const size_t row = (size_t)tok[r] * a.s.n_heads + hd[r];
+            if (tk.n_prefix + tk.n_own == 1) {
+                const float f = sum[r][0] == 0.0f && m[r] == -INFINITY ? 0.0f : sv / sum[r][0];
+                uint16_t* out = a.out + row * kHeadDim + g4 * 4;
+#pragma unroll
+                for (int d = 0; d < 8; ++d)
+                    if (d < nd) {
+                        const f32x4 x = o[d][r] * f;
+                        const uint2 w = make_uint2(
+                            (uint32_t)f32_to_bf16(x[0]) | (uint32_t)f32_to_bf16(x[1]) << 16,
+                            (uint32_t)f32_to_bf16(x[2]) | (uint32_t)f32_to_bf16(x[3]) << 16);
+                        *reinterpret_cast<uint2*>(out + (d0 + d) * 16) = w;
+                    }
+            } else {
+                const size_t slot = row * a.s.parts() + (u.prefix ? 0 : tk.n_prefix) + u.part;
+                if (g4 == 0 && d0 == 0) a.part_ml[slot] = make_float2(m[r], sum[r][0]);
+#pragma unroll
+                for (int d = 0; d < 8; ++d)
+                    if (d < nd)
+                        *reinterpret_cast<f32x4*>(a.part_o + slot * kHeadDim + (d0 + d) * 16 + g4 * 4) = o[d][r];
+            }
+        }
+    }
+};
+
+// The ids of the 64 pages from p on, one a lane. A load among the pages' own
+// would be waited for with all of them, so a run goes in blocks of 64 pages.
+__device__ __forceinline__ int page_ids(const AttnArgs& a, const Unit& u, int p)
+{
+    const int n = p + (threadIdx.x & 63);
+    return n < a.table_pages ? a.table[(size_t)u.seq * a.table_pages + n] : -1;
+}
+
+// s_waitcnt: at most N of this wave's vector memory operations and no LDS one left.
+template <int N>
+__device__ __forceinline__ void wait_vm()
+{
+    __builtin_amdgcn_s_waitcnt(0x0070 | (N & 15) | (N >> 4) << 14);
+    asm volatile("" ::: "memory");
+}
+
+// Up to 64 rows: a wave takes 16 of them and, where that leaves waves, every
+// KW-th page of the run. Bound by the stream of K and V: the next page's 16 KB
+// a wave are on their way into registers while one is worked on.
+__device__ __forceinline__ void attend_narrow(const AttnArgs& a, const Unit& u, int head, uint8_t* lds)
+{
+    const int l = threadIdx.x & 63, c = l & 15, g4 = l >> 4, n_kv = a.s.n_kv;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int KW = u.rows <= 16 ? 4 : u.rows <= 32 ? 2 : 1, kw = wave % KW;
+    Rows<1> x;
+    x.init(a, u, head, wave / KW * 16);
+    const int end = min(u.page0 + u.pages, (x.hi + kPage - 1) / kPage);
+    const float sc = a.kv_scale[head] * (0.08838834764831845f * 1.4426950408889634f);
+    auto place = [&](int id) {
+        // (a page that is not there is not used: any address in the pool)
+        const int at = id >= 0 && id < a.n_pages ? id : 0;
+        return ((size_t)at * n_kv + head) * kPageBytes + c * 64 + g4 * 16;
+    };
+    struct Page {
+        i32x4 k[8], v[8];
+        int id;
+    } p0, p1;
+    int ids = 0, first = 0, last = 0;
+    // (past the run its last page again: a load that is left out on some path would make
+    // the waits for the page before count without it, and hold up the one behind)
+    auto load = [&](Page& p, int n) {
+        p.id = __builtin_amdgcn_readlane(ids, min(n, last - 1) - first);
+        const size_t o = place(p.id);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) p.k[i] = ldg16(a.k_pages + o + i * 1024);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) p.v[i] = ldg16(a.v_pages + o + i * 1024);
+    };
+    auto work = [&](Page& p, int n) {
+        if (p.id < 0 || p.id >= a.n_pages) return;
+        auto half = [](const i32x4& w, int h) { return bf16_of_codes(w[2 * h], w[2 * h + 1]); };
+        auto clear = [&] {
+            bool any = false;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) any |= clear_nan(p.v[i]);
+            return __any(any);
+        };
+        x.page<false>(n, sc, [&](int i, int h) { return half(p.k[i], h); },
+                      [&](int i, int h) { return half(p.v[i], h); }, clear,
+                      a.v_pages + place(p.id));
+    };
+    for (first = u.page0; first < end; first += 64) {
+        last = min(first + 64, end);
+        ids = page_ids(a, u, first);
+        wait_vm<0>();           // (nothing but pages on its way below)
+        int n = first + kw;
+        load(p0, n);
+        while (n < last) {
+            load(p1, n + KW);
+            work(p0, n);
+            n += KW;
+            if (n >= last) break;
+            load(p0, n + KW);
+            work(p1, n);
+            n += KW;
+        }
+    }
 
     // Waves on the same rows join: each takes 8 / KW of the dim tiles.
     int d0 = 0, nd = 8;
     if (KW > 1) {
+        f32x4* lds_o = reinterpret_cast<f32x4*>(lds);
+        float2* lds_ml = reinterpret_cast<float2*>(lds + 4 * 8 * 64 * sizeof(f32x4));
+        if (g4 == 0) lds_ml[wave * 16 + c] = make_float2(x.m[0], x.sum[0][0]);
 #pragma unroll
-        for (int r = 0; r < RT; ++r) {
-            if (g4 == 0) lds_ml[wave * 32 + r * 16 + c] = make_float2(m[r], sum[r]);
-#pragma unroll
-            for (int d = 0; d < 8; ++d) lds_o[((wave * RT + r) * 8 + d) * 64 + l] = o[d][r];
-        }
+        for (int d = 0; d < 8; ++d) lds_o[(wave * 8 + d) * 64 + l] = x.o[d][0];
         __syncthreads();
         nd = 8 / KW;
         d0 = kw * nd;
         const int w0 = wave - kw;
+        float top = -INFINITY, total = 0.0f;
+        for (int w = 0; w < KW; ++w) top = fmaxf(top, lds_ml[(w0 + w) * 16 + c].x);
+        f32x4 o[4] = {};
+        for (int w = 0; w < KW; ++w) {
+            const float2 ml = lds_ml[(w0 + w) * 16 + c];
+            const float f = weight(ml.x, top);
+            total = __builtin_fmaf(ml.y, f, total);
 #pragma unroll
-        for (int r = 0; r < RT; ++r) {
-            float top = -INFINITY, total = 0.0f;
-            for (int w = 0; w < KW; ++w) top = fmaxf(top, lds_ml[(w0 + w) * 32 + r * 16 + c].x);
-            f32x4 x[4] = {};
-            for (int w = 0; w < KW; ++w) {
-                const float2 ml = lds_ml[(w0 + w) * 32 + r * 16 + c];
-                const float f = weight(ml.x, top);
-                total = __builtin_fmaf(ml.y, f, total);
+            for (int d = 0; d < 4; ++d)
+                if (d < nd) o[d] += lds_o[((w0 + w) * 8 + d0 + d) * 64 + l] * f;
+        }
+        x.m[0] = top;
+        x.sum[0][0] = total;
 #pragma unroll
-                for (int d = 0; d < 4; ++d)
-                    if (d < nd) x[d] += lds_o[(((w0 + w) * RT + r) * 8 + d0 + d) * 64 + l] * f;
+        for (int d = 0; d < 4; ++d) x.o[d][0] = o[d];
+    }
+    x.store(a, u, head, d0, nd);
+}
+
+// Up to 128 rows, 32 a wave. Bound by the matrix cores and the VALU's share beside
+// them (exp2, maxima, conversions), so each wave converts a quarter of a page's codes
+// to bf16 for all four, into one of two buffers in LDS in the operands' lane order
+// (linear: free of bank conflicts), while the other is worked on; the codes of the
+// page after that are on their way in registers.
+constexpr int kWidePage = 2 * 2 * kPageBytes;      // K and V as bf16
+
+// LDS accesses of the workgroup before and behind it are ordered; loads from
+// memory stay in flight (__syncthreads would wait for them).
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+__device__ __forceinline__ void attend_wide(const AttnArgs& a, const Unit& u, int head, uint8_t* lds)
+{
+    __shared__ int nan_page[2], lows[4];       // of each buffer's page; each wave's smallest limit
+    const int l = threadIdx.x & 63, c = l & 15, g4 = l >> 4, n_kv = a.s.n_kv;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    Rows<2> x;
+    x.init(a, u, head, wave * 32);
+    // The run's end for all waves: a sequence's last row sees most.
+    int end = u.page0 + u.pages;
+    if (!u.prefix) {
+        const int last = u.tok0 + (u.row0 + u.rows - 1) / a.s.group();
+        end = min(end, (plan_tokens(a.plan)[last].limit + kPage - 1) / kPage);
+    }
+    end = __builtin_amdgcn_readfirstlane(end);
+    if (l == 0) lows[wave] = x.lo;
+    __syncthreads();
+    // pages that some row does not see all of: their V goes to LDS without NaN
+    const int lo = __builtin_amdgcn_readfirstlane(min(min(lows[0], lows[1]), min(lows[2], lows[3])));
+    const float sc = a.kv_scale[head] * (0.08838834764831845f * 1.4426950408889634f);
+    // waves 0, 1: K's 1 KB tiles 0..3, 4..7; waves 2, 3: V's
+    const uint8_t* pool = (wave < 2 ? a.k_pages : a.v_pages) + (wave & 1) * 4096 + c * 64 + g4 * 16;
+    for (int first = u.page0; first < end; first += 64) {
+        const int last = min(first + 64, end), ids = page_ids(a, u, first);
+        wait_vm<0>();           // (nothing but pages on its way below)
+        auto id_of = [&](int n) { return __builtin_amdgcn_readlane(ids, n - first); };
+        i32x4 w[4];
+        auto load = [&](int n) {
+            const int id = id_of(n), at = id >= 0 && id < a.n_pages ? id : 0;
+            const uint8_t* p = pool + ((size_t)at * n_kv + head) * kPageBytes;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = ldg16(p + i * 1024);
+        };
+        auto buffer = [&](int n) { return lds + ((n - first) & 1) * kWidePage + l * 16; };
+        auto convert = [&](int n) {
+            uint8_t* to = buffer(n) + wave * 8192;
+            if (wave >= 2 && (n + 1) * kPage > lo) {
+                bool any = false;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) any |= clear_nan(w[i]);
+                if (__any(any) && l == 0) nan_page[(n - first) & 1] = n;
             }
-            m[r] = top;
-            sum[r] = total;
 #pragma unroll
-            for (int d = 0; d < 4; ++d) o[d][r] = x[d];
+            for (int i = 0; i < 4; ++i) {
+                *reinterpret_cast<bf16x8*>(to + i * 2048) = bf16_of_codes(w[i][0], w[i][1]);
+                *reinterpret_cast<bf16x8*>(to + i * 2048 + 1024) = bf16_of_codes(w[i][2], w[i][3]);
+            }
+        };
+        load(first);
+        if (threadIdx.x < 2) nan_page[threadIdx.x] = -1;
+        lds_barrier();          // (the last block's pages are read)
+        convert(first);
+        if (first + 1 < last) load(first + 1);
+        lds_barrier();
+        for (int n = first; n < last; ++n) {
+            if (n + 1 < last) convert(n + 1);
+            if (n + 2 < last) load(n + 2);
+            const int id = id_of(n);
+            if (id >= 0 && id < a.n_pages && n * kPage < x.hi) {
+                const uint8_t* base = buffer(n);
+                auto k = [&](int i, int h) { return *reinterpret_cast<const bf16x8*>(base + (2 * i + h) * 1024); };
+                auto v = [&](int i, int h) { return k(8 + i, h); };
+                auto clear = [&] { return nan_page[(n - first) & 1] == n; };
+                x.page<true>(n, sc, k, v, clear,
+                             a.v_pages + ((size_t)id * n_kv + head) * kPageBytes + c * 64 + g4 * 16);
+            }
+            lds_barrier();
         }
     }
-    const float sv = a.kv_scale[n_kv + head];
-#pragma unroll
-    for (int r = 0; r < RT; ++r) {
-        if (tok[r] < 0) continue;
-        const Token tk = tokens[tok[r]];
-        const int own_first = u.prefix ? 0 : tk.n_prefix;
-        if (u.part >= (u.prefix ? tk.n_prefix : tk.n_own)) continue;       // none of its keys here
-        const size_t row = (size_t)tok[r] * H + hd[r];
-        if (tk.n_prefix + tk.n_own == 1) {
-            const float f = sum[r] == 0.0f && m[r] == -INFINITY ? 0.0f : sv / sum[r];
-            uint16_t* out = a.out + row * kHeadDim + g4 * 4;
-#pragma unroll
-            for (int d = 0; d < 8; ++d)
-                if (d < nd) {
-                    const f32x4 x = o[d][r] * f;
-                    const uint2 w = make_uint2(
-                        (uint32_t)f32_to_bf16(x[0]) | (uint32_t)f32_to_bf16(x[1]) << 16,
-                        (uint32_t)f32_to_bf16(x[2]) | (uint32_t)f32_to_bf16(x[3]) << 16);
-                    *reinterpret_cast<uint2*>(out + (d0 + d) * 16) = w;
-                }
-        } else {
-            const size_t slot = row * a.s.parts() + own_first + u.part;
-            if (g4 == 0 && d0 == 0) a.part_ml[slot] = make_float2(m[r], sum[r]);
-#pragma unroll
-            for (int d = 0; d < 8; ++d)
-                if (d < nd)
-                    *reinterpret_cast<f32x4*>(a.part_o + slot * kHeadDim + (d0 + d) * 16 + g4 * 4) = o[d][r];
-        }
-    }
+    x.store(a, u, head, 0, 8);
 }
 
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void attention_kernel(AttnArgs a)
 {
-    __shared__ f32x4 lds_o[4 * 2 * 8 * 64];
-    __shared__ float2 lds_ml[4 * 32];
+    __shared__ __attribute__((aligned(16))) uint8_t lds[2 * kWidePage];
     const PlanHeader h = *a.plan;
     const int n_kv = a.s.n_kv, unit = blockIdx.x / n_kv, head = blockIdx.x % n_kv;
     if (!plan_fits(h, a) || unit >= h.n_units) return;
     const Unit u = plan_units(a.plan, a.s.n_tok)[unit];
-    const int wave = threadIdx.x >> 6;
-    if (u.rows <= 16) {
-        attend<1>(a, u, head, 0, wave, 4, lds_o, lds_ml);
-    } else {
-        const int KW = u.rows <= 32 ? 4 : u.rows <= 64 ? 2 : 1;
-        attend<2>(a, u, head, wave / KW * 32, wave % KW, KW, lds_o, lds_ml);
-    }
+    if (u.rows <= 64) attend_narrow(a, u, head, lds);
+    else attend_wide(a, u, head, lds);
 }
 
-// Joins the partial results of a row: one wave a row, two dims a lane. A row of
-// one unit is finished already.
-__global__ __launch_bounds__(256) void merge_kernel(AttnArgs a)
+// Joins the partial results of a row, two dims a lane. A row of one unit is
+// finished already.
+__device__ __forceinline__ void merge_row(const AttnArgs& a, long row, int l)
 {
-    if (!plan_fits(*a.plan, a)) return;
-    const long row = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (row >= a.s.rows()) return;
-    const int l = threadIdx.x & 63, t = (int)(row / a.s.n_heads), h = (int)(row % a.s.n_heads);
+    const int t = (int)(row / a.s.n_heads), h = (int)(row % a.s.n_heads);
     const Token tk = plan_tokens(a.plan)[t];
     const int n = min(tk.n_prefix + tk.n_own, a.s.parts());
     if (tk.limit < 0 || n == 1) return;
@@ -652,17 +817,36 @@ __global__ __launch_bounds__(256) void merge_kernel(AttnArgs a)
     top = wave_fold_max64(top);
     const float f0 = weight(ml[0].x, top), f1 = weight(ml[1].x, top);
     const float sum = wave_fold_sum64(__builtin_fmaf(ml[0].y, f0, ml[1].y * f1));
+    const float2* part = reinterpret_cast<const float2*>(a.part_o + slot * kHeadDim) + l;
     float x = 0.0f, y = 0.0f;
-    for (int k = 0; k < n; ++k) {
-        const float f = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(k < 64 ? f0 : f1), k & 63));
-        const float2 o = *reinterpret_cast<const float2*>(a.part_o + (slot + k) * kHeadDim + 2 * l);
-        x = __builtin_fmaf(o.x, f, x);
-        y = __builtin_fmaf(o.y, f, y);
+    for (int k = 0; k < n; k += 8) {
+        float2 o[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) o[i] = part[(size_t)min(k + i, n - 1) * (kHeadDim / 2)];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float f = __int_as_float(__builtin_amdgcn_readlane(
+                __float_as_int(k + i < 64 ? f0 : f1), (k + i) & 63));
+            if (k + i < n) {
+                x = __builtin_fmaf(o[i].x, f, x);
+                y = __builtin_fmaf(o[i].y, f, y);
+            }
+        }
     }
     const float f = sum == 0.0f && top == -INFINITY ? 0.0f
                                                     : a.kv_scale[a.s.n_kv + h / a.s.group()] / sum;
     *reinterpret_cast<uint32_t*>(a.out + row * kHeadDim + 2 * l) =
         (uint32_t)f32_to_bf16(x * f) | (uint32_t)f32_to_bf16(y * f) << 16;
+}
+
+// One wave a row at a time; nothing to do where every row has one unit.
+constexpr int kMergeBlocks = 2048;
+__global__ __launch_bounds__(256) void merge_kernel(AttnArgs a)
+{
+    const PlanHeader head = *a.plan;
+    if (!plan_fits(head, a) || !head.merges) return;
+    for (long row = (long)blockIdx.x * 4 + (threadIdx.x >> 6); row < a.s.rows(); row += (long)gridDim.x * 4)
+        merge_row(a, row, threadIdx.x & 63);
 }
 
 bool sizes_ok(int n_tok, int n_seqs, int n_groups, int n_heads, int n_kv)
@@ -735,8 +919,9 @@ int heph_pages_attention(void* out_bf16, const void* q_bf16, int64_t q_stride,
         return HEPH_ERR_WORKSPACE;
     AttnArgs a;
     a.s = Sizes{n_tok, n_seqs, n_groups, n_heads, n_kv_heads};
-    const long blocks = a.s.max_units() * n_kv_heads, merges = (a.s.rows() + 3) / 4;
-    if (blocks > INT32_MAX || merges > INT32_MAX) return HEPH_ERR_UNSUPPORTED;
+    const long blocks = a.s.max_units() * n_kv_heads;
+    const long merges = std::min((a.s.rows() + 3) / 4, (long)kMergeBlocks);
+    if (blocks > INT32_MAX) return HEPH_ERR_UNSUPPORTED;
     if (int st = check_device()) return st;
     a.out = static_cast<uint16_t*>(out_bf16);
     a.q = static_cast<const uint16_t*>(q_bf16);
