@@ -26,9 +26,9 @@
 namespace heph {
 namespace {
 
-constexpr int kMagic = 0x41505032;
-constexpr int kTargetUnits = 512;     // workgroups the split of long key runs aims at: two a CU
-constexpr int kPlanThreads = 1024;
+constexpr int kMagic = 0x41505033;
+constexpr int kSlots = 512;           // workgroups that run at once: two a CU
+constexpr int kMaxSeqs = HEPH_PAGES_MAX_SEQS;
 
 struct PlanHeader {
     int magic, n_tok, n_seqs, n_groups, table_pages, n_heads, n_kv, n_units;
@@ -47,6 +47,16 @@ struct Token {
     int limit, n_prefix, n_own, pad;
 };
 
+// Query rows of a unit by how many there are: 16, 32 or 64 (attend_narrow: a
+// wave takes 16 rows, waves left over split the pages) or as many whole tokens
+// as 128 rows hold (attend_wide).
+constexpr int kNarrow = 64;
+__host__ __device__ __forceinline__ int wide_rows(int G) { return 128 / G * G; }
+
+// Pages a unit has at least: fewer would not keep the four waves of a narrow one
+// busy, and writing and joining a wide one's 128 rows would outweigh its pages.
+constexpr int kMinNarrow = 4, kMinWide = 8;
+
 struct Sizes {
     int n_tok, n_seqs, n_groups, n_heads, n_kv;
     __host__ __device__ int group() const { return n_heads / n_kv; }
@@ -57,12 +67,15 @@ struct Sizes {
         const long p = (1L << 17) / rows();
         return (int)(p < 2 ? 2 : p > 96 ? 96 : p);
     }
-    // Units a plan may hold: runs split to the target, one more for each
-    // tile of each sequence and group.
+    // Slots of one kv head.
+    __host__ __device__ int slots() const { return kSlots / n_kv > 0 ? kSlots / n_kv : 1; }
+    // Units a plan may hold: one a tile (each sequence's and each group's last
+    // one may be short), and a round more where long runs are split and where
+    // the last round's tiles are.
     __host__ __device__ long max_units() const
     {
-        const long tiles = (long)n_tok * group() / 128;
-        return kTargetUnits / n_kv + 1 + n_seqs + n_groups + 2 * tiles;
+        const long tiles = (long)n_tok * group() / wide_rows(group());
+        return 2L * slots() + n_seqs + n_groups + 2 * tiles;
     }
 };
 
@@ -75,14 +88,7 @@ __host__ __device__ inline Unit* plan_units(PlanHeader* p, int n_tok)
 // ------------------------------------------------------------------- plan ----
 
 __device__ __forceinline__ int clampi(int v, int lo, int hi) { return min(max(v, lo), hi); }
-
-// Query rows of a unit by how many there are: 16, 32 or 64 (attend_narrow: a
-// wave takes 16 rows, waves left over split the pages) or 128 (attend_wide).
-__device__ __forceinline__ int tile_rows(int rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128; }
-
-struct Source {
-    int seq, tok0, n_tok, page0, pages;
-};
+__device__ __forceinline__ int ceil_div(int a, int b) { return (int)(((unsigned)a + (unsigned)b - 1) / (unsigned)b); }
 
 struct PlanArgs {
     PlanHeader* plan;
@@ -94,51 +100,101 @@ struct PlanArgs {
     int table_pages;
 };
 
+// The plan kernel's inputs in LDS, loaded all at once: what follows reads them
+// in chains.
+struct PlanLds {
+    int32_t q_start[kMaxSeqs + 1], kv_len[kMaxSeqs], group_start[kMaxSeqs + 1], shared[kMaxSeqs];
+};
+
+// Rows that work on the same pages: a group's on its shared ones, or one
+// sequence's on its own. Tiles are numbered over all sources from `base` on, a
+// sequence's last (longest) tile first.
+struct Source {
+    int seq, tok0, n_tok, page0, pages, kv;     // kv: 0 for a group
+    int tile, tiles, base;
+    int chunks;                                 // a tile's units before the last round
+};
+
+struct SeqTokens {
+    Source x;
+    int group;
+};
+
+// How the last round's tiles are cut.
+struct Rounds {
+    int first, chunks;
+};
+
+__device__ __forceinline__ void set_tiles(Source& x, int G)
+{
+    const int rows = x.n_tok * G;
+    x.tile = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= kNarrow ? kNarrow : wide_rows(G);
+    x.tiles = x.pages > 0 ? ceil_div(rows, x.tile) : 0;
+}
+
 // The group's sequences and shared pages; none where sharing gains nothing: a
 // single sequence, or sequences that bring 64 rows or more each, whose own
 // units are bound by the matrix cores and re-read a prefix from the caches.
-__device__ Source group_source(const PlanArgs& a, int g)
+__device__ Source group_source(const PlanLds& in, const PlanArgs& a, int g)
 {
-    const int s0 = clampi(a.group_start[g], 0, a.s.n_seqs);
-    const int s1 = clampi(a.group_start[g + 1], s0, a.s.n_seqs);
-    const int t0 = clampi(a.q_start[s0], 0, a.s.n_tok), t1 = clampi(a.q_start[s1], t0, a.s.n_tok);
+    const int s0 = clampi(in.group_start[g], 0, a.s.n_seqs);
+    const int s1 = clampi(in.group_start[g + 1], s0, a.s.n_seqs);
+    const int t0 = clampi(in.q_start[s0], 0, a.s.n_tok), t1 = clampi(in.q_start[s1], t0, a.s.n_tok);
     const int n = s1 - s0;
-    int pages = clampi(a.shared[g], 0, a.table_pages);
+    int pages = clampi(in.shared[g], 0, a.table_pages);
     if (n < 2 || (long)(t1 - t0) * a.s.group() >= 64L * n) pages = 0;
-    return Source{s0, t0, pages ? t1 - t0 : 0, 0, pages};
+    Source x{s0, t0, t1 - t0, 0, pages, 0};
+    set_tiles(x, a.s.group());
+    return x;
 }
 
-__device__ Source seq_source(const PlanArgs& a, int s, int& kv)
+__device__ Source seq_source(const PlanLds& in, const PlanArgs& a, int s, int& group)
 {
-    const int t0 = clampi(a.q_start[s], 0, a.s.n_tok), t1 = clampi(a.q_start[s + 1], t0, a.s.n_tok);
-    kv = clampi(a.kv_len[s], 0, a.table_pages * kPage);
+    const int t0 = clampi(in.q_start[s], 0, a.s.n_tok), t1 = clampi(in.q_start[s + 1], t0, a.s.n_tok);
+    const int kv = clampi(in.kv_len[s], 0, a.table_pages * kPage);
     int lo = 0, hi = a.s.n_groups;            // the last group that starts at s or before
     while (lo < hi) {
         const int mid = (lo + hi) / 2;
-        if (a.group_start[mid] <= s) lo = mid + 1;
+        if (in.group_start[mid] <= s) lo = mid + 1;
         else hi = mid;
     }
-    int page0 = 0;
-    if (lo > 0 && s < a.group_start[lo]) page0 = group_source(a, lo - 1).pages;
-    return Source{s, t0, t1 - t0, page0, max((kv + kPage - 1) / kPage - page0, 0)};
+    group = lo > 0 && s < in.group_start[lo] ? lo - 1 : -1;
+    const int page0 = group >= 0 ? group_source(in, a, group).pages : 0;
+    Source x{s, t0, t1 - t0, page0, max((kv + kPage - 1) / kPage - page0, 0), kv};
+    set_tiles(x, a.s.group());
+    return x;
 }
 
-__device__ long sum_block(long v, long* red)
+// Keys that token i of the source attends to.
+__device__ __forceinline__ int limit_of(const Source& x, int i) { return max(x.kv - x.n_tok + i + 1, 0); }
+
+// Units of tile r and pages of each: a sequence's tile sees its last token's keys.
+struct Cut {
+    int per, chunks;
+};
+__device__ __forceinline__ Cut cut_tile(const Source& x, const Rounds& rounds, int G, int r)
 {
-    const int t = threadIdx.x;
-    for (int o = 32; o; o >>= 1) v += __shfl_down(v, o);
-    __syncthreads();
-    if (t % 64 == 0) red[t / 64] = v;
-    __syncthreads();
-    long r = 0;
-    for (int i = 0; i < kPlanThreads / 64; ++i) r += red[i];
-    return r;
+    int pages = x.pages;
+    if (x.kv > 0 && x.tiles > 1) {
+        const int last = (int)min((unsigned)((r + 1) * x.tile) / (unsigned)G, (unsigned)x.n_tok) - 1;
+        pages = clampi((limit_of(x, last) + kPage - 1) / kPage - x.page0, 0, pages);
+    }
+    Cut c;
+    c.chunks = x.tile > kNarrow && x.base + x.tiles - 1 - r >= rounds.first ? rounds.chunks : x.chunks;
+    c.per = max(ceil_div(pages, c.chunks), 1);
+    return c;
+}
+
+// Units of c that hold any of the first `keys` keys.
+__device__ __forceinline__ int parts_seen(int keys, const Cut& c)
+{
+    return keys <= 0 ? 0 : min(c.chunks, ceil_div((keys + kPage - 1) / kPage, c.per));
 }
 
 // Exclusive prefix sum over the workgroup, and the total.
 __device__ int scan_block(int v, int* red, int& total)
 {
-    const int t = threadIdx.x, l = t & 63;
+    const int t = threadIdx.x, l = t & 63, waves = blockDim.x / 64;
     int x = v;
     for (int o = 1; o < 64; o <<= 1) {
         const int y = __shfl_up(x, o);
@@ -149,135 +205,125 @@ __device__ int scan_block(int v, int* red, int& total)
     __syncthreads();
     int before = 0;
     total = 0;
-    for (int i = 0; i < kPlanThreads / 64; ++i) {
+    for (int i = 0; i < waves; ++i) {
         if (i < t / 64) before += red[i];
         total += red[i];
     }
     return before + x - v;
 }
 
-// How a source is cut: row tiles, and pages a unit so that its time is about tau
-// (a page of a narrow unit costs the stream of its 16 KB, one of a wide unit
-// twice that in matrix work), but not so few that writing and joining 128 rows'
-// results outweighs their pages.
-struct Cut {
-    int tile, tiles, per, chunks;
-};
-__device__ __forceinline__ int page_cost(int tile) { return tile == 128 ? 2 : 1; }
-__device__ __forceinline__ int min_pages(int tile) { return tile == 128 ? 8 : 4; }
-__device__ Cut cut_source(const Source& x, int G, long tau, int cap)
+// One thread a sequence and a group. Every workgroup repeats that and writes a share
+// of the tokens; the first one also writes the units and the header.
+constexpr int kPlanTokens = 256;
+__global__ __launch_bounds__(kMaxSeqs) void plan_kernel(PlanArgs a)
 {
-    Cut c;
-    const int rows = x.n_tok * G;
-    c.tile = tile_rows(rows);
-    c.tiles = (rows + c.tile - 1) / c.tile;
-    const int w = page_cost(c.tile);
-    const long per = max((tau + w - 1) / w, (long)min_pages(c.tile));
-    c.per = max((int)min(per, (long)max(x.pages, 1)), (x.pages + cap - 1) / cap);
-    c.chunks = (x.pages + c.per - 1) / c.per;
-    if (c.chunks > 0) c.per = (x.pages + c.chunks - 1) / c.chunks;     // even
-    if (c.chunks > 0) c.chunks = (x.pages + c.per - 1) / c.per;
-    return c;
-}
-
-__device__ __forceinline__ int parts_seen(int keys, const Cut& c)
-{
-    return keys <= 0 ? 0 : min(c.chunks, (keys + c.per * kPage - 1) / (c.per * kPage));
-}
-
-__global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanArgs a)
-{
-    __shared__ long red_l[kPlanThreads / 64];
-    __shared__ int red_i[kPlanThreads / 64];
-    __shared__ int32_t in_lds[4][kPlanThreads + 1];
-    __shared__ int merges;
-    const int t = threadIdx.x, G = a.s.group(), n_src = a.s.n_groups + a.s.n_seqs;
+    __shared__ PlanLds in;
+    __shared__ Source groups[kMaxSeqs];
+    __shared__ SeqTokens seqs[kMaxSeqs];
+    __shared__ float red_f[kMaxSeqs / 64];
+    __shared__ int red_i[kMaxSeqs / 64], merges;
+    const int t = threadIdx.x, G = a.s.group(), nt = blockDim.x;
     const int cap = a.s.parts(), cap_prefix = a.s.n_groups ? cap / 2 : 0, cap_own = cap - cap_prefix;
-    const long max_units = a.s.max_units();
     Token* tokens = plan_tokens(a.plan);
     Unit* units = plan_units(a.plan, a.s.n_tok);
-    // The lengths, all on their way at once: what follows reads them in chains.
-    if (a.s.n_seqs <= kPlanThreads) {
-        if (t < a.s.n_seqs) in_lds[1][t] = a.kv_len[t];
-        for (int i = t; i <= a.s.n_seqs; i += kPlanThreads) in_lds[0][i] = a.q_start[i];
-        if (a.s.n_groups) {
-            if (t < a.s.n_groups) in_lds[3][t] = a.shared[t];
-            for (int i = t; i <= a.s.n_groups; i += kPlanThreads) in_lds[2][i] = a.group_start[i];
-        }
-        a.q_start = in_lds[0];
-        a.kv_len = in_lds[1];
-        a.group_start = in_lds[2];
-        a.shared = in_lds[3];
+    for (int i = t; i <= a.s.n_seqs; i += nt) in.q_start[i] = a.q_start[i];
+    if (t < a.s.n_seqs) in.kv_len[t] = a.kv_len[t];
+    if (a.s.n_groups) {
+        for (int i = t; i <= a.s.n_groups; i += nt) in.group_start[i] = a.group_start[i];
+        if (t < a.s.n_groups) in.shared[t] = a.shared[t];
     }
     if (t == 0) merges = 0;
-    // rows of no sequence
-    for (int i = t; i < a.s.n_tok; i += kPlanThreads) tokens[i] = Token{-1, 0, 0, 0};
     __syncthreads();
-    auto source = [&](int j, int& kv) {
-        kv = 0;
-        return j < a.s.n_groups ? group_source(a, j) : seq_source(a, j - a.s.n_groups, kv);
+    Source xg{}, xs{};
+    int group = -1;
+    if (t < a.s.n_groups) xg = group_source(in, a, t);
+    if (t < a.s.n_seqs) xs = seq_source(in, a, t, group);
+
+    // Work: a page of a narrow unit costs the stream of its 16 KB, one of a wide
+    // unit about twice that in matrix work. (In f32: it only sets a split.)
+    auto wide = [](const Source& x) { return x.tile > kNarrow; };
+    auto cost = [&](const Source& x) { return (float)x.tiles * (float)x.pages * (wide(x) ? 2.0f : 1.0f); };
+    float work = cost(xg) + cost(xs);
+    for (int o = 32; o; o >>= 1) work += __shfl_xor(work, o);
+    if ((t & 63) == 0) red_f[t / 64] = work;
+    int wide_g, wide_s;
+    xg.base = scan_block(wide(xg) ? xg.tiles : 0, red_i, wide_g);
+    xs.base = wide_g + scan_block(wide(xs) ? xs.tiles : 0, red_i, wide_s);
+    work = 0.0f;
+    for (int i = 0; i < nt / 64; ++i) work += red_f[i];
+
+    // Runs are split so that the units fill the slots of a kv head; wide tiles
+    // that fill them by themselves stay whole but for those of a last round that
+    // would leave half of the slots or more empty.
+    const int slots = a.s.slots(), wide_tiles = wide_g + wide_s, rest = wide_tiles % slots;
+    const float tau = work / (float)slots;
+    auto chunks = [&](const Source& x, int cap) {
+        if (wide(x) && wide_tiles >= slots) return 1;
+        const float per = fmaxf(tau * (wide(x) ? 0.5f : 1.0f), (float)(wide(x) ? kMinWide : kMinNarrow));
+        return clampi((int)ceilf((float)x.pages / per), 1, cap);
     };
-    long cost = 0;
-    for (int j = t; j < n_src; j += kPlanThreads) {
-        int kv;
-        const Source x = source(j, kv);
-        const int rows = x.n_tok * G, tile = tile_rows(rows);
-        cost += (long)((rows + tile - 1) / tile) * x.pages * page_cost(tile);
-    }
-    cost = sum_block(cost, red_l) * a.s.n_kv;
-    const long tau = (cost + kTargetUnits - 1) / kTargetUnits;
-    int base = 0;
-    for (int j0 = 0; j0 < n_src; j0 += kPlanThreads) {
-        const int j = j0 + t;
-        int kv = 0;
-        Source x{0, 0, 0, 0, 0};
-        if (j < n_src) x = source(j, kv);
-        const bool prefix = j < a.s.n_groups;
-        const Cut c = cut_source(x, G, tau, prefix ? cap_prefix : cap_own);
-        const int n = c.tiles * c.chunks;
-        int total;
-        int u = base + scan_block(n, red_i, total);
-        base += total;
-        for (int k = 0; k < c.chunks; ++k)
-            for (int r = 0; r < c.tiles; ++r, ++u)
+    Rounds rounds{INT32_MAX, 1};
+    if (wide_tiles >= slots && rest > 0) rounds = Rounds{wide_tiles - rest, slots / rest};
+    rounds.chunks = min(min(rounds.chunks, a.s.n_groups ? cap_prefix : cap_own),
+                        ceil_div(a.table_pages, kMinNarrow));
+    xg.chunks = chunks(xg, cap_prefix);
+    xs.chunks = chunks(xs, cap_own);
+    if (t < a.s.n_groups) groups[t] = xg;
+
+    auto count = [&](const Source& x) {
+        if (!wide(x)) return x.tiles * x.chunks;
+        const int last = clampi(x.base + x.tiles - rounds.first, 0, x.tiles);    // of the last round
+        return (x.tiles - last) * x.chunks + last * rounds.chunks;
+    };
+    int units_g, units_s;
+    const int at_g = scan_block(count(xg), red_i, units_g);
+    const int at_s = units_g + scan_block(count(xs), red_i, units_s);      // (groups[] is there)
+    const int max_units = (int)min(a.s.max_units(), (long)INT32_MAX);
+    auto emit = [&](const Source& x, int u, int prefix) {
+        const int rows = x.n_tok * G;
+        for (int r = x.tiles - 1; r >= 0; --r) {
+            const Cut c = cut_tile(x, rounds, G, r);
+            for (int k = 0; k < c.chunks; ++k, ++u)
                 if (u < max_units)
-                    units[u] = Unit{x.seq, x.tok0, r * c.tile, min(c.tile, x.n_tok * G - r * c.tile),
+                    units[u] = Unit{x.seq, x.tok0, r * x.tile, min(x.tile, rows - r * x.tile),
                                     x.page0 + k * c.per, min(c.per, x.pages - k * c.per), k, prefix};
-        // the sequence's tokens: its own thread writes a few, the wave many
-        Cut cp{16, 0, 1, 0};
-        if (j < n_src && !prefix && x.page0 > 0) {
-            // the group's cut, as its own thread made it
-            int lo = 0, hi = a.s.n_groups;
-            while (lo < hi) {
-                const int mid = (lo + hi) / 2;
-                if (a.group_start[mid] <= x.seq) lo = mid + 1;
-                else hi = mid;
-            }
-            cp = cut_source(group_source(a, lo - 1), G, tau, cap_prefix);
         }
-        auto token = [&](int i, int tok0, int n_tok, int kv_, int page0, const Cut& p, const Cut& o) {
-            const int limit = max(kv_ - n_tok + i + 1, 0);
-            const int np = parts_seen(limit, p), no = parts_seen(limit - page0 * kPage, o);
-            tokens[tok0 + i] = Token{limit, np, no, 0};
-            if (np + no != 1) merges = 1;
-        };
-        const int mine = j < n_src && !prefix ? x.n_tok : 0;
-        if (mine <= 4)
-            for (int i = 0; i < mine; ++i) token(i, x.tok0, x.n_tok, kv, x.page0, cp, c);
-        unsigned long long many = __ballot(mine > 4);
-        while (many) {
-            const int l = __ffsll((long long)many) - 1;
-            many &= many - 1;
-            auto from = [&](int v) { return __shfl(v, l); };
-            const int tok0 = from(x.tok0), nt = from(x.n_tok), kv_ = from(kv), page0 = from(x.page0);
-            const Cut p{0, 0, from(cp.per), from(cp.chunks)}, o{0, 0, from(c.per), from(c.chunks)};
-            for (int i = t & 63; i < nt; i += 64) token(i, tok0, nt, kv_, page0, p, o);
-        }
-    }
+    };
+    // a row of another number of units than one: behind a prefix, in a split run, without keys
+    if (xg.tiles > 0 || (xs.n_tok > 0 && (xs.kv < xs.n_tok || xs.tiles == 0 || count(xs) > xs.tiles)))
+        merges = 1;
+    if (t < a.s.n_seqs) seqs[t] = SeqTokens{xs, group};
     __syncthreads();
-    if (t == 0)
-        *a.plan = PlanHeader{kMagic, a.s.n_tok, a.s.n_seqs, a.s.n_groups, a.table_pages, a.s.n_heads,
-                             a.s.n_kv, (int)min((long)base, max_units), merges, {}};
+    if (blockIdx.x == 0) {
+        emit(xg, at_g, 1);
+        emit(xs, at_s, 0);
+        if (t == 0)
+            *a.plan = PlanHeader{kMagic, a.s.n_tok, a.s.n_seqs, a.s.n_groups, a.table_pages, a.s.n_heads,
+                                 a.s.n_kv, min(units_g + units_s, max_units), merges, {}};
+    }
+    for (int i = blockIdx.x * kPlanTokens + t; i < min(a.s.n_tok, ((int)blockIdx.x + 1) * kPlanTokens); i += nt) {
+        int lo = 0, hi = a.s.n_seqs;              // the last sequence that starts at i or before
+        while (lo < hi) {
+            const int mid = (lo + hi) / 2;
+            if (in.q_start[mid] <= i) lo = mid + 1;
+            else hi = mid;
+        }
+        Token tk{-1, 0, 0, 0};
+        if (lo > 0 && i < in.q_start[lo]) {
+            const Source& x = seqs[lo - 1].x;
+            const int g = seqs[lo - 1].group, at = i - x.tok0;
+            tk.limit = limit_of(x, at);
+            if (x.tiles > 0)
+                tk.n_own = parts_seen(tk.limit - x.page0 * kPage,
+                                      cut_tile(x, rounds, G, (unsigned)(at * G) / (unsigned)x.tile));
+            if (g >= 0 && groups[g].tiles > 0)
+                tk.n_prefix = parts_seen(
+                    min(tk.limit, x.page0 * kPage),
+                    cut_tile(groups[g], rounds, G,
+                             (unsigned)((i - groups[g].tok0) * G) / (unsigned)groups[g].tile));
+        }
+        tokens[i] = tk;
+    }
 }
 
 // -------------------------------------------------------------- attention ----
@@ -794,7 +840,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     const int n_kv = a.s.n_kv, unit = blockIdx.x / n_kv, head = blockIdx.x % n_kv;
     if (!plan_fits(h, a) || unit >= h.n_units) return;
     const Unit u = plan_units(a.plan, a.s.n_tok)[unit];
-    if (u.rows <= 64) attend_narrow(a, u, head, lds);
+    if (u.rows <= kNarrow) attend_narrow(a, u, head, lds);
     else attend_wide(a, u, head, lds);
 }
 
@@ -852,7 +898,7 @@ __global__ __launch_bounds__(256) void merge_kernel(AttnArgs a)
 bool sizes_ok(int n_tok, int n_seqs, int n_groups, int n_heads, int n_kv)
 {
     return heads_ok(n_heads, n_kv, kHeadDim) && n_tok >= 1 && n_seqs >= 1 && n_groups >= 0 &&
-           n_groups <= n_seqs && n_tok <= (1 << 20) && n_seqs <= (1 << 16) && n_heads <= 4096;
+           n_groups <= n_seqs && n_tok <= (1 << 20) && n_seqs <= kMaxSeqs && n_heads <= 4096;
 }
 
 }  // namespace
@@ -894,7 +940,8 @@ int heph_pages_attention_plan(void* plan, size_t plan_bytes, const int32_t* q_st
     if (int st = check_device()) return st;
     const PlanArgs a{static_cast<PlanHeader*>(plan), q_start, kv_len, group_start, shared_pages,
                      Sizes{n_tok, n_seqs, n_groups, n_heads, n_kv_heads}, table_pages};
-    plan_kernel<<<1, kPlanThreads, 0, static_cast<hipStream_t>(stream)>>>(a);
+    const int threads = std::max(256, (n_seqs + 63) / 64 * 64);
+    plan_kernel<<<(n_tok + kPlanTokens - 1) / kPlanTokens, threads, 0, static_cast<hipStream_t>(stream)>>>(a);
     return status_of(hipGetLastError());
 }
 
@@ -919,7 +966,10 @@ int heph_pages_attention(void* out_bf16, const void* q_bf16, int64_t q_stride,
         return HEPH_ERR_WORKSPACE;
     AttnArgs a;
     a.s = Sizes{n_tok, n_seqs, n_groups, n_heads, n_kv_heads};
-    const long blocks = a.s.max_units() * n_kv_heads;
+    // no unit has fewer pages than kMinNarrow unless it is its rows' only one
+    const long tiles = (long)n_tok * a.s.group() / wide_rows(a.s.group()) * 2 + n_seqs + n_groups;
+    const long blocks = std::min(a.s.max_units(), tiles * ((table_pages + kMinNarrow - 1) / kMinNarrow)) *
+                        n_kv_heads;
     const long merges = std::min((a.s.rows() + 3) / 4, (long)kMergeBlocks);
     if (blocks > INT32_MAX) return HEPH_ERR_UNSUPPORTED;
     if (int st = check_device()) return st;

@@ -33,34 +33,51 @@ _U8 = (torch.uint8, torch.float8_e4m3fn)
 _I32, _BF16, _F32 = (torch.int32,), (torch.bfloat16,), (torch.float32,)
 
 
-def _dev(t, name: str, dtypes, numel: int | None = None) -> int:
-    """Pointer of a contiguous tensor on the current device with at least
-    numel elements."""
-    p = HK._dev(t, name, dtypes)
-    if t.device.index != torch.cuda.current_device():
+def _dev(t, name: str, dtypes, numel: int, dev: int) -> int:
+    """Pointer of a contiguous tensor on device dev with at least numel elements."""
+    if isinstance(t, torch.Tensor) and t.dtype in dtypes and t.get_device() == dev and \
+            t.is_contiguous() and t.numel() >= numel:
+        return t.data_ptr()
+    HK._dev(t, name, dtypes)
+    if t.get_device() != dev:
         raise ValueError(f"{name} is on {t.device}, not on the current device")
-    if numel is not None and t.numel() < numel:
-        raise ValueError(f"{name} has {t.numel()} elements, {numel} are needed")
-    return p
+    raise ValueError(f"{name} has {t.numel()} elements, {numel} are needed")
 
 
-def _rows(t, name: str, n: int, width: int) -> tuple[int, int]:
+def _rows(t, name: str, n: int, width: int, dev: int) -> tuple[int, int]:
     """Pointer and row stride (elements) of n rows of width bf16 values; the
     rows may lie apart (a slice of a wider buffer)."""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch tensor")
-    if t.device.type != "cuda" or t.device.index != torch.cuda.current_device():
+    if t.get_device() != dev:
         raise ValueError(f"{name} must be in the current device's memory (got {t.device})")
     if t.dtype != torch.bfloat16:
         raise TypeError(f"{name} has dtype {t.dtype}, expected torch.bfloat16")
-    if t.dim() < 2 or t.shape[0] < n or t[0].numel() != width or not t[0].is_contiguous():
-        raise ValueError(f"{name} of shape {tuple(t.shape)} is not {n} rows of {width} "
-                         "consecutive values")
-    return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else max(width, t.stride(0))
+    if t.dim() >= 2 and t.shape[0] >= n:
+        if t.is_contiguous():
+            if t.numel() == t.shape[0] * width:
+                return t.data_ptr(), width
+        elif t[0].numel() == width and t[0].is_contiguous():
+            return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else width
+    raise ValueError(f"{name} of shape {tuple(t.shape)} is not {n} rows of {width} "
+                     "consecutive values")
+
+
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def _at(ctx) -> tuple[int, int]:
+    """The current device and the stream of a call: ctx, or its current one."""
+    dev = torch.cuda.current_device()
+    if ctx is None and _raw_stream is not None:
+        return dev, _raw_stream(dev)
+    return dev, HK._stream(ctx)
 
 
 def _call(name: str, *args) -> None:
-    HK._check(getattr(L.lib(), name)(*args), name)
+    status = getattr(L.lib(), name)(*args)
+    if status != L.HEPH_OK:
+        raise HephError(status, name)
 
 
 def v_place(j: int) -> int:
@@ -74,16 +91,18 @@ def rope_table_f32(n_pos: int, theta: float = 1e6, device="cuda", ctx=None) -> t
     """(cos, sin) in f32 of the 64 pairs of a 128-wide head at positions
     0..n_pos-1, [n_pos, 64, 2], the angles in double."""
     t = torch.empty(n_pos, 64, 2, dtype=torch.float32, device=device)
-    _call("heph_rope_table_f32", _dev(t, "table", _F32), n_pos, 128, theta, HK._stream(ctx))
+    dev, stream = _at(ctx)
+    _call("heph_rope_table_f32", _dev(t, "table", _F32, 0, dev), n_pos, 128, theta, stream)
     return t
 
 
-def _pools(k_pages, v_pages, n_kv: int) -> tuple[int, int, int]:
-    if k_pages.dim() < 5 or tuple(k_pages.shape[-4:]) != (n_kv, 2, PAGE, 64) or \
-            tuple(v_pages.shape) != tuple(k_pages.shape[:-3]) + (128, PAGE):
+def _pools(k_pages, v_pages, n_kv: int, dev: int) -> tuple[int, int, int]:
+    """Pointers of the K and V pools and how many pages a layer of them has."""
+    ks = k_pages.shape
+    if len(ks) < 5 or ks[-4:] != (n_kv, 2, PAGE, 64) or v_pages.shape != ks[:-3] + (128, PAGE):
         raise ValueError(f"pools of shapes {tuple(k_pages.shape)} and {tuple(v_pages.shape)} are "
                          f"not [n_pages, {n_kv}, 2, 64, 64] and [n_pages, {n_kv}, 128, 64]")
-    return _dev(k_pages, "k_pages", _U8), _dev(v_pages, "v_pages", _U8), k_pages.shape[-5]
+    return _dev(k_pages, "k_pages", _U8, 0, dev), _dev(v_pages, "v_pages", _U8, 0, dev), ks[-5]
 
 
 def qk_norm_rope_pages(q_out, qkv, q_gamma, k_gamma, k_pages, v_pages, kv_inv, rope, positions,
@@ -94,25 +113,31 @@ def qk_norm_rope_pages(q_out, qkv, q_gamma, k_gamma, k_pages, v_pages, kv_inv, r
     v_pages [n_pages, n_kv, 128, 64]. qkv: [n_tok, n_heads + 2 n_kv, 128], its
     rows may lie apart; q_out may be qkv[:, :n_heads]. A position outside
     rope skips the token, a slot outside the pools the cache write."""
-    n_tok, n_heads = q_out.shape[0], q_out[0].numel() // 128
-    n_kv = k_pages.shape[-4]
-    qp, qs = _rows(q_out, "q_out", n_tok, n_heads * 128)
-    xp, xs = _rows(qkv, "qkv", n_tok, (n_heads + 2 * n_kv) * 128)
-    kp, vp, n_pages = _pools(k_pages, v_pages, n_kv)
-    if rope.dim() != 3 or tuple(rope.shape[1:]) != (64, 2):
+    dev, stream = _at(ctx)
+    if q_out.dim() != 3 or q_out.shape[2] != 128 or k_pages.dim() != 5:
+        raise ValueError(f"q_out of shape {tuple(q_out.shape)} and k_pages of shape "
+                         f"{tuple(k_pages.shape)} are not [n_tok, n_heads, 128] and one layer's pool")
+    n_tok, n_heads = q_out.shape[0], q_out.shape[1]
+    n_kv = k_pages.shape[1]
+    qp, qs = _rows(q_out, "q_out", n_tok, n_heads * 128, dev)
+    xp, xs = _rows(qkv, "qkv", n_tok, (n_heads + 2 * n_kv) * 128, dev)
+    if n_tok == 1 and qp == xp:
+        qs = xs                   # (one row has no stride of its own)
+    kp, vp, n_pages = _pools(k_pages, v_pages, n_kv, dev)
+    if rope.dim() != 3 or rope.shape[1:] != (64, 2):
         raise ValueError(f"rope of shape {tuple(rope.shape)} is not [n_pos, 64, 2]")
-    _call("heph_qk_norm_rope_pages", qp, qs, xp, xs, _dev(q_gamma, "q_gamma", _BF16, 128),
-          _dev(k_gamma, "k_gamma", _BF16, 128), kp, vp, n_pages,
-          _dev(kv_inv, "kv_inv", _F32, 2 * n_kv), _dev(rope, "rope", _F32), rope.shape[0],
-          _dev(positions, "positions", _I32, n_tok), _dev(slots, "slots", _I32, n_tok), n_tok,
-          n_heads, n_kv, 128, eps, HK._stream(ctx))
+    _call("heph_qk_norm_rope_pages", qp, qs, xp, xs, _dev(q_gamma, "q_gamma", _BF16, 128, dev),
+          _dev(k_gamma, "k_gamma", _BF16, 128, dev), kp, vp, n_pages,
+          _dev(kv_inv, "kv_inv", _F32, 2 * n_kv, dev), _dev(rope, "rope", _F32, 0, dev),
+          rope.shape[0], _dev(positions, "positions", _I32, n_tok, dev),
+          _dev(slots, "slots", _I32, n_tok, dev), n_tok, n_heads, n_kv, 128, eps, stream)
 
 
 class AttentionPlan:
     """The layout of one step's attention and its workspace: update() it from
     the step's lengths in device memory, then call attention_pages for every
     layer. All sizes are fixed, so a captured step can be replayed with other
-    lengths."""
+    lengths. Calls that share a plan are ordered by the caller."""
 
     def __init__(self, n_seqs: int, n_tok: int, n_heads: int, n_kv: int, table_pages: int,
                  n_groups: int = 0, device="cuda"):
@@ -124,8 +149,8 @@ class AttentionPlan:
             raise HephError(L.HEPH_ERR_SHAPE, "AttentionPlan")
         # (zeros: no plan until the first update)
         self.plan = torch.zeros(nb, dtype=torch.uint8, device=device)
-        self.ws = torch.empty(max(16, L.lib().heph_pages_attention_ws_bytes(*sizes)),
-                              dtype=torch.uint8, device=device)
+        self.ws = torch.empty(L.lib().heph_pages_attention_ws_bytes(*sizes), dtype=torch.uint8,
+                              device=device)
 
     def update(self, q_start, kv_len, group_start=None, shared_pages=None, ctx=None) -> None:
         """q_start int32 [n_seqs + 1], kv_len int32 [n_seqs]; with groups
@@ -134,13 +159,14 @@ class AttentionPlan:
         if g != (group_start is not None) or g != (shared_pages is not None):
             raise ValueError(f"a plan of {self.n_groups} groups "
                              + ("needs" if g else "takes no") + " group_start and shared_pages")
-        _call("heph_pages_attention_plan", _dev(self.plan, "plan", _U8), self.plan.numel(),
-              _dev(q_start, "q_start", _I32, self.n_seqs + 1),
-              _dev(kv_len, "kv_len", _I32, self.n_seqs),
-              _dev(group_start, "group_start", _I32, self.n_groups + 1) if g else None,
-              _dev(shared_pages, "shared_pages", _I32, self.n_groups) if g else None,
+        dev, stream = _at(ctx)
+        _call("heph_pages_attention_plan", _dev(self.plan, "plan", _U8, 0, dev), self.plan.numel(),
+              _dev(q_start, "q_start", _I32, self.n_seqs + 1, dev),
+              _dev(kv_len, "kv_len", _I32, self.n_seqs, dev),
+              _dev(group_start, "group_start", _I32, self.n_groups + 1, dev) if g else None,
+              _dev(shared_pages, "shared_pages", _I32, self.n_groups, dev) if g else None,
               self.n_tok, self.n_seqs, self.n_groups, self.table_pages, self.n_heads, self.n_kv,
-              HK._stream(ctx))
+              stream)
 
 
 def attention_pages(out, q, k_pages, v_pages, kv_scale, page_table, plan: AttentionPlan,
@@ -150,16 +176,17 @@ def attention_pages(out, q, k_pages, v_pages, kv_scale, page_table, plan: Attent
     128] (rows may lie apart), out contiguous; page_table int32 [n_seqs,
     table_pages]."""
     p = plan
-    if tuple(page_table.shape) != (p.n_seqs, p.table_pages):
+    dev, stream = _at(ctx)
+    if page_table.shape != (p.n_seqs, p.table_pages):
         raise ValueError(f"page_table of shape {tuple(page_table.shape)} is not "
                          f"[{p.n_seqs}, {p.table_pages}] as planned")
-    qp, qs = _rows(q, "q", p.n_tok, p.n_heads * 128)
-    kp, vp, n_pages = _pools(k_pages, v_pages, p.n_kv)
-    _call("heph_pages_attention", _dev(out, "out", _BF16, p.n_tok * p.n_heads * 128), qp, qs, kp,
-          vp, n_pages, _dev(kv_scale, "kv_scale", _F32, 2 * p.n_kv),
-          _dev(page_table, "page_table", _I32), p.table_pages, _dev(p.plan, "plan", _U8),
-          p.plan.numel(), _dev(p.ws, "ws", _U8), p.ws.numel(), p.n_tok, p.n_seqs, p.n_groups,
-          p.n_heads, p.n_kv, 128, HK._stream(ctx))
+    qp, qs = _rows(q, "q", p.n_tok, p.n_heads * 128, dev)
+    kp, vp, n_pages = _pools(k_pages, v_pages, p.n_kv, dev)
+    _call("heph_pages_attention", _dev(out, "out", _BF16, p.n_tok * p.n_heads * 128, dev), qp, qs,
+          kp, vp, n_pages, _dev(kv_scale, "kv_scale", _F32, 2 * p.n_kv, dev),
+          _dev(page_table, "page_table", _I32, 0, dev), p.table_pages,
+          _dev(p.plan, "plan", _U8, 0, dev), p.plan.numel(), _dev(p.ws, "ws", _U8, 0, dev),
+          p.ws.numel(), p.n_tok, p.n_seqs, p.n_groups, p.n_heads, p.n_kv, 128, stream)
 
 
 def copy_pages(k_pools, v_pools, src, dst, ctx=None) -> None:
@@ -168,18 +195,21 @@ def copy_pages(k_pools, v_pools, src, dst, ctx=None) -> None:
     neither repeat nor be a source."""
     if k_pools.dim() != 6:
         raise ValueError(f"k_pools of shape {tuple(k_pools.shape)} has no layers")
-    kp, vp, n_pages = _pools(k_pools, v_pools, k_pools.shape[2])
+    dev, stream = _at(ctx)
+    kp, vp, n_pages = _pools(k_pools, v_pools, k_pools.shape[2], dev)
     s, d = np.asarray(src, dtype=np.int32).reshape(-1), np.asarray(dst, dtype=np.int32).reshape(-1)
     if s.size != d.size:
         raise ValueError(f"{s.size} sources and {d.size} destinations")
+    s, d = np.ascontiguousarray(s), np.ascontiguousarray(d)
     _call("heph_copy_pages", kp, vp, k_pools.shape[0], n_pages, k_pools.shape[2], s.ctypes.data,
-          d.ctypes.data, int(s.size), HK._stream(ctx))
+          d.ctypes.data, s.size, stream)
 
 
 class LoraPlan:
     """The rows of a step grouped by adapter, and the workspace of lora_add for
     projections of up to rank x k -> n: update() it from the rows' adapter ids
-    in device memory (an id outside [0, n_adapters): no adapter)."""
+    in device memory (an id outside [0, n_adapters): no adapter). Calls that
+    share a plan are ordered by the caller."""
 
     def __init__(self, m: int, n_adapters: int, rank: int, k: int, n: int | None = None,
                  device="cuda"):
@@ -189,11 +219,12 @@ class LoraPlan:
         if nb == 0 or wb == 0:
             raise HephError(L.HEPH_ERR_SHAPE, "LoraPlan")
         self.plan = torch.zeros(nb, dtype=torch.uint8, device=device)
-        self.ws = torch.empty(max(16, wb), dtype=torch.uint8, device=device)
+        self.ws = torch.empty(wb, dtype=torch.uint8, device=device)
 
     def update(self, ids, ctx=None) -> None:
-        _call("heph_lora_plan", _dev(self.plan, "plan", _U8), self.plan.numel(),
-              _dev(ids, "ids", _I32, self.m), self.m, self.n_adapters, HK._stream(ctx))
+        dev, stream = _at(ctx)
+        _call("heph_lora_plan", _dev(self.plan, "plan", _U8, 0, dev), self.plan.numel(),
+              _dev(ids, "ids", _I32, self.m, dev), self.m, self.n_adapters, stream)
 
 
 def lora_add(c, base, x, a, b, scale, plan: LoraPlan, ctx=None) -> None:
@@ -201,20 +232,23 @@ def lora_add(c, base, x, a, b, scale, plan: LoraPlan, ctx=None) -> None:
     that plan holds for it (c may be base, the projection's own output).
     a [n_adapters, rank, k], b [n_adapters, n, rank], x [m, k] bf16; c and base
     [m, n] bf16 or f32."""
-    if a.dim() != 3 or b.dim() != 3 or a.shape[0] != b.shape[0] or a.shape[1] != b.shape[2]:
-        raise ValueError(f"a {tuple(a.shape)} and b {tuple(b.shape)} are not [adapters, rank, k] "
+    sa, sb, m = a.shape, b.shape, plan.m
+    if len(sa) != 3 or len(sb) != 3 or sa[0] != sb[0] or sa[1] != sb[2]:
+        raise ValueError(f"a {tuple(sa)} and b {tuple(sb)} are not [adapters, rank, k] "
                          "and [adapters, n, rank]")
-    if a.shape[0] != plan.n_adapters:
-        raise ValueError(f"{a.shape[0]} adapters, planned for {plan.n_adapters}")
-    rank, k, n, m = a.shape[1], a.shape[2], b.shape[1], plan.m
+    if sa[0] != plan.n_adapters:
+        raise ValueError(f"{sa[0]} adapters, planned for {plan.n_adapters}")
     if c.dtype not in HK._OUT or base.dtype != c.dtype:
         raise TypeError(f"lora_add: c {c.dtype} and base {base.dtype} not supported")
-    dt = (c.dtype,)
-    _call("heph_lora_add", _dev(c, "c", dt, m * n), HK._OUT[c.dtype],
-          _dev(base, "base", dt, m * n), _dev(x, "x", _BF16, m * k), _dev(a, "a", _BF16),
-          _dev(b, "b", _BF16), _dev(scale, "scale", _F32, plan.n_adapters),
-          _dev(plan.plan, "plan", _U8), plan.plan.numel(), _dev(plan.ws, "ws", _U8),
-          plan.ws.numel(), m, n, k, rank, plan.n_adapters, HK._stream(ctx))
+    rank, k, n, dt = sa[1], sa[2], sb[1], (c.dtype,)
+    dev, stream = _at(ctx)
+    _call("heph_lora_add", _dev(c, "c", dt, m * n, dev), HK._OUT[c.dtype],
+          _dev(base, "base", dt, m * n, dev), _dev(x, "x", _BF16, m * k, dev),
+          _dev(a, "a", _BF16, 0, dev), _dev(b, "b", _BF16, 0, dev),
+          _dev(scale, "scale", _F32, plan.n_adapters, dev),
+          _dev(plan.plan, "plan", _U8, 0, dev), plan.plan.numel(),
+          _dev(plan.ws, "ws", _U8, 0, dev), plan.ws.numel(), m, n, k, rank, plan.n_adapters,
+          stream)
 
 
 # --------------------------------------------------------------- the cache ----

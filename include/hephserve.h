@@ -36,6 +36,8 @@ extern "C" {
  * order in which the scores of those keys lie in that lane).
  */
 #define HEPH_PAGE_KEYS 64
+/* Most sequences of one attention call. */
+#define HEPH_PAGES_MAX_SEQS 1024
 
 /*
  * Rotation table: table[pos][p] = (cos, sin) of pair p < head_dim/2 at
@@ -79,7 +81,9 @@ int heph_qk_norm_rope_pages(void* q_out_bf16, int64_t q_stride, const void* qkv_
  * with kv_scale (n_kv_heads K entries, then V). Scores, softmax statistics and
  * sums are f32; the unnormalized probabilities are rounded to bf16 for the
  * product with V, and out once to bf16. A token without keys gives a zero row.
- * n_heads is a multiple of n_kv_heads, at most 64 times it.
+ * n_heads is a multiple of n_kv_heads, at most 64 times it; n_seqs is at most
+ * HEPH_PAGES_MAX_SEQS. kv_scale > 0. A token whose every score is -inf gives a
+ * zero row.
  *
  * Shared prefixes: group g is the sequences group_start[g] ..
  * group_start[g+1]-1 (n_groups + 1 entries, not decreasing), whose first
@@ -95,9 +99,11 @@ int heph_qk_norm_rope_pages(void* q_out_bf16, int64_t q_stride, const void* qkv_
  * 16-byte aligned; calls that share a ws are ordered by the caller. A larger
  * ws is not used.
  *
- * On the device: q_start is clamped to [0, n_tok] and to not decreasing,
- * kv_len to [0, 64 * table_pages]; the keys of a page id outside [0, n_pages)
- * are left out as if masked. Rows of no sequence are left as they were.
+ * On the device: q_start is clamped to [0, n_tok], kv_len to [0, 64 *
+ * table_pages]; the keys of a page id outside [0, n_pages) are left out as if
+ * masked. Rows of no sequence are left as they were; rows that a decreasing
+ * q_start gives to two sequences, or that a decreasing group_start gives to two
+ * groups, are undefined.
  * q + t * q_stride: [n_heads, 128] (q_stride in elements, a multiple of 8);
  * out: [n_tok, n_heads, 128], not overlapping q.
  * Replaces, for a batch, attention (src/hephaestus/kernels.mojo:923-1240) as

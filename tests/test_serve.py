@@ -57,7 +57,8 @@ def attn(lib, **kw):
     *[({f: None}, L.HEPH_ERR_NULL) for f in ("out", "q", "k", "v", "sc", "table", "plan", "ws")],
     *[({f: ODD}, L.HEPH_ERR_ALIGN) for f in ("out", "q", "k", "v", "plan", "ws")],
     (dict(qs=4088), L.HEPH_ERR_SHAPE), (dict(qs=4100), L.HEPH_ERR_ALIGN),
-    (dict(T=0), L.HEPH_ERR_SHAPE), (dict(S=0), L.HEPH_ERR_SHAPE), (dict(G=3), L.HEPH_ERR_SHAPE),
+    (dict(T=0), L.HEPH_ERR_SHAPE), (dict(S=0), L.HEPH_ERR_SHAPE),
+    (dict(S=1025, T=2000), L.HEPH_ERR_SHAPE), (dict(G=3), L.HEPH_ERR_SHAPE),
     (dict(G=-1), L.HEPH_ERR_SHAPE), (dict(np=0), L.HEPH_ERR_SHAPE), (dict(tp=0), L.HEPH_ERR_SHAPE),
     (dict(tp=4097), L.HEPH_ERR_SHAPE), (dict(D=64), L.HEPH_ERR_SHAPE), (dict(H=36), L.HEPH_ERR_SHAPE),
     (dict(H=65, KV=1, qs=1 << 20), L.HEPH_ERR_SHAPE),
@@ -141,7 +142,8 @@ def test_valid_calls_without_a_gpu_report_the_device(lib):
     assert lib.heph_lora_plan(FAKE, 1 << 20, FAKE, 4, 3, None) == L.HEPH_ERR_DEVICE
 
 
-def test_python_rejects_host_tensors():
+def test_python_rejects_host_tensors(monkeypatch):
+    monkeypatch.setattr(S, "_at", lambda ctx: (0, 0))          # (no device to ask here)
     t = torch.zeros(2, 8, 128, dtype=torch.bfloat16)
     k, v = torch.zeros(4, 2, 2, 64, 64, dtype=torch.uint8), torch.zeros(4, 2, 128, 64, dtype=torch.uint8)
     i = torch.zeros(2, dtype=torch.int32)
@@ -151,7 +153,10 @@ def test_python_rejects_host_tensors():
     with pytest.raises(ValueError):
         S.copy_pages(k[None], v[None], [0], [1])
     with pytest.raises(ValueError):
-        S.lora_add(t[0], t[0], t[0], t, t, i, None)
+        plan = S.LoraPlan.__new__(S.LoraPlan)                  # (without its device buffers)
+        plan.m, plan.n_adapters = 2, 2
+        S.lora_add(t[0], t[0], t[0], torch.zeros(2, 8, 128, dtype=torch.bfloat16),
+                   torch.zeros(2, 128, 8, dtype=torch.bfloat16), torch.ones(2), plan)
 
 
 def test_v_place_is_a_permutation_that_keeps_runs_of_four():
