@@ -146,7 +146,8 @@ int heph_copy_pages(uint8_t* k_pages, uint8_t* v_pages, int n_layers, int n_page
  * 16 bits of mantissa (a bf16 and a bf16 of its remainder) for the product
  * with b; c is rounded once.
  * N % 16 == 0, K % 16 == 0, rank % 8 == 0 and 8 <= rank <= 128 (adapters of
- * less rank are padded with zeros).
+ * less rank are padded with zeros); n_adapters at most HEPH_LORA_MAX_ADAPTERS.
+ * base and c are the same buffer or do not overlap.
  *
  * heph_lora_plan (one small launch) groups the rows by adapter from the ids in
  * device memory; one plan serves every projection of a step. heph_lora_add
@@ -155,6 +156,7 @@ int heph_copy_pages(uint8_t* k_pages, uint8_t* v_pages, int n_layers, int n_page
  * calls that share a ws are ordered by the caller.
  * No counterpart in the reference.
  */
+#define HEPH_LORA_MAX_ADAPTERS 4096
 size_t heph_lora_plan_bytes(int M, int n_adapters);
 size_t heph_lora_ws_bytes(int M, int n_adapters, int K, int rank);
 int heph_lora_plan(void* plan, size_t plan_bytes, const int32_t* ids, int M, int n_adapters,
