@@ -55,7 +55,20 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanHeader* plan, co
         const int id = ids[m];
         return id >= 0 && id < n_adapters ? id : n_adapters;         // none: the last group
     };
-    for (int m = t; m < M; m += nt) atomicAdd(&count[group_of(m)], 1);
+    // A place in the row's group. A prompt's neighbours share an adapter: one atomic for
+    // a wave of them instead of 64 on one address.
+    auto place = [&](int m) -> int {
+        const int g = group_of(m);
+        if (__all(g == __builtin_amdgcn_readfirstlane(g))) {
+            const unsigned long long here = __ballot(1);
+            int at = 0;
+            if ((t & 63) == __ffsll((long long)here) - 1) at = atomicAdd(&count[g], __popcll(here));
+            return __builtin_amdgcn_readfirstlane(at) +
+                   __popcll(here & ((1ull << (t & 63)) - 1));
+        }
+        return atomicAdd(&count[g], 1);
+    };
+    for (int m = t; m < M; m += nt) place(m);
     __syncthreads();
     int row0 = 0, tile0 = 0;                                         // of the groups before
     for (int g0 = 0; g0 < groups; g0 += nt) {
@@ -91,7 +104,7 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanHeader* plan, co
         tile0 += tile_sum;
         __syncthreads();
     }
-    for (int m = t; m < M; m += nt) rows[atomicAdd(&count[group_of(m)], 1)] = m;
+    for (int m = t; m < M; m += nt) rows[place(m)] = m;
     if (t == 0) *plan = PlanHeader{kMagic, M, n_adapters, tile0};
 }
 
@@ -112,196 +125,335 @@ __device__ __forceinline__ bool plan_fits(const PlanHeader& h, const LoraArgs& g
     return h.magic == kMagic && h.m == g.M && h.n_adapters == g.n_adapters;
 }
 
-__device__ __forceinline__ bf16x8 load8(const uint16_t* p, bool there)
+__device__ __forceinline__ bf16x8 load8(const uint16_t* p) { return __builtin_bit_cast(bf16x8, ldg16(p)); }
+__device__ __forceinline__ bf16x8 zero_unless(bf16x8 x, bool there)
 {
-    const i32x4 zero = {0, 0, 0, 0};
-    return __builtin_bit_cast(bf16x8, there ? ldg16(p) : zero);
+    const i32x4 w = __builtin_bit_cast(i32x4, x), zero = {0, 0, 0, 0};
+    return __builtin_bit_cast(bf16x8, there ? w : zero);
 }
 
-// Steps of 64 K: a lane holds 16 consecutive elements of a row of x and of a, two
-// matrix instructions' worth (their order along K is the same on both sides).
+// s_waitcnt: at most N of this wave's vector memory operations and no LDS one left.
+template <int N>
+__device__ __forceinline__ void wait_vm()
+{
+    static_assert(N < 64, "vmcnt has six bits");
+    __builtin_amdgcn_s_waitcnt(0x0070 | (N & 15) | (N >> 4) << 14);
+    asm volatile("" ::: "memory");
+}
+// The wait for a step with `left` later steps of P operations on their way.
+template <int P, int MAX>
+__device__ __forceinline__ void wait_steps(int left)
+{
+    if constexpr (MAX == 0) {
+        wait_vm<0>();
+    } else {
+        if (left >= MAX) wait_vm<MAX * P>();
+        else wait_steps<P, MAX - 1>(left);
+    }
+}
+__device__ __forceinline__ void stage_barrier() { asm volatile("s_barrier" ::: "memory"); }
+
+// K goes in steps of 64: two matrix instructions, 64 bytes of a row in each load.
 constexpr int kStep = 64;
 
-// RT 16-row tiles, RK 16-rank tiles. The workgroup's part of K goes in steps to its
-// four waves, whose sums meet in LDS.
-template <int RT, int RK>
+// Decode tiles: four waves take every fourth step of the workgroup's part of K, and
+// their sums meet in LDS; RK tiles of 16 ranks. Bound by the stream of a, and by the
+// latency of the loads in front of it.
+template <int RK>
 __global__ __launch_bounds__(256) void shrink_kernel(LoraArgs g)
 {
-    __shared__ f32x4 lds[3][RT * RK][64];
+    __shared__ f32x4 lds[3][RK][64];
     const PlanHeader h = *g.plan;
     const int tile = blockIdx.x / g.splits, split = blockIdx.x % g.splits;
     if (!plan_fits(h, g) || tile >= h.n_tiles) return;
     const Tile tl = plan_tiles(g.plan)[tile];
     if (tl.adapter < 0) return;
-    const int l = threadIdx.x & 63, wave = threadIdx.x >> 6, c = l & 15, g4 = l >> 4;
+    const int l = threadIdx.x & 63, c = l & 15, g4 = l >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int steps = (g.K + kStep - 1) / kStep;
     const int s0 = (int)((long)steps * split / g.splits), s1 = (int)((long)steps * (split + 1) / g.splits);
-    const int* rows = plan_rows(g.plan, g.M, g.n_adapters) + tl.start;
-    const uint16_t *x[RT], *a[RK];
-#pragma unroll
-    for (int i = 0; i < RT; ++i)      // (rows past the tile's end: its last one again)
-        x[i] = g.x + (size_t)rows[min(i * 16 + c, tl.count - 1)] * g.K + g4 * 16;
+    // (rows past the tile's end: its last one again)
+    const int row = plan_rows(g.plan, g.M, g.n_adapters)[tl.start + min(c, tl.count - 1)];
+    const uint16_t *x = g.x + (size_t)row * g.K, *a[RK];
 #pragma unroll
     for (int j = 0; j < RK; ++j)
-        a[j] = g.a + ((size_t)tl.adapter * g.r + min(j * 16 + c, g.r - 1)) * g.K + g4 * 16;
-    f32x4 acc[RT][RK];
+        a[j] = g.a + ((size_t)tl.adapter * g.r + min(j * 16 + c, g.r - 1)) * g.K;
+    f32x4 acc[RK];
 #pragma unroll
-    for (int i = 0; i < RT; ++i)
-#pragma unroll
-        for (int j = 0; j < RK; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
-#pragma unroll 2
+    for (int j = 0; j < RK; ++j) acc[j] = f32x4{0, 0, 0, 0};
     for (int s = s0 + wave; s < s1; s += 4) {
-        const int k = s * kStep;
-        const bool there = k + g4 * 16 < g.K;
-        bf16x8 xs[RT][2], as[RK][2];
+        bf16x8 xs[2], as[RK][2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
+            // a piece past K: the row's end again, dropped below
+            const int k = s * kStep + e * 32 + g4 * 8, at = min(k, g.K - 8);
+            xs[e] = load8(x + at);
 #pragma unroll
-            for (int j = 0; j < RK; ++j) as[j][e] = load8(a[j] + k + 8 * e, there);
-#pragma unroll
-            for (int i = 0; i < RT; ++i) xs[i][e] = load8(x[i] + k + 8 * e, there);
+            for (int j = 0; j < RK; ++j) as[j][e] = load8(a[j] + at);
         }
+        if (s * kStep + kStep > g.K)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const bool there = s * kStep + e * 32 + g4 * 8 < g.K;
+                xs[e] = zero_unless(xs[e], there);
+#pragma unroll
+                for (int j = 0; j < RK; ++j) as[j][e] = zero_unless(as[j][e], there);
+            }
 #pragma unroll
         for (int e = 0; e < 2; ++e)
 #pragma unroll
-            for (int i = 0; i < RT; ++i)
-#pragma unroll
-                for (int j = 0; j < RK; ++j) acc[i][j] = mfma_bf16(as[j][e], xs[i][e], acc[i][j]);
+            for (int j = 0; j < RK; ++j) acc[j] = mfma_bf16(as[j][e], xs[e], acc[j]);
     }
     if (wave > 0)
 #pragma unroll
-        for (int i = 0; i < RT; ++i)
-#pragma unroll
-            for (int j = 0; j < RK; ++j) lds[wave - 1][i * RK + j][l] = acc[i][j];
+        for (int j = 0; j < RK; ++j) lds[wave - 1][j][l] = acc[j];
     __syncthreads();
+    if (wave > 0) return;
     // lane: ranks 4 g4 .. of row c
-    if (wave == 0)
 #pragma unroll
-        for (int i = 0; i < RT; ++i)
-#pragma unroll
-            for (int j = 0; j < RK; ++j) {
-                const f32x4 v = ((acc[i][j] + lds[0][i * RK + j][l]) + lds[1][i * RK + j][l]) + lds[2][i * RK + j][l];
-                const int row = i * 16 + c, rank = j * 16 + g4 * 4;
-                if (row < tl.count && rank < g.r)
-                    *reinterpret_cast<f32x4*>(g.part + ((size_t)split * g.M + tl.start + row) * g.r + rank) = v;
-            }
+    for (int j = 0; j < RK; ++j) {
+        const f32x4 v = ((acc[j] + lds[0][j][l]) + lds[1][j][l]) + lds[2][j][l];
+        const int rank = j * 16 + g4 * 4;
+        if (c < tl.count && rank < g.r)
+            *reinterpret_cast<f32x4*>(g.part + ((size_t)split * g.M + tl.start + c) * g.r + rank) = v;
+    }
 }
 
-// F operand pieces of 32 ranks (F = 0: 16 ranks, the remainders in the other half
-// of one piece). Outputs transposed, b as the first operand with its rows in the
-// order that leaves eight consecutive columns of a row in a lane.
-template <int RT, int F, bool F32>
+// Prompt tiles: 64 rows, 16 a wave, x and a through a ring of D steps in LDS, filled by
+// DMA in the operands' lane order (a lane's 16 bytes at 16 * lane of a 1 KB piece: 16
+// rows x 64 bytes). Bound by the stream of x; a tile reads its adapter's a once for 64
+// rows.
+template <int RK, int D>
+__global__ __launch_bounds__(256) void shrink_ring_kernel(LoraArgs g)
+{
+    constexpr int PIECES = (4 + RK) * 2, PW = (PIECES + 3) / 4;       // a step's; a wave's
+    __shared__ __attribute__((aligned(16))) uint8_t lds[D][PIECES * 1024];
+    const PlanHeader h = *g.plan;
+    const int tile = blockIdx.x / g.splits, split = blockIdx.x % g.splits;
+    if (!plan_fits(h, g) || tile >= h.n_tiles) return;
+    const Tile tl = plan_tiles(g.plan)[tile];
+    if (tl.adapter < 0) return;
+    const int l = threadIdx.x & 63, c = l & 15, g4 = l >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int steps = (g.K + kStep - 1) / kStep;
+    const int s0 = (int)((long)steps * split / g.splits), s1 = (int)((long)steps * (split + 1) / g.splits);
+    const int* rows = plan_rows(g.plan, g.M, g.n_adapters) + tl.start;
+    // Piece 2 i + e: half e of a step of x's rows 16 i .. (i < 4), then of a's ranks
+    // 16 (i - 4) .. A wave's spare turn repeats the last piece.
+    const uint16_t* from[PW];
+    int piece[PW];
+#pragma unroll
+    for (int i = 0; i < PW; ++i) {
+        piece[i] = min(wave * PW + i, PIECES - 1);
+        const int t16 = piece[i] / 2;
+        from[i] = t16 < 4 ? g.x + (size_t)rows[min(t16 * 16 + c, tl.count - 1)] * g.K
+                          : g.a + ((size_t)tl.adapter * g.r + min((t16 - 4) * 16 + c, g.r - 1)) * g.K;
+    }
+    auto fetch = [&](int s) {
+#pragma unroll
+        for (int i = 0; i < PW; ++i) {
+            // (a piece past K: the row's end again, dropped below)
+            const int k = min(s * kStep + piece[i] % 2 * 32 + g4 * 8, g.K - 8);
+            __builtin_amdgcn_global_load_lds(
+                (const __attribute__((address_space(1))) void*)(from[i] + k),
+                (__attribute__((address_space(3))) void*)(lds[(s - s0) % D] + piece[i] * 1024), 16, 0, 0);
+        }
+    };
+    f32x4 acc[RK];
+#pragma unroll
+    for (int j = 0; j < RK; ++j) acc[j] = f32x4{0, 0, 0, 0};
+    wait_vm<0>();               // (nothing but steps on its way below)
+    for (int s = s0; s < min(s0 + D - 1, s1); ++s) fetch(s);
+    for (int s = s0; s < s1; ++s) {
+        wait_steps<PW, D - 2>(min(D - 2, s1 - 1 - s));
+        stage_barrier();        // the step is there, and nobody reads the one before it
+        if (s + D - 1 < s1) fetch(s + D - 1);
+        const uint8_t* base = lds[(s - s0) % D] + l * 16;
+        bf16x8 x[2], a[RK][2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            x[e] = *reinterpret_cast<const bf16x8*>(base + (2 * wave + e) * 1024);
+#pragma unroll
+            for (int j = 0; j < RK; ++j)
+                a[j][e] = *reinterpret_cast<const bf16x8*>(base + (8 + 2 * j + e) * 1024);
+        }
+        if (s * kStep + kStep > g.K)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const bool there = s * kStep + e * 32 + g4 * 8 < g.K;
+                x[e] = zero_unless(x[e], there);
+#pragma unroll
+                for (int j = 0; j < RK; ++j) a[j][e] = zero_unless(a[j][e], there);
+            }
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+#pragma unroll
+            for (int j = 0; j < RK; ++j) acc[j] = mfma_bf16(a[j][e], x[e], acc[j]);
+    }
+    const int row = wave * 16 + c;
+#pragma unroll
+    for (int j = 0; j < RK; ++j) {
+        const int rank = j * 16 + g4 * 4;
+        if (row < tl.count && rank < g.r)
+            *reinterpret_cast<f32x4*>(g.part + ((size_t)split * g.M + tl.start + row) * g.r + rank) = acc[j];
+    }
+}
+
+// F operand pieces of 32 ranks (F = 0: 16 ranks, the remainders in the other half of
+// one piece). Outputs transposed, b as the first operand with its rows in the order that
+// leaves eight consecutive columns of a row in a lane. A wave takes U steps of 32 columns
+// at a time, all their loads of base and b at once, the first ones before t is joined.
+// Bound by these streams.
+template <int RT, int F, bool F32, int U>
 __global__ __launch_bounds__(256) void expand_kernel(LoraArgs g)
 {
-    constexpr int P = F == 0 ? 1 : F, PARTS = F == 0 ? 1 : 2;
+    constexpr int P = F == 0 ? 1 : F, PARTS = F == 0 ? 1 : 2, BW = F32 ? 2 : 1;
     __shared__ bf16x8 lds[RT][P][PARTS][64];
     const PlanHeader h = *g.plan;
     const int chunks = (g.N + g.n_chunk - 1) / g.n_chunk;
     const int tile = blockIdx.x / chunks, n0 = blockIdx.x % chunks * g.n_chunk;
     if (!plan_fits(h, g) || tile >= h.n_tiles) return;
     const Tile tl = plan_tiles(g.plan)[tile];
-    const bool copy = tl.adapter < 0;
-    if (copy && g.c == g.base) return;
-    const int l = threadIdx.x & 63, wave = threadIdx.x >> 6, c = l & 15, g4 = l >> 4;
-    if (!copy) {
-        const float scale = g.scale[tl.adapter];
-        for (int u = threadIdx.x; u < RT * P * 64; u += 256) {
-            const int i = u / (P * 64), f = u / 64 % P, ul = u & 63, row = i * 16 + (ul & 15);
-            const int rank = F == 0 ? (ul >> 4 & 1) * 8 : f * 32 + (ul >> 4) * 8;
-            f32x4 s[2] = {};
-            if (row < tl.count && rank < g.r) {
-                const float* p = g.part + (size_t)(tl.start + row) * g.r + rank;
-                for (int k = 0; k < g.splits; ++k, p += (size_t)g.M * g.r) {
-                    s[0] += *reinterpret_cast<const f32x4*>(p);
-                    s[1] += *reinterpret_cast<const f32x4*>(p + 4);
-                }
-            }
-            bf16x8 hi, lo;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float v = s[e / 4][e % 4] * scale;
-                hi[e] = (__bf16)v;
-                lo[e] = (__bf16)(v - (float)hi[e]);
-            }
-            if constexpr (F == 0) {
-                lds[i][0][0][ul] = ul < 32 ? hi : lo;
-            } else {
-                lds[i][f][0][ul] = hi;
-                lds[i][f][1][ul] = lo;
+    const int l = threadIdx.x & 63, c = l & 15, g4 = l >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int n_end = min(n0 + g.n_chunk, g.N);
+    const int* rows = plan_rows(g.plan, g.M, g.n_adapters) + tl.start;
+    if (tl.adapter < 0) {                       // no adapter: c = base
+        if (g.c == g.base) return;
+        constexpr int E = F32 ? 4 : 8;
+        for (int r = 0; r < tl.count; ++r) {
+            const size_t o = (size_t)rows[r] * g.N;
+            for (int n = n0 + (int)threadIdx.x * E; n < n_end; n += 256 * E) {
+                const size_t at = (o + n) * (F32 ? 4 : 2);
+                *reinterpret_cast<i32x4*>(static_cast<uint8_t*>(g.c) + at) =
+                    ldg16(static_cast<const uint8_t*>(g.base) + at);
             }
         }
-        __syncthreads();
+        return;
     }
-    bf16x8 t[RT][P][PARTS];
     int row[RT];
-    const int* rows = plan_rows(g.plan, g.M, g.n_adapters) + tl.start;
 #pragma unroll
-    for (int i = 0; i < RT; ++i) {
-        row[i] = i * 16 + c < tl.count ? rows[i * 16 + c] : -1;
+    for (int i = 0; i < RT; ++i) row[i] = rows[min(i * 16 + c, tl.count - 1)];
+    const uint16_t* b = g.b + (size_t)tl.adapter * g.N * g.r;
+    // Past the chunk's end the last columns again, past the tile's its last row: what is
+    // not stored.
+    const int rank0 = F == 0 ? (g4 & 1) * 8 : g4 * 8;
+    i32x4 base[U][RT][BW];
+    bf16x8 bs[U][2][P];
+    auto load = [&](int n) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int at = n + u * 128;
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const int bn = min(at + (c >> 2) * 8 + j * 4 + (c & 3), n_end - 1);
+#pragma unroll
+                for (int f = 0; f < P; ++f)
+                    bs[u][j][f] = load8(b + (size_t)bn * g.r + min(f * 32 + rank0, g.r - 8));
+            }
+            const int col = min(at + g4 * 8, n_end - 8);
+#pragma unroll
+            for (int i = 0; i < RT; ++i)
+#pragma unroll
+                for (int e = 0; e < BW; ++e)
+                    base[u][i][e] = ldg16(static_cast<const uint8_t*>(g.base) +
+                                          ((size_t)row[i] * g.N + col) * (F32 ? 4 : 2) + e * 16);
+        }
+    };
+    int n = n0 + wave * 32;
+    load(n);
+
+    // t = scale * the sum of K's parts, in the operands' lane order.
+    const float scale = g.scale[tl.adapter];
+    const size_t split = (size_t)g.M * g.r;
+    for (int u = threadIdx.x; u < RT * P * 64; u += 256) {
+        const int i = u / (P * 64), f = u / 64 % P, ul = u & 63, r = i * 16 + (ul & 15);
+        const int rank = F == 0 ? (ul >> 4 & 1) * 8 : f * 32 + (ul >> 4) * 8;
+        const bool there = r < tl.count && rank < g.r;
+        const float* p = g.part + (size_t)(tl.start + min(r, tl.count - 1)) * g.r + min(rank, g.r - 8);
+        f32x4 s[2] = {};
+        for (int k = 0; k < g.splits; k += 8) {
+            f32x4 v[8][2];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float* q = p + (size_t)min(k + e, g.splits - 1) * split;
+                v[e][0] = *reinterpret_cast<const f32x4*>(q);
+                v[e][1] = *reinterpret_cast<const f32x4*>(q + 4);
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (k + e < g.splits) {
+                    s[0] += v[e][0];
+                    s[1] += v[e][1];
+                }
+        }
+        bf16x8 hi, lo;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float v = there ? s[e / 4][e % 4] * scale : 0.0f;
+            hi[e] = (__bf16)v;
+            lo[e] = (__bf16)(v - (float)hi[e]);
+        }
+        if constexpr (F == 0) {
+            lds[i][0][0][ul] = ul < 32 ? hi : lo;
+        } else {
+            lds[i][f][0][ul] = hi;
+            lds[i][f][1][ul] = lo;
+        }
+    }
+    __syncthreads();
+    bf16x8 t[RT][P][PARTS];
+#pragma unroll
+    for (int i = 0; i < RT; ++i)
 #pragma unroll
         for (int f = 0; f < P; ++f)
 #pragma unroll
             for (int e = 0; e < PARTS; ++e) t[i][f][e] = lds[i][f][e][l];
-    }
-    const uint16_t* b = g.b + (size_t)(copy ? 0 : tl.adapter) * g.N * g.r;
-    const int n_end = min(n0 + g.n_chunk, g.N);
-    for (int n = n0 + wave * 32; n < n_end; n += 128) {
-        // this lane's eight columns are all inside N or all past it (N % 16 == 0)
-        const int col = n + g4 * 8;
-        const bool inside = col < g.N;
-        f32x4 v[RT][2];
+    while (true) {
 #pragma unroll
-        for (int i = 0; i < RT; ++i) {
-            v[i][0] = v[i][1] = f32x4{0, 0, 0, 0};
-            if (row[i] >= 0 && inside) {
-                const size_t o = (size_t)row[i] * g.N + col;
+        for (int u = 0; u < U; ++u) {
+            const int col = n + u * 128 + g4 * 8;       // N % 16 == 0: all eight inside or past the end
+#pragma unroll
+            for (int i = 0; i < RT; ++i) {
+                f32x4 v[2];
                 if constexpr (F32) {
-                    const f32x4* p = reinterpret_cast<const f32x4*>(static_cast<const float*>(g.base) + o);
-                    v[i][0] = p[0];
-                    v[i][1] = p[1];
+                    v[0] = __builtin_bit_cast(f32x4, base[u][i][0]);
+                    v[1] = __builtin_bit_cast(f32x4, base[u][i][1]);
                 } else {
-                    const uint4 w = ldg16u(static_cast<const uint16_t*>(g.base) + o);
-                    v[i][0] = f32x4{bf16lo(w.x), bf16hi(w.x), bf16lo(w.y), bf16hi(w.y)};
-                    v[i][1] = f32x4{bf16lo(w.z), bf16hi(w.z), bf16lo(w.w), bf16hi(w.w)};
-                }
-            }
-        }
-        if (!copy) {
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const int bn = n + (c >> 2) * 8 + j * 4 + (c & 3);
-                bf16x8 w[P];
-#pragma unroll
-                for (int f = 0; f < P; ++f) {
-                    const int rank = F == 0 ? (g4 & 1) * 8 : f * 32 + g4 * 8;
-                    w[f] = load8(b + (size_t)min(bn, g.N - 1) * g.r + rank, rank < g.r);
+                    const i32x4 x = base[u][i][0];
+                    v[0] = f32x4{bf16lo(x[0]), bf16hi(x[0]), bf16lo(x[1]), bf16hi(x[1])};
+                    v[1] = f32x4{bf16lo(x[2]), bf16hi(x[2]), bf16lo(x[3]), bf16hi(x[3])};
                 }
 #pragma unroll
-                for (int i = 0; i < RT; ++i) {
+                for (int j = 0; j < 2; ++j) {
                     f32x4 d = {0, 0, 0, 0};
 #pragma unroll
-                    for (int f = 0; f < P; ++f)
+                    for (int f = 0; f < P; ++f) {
+                        // (a rank past r: t is 0 there, and what was loaded must not be NaN)
+                        const bf16x8 w = zero_unless(bs[u][j][f], f * 32 + rank0 < g.r);
 #pragma unroll
-                        for (int e = PARTS - 1; e >= 0; --e) d = mfma_bf16(w[f], t[i][f][e], d);
-                    v[i][j] += d;
+                        for (int e = PARTS - 1; e >= 0; --e) d = mfma_bf16(w, t[i][f][e], d);
+                    }
+                    v[j] += d;
+                }
+                if (i * 16 + c < tl.count && col < n_end) {
+                    const size_t o = (size_t)row[i] * g.N + col;
+                    if constexpr (F32) {
+                        f32x4* p = reinterpret_cast<f32x4*>(static_cast<float*>(g.c) + o);
+                        p[0] = v[0];
+                        p[1] = v[1];
+                    } else {
+                        auto two = [](float x, float y) { return (uint32_t)f32_to_bf16(x) | (uint32_t)f32_to_bf16(y) << 16; };
+                        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(g.c) + o) =
+                            make_uint4(two(v[0][0], v[0][1]), two(v[0][2], v[0][3]),
+                                       two(v[1][0], v[1][1]), two(v[1][2], v[1][3]));
+                    }
                 }
             }
         }
-#pragma unroll
-        for (int i = 0; i < RT; ++i)
-            if (row[i] >= 0 && inside) {
-                const size_t o = (size_t)row[i] * g.N + col;
-                if constexpr (F32) {
-                    f32x4* p = reinterpret_cast<f32x4*>(static_cast<float*>(g.c) + o);
-                    p[0] = v[i][0];
-                    p[1] = v[i][1];
-                } else {
-                    auto two = [](float x, float y) { return (uint32_t)f32_to_bf16(x) | (uint32_t)f32_to_bf16(y) << 16; };
-                    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(g.c) + o) =
-                        make_uint4(two(v[i][0][0], v[i][0][1]), two(v[i][0][2], v[i][0][3]),
-                                   two(v[i][1][0], v[i][1][1]), two(v[i][1][2], v[i][1][3]));
-                }
-            }
+        n += U * 128;
+        if (n >= n_end) break;
+        load(n);
     }
 }
 
@@ -318,22 +470,30 @@ int k_splits(int M, int n_adapters, int K)
     return std::max(1, std::min(std::min((steps + 3) / 4, want), 16));
 }
 
-template <int RT>
 void launch_shrink(const LoraArgs& g, unsigned blocks, hipStream_t s)
 {
-    if (g.r <= 16) shrink_kernel<RT, 1><<<blocks, 256, 0, s>>>(g);
-    else if (g.r <= 32) shrink_kernel<RT, 2><<<blocks, 256, 0, s>>>(g);
-    else if (g.r <= 64) shrink_kernel<RT, 4><<<blocks, 256, 0, s>>>(g);
-    else shrink_kernel<RT, 8><<<blocks, 256, 0, s>>>(g);
+    if (g.r <= 16) shrink_kernel<1><<<blocks, 256, 0, s>>>(g);
+    else if (g.r <= 32) shrink_kernel<2><<<blocks, 256, 0, s>>>(g);
+    else if (g.r <= 64) shrink_kernel<4><<<blocks, 256, 0, s>>>(g);
+    else shrink_kernel<8><<<blocks, 256, 0, s>>>(g);
+}
+
+void launch_shrink_ring(const LoraArgs& g, unsigned blocks, hipStream_t s)
+{
+    if (g.r <= 16) shrink_ring_kernel<1, 6><<<blocks, 256, 0, s>>>(g);
+    else if (g.r <= 32) shrink_ring_kernel<2, 5><<<blocks, 256, 0, s>>>(g);
+    else if (g.r <= 64) shrink_ring_kernel<4, 4><<<blocks, 256, 0, s>>>(g);
+    else shrink_ring_kernel<8, 3><<<blocks, 256, 0, s>>>(g);
 }
 
 template <int RT, bool F32>
 void launch_expand(const LoraArgs& g, unsigned blocks, hipStream_t s)
 {
-    if (g.r <= 16) expand_kernel<RT, 0, F32><<<blocks, 256, 0, s>>>(g);
-    else if (g.r <= 32) expand_kernel<RT, 1, F32><<<blocks, 256, 0, s>>>(g);
-    else if (g.r <= 64) expand_kernel<RT, 2, F32><<<blocks, 256, 0, s>>>(g);
-    else expand_kernel<RT, 4, F32><<<blocks, 256, 0, s>>>(g);
+    constexpr int U = RT == 1 ? 4 : 2, U4 = RT == 1 ? 2 : 1;
+    if (g.r <= 16) expand_kernel<RT, 0, F32, U><<<blocks, 256, 0, s>>>(g);
+    else if (g.r <= 32) expand_kernel<RT, 1, F32, U><<<blocks, 256, 0, s>>>(g);
+    else if (g.r <= 64) expand_kernel<RT, 2, F32, U><<<blocks, 256, 0, s>>>(g);
+    else expand_kernel<RT, 4, F32, U4><<<blocks, 256, 0, s>>>(g);
 }
 
 }  // namespace
@@ -386,8 +546,10 @@ int heph_lora_add(void* c, int c_dtype, const void* base, const uint16_t* x_bf16
         ws_bytes < heph_lora_ws_bytes(M, n_adapters, K, rank))
         return HEPH_ERR_WORKSPACE;
     const int tiles = max_tiles(M, n_adapters), splits = k_splits(M, n_adapters, K);
-    // columns a workgroup: more where that still leaves work for the device
-    const int n_chunk = (long)tiles * N >= 512L * 4 * kPlanCUs ? 512 : 128;
+    // Columns a workgroup: few enough for two workgroups a CU, each of which joins the
+    // parts of t for itself.
+    const int chunks = std::max(1, std::min((2 * kPlanCUs + tiles - 1) / tiles, (N + 127) / 128));
+    const int n_chunk = ((N + chunks - 1) / chunks + 127) / 128 * 128;
     const int64_t expand = (int64_t)tiles * ((N + n_chunk - 1) / n_chunk);
     if (expand > INT32_MAX) return HEPH_ERR_UNSUPPORTED;
     if (int st = check_device()) return st;
@@ -397,10 +559,10 @@ int heph_lora_add(void* c, int c_dtype, const void* base, const uint16_t* x_bf16
     hipStream_t s = static_cast<hipStream_t>(stream);
     const bool f32 = c_dtype == HEPH_DTYPE_F32;
     if (tile_rows(M) == 16) {
-        launch_shrink<1>(g, (unsigned)(tiles * splits), s);
+        launch_shrink(g, (unsigned)(tiles * splits), s);
         f32 ? launch_expand<1, true>(g, (unsigned)expand, s) : launch_expand<1, false>(g, (unsigned)expand, s);
     } else {
-        launch_shrink<4>(g, (unsigned)(tiles * splits), s);
+        launch_shrink_ring(g, (unsigned)(tiles * splits), s);
         f32 ? launch_expand<4, true>(g, (unsigned)expand, s) : launch_expand<4, false>(g, (unsigned)expand, s);
     }
     return status_of(hipGetLastError());
