@@ -9,6 +9,7 @@
 // bf16 of its remainder (16 bits of mantissa): the product has matrix cores to
 // spare, as both launches are bound by what they stream.
 #include <algorithm>
+#include <type_traits>
 
 #include "pages.h"
 
@@ -117,7 +118,7 @@ struct LoraArgs {
     const float* scale;
     PlanHeader* plan;
     float* part;             // [splits][M][r], rows in the plan's order
-    int M, N, K, r, n_adapters, splits, n_chunk;
+    int M, N, K, r, n_adapters, splits, n_chunk, xcds;
 };
 
 __device__ __forceinline__ bool plan_fits(const PlanHeader& h, const LoraArgs& g)
@@ -153,6 +154,23 @@ __device__ __forceinline__ void wait_steps(int left)
 }
 __device__ __forceinline__ void stage_barrier() { asm volatile("s_barrier" ::: "memory"); }
 
+// Workgroups go to the XCDs in turn. With tiles for all of them (xcds = 8) a tile's parts
+// all go to one, in both launches, so that t's parts are read through the L2 that wrote
+// them and a tile's x, a and b stay in one L2; with few tiles (xcds = 1) they spread.
+constexpr int kXcds = 8;
+inline int xcds_for(int tiles) { return tiles >= 8 * kXcds ? kXcds : 1; }
+inline int64_t blocks_for(int tiles, int parts)
+{
+    const int x = xcds_for(tiles);
+    return (int64_t)((tiles + x - 1) / x * x) * parts;
+}
+__device__ __forceinline__ void tile_and_part(int xcds, int parts, int& tile, int& part)
+{
+    const int k = blockIdx.x / xcds;
+    tile = k / parts * xcds + blockIdx.x % xcds;
+    part = k % parts;
+}
+
 // K goes in steps of 64: two matrix instructions, 64 bytes of a row in each load.
 constexpr int kStep = 64;
 
@@ -164,7 +182,8 @@ __global__ __launch_bounds__(256) void shrink_kernel(LoraArgs g)
 {
     __shared__ f32x4 lds[3][RK][64];
     const PlanHeader h = *g.plan;
-    const int tile = blockIdx.x / g.splits, split = blockIdx.x % g.splits;
+    int tile, split;
+    tile_and_part(g.xcds, g.splits, tile, split);
     if (!plan_fits(h, g) || tile >= h.n_tiles) return;
     const Tile tl = plan_tiles(g.plan)[tile];
     if (tl.adapter < 0) return;
@@ -220,16 +239,18 @@ __global__ __launch_bounds__(256) void shrink_kernel(LoraArgs g)
 }
 
 // Prompt tiles: 64 rows, 16 a wave, x and a through a ring of D steps in LDS, filled by
-// DMA in the operands' lane order (a lane's 16 bytes at 16 * lane of a 1 KB piece: 16
-// rows x 64 bytes). Bound by the stream of x; a tile reads its adapter's a once for 64
-// rows.
+// DMA. Bound by the stream of x; a tile reads its adapter's a once for 64 rows. A DMA
+// moves 8 rows x 128 bytes, whole lines: in the operands' own order, 16 rows x 64 bytes,
+// the L2 gave half the rate. The 16-byte pieces of a row lie in LDS XOR-ed by the row, so
+// that the operands' reads have no bank conflicts.
 template <int RK, int D>
 __global__ __launch_bounds__(256) void shrink_ring_kernel(LoraArgs g)
 {
     constexpr int PIECES = (4 + RK) * 2, PW = (PIECES + 3) / 4;       // a step's; a wave's
     __shared__ __attribute__((aligned(16))) uint8_t lds[D][PIECES * 1024];
     const PlanHeader h = *g.plan;
-    const int tile = blockIdx.x / g.splits, split = blockIdx.x % g.splits;
+    int tile, split;
+    tile_and_part(g.xcds, g.splits, tile, split);
     if (!plan_fits(h, g) || tile >= h.n_tiles) return;
     const Tile tl = plan_tiles(g.plan)[tile];
     if (tl.adapter < 0) return;
@@ -238,44 +259,46 @@ __global__ __launch_bounds__(256) void shrink_ring_kernel(LoraArgs g)
     const int steps = (g.K + kStep - 1) / kStep;
     const int s0 = (int)((long)steps * split / g.splits), s1 = (int)((long)steps * (split + 1) / g.splits);
     const int* rows = plan_rows(g.plan, g.M, g.n_adapters) + tl.start;
-    // Piece 2 i + e: half e of a step of x's rows 16 i .. (i < 4), then of a's ranks
-    // 16 (i - 4) .. A wave's spare turn repeats the last piece.
+    // Piece p: rows 8 p .. of x (p < 8), then ranks 8 (p - 8) .. of a. A wave's spare turn
+    // repeats the last piece.
     const uint16_t* from[PW];
     int piece[PW];
+    const int k_lane = ((l & 7) ^ (l >> 3)) * 8;
 #pragma unroll
     for (int i = 0; i < PW; ++i) {
         piece[i] = min(wave * PW + i, PIECES - 1);
-        const int t16 = piece[i] / 2;
-        from[i] = t16 < 4 ? g.x + (size_t)rows[min(t16 * 16 + c, tl.count - 1)] * g.K
-                          : g.a + ((size_t)tl.adapter * g.r + min((t16 - 4) * 16 + c, g.r - 1)) * g.K;
+        const int r = piece[i] * 8 + (l >> 3);
+        from[i] = piece[i] < 8 ? g.x + (size_t)rows[min(r, tl.count - 1)] * g.K
+                               : g.a + ((size_t)tl.adapter * g.r + min(r - 64, g.r - 1)) * g.K;
     }
     auto fetch = [&](int s) {
+        // (a piece past K: the row's end again, dropped below)
+        const int k = min(s * kStep + k_lane, g.K - 8);
 #pragma unroll
-        for (int i = 0; i < PW; ++i) {
-            // (a piece past K: the row's end again, dropped below)
-            const int k = min(s * kStep + piece[i] % 2 * 32 + g4 * 8, g.K - 8);
+        for (int i = 0; i < PW; ++i)
             __builtin_amdgcn_global_load_lds(
                 (const __attribute__((address_space(1))) void*)(from[i] + k),
                 (__attribute__((address_space(3))) void*)(lds[(s - s0) % D] + piece[i] * 1024), 16, 0, 0);
-        }
     };
     f32x4 acc[RK];
 #pragma unroll
     for (int j = 0; j < RK; ++j) acc[j] = f32x4{0, 0, 0, 0};
     wait_vm<0>();               // (nothing but steps on its way below)
     for (int s = s0; s < min(s0 + D - 1, s1); ++s) fetch(s);
+    // the lane's row c, K pieces g4 and 4 + g4 of the step
+    const int at[2] = {c * 128 + (g4 ^ (c & 7)) * 16, c * 128 + ((4 + g4) ^ (c & 7)) * 16};
     for (int s = s0; s < s1; ++s) {
         wait_steps<PW, D - 2>(min(D - 2, s1 - 1 - s));
         stage_barrier();        // the step is there, and nobody reads the one before it
         if (s + D - 1 < s1) fetch(s + D - 1);
-        const uint8_t* base = lds[(s - s0) % D] + l * 16;
+        const uint8_t* base = lds[(s - s0) % D];
         bf16x8 x[2], a[RK][2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-            x[e] = *reinterpret_cast<const bf16x8*>(base + (2 * wave + e) * 1024);
+            x[e] = *reinterpret_cast<const bf16x8*>(base + wave * 2048 + at[e]);
 #pragma unroll
             for (int j = 0; j < RK; ++j)
-                a[j][e] = *reinterpret_cast<const bf16x8*>(base + (8 + 2 * j + e) * 1024);
+                a[j][e] = *reinterpret_cast<const bf16x8*>(base + (4 + j) * 2048 + at[e]);
         }
         if (s * kStep + kStep > g.K)
 #pragma unroll
@@ -311,7 +334,9 @@ __global__ __launch_bounds__(256) void expand_kernel(LoraArgs g)
     __shared__ bf16x8 lds[RT][P][PARTS][64];
     const PlanHeader h = *g.plan;
     const int chunks = (g.N + g.n_chunk - 1) / g.n_chunk;
-    const int tile = blockIdx.x / chunks, n0 = blockIdx.x % chunks * g.n_chunk;
+    int tile, n0;
+    tile_and_part(g.xcds, chunks, tile, n0);
+    n0 *= g.n_chunk;
     if (!plan_fits(h, g) || tile >= h.n_tiles) return;
     const Tile tl = plan_tiles(g.plan)[tile];
     const int l = threadIdx.x & 63, c = l & 15, g4 = l >> 4;
@@ -320,14 +345,20 @@ __global__ __launch_bounds__(256) void expand_kernel(LoraArgs g)
     const int* rows = plan_rows(g.plan, g.M, g.n_adapters) + tl.start;
     if (tl.adapter < 0) {                       // no adapter: c = base
         if (g.c == g.base) return;
-        constexpr int E = F32 ? 4 : 8;
-        for (int r = 0; r < tl.count; ++r) {
-            const size_t o = (size_t)rows[r] * g.N;
-            for (int n = n0 + (int)threadIdx.x * E; n < n_end; n += 256 * E) {
-                const size_t at = (o + n) * (F32 ? 4 : 2);
-                *reinterpret_cast<i32x4*>(static_cast<uint8_t*>(g.c) + at) =
-                    ldg16(static_cast<const uint8_t*>(g.base) + at);
+        constexpr int E = F32 ? 4 : 8, B = 4;
+        const int per = (n_end - n0) / E, all = per * tl.count;
+        for (int v = threadIdx.x; v < all; v += 256 * B) {
+            i32x4 w[B];
+            size_t at[B];
+#pragma unroll
+            for (int i = 0; i < B; ++i) {
+                const int e = min(v + i * 256, all - 1);
+                at[i] = ((size_t)rows[e / per] * g.N + n0 + e % per * E) * (F32 ? 4 : 2);
+                w[i] = ldg16(static_cast<const uint8_t*>(g.base) + at[i]);
             }
+#pragma unroll
+            for (int i = 0; i < B; ++i)
+                *reinterpret_cast<i32x4*>(static_cast<uint8_t*>(g.c) + at[i]) = w[i];
         }
         return;
     }
@@ -343,7 +374,7 @@ __global__ __launch_bounds__(256) void expand_kernel(LoraArgs g)
     auto load = [&](int n) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int at = n + u * 128;
+            const int at = n + u * 32;
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 const int bn = min(at + (c >> 2) * 8 + j * 4 + (c & 3), n_end - 1);
@@ -360,33 +391,41 @@ __global__ __launch_bounds__(256) void expand_kernel(LoraArgs g)
                                           ((size_t)row[i] * g.N + col) * (F32 ? 4 : 2) + e * 16);
         }
     };
-    int n = n0 + wave * 32;
+    int n = n0 + wave * (U * 32);
     load(n);
 
     // t = scale * the sum of K's parts, in the operands' lane order.
     const float scale = g.scale[tl.adapter];
     const size_t split = (size_t)g.M * g.r;
-    for (int u = threadIdx.x; u < RT * P * 64; u += 256) {
+    constexpr int ITEMS = (RT * P * 64 + 255) / 256;
+#pragma unroll
+    for (int it = 0; it < ITEMS; ++it) {
+        const int u = threadIdx.x + it * 256;
+        if (RT * P * 64 % 256 != 0 && u >= RT * P * 64) break;
         const int i = u / (P * 64), f = u / 64 % P, ul = u & 63, r = i * 16 + (ul & 15);
         const int rank = F == 0 ? (ul >> 4 & 1) * 8 : f * 32 + (ul >> 4) * 8;
         const bool there = r < tl.count && rank < g.r;
         const float* p = g.part + (size_t)(tl.start + min(r, tl.count - 1)) * g.r + min(rank, g.r - 8);
         f32x4 s[2] = {};
-        for (int k = 0; k < g.splits; k += 8) {
-            f32x4 v[8][2];
+        auto parts = [&](auto n, int k0) {
+            constexpr int NP = decltype(n)::value;
+            f32x4 v[NP][2];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float* q = p + (size_t)min(k + e, g.splits - 1) * split;
+            for (int e = 0; e < NP; ++e) {
+                const float* q = p + (size_t)min(k0 + e, g.splits - 1) * split;
                 v[e][0] = *reinterpret_cast<const f32x4*>(q);
                 v[e][1] = *reinterpret_cast<const f32x4*>(q + 4);
             }
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if (k + e < g.splits) {
+            for (int e = 0; e < NP; ++e)
+                if (k0 + e < g.splits) {
                     s[0] += v[e][0];
                     s[1] += v[e][1];
                 }
-        }
+        };
+        if (g.splits <= 4) parts(std::integral_constant<int, 4>{}, 0);
+        else
+            for (int k = 0; k < g.splits; k += 8) parts(std::integral_constant<int, 8>{}, k);
         bf16x8 hi, lo;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
@@ -412,7 +451,7 @@ __global__ __launch_bounds__(256) void expand_kernel(LoraArgs g)
     while (true) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int col = n + u * 128 + g4 * 8;       // N % 16 == 0: all eight inside or past the end
+            const int col = n + u * 32 + g4 * 8;        // N % 16 == 0: all eight inside or past the end
 #pragma unroll
             for (int i = 0; i < RT; ++i) {
                 f32x4 v[2];
@@ -463,10 +502,12 @@ bool sizes_ok(int M, int n_adapters)
 }
 bool rank_ok(int rank) { return rank >= 8 && rank <= 128 && rank % 8 == 0; }
 
-// Parts of K: as many as fill the device twice over, each at least a step a wave.
+// Parts of K: as many as fill the device, with few tiles twice over, each at least a step
+// a wave.
 int k_splits(int M, int n_adapters, int K)
 {
-    const int steps = (K + kStep - 1) / kStep, want = 2 * kPlanCUs / max_tiles(M, n_adapters);
+    const int steps = (K + kStep - 1) / kStep, tiles = max_tiles(M, n_adapters);
+    const int want = (tiles < 64 ? 2 : 1) * kPlanCUs / tiles;
     return std::max(1, std::min(std::min((steps + 3) / 4, want), 16));
 }
 
@@ -550,19 +591,19 @@ int heph_lora_add(void* c, int c_dtype, const void* base, const uint16_t* x_bf16
     // parts of t for itself.
     const int chunks = std::max(1, std::min((2 * kPlanCUs + tiles - 1) / tiles, (N + 127) / 128));
     const int n_chunk = ((N + chunks - 1) / chunks + 127) / 128 * 128;
-    const int64_t expand = (int64_t)tiles * ((N + n_chunk - 1) / n_chunk);
+    const int64_t expand = blocks_for(tiles, (N + n_chunk - 1) / n_chunk);
     if (expand > INT32_MAX) return HEPH_ERR_UNSUPPORTED;
     if (int st = check_device()) return st;
     const LoraArgs g{c, base, x_bf16, a_bf16, b_bf16, scale,
                      static_cast<PlanHeader*>(const_cast<void*>(plan)), static_cast<float*>(ws), M, N, K,
-                     rank, n_adapters, splits, n_chunk};
+                     rank, n_adapters, splits, n_chunk, xcds_for(tiles)};
     hipStream_t s = static_cast<hipStream_t>(stream);
     const bool f32 = c_dtype == HEPH_DTYPE_F32;
     if (tile_rows(M) == 16) {
-        launch_shrink(g, (unsigned)(tiles * splits), s);
+        launch_shrink(g, (unsigned)blocks_for(tiles, splits), s);
         f32 ? launch_expand<1, true>(g, (unsigned)expand, s) : launch_expand<1, false>(g, (unsigned)expand, s);
     } else {
-        launch_shrink_ring(g, (unsigned)(tiles * splits), s);
+        launch_shrink_ring(g, (unsigned)blocks_for(tiles, splits), s);
         f32 ? launch_expand<4, true>(g, (unsigned)expand, s) : launch_expand<4, false>(g, (unsigned)expand, s);
     }
     return status_of(hipGetLastError());
