@@ -322,6 +322,18 @@ __global__ __launch_bounds__(256) void shrink_ring_kernel(LoraArgs g)
     }
 }
 
+// The values of lanes 0..31 (j = 0) or 32..63 (j = 1) in both halves of the wave.
+__device__ __forceinline__ bf16x8 half_of(const bf16x8& x, int j)
+{
+    i32x4 w = __builtin_bit_cast(i32x4, x);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const auto r = __builtin_amdgcn_permlane32_swap((unsigned)w[i], (unsigned)w[i], false, false);
+        w[i] = (int)r[j];
+    }
+    return __builtin_bit_cast(bf16x8, w);
+}
+
 // F operand pieces of 32 ranks (F = 0: 16 ranks, the remainders in the other half of
 // one piece). Outputs transposed, b as the first operand with its rows in the order that
 // leaves eight consecutive columns of a row in a lane. A wave takes U steps of 32 columns
@@ -370,14 +382,16 @@ __global__ __launch_bounds__(256) void expand_kernel(LoraArgs g)
     // not stored.
     const int rank0 = F == 0 ? (g4 & 1) * 8 : g4 * 8;
     i32x4 base[U][RT][BW];
-    bf16x8 bs[U][2][P];
+    // (16 ranks: one load brings both halves of the columns, j = lane / 32)
+    constexpr int BJ = F == 0 ? 1 : 2;
+    bf16x8 bs[U][BJ][P];
     auto load = [&](int n) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int at = n + u * 32;
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const int bn = min(at + (c >> 2) * 8 + j * 4 + (c & 3), n_end - 1);
+            for (int j = 0; j < BJ; ++j) {
+                const int bn = min(at + (c >> 2) * 8 + (F == 0 ? g4 >> 1 : j) * 4 + (c & 3), n_end - 1);
 #pragma unroll
                 for (int f = 0; f < P; ++f)
                     bs[u][j][f] = load8(b + (size_t)bn * g.r + min(f * 32 + rank0, g.r - 8));
@@ -469,7 +483,8 @@ __global__ __launch_bounds__(256) void expand_kernel(LoraArgs g)
 #pragma unroll
                     for (int f = 0; f < P; ++f) {
                         // (a rank past r: t is 0 there, and what was loaded must not be NaN)
-                        const bf16x8 w = zero_unless(bs[u][j][f], f * 32 + rank0 < g.r);
+                        bf16x8 w = zero_unless(bs[u][F == 0 ? 0 : j][f], f * 32 + rank0 < g.r);
+                        if constexpr (F == 0) w = half_of(w, j);
 #pragma unroll
                         for (int e = PARTS - 1; e >= 0; --e) d = mfma_bf16(w, t[i][f][e], d);
                     }
@@ -502,12 +517,12 @@ bool sizes_ok(int M, int n_adapters)
 }
 bool rank_ok(int rank) { return rank >= 8 && rank <= 128 && rank % 8 == 0; }
 
-// Parts of K: as many as fill the device, with few tiles twice over, each at least a step
-// a wave.
+// Parts of K: as many as fill the device, with few prompt tiles twice over, each at least
+// a step a wave.
 int k_splits(int M, int n_adapters, int K)
 {
     const int steps = (K + kStep - 1) / kStep, tiles = max_tiles(M, n_adapters);
-    const int want = (tiles < 64 ? 2 : 1) * kPlanCUs / tiles;
+    const int want = (tile_rows(M) > 16 && tiles < 64 ? 2 : 1) * kPlanCUs / tiles;
     return std::max(1, std::min(std::min((steps + 3) / 4, want), 16));
 }
 
@@ -527,14 +542,26 @@ void launch_shrink_ring(const LoraArgs& g, unsigned blocks, hipStream_t s)
     else shrink_ring_kernel<8, 3><<<blocks, 256, 0, s>>>(g);
 }
 
+// Steps of 32 columns a wave loads at once (of `big` launches, whose workgroups have them
+// for all four waves).
 template <int RT, bool F32>
-void launch_expand(const LoraArgs& g, unsigned blocks, hipStream_t s)
+constexpr int expand_steps(int r)
 {
-    constexpr int U = RT == 1 ? 4 : 2, U4 = RT == 1 ? 2 : 1;
-    if (g.r <= 16) expand_kernel<RT, 0, F32, U><<<blocks, 256, 0, s>>>(g);
-    else if (g.r <= 32) expand_kernel<RT, 1, F32, U><<<blocks, 256, 0, s>>>(g);
-    else if (g.r <= 64) expand_kernel<RT, 2, F32, U><<<blocks, 256, 0, s>>>(g);
-    else expand_kernel<RT, 4, F32, U4><<<blocks, 256, 0, s>>>(g);
+    return RT > 1 ? (r <= 64 ? 2 : 1) : r <= 16 ? (F32 ? 6 : 8) : r <= 64 ? 4 : 2;
+}
+
+template <int RT, bool F32>
+void launch_expand(const LoraArgs& g, bool big, unsigned blocks, hipStream_t s)
+{
+    auto go = [&](auto f, auto steps) {
+        constexpr int F = decltype(f)::value, U = decltype(steps)::value;
+        if (big) expand_kernel<RT, F, F32, U><<<blocks, 256, 0, s>>>(g);
+        else expand_kernel<RT, F, F32, 1><<<blocks, 256, 0, s>>>(g);
+    };
+    if (g.r <= 16) go(std::integral_constant<int, 0>{}, std::integral_constant<int, expand_steps<RT, F32>(16)>{});
+    else if (g.r <= 32) go(std::integral_constant<int, 1>{}, std::integral_constant<int, expand_steps<RT, F32>(32)>{});
+    else if (g.r <= 64) go(std::integral_constant<int, 2>{}, std::integral_constant<int, expand_steps<RT, F32>(64)>{});
+    else go(std::integral_constant<int, 4>{}, std::integral_constant<int, expand_steps<RT, F32>(128)>{});
 }
 
 }  // namespace
@@ -588,9 +615,14 @@ int heph_lora_add(void* c, int c_dtype, const void* base, const uint16_t* x_bf16
         return HEPH_ERR_WORKSPACE;
     const int tiles = max_tiles(M, n_adapters), splits = k_splits(M, n_adapters, K);
     // Columns a workgroup: few enough for two workgroups a CU, each of which joins the
-    // parts of t for itself.
+    // parts of t for itself; whole rounds of its four waves.
+    const bool f32 = c_dtype == HEPH_DTYPE_F32, decode = tile_rows(M) == 16;
+    const int round = 128 * (decode ? (f32 ? expand_steps<1, true>(rank) : expand_steps<1, false>(rank))
+                                    : expand_steps<4, false>(rank));
     const int chunks = std::max(1, std::min((2 * kPlanCUs + tiles - 1) / tiles, (N + 127) / 128));
-    const int n_chunk = ((N + chunks - 1) / chunks + 127) / 128 * 128;
+    const int want = (N + chunks - 1) / chunks;
+    const bool big = want >= round;
+    const int n_chunk = big ? (want + round - 1) / round * round : (want + 127) / 128 * 128;
     const int64_t expand = blocks_for(tiles, (N + n_chunk - 1) / n_chunk);
     if (expand > INT32_MAX) return HEPH_ERR_UNSUPPORTED;
     if (int st = check_device()) return st;
@@ -598,13 +630,14 @@ int heph_lora_add(void* c, int c_dtype, const void* base, const uint16_t* x_bf16
                      static_cast<PlanHeader*>(const_cast<void*>(plan)), static_cast<float*>(ws), M, N, K,
                      rank, n_adapters, splits, n_chunk, xcds_for(tiles)};
     hipStream_t s = static_cast<hipStream_t>(stream);
-    const bool f32 = c_dtype == HEPH_DTYPE_F32;
-    if (tile_rows(M) == 16) {
+    if (decode) {
         launch_shrink(g, (unsigned)blocks_for(tiles, splits), s);
-        f32 ? launch_expand<1, true>(g, (unsigned)expand, s) : launch_expand<1, false>(g, (unsigned)expand, s);
+        f32 ? launch_expand<1, true>(g, big, (unsigned)expand, s)
+            : launch_expand<1, false>(g, big, (unsigned)expand, s);
     } else {
         launch_shrink_ring(g, (unsigned)blocks_for(tiles, splits), s);
-        f32 ? launch_expand<4, true>(g, (unsigned)expand, s) : launch_expand<4, false>(g, (unsigned)expand, s);
+        f32 ? launch_expand<4, true>(g, big, (unsigned)expand, s)
+            : launch_expand<4, false>(g, big, (unsigned)expand, s);
     }
     return status_of(hipGetLastError());
 }
