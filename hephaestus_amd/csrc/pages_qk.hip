@@ -118,9 +118,8 @@ __device__ __forceinline__ void qk_heads(const QkArgs& a, long unit)
 // are single bytes 64 apart; where four tokens fill an aligned run of four slots (a
 // prompt's do) their bytes are neighbours. The codes meet in LDS; then sixteen lanes write
 // the dwords of up to sixteen such runs, a whole 64-byte line of a dim where the window
-// fills a page, and the tokens left over go as bytes. Lines written in part cost most:
-// 4090 prompt tokens with four of them a run written by waves of 16 tokens 64 us, 128
-// scattered ones 12.5.
+// fills a page, and the tokens left over go as bytes. (4096 tokens, 32 + 8 heads: in
+// runs 18.5 us, all scattered 41.5; without any cache write 15.1.)
 template <int W>
 __device__ __forceinline__ void v_window(const QkArgs& a, long unit)
 {
@@ -138,9 +137,20 @@ __device__ __forceinline__ void v_window(const QkArgs& a, long unit)
     }
     const float inv = a.kv_inv[a.n_kv + h];
     const uint16_t* rows = a.qkv + (int64_t)t0 * a.qkv_stride + (size_t)(a.n_heads + a.n_kv + h) * kHeadDim;
-    for (int i = tid; i < n * 16; i += 256) {
+    // (all loads at once; past the batch its last row again, not used)
+    constexpr int LOADS = (W * 16 + 255) / 256;
+    uint4 x[LOADS];
+#pragma unroll
+    for (int k = 0; k < LOADS; ++k) {
+        const int i = min(tid + k * 256, n * 16 - 1);
+        x[k] = ldg16u(rows + (int64_t)(i / 16) * a.qkv_stride + i % 16 * 8);
+    }
+#pragma unroll
+    for (int k = 0; k < LOADS; ++k) {
+        const int i = tid + k * 256;
+        if (i >= n * 16) break;
         float f[8];
-        unpack8(ldg16u(rows + (int64_t)(i / 16) * a.qkv_stride + i % 16 * 8), f);
+        unpack8(x[k], f);
         const uint2 w = codes8(f, inv);
         uint32_t* to = lds + (i / 16) * (PITCH / 4) + i % 16 * 2;
         to[0] = w.x;
@@ -148,7 +158,10 @@ __device__ __forceinline__ void v_window(const QkArgs& a, long unit)
     }
     bool leads = slot >= 0 && slot % 4 == 0 && l + 3 < W;
 #pragma unroll
-    for (int i = 1; i < 4; ++i) leads = leads && __shfl(slot, min(l + i, 63)) == slot + i;
+    for (int i = 1; i < 4; ++i) {
+        const int later = __shfl(slot, min(l + i, 63));       // (by all lanes)
+        leads = leads && later == slot + i;
+    }
     const unsigned long long lead = __ballot(leads);
     const int first = l - (slot & 3);                  // where slot's run of four would start
     const bool alone = slot >= 0 && !(first >= 0 && (lead >> first & 1));

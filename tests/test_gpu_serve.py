@@ -138,6 +138,34 @@ def test_qk_runs_of_slots():
     check_qk(c, 8, 4)
 
 
+def test_qk_long_batches_in_runs():
+    # windows of 64 tokens: prompts from any slot, some tokens left out, and the bytes
+    # of a batch alike however its tokens are cut into calls
+    for first in (0, 64, 37, 3):
+        c = qk_case(777, 8, 3, seed=first)
+        c["slot"] = torch.arange(first, first + 777, dtype=torch.int32, device="cuda")
+        c["pos"][[0, 100, 101, 640]] = -1
+        c["slot"][[7, 63, 64, 700]] = -1
+        check_qk(c, 8, 3)
+    c = qk_case(700, 8, 4, seed=20)
+    a = torch.arange(2000, 2350)
+    c["slot"] = torch.cat([a, torch.randperm(1900)[:200], torch.arange(1999, 1849, -1)]).int().cuda()
+    check_qk(c, 8, 4)
+    whole, parts = qk_case(600, 8, 4, seed=21), qk_case(600, 8, 4, seed=21)
+    for d in (whole, parts):
+        d["slot"] = torch.arange(5, 605, dtype=torch.int32, device="cuda")
+    check_qk(whole, 8, 4)
+    rope = S.rope_table_f32(whole["n_pos"])
+    for lo in range(0, 600, 50):
+        s = slice(lo, lo + 50)
+        S.qk_norm_rope_pages(parts["q"][s], parts["qkv"][s], parts["gam"][0], parts["gam"][1],
+                             parts["k"], parts["v"], parts["inv"], rope, parts["pos"][s].clone(),
+                             parts["slot"][s].clone())
+    torch.cuda.synchronize()
+    assert torch.equal(whole["k"], parts["k"]) and torch.equal(whole["v"], parts["v"])
+    assert torch.equal(whole["q"], parts["q"])
+
+
 def test_qk_padding_rows():
     c = qk_case(40, 8, 4, seed=3)
     c["pos"][[0, 7, 39]] = torch.tensor([-1, 5000, 2 ** 31 - 1], dtype=torch.int32, device="cuda")
