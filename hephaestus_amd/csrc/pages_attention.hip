@@ -41,10 +41,11 @@ struct PlanHeader {
 struct Unit {
     int seq, tok0, row0, rows, page0, pages, part, prefix;
 };
-// Per token: keys it attends to (-1: no sequence), and how many prefix and own
-// units hold any of them.
+// Per token: keys it attends to (-1: no sequence), how many prefix and own units hold
+// any of them, and where its first row's partial results lie among a kv head's: those of
+// unit k at prefix + k * prefix_step, own + k * own_step.
 struct Token {
-    int limit, n_prefix, n_own, pad;
+    int limit, n_prefix, n_own, prefix, prefix_step, own, own_step, pad;
 };
 
 // Query rows of a unit by how many there are: 16, 32 or 64 (attend_narrow: a
@@ -61,14 +62,14 @@ struct Sizes {
     int n_tok, n_seqs, n_groups, n_heads, n_kv;
     __host__ __device__ int group() const { return n_heads / n_kv; }
     __host__ __device__ long rows() const { return (long)n_tok * n_heads; }
-    // Workspace slots a row: as many partial results as its units may write.
-    __host__ __device__ int parts() const
-    {
-        const long p = (1L << 17) / rows();
-        return (int)(p < 2 ? 2 : p > 96 ? 96 : p);
-    }
-    // Slots of one kv head.
+    // Workgroups of one kv head that run at once.
     __host__ __device__ int slots() const { return kSlots / n_kv > 0 ? kSlots / n_kv : 1; }
+    // Partial results a kv head may write: every row twice (behind a prefix, and its
+    // own), and the rows of the units that splitting adds.
+    __host__ __device__ long max_parts() const
+    {
+        return 2L * n_tok * group() + 3L * slots() * wide_rows(group());
+    }
     // Units a plan may hold: one a tile (each sequence's and each group's last
     // one may be short), and a round more where long runs are split and where
     // the last round's tiles are.
@@ -113,6 +114,7 @@ struct Source {
     int seq, tok0, n_tok, page0, pages, kv;     // kv: 0 for a group
     int tile, tiles, base;
     int chunks;                                 // a tile's units before the last round
+    int parts;                                  // where its partial results start
 };
 
 struct SeqTokens {
@@ -168,6 +170,12 @@ __device__ Source seq_source(const PlanLds& in, const PlanArgs& a, int s, int& g
 // Keys that token i of the source attends to.
 __device__ __forceinline__ int limit_of(const Source& x, int i) { return max(x.kv - x.n_tok + i + 1, 0); }
 
+// Tiles of the source that belong to the last round: those numbered last, r < the result.
+__device__ __forceinline__ int last_round(const Source& x, const Rounds& rounds)
+{
+    return x.tile > kNarrow ? clampi(x.base + x.tiles - rounds.first, 0, x.tiles) : 0;
+}
+
 // Units of tile r and pages of each: a sequence's tile sees its last token's keys.
 struct Cut {
     int per, chunks;
@@ -180,9 +188,16 @@ __device__ __forceinline__ Cut cut_tile(const Source& x, const Rounds& rounds, i
         pages = clampi((limit_of(x, last) + kPage - 1) / kPage - x.page0, 0, pages);
     }
     Cut c;
-    c.chunks = x.tile > kNarrow && x.base + x.tiles - 1 - r >= rounds.first ? rounds.chunks : x.chunks;
+    c.chunks = r < last_round(x, rounds) ? rounds.chunks : x.chunks;
     c.per = max(ceil_div(pages, c.chunks), 1);
     return c;
+}
+
+// Partial results of the tiles before r, which are full ones: one a row and unit.
+__device__ __forceinline__ int parts_before(const Source& x, const Rounds& rounds, int r)
+{
+    const int last = last_round(x, rounds);
+    return x.tile * (min(r, last) * rounds.chunks + max(r - last, 0) * x.chunks);
 }
 
 // Units of c that hold any of the first `keys` keys.
@@ -191,25 +206,35 @@ __device__ __forceinline__ int parts_seen(int keys, const Cut& c)
     return keys <= 0 ? 0 : min(c.chunks, ceil_div((keys + kPage - 1) / kPage, c.per));
 }
 
-// Exclusive prefix sum over the workgroup, and the total.
-__device__ int scan_block(int v, int* red, int& total)
+// Exclusive prefix sums over the workgroup of the groups' values and, behind them all, the
+// sequences'; the total.
+__device__ int scan_block(int& g, int& s, int2* red)
 {
     const int t = threadIdx.x, l = t & 63, waves = blockDim.x / 64;
-    int x = v;
+    int x = g, y = s;
     for (int o = 1; o < 64; o <<= 1) {
-        const int y = __shfl_up(x, o);
-        if (l >= o) x += y;
+        const int a = __shfl_up(x, o), b = __shfl_up(y, o);
+        if (l >= o) {
+            x += a;
+            y += b;
+        }
     }
     __syncthreads();
-    if (l == 63) red[t / 64] = x;
+    if (l == 63) red[t / 64] = make_int2(x, y);
     __syncthreads();
-    int before = 0;
-    total = 0;
+    int before_g = 0, before_s = 0, all_g = 0, all_s = 0;
     for (int i = 0; i < waves; ++i) {
-        if (i < t / 64) before += red[i];
-        total += red[i];
+        const int2 r = red[i];
+        if (i < t / 64) {
+            before_g += r.x;
+            before_s += r.y;
+        }
+        all_g += r.x;
+        all_s += r.y;
     }
-    return before + x - v;
+    g = before_g + x - g;
+    s = all_g + before_s + y - s;
+    return all_g + all_s;
 }
 
 // One thread a sequence and a group. Every workgroup repeats that and writes a share
@@ -220,10 +245,11 @@ __global__ __launch_bounds__(kMaxSeqs) void plan_kernel(PlanArgs a)
     __shared__ PlanLds in;
     __shared__ Source groups[kMaxSeqs];
     __shared__ SeqTokens seqs[kMaxSeqs];
-    __shared__ float red_f[kMaxSeqs / 64];
-    __shared__ int red_i[kMaxSeqs / 64], merges;
+    __shared__ float2 red_f[kMaxSeqs / 64];
+    __shared__ int2 red_i[kMaxSeqs / 64];
+    __shared__ int merges;
     const int t = threadIdx.x, G = a.s.group(), nt = blockDim.x;
-    const int cap = a.s.parts(), cap_prefix = a.s.n_groups ? cap / 2 : 0, cap_own = cap - cap_prefix;
+    constexpr int cap = 64;                    // (merge_row takes two lanes' worth)
     Token* tokens = plan_tokens(a.plan);
     Unit* units = plan_units(a.plan, a.s.n_tok);
     for (int i = t; i <= a.s.n_seqs; i += nt) in.q_start[i] = a.q_start[i];
@@ -239,59 +265,72 @@ __global__ __launch_bounds__(kMaxSeqs) void plan_kernel(PlanArgs a)
     if (t < a.s.n_groups) xg = group_source(in, a, t);
     if (t < a.s.n_seqs) xs = seq_source(in, a, t, group);
 
-    // Work: a page of a narrow unit costs the stream of its 16 KB, one of a wide
-    // unit about twice that in matrix work. (In f32: it only sets a split.)
+    // Work: a page of a narrow unit costs the stream of its 16 KB, one of a wide unit
+    // about twice that in matrix work. (In f32: it only sets a split.)
     auto wide = [](const Source& x) { return x.tile > kNarrow; };
-    auto cost = [&](const Source& x) { return (float)x.tiles * (float)x.pages * (wide(x) ? 2.0f : 1.0f); };
-    float work = cost(xg) + cost(xs);
-    for (int o = 32; o; o >>= 1) work += __shfl_xor(work, o);
-    if ((t & 63) == 0) red_f[t / 64] = work;
-    int wide_g, wide_s;
-    xg.base = scan_block(wide(xg) ? xg.tiles : 0, red_i, wide_g);
-    xs.base = wide_g + scan_block(wide(xs) ? xs.tiles : 0, red_i, wide_s);
-    work = 0.0f;
-    for (int i = 0; i < nt / 64; ++i) work += red_f[i];
+    auto pages = [&](const Source& x, bool w) { return wide(x) == w ? (float)x.tiles * (float)x.pages : 0.0f; };
+    float work_n = pages(xg, false) + pages(xs, false), work_w = pages(xg, true) + pages(xs, true);
+    for (int o = 32; o; o >>= 1) {
+        work_n += __shfl_xor(work_n, o);
+        work_w += __shfl_xor(work_w, o);
+    }
+    if ((t & 63) == 0) red_f[t / 64] = make_float2(work_n, work_w);
+    xg.base = wide(xg) ? xg.tiles : 0;
+    xs.base = wide(xs) ? xs.tiles : 0;
+    const int wide_tiles = scan_block(xg.base, xs.base, red_i);
+    work_n = work_w = 0.0f;
+    for (int i = 0; i < nt / 64; ++i) {
+        work_n += red_f[i].x;
+        work_w += red_f[i].y;
+    }
 
-    // Runs are split so that the units fill the slots of a kv head; wide tiles
-    // that fill them by themselves stay whole but for those of a last round that
-    // would leave half of the slots or more empty.
-    const int slots = a.s.slots(), wide_tiles = wide_g + wide_s, rest = wide_tiles % slots;
-    const float tau = work / (float)slots;
-    auto chunks = [&](const Source& x, int cap) {
-        if (wide(x) && wide_tiles >= slots) return 1;
-        const float per = fmaxf(tau * (wide(x) ? 0.5f : 1.0f), (float)(wide(x) ? kMinWide : kMinNarrow));
-        return clampi((int)ceilf((float)x.pages / per), 1, cap);
+    // Narrow runs are split so that the units fill the slots of a kv head. Wide tiles get
+    // their share of the slots, of half of them where narrow units are a good part of the
+    // work: a CU then streams for one while it multiplies for the other. Wide tiles that
+    // fill the slots by themselves stay whole, but for those of a last round that would
+    // leave half of the slots or more empty.
+    const int slots = a.s.slots(), rest = wide_tiles % slots;
+    const float tau = fmaxf((work_n + 2.0f * work_w) / (float)slots, (float)kMinNarrow);
+    const float share = (float)(work_n > 0.5f * work_w ? (slots + 1) / 2 : slots) / fmaxf(work_w, 1.0f);
+    auto chunks = [&](const Source& x) {
+        if (!wide(x)) return clampi((int)ceilf((float)x.pages / tau), 1, cap);
+        if (wide_tiles >= slots) return 1;
+        return clampi(min((int)((float)x.pages * share), x.pages / kMinWide), 1, cap);
     };
     Rounds rounds{INT32_MAX, 1};
-    if (wide_tiles >= slots && rest > 0) rounds = Rounds{wide_tiles - rest, slots / rest};
-    rounds.chunks = min(min(rounds.chunks, a.s.n_groups ? cap_prefix : cap_own),
-                        ceil_div(a.table_pages, kMinNarrow));
-    xg.chunks = chunks(xg, cap_prefix);
-    xs.chunks = chunks(xs, cap_own);
-    if (t < a.s.n_groups) groups[t] = xg;
-
+    if (wide_tiles >= slots && rest > 0)
+        rounds = Rounds{wide_tiles - rest, min(min(slots / rest, cap), ceil_div(a.table_pages, kMinNarrow))};
+    xg.chunks = chunks(xg);
+    xs.chunks = chunks(xs);
     auto count = [&](const Source& x) {
-        if (!wide(x)) return x.tiles * x.chunks;
-        const int last = clampi(x.base + x.tiles - rounds.first, 0, x.tiles);    // of the last round
+        const int last = last_round(x, rounds);
         return (x.tiles - last) * x.chunks + last * rounds.chunks;
     };
-    int units_g, units_s;
-    const int at_g = scan_block(count(xg), red_i, units_g);
-    const int at_s = units_g + scan_block(count(xs), red_i, units_s);      // (groups[] is there)
+    auto rows_in = [&](const Source& x, int r) { return min(x.tile, x.n_tok * G - r * x.tile); };
+    auto parts = [&](const Source& x) {
+        if (x.tiles == 0) return 0;
+        const int r = x.tiles - 1;
+        return parts_before(x, rounds, r) + rows_in(x, r) * cut_tile(x, rounds, G, r).chunks;
+    };
+    xg.parts = parts(xg);
+    xs.parts = parts(xs);
+    scan_block(xg.parts, xs.parts, red_i);
+    if (t < a.s.n_groups) groups[t] = xg;
+    int at_g = count(xg), at_s = count(xs);
+    // a row of another number of units than one: behind a prefix, in a split run, without keys
+    if (xg.tiles > 0 || (xs.n_tok > 0 && (xs.kv < xs.n_tok || xs.tiles == 0 || at_s > xs.tiles)))
+        merges = 1;
+    const int all_units = scan_block(at_g, at_s, red_i);
     const int max_units = (int)min(a.s.max_units(), (long)INT32_MAX);
     auto emit = [&](const Source& x, int u, int prefix) {
-        const int rows = x.n_tok * G;
         for (int r = x.tiles - 1; r >= 0; --r) {
             const Cut c = cut_tile(x, rounds, G, r);
             for (int k = 0; k < c.chunks; ++k, ++u)
                 if (u < max_units)
-                    units[u] = Unit{x.seq, x.tok0, r * x.tile, min(x.tile, rows - r * x.tile),
+                    units[u] = Unit{x.seq, x.tok0, r * x.tile, rows_in(x, r),
                                     x.page0 + k * c.per, min(c.per, x.pages - k * c.per), k, prefix};
         }
     };
-    // a row of another number of units than one: behind a prefix, in a split run, without keys
-    if (xg.tiles > 0 || (xs.n_tok > 0 && (xs.kv < xs.n_tok || xs.tiles == 0 || count(xs) > xs.tiles)))
-        merges = 1;
     if (t < a.s.n_seqs) seqs[t] = SeqTokens{xs, group};
     __syncthreads();
     if (blockIdx.x == 0) {
@@ -299,7 +338,7 @@ __global__ __launch_bounds__(kMaxSeqs) void plan_kernel(PlanArgs a)
         emit(xs, at_s, 0);
         if (t == 0)
             *a.plan = PlanHeader{kMagic, a.s.n_tok, a.s.n_seqs, a.s.n_groups, a.table_pages, a.s.n_heads,
-                                 a.s.n_kv, min(units_g + units_s, max_units), merges, {}};
+                                 a.s.n_kv, min(all_units, max_units), merges, {}};
     }
     for (int i = blockIdx.x * kPlanTokens + t; i < min(a.s.n_tok, ((int)blockIdx.x + 1) * kPlanTokens); i += nt) {
         int lo = 0, hi = a.s.n_seqs;              // the last sequence that starts at i or before
@@ -308,19 +347,21 @@ __global__ __launch_bounds__(kMaxSeqs) void plan_kernel(PlanArgs a)
             if (in.q_start[mid] <= i) lo = mid + 1;
             else hi = mid;
         }
-        Token tk{-1, 0, 0, 0};
+        Token tk{-1, 0, 0, 0, 0, 0, 0, 0};
         if (lo > 0 && i < in.q_start[lo]) {
             const Source& x = seqs[lo - 1].x;
-            const int g = seqs[lo - 1].group, at = i - x.tok0;
-            tk.limit = limit_of(x, at);
-            if (x.tiles > 0)
-                tk.n_own = parts_seen(tk.limit - x.page0 * kPage,
-                                      cut_tile(x, rounds, G, (unsigned)(at * G) / (unsigned)x.tile));
-            if (g >= 0 && groups[g].tiles > 0)
-                tk.n_prefix = parts_seen(
-                    min(tk.limit, x.page0 * kPage),
-                    cut_tile(groups[g], rounds, G,
-                             (unsigned)((i - groups[g].tok0) * G) / (unsigned)groups[g].tile));
+            const int g = seqs[lo - 1].group;
+            tk.limit = limit_of(x, i - x.tok0);
+            // units of the row's tile that hold any of `keys` keys, and where their results lie
+            auto look = [&](const Source& y, int keys, int& n, int& at, int& step) {
+                if (y.tiles == 0) return;
+                const int row = (i - y.tok0) * G, r = (unsigned)row / (unsigned)y.tile;
+                n = parts_seen(keys, cut_tile(y, rounds, G, r));
+                at = y.parts + parts_before(y, rounds, r) + row - r * y.tile;
+                step = rows_in(y, r);
+            };
+            look(x, tk.limit - x.page0 * kPage, tk.n_own, tk.own, tk.own_step);
+            if (g >= 0) look(groups[g], min(tk.limit, x.page0 * kPage), tk.n_prefix, tk.prefix, tk.prefix_step);
         }
         tokens[i] = tk;
     }
@@ -337,8 +378,8 @@ struct AttnArgs {
     const float* kv_scale;
     const int32_t* table;
     PlanHeader* plan;
-    float* part_o;          // [rows][parts][128], unnormalized
-    float2* part_ml;        // [rows][parts]: maximum (log2), sum
+    float* part_o;          // [n_kv][max_parts][128], unnormalized
+    float2* part_ml;        // [n_kv][max_parts]: maximum (log2), sum
     Sizes s;
     int n_pages, table_pages;
 };
@@ -631,7 +672,10 @@ struct Rows {
                         *reinterpret_cast<uint2*>(out + (d0 + d) * 16) = w;
                     }
             } else {
-                const size_t slot = row * a.s.parts() + (u.prefix ? 0 : tk.n_prefix) + u.part;
+                const long part = (u.prefix ? tk.prefix + u.part * tk.prefix_step : tk.own + u.part * tk.own_step) +
+                                  (hd[r] - head * a.s.group());
+                if (part >= a.s.max_parts()) continue;          // (a plan never asks for it)
+                const size_t slot = (size_t)head * a.s.max_parts() + part;
                 if (g4 == 0 && d0 == 0) a.part_ml[slot] = make_float2(m[r], sum[r][0]);
 #pragma unroll
                 for (int d = 0; d < 8; ++d)
@@ -850,25 +894,30 @@ __device__ __forceinline__ void merge_row(const AttnArgs& a, long row, int l)
 {
     const int t = (int)(row / a.s.n_heads), h = (int)(row % a.s.n_heads);
     const Token tk = plan_tokens(a.plan)[t];
-    const int n = min(tk.n_prefix + tk.n_own, a.s.parts());
+    const int n = min(tk.n_prefix + tk.n_own, 128), G = a.s.group();
     if (tk.limit < 0 || n == 1) return;
-    const size_t slot = (size_t)row * a.s.parts();
+    const long max_parts = a.s.max_parts();
+    auto slot = [&](int k) {
+        const long part = (k < tk.n_prefix ? tk.prefix + k * tk.prefix_step
+                                           : tk.own + (k - tk.n_prefix) * tk.own_step) + h % G;
+        return (size_t)(h / G) * max_parts + (part < max_parts ? part : 0);
+    };
     float2 ml[2];
     float top = -INFINITY;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-        ml[i] = i * 64 + l < n ? a.part_ml[slot + i * 64 + l] : make_float2(-INFINITY, 0.0f);
+        ml[i] = i * 64 + l < n ? a.part_ml[slot(i * 64 + l)] : make_float2(-INFINITY, 0.0f);
         top = fmaxf(top, ml[i].x);
     }
     top = wave_fold_max64(top);
     const float f0 = weight(ml[0].x, top), f1 = weight(ml[1].x, top);
     const float sum = wave_fold_sum64(__builtin_fmaf(ml[0].y, f0, ml[1].y * f1));
-    const float2* part = reinterpret_cast<const float2*>(a.part_o + slot * kHeadDim) + l;
+    const float2* part = reinterpret_cast<const float2*>(a.part_o) + l;
     float x = 0.0f, y = 0.0f;
     for (int k = 0; k < n; k += 8) {
         float2 o[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) o[i] = part[(size_t)min(k + i, n - 1) * (kHeadDim / 2)];
+        for (int i = 0; i < 8; ++i) o[i] = part[slot(min(k + i, n - 1)) * (kHeadDim / 2)];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const float f = __int_as_float(__builtin_amdgcn_readlane(
@@ -921,7 +970,7 @@ size_t heph_pages_attention_ws_bytes(int n_tok, int n_seqs, int n_groups, int n_
 {
     if (!sizes_ok(n_tok, n_seqs, n_groups, n_heads, n_kv_heads)) return 0;
     const Sizes s{n_tok, n_seqs, n_groups, n_heads, n_kv_heads};
-    return (size_t)s.rows() * s.parts() * (kHeadDim * sizeof(float) + sizeof(float2));
+    return (size_t)n_kv_heads * s.max_parts() * (kHeadDim * sizeof(float) + sizeof(float2));
 }
 
 int heph_pages_attention_plan(void* plan, size_t plan_bytes, const int32_t* q_start,
@@ -982,7 +1031,7 @@ int heph_pages_attention(void* out_bf16, const void* q_bf16, int64_t q_stride,
     a.table = page_table;
     a.plan = static_cast<PlanHeader*>(const_cast<void*>(plan));
     a.part_o = static_cast<float*>(ws);
-    a.part_ml = reinterpret_cast<float2*>(a.part_o + (size_t)a.s.rows() * a.s.parts() * kHeadDim);
+    a.part_ml = reinterpret_cast<float2*>(a.part_o + (size_t)n_kv_heads * a.s.max_parts() * kHeadDim);
     a.n_pages = n_pages;
     a.table_pages = table_pages;
     hipStream_t s = static_cast<hipStream_t>(stream);
