@@ -20,6 +20,7 @@
 // units out from the lengths in device memory; units of the same row meet in
 // the workspace and merge_kernel joins them.
 #include <algorithm>
+#include <type_traits>
 
 #include "pages.h"
 
@@ -206,19 +207,29 @@ __device__ __forceinline__ int parts_seen(int keys, const Cut& c)
     return keys <= 0 ? 0 : min(c.chunks, ceil_div((keys + kPage - 1) / kPage, c.per));
 }
 
+// Inclusive prefix sum over the wave: within rows of 16 lanes by shifts, then each row's
+// total to the rows behind it.
+__device__ __forceinline__ int wave_scan(int v)
+{
+    auto add = [&](auto ctrl, auto rows) {
+        v += __builtin_amdgcn_update_dpp(0, v, decltype(ctrl)::value, decltype(rows)::value, 0xF, false);
+    };
+    using std::integral_constant;
+    add(integral_constant<int, 0x111>{}, integral_constant<int, 0xF>{});
+    add(integral_constant<int, 0x112>{}, integral_constant<int, 0xF>{});
+    add(integral_constant<int, 0x114>{}, integral_constant<int, 0xF>{});
+    add(integral_constant<int, 0x118>{}, integral_constant<int, 0xF>{});
+    add(integral_constant<int, 0x142>{}, integral_constant<int, 0xA>{});      // row_bcast 15
+    add(integral_constant<int, 0x143>{}, integral_constant<int, 0xC>{});      // row_bcast 31
+    return v;
+}
+
 // Exclusive prefix sums over the workgroup of the groups' values and, behind them all, the
 // sequences'; the total.
 __device__ int scan_block(int& g, int& s, int2* red)
 {
     const int t = threadIdx.x, l = t & 63, waves = blockDim.x / 64;
-    int x = g, y = s;
-    for (int o = 1; o < 64; o <<= 1) {
-        const int a = __shfl_up(x, o), b = __shfl_up(y, o);
-        if (l >= o) {
-            x += a;
-            y += b;
-        }
-    }
+    const int x = wave_scan(g), y = wave_scan(s);
     __syncthreads();
     if (l == 63) red[t / 64] = make_int2(x, y);
     __syncthreads();
@@ -239,7 +250,7 @@ __device__ int scan_block(int& g, int& s, int2* red)
 
 // One thread a sequence and a group. Every workgroup repeats that and writes a share
 // of the tokens; the first one also writes the units and the header.
-constexpr int kPlanTokens = 256;
+constexpr int kPlanTokens = 64;
 __global__ __launch_bounds__(kMaxSeqs) void plan_kernel(PlanArgs a)
 {
     __shared__ PlanLds in;
@@ -882,8 +893,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     __shared__ __attribute__((aligned(16))) uint8_t lds[2 * kWidePage];
     const PlanHeader h = *a.plan;
     const int n_kv = a.s.n_kv, unit = blockIdx.x / n_kv, head = blockIdx.x % n_kv;
+    const Unit u = plan_units(a.plan, a.s.n_tok)[unit];        // (the plan has room for all of the grid's)
     if (!plan_fits(h, a) || unit >= h.n_units) return;
-    const Unit u = plan_units(a.plan, a.s.n_tok)[unit];
     if (u.rows <= kNarrow) attend_narrow(a, u, head, lds);
     else attend_wide(a, u, head, lds);
 }
@@ -940,8 +951,18 @@ __global__ __launch_bounds__(256) void merge_kernel(AttnArgs a)
 {
     const PlanHeader head = *a.plan;
     if (!plan_fits(head, a) || !head.merges) return;
-    for (long row = (long)blockIdx.x * 4 + (threadIdx.x >> 6); row < a.s.rows(); row += (long)gridDim.x * 4)
-        merge_row(a, row, threadIdx.x & 63);
+    // each lane looks at one of the wave's next 64 rows
+    const long step = (long)gridDim.x * 4, rows = a.s.rows();
+    for (long row0 = (long)blockIdx.x * 4 + (threadIdx.x >> 6); row0 < rows; row0 += 64 * step) {
+        const long row = row0 + (threadIdx.x & 63) * step;
+        bool todo = false;
+        if (row < rows) {
+            const Token tk = plan_tokens(a.plan)[row / a.s.n_heads];
+            todo = tk.limit >= 0 && tk.n_prefix + tk.n_own != 1;
+        }
+        for (unsigned long long m = __ballot(todo); m; m &= m - 1)
+            merge_row(a, row0 + (__ffsll((long long)m) - 1) * step, threadIdx.x & 63);
+    }
 }
 
 bool sizes_ok(int n_tok, int n_seqs, int n_groups, int n_heads, int n_kv)
@@ -989,7 +1010,7 @@ int heph_pages_attention_plan(void* plan, size_t plan_bytes, const int32_t* q_st
     if (int st = check_device()) return st;
     const PlanArgs a{static_cast<PlanHeader*>(plan), q_start, kv_len, group_start, shared_pages,
                      Sizes{n_tok, n_seqs, n_groups, n_heads, n_kv_heads}, table_pages};
-    const int threads = std::max(256, (n_seqs + 63) / 64 * 64);
+    const int threads = (n_seqs + 63) / 64 * 64;
     plan_kernel<<<(n_tok + kPlanTokens - 1) / kPlanTokens, threads, 0, static_cast<hipStream_t>(stream)>>>(a);
     return status_of(hipGetLastError());
 }
