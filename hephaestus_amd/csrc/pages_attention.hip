@@ -531,43 +531,58 @@ struct Rows {
     // number in the sequence. Where some row does not see all of it, clear() takes the
     // NaN out of what v gives and says whether there was any: a NaN must reach the rows
     // that see its key and no other, and 0 * NaN is NaN; vp reads V's codes again for
-    // them. AHEAD: operands come from LDS, eight of them a step ahead of their products.
+    // them. AHEAD: operands come from LDS, four of them a step ahead of their products.
     template <bool AHEAD, class K, class V, class C>
     __device__ __forceinline__ void page(int page, float sc, K k, V v, C clear, const uint8_t* vp)
     {
         const int g4 = (threadIdx.x & 63) >> 4;
         f32x4 s[4][RT];
-        bf16x8 w0[8], w1[8];
-        auto k8 = [&](bf16x8 (&w)[8], int g) {
+        bf16x8 w0[4], w1[4];
+        auto k4 = [&](bf16x8 (&w)[4], int kt) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) w[i] = k(i % 4 / 2 * 4 + 2 * g + i / 4, i % 2);
+            for (int i = 0; i < 4; ++i) w[i] = k(i / 2 * 4 + kt, i % 2);
         };
-        auto v8 = [&](bf16x8 (&w)[8], int g) {
+        auto v4 = [&](bf16x8 (&w)[4], int g) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) w[i] = v(4 * g + i / 2, i % 2);
+            for (int i = 0; i < 4; ++i) w[i] = v(2 * g + i / 2, i % 2);
         };
-        auto scores8 = [&](const bf16x8 (&w)[8], int g) {
+        auto scores4 = [&](const bf16x8 (&w)[4], int kt) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
+            for (int i = 0; i < 4; ++i)
 #pragma unroll
                 for (int r = 0; r < RT; ++r) {
                     const f32x4 zero = {0, 0, 0, 0};
-                    f32x4& x = s[2 * g + i / 4][r];
-                    x = mfma_bf16(w[i], q[r][i % 4], i % 4 ? x : zero);
+                    s[kt][r] = mfma_bf16(w[i], q[r][i], i ? s[kt][r] : zero);
                 }
         };
+        // Keeps what is on its two sides apart, so that reads stay a step ahead.
         auto step = [] { if constexpr (AHEAD) __builtin_amdgcn_sched_barrier(0); };
-        k8(w0, 0);
-        step();
-        if constexpr (AHEAD) k8(w1, 1);
-        step();
-        scores8(w0, 0);
-        step();
-        if constexpr (AHEAD) v8(w0, 0);
-        else k8(w1, 1);
-        step();
-        scores8(w1, 1);
-        step();
+        if constexpr (AHEAD) {
+            k4(w0, 0);
+            step();
+            k4(w1, 1);
+            step();
+            scores4(w0, 0);
+            step();
+            k4(w0, 2);
+            step();
+            scores4(w1, 1);
+            step();
+            k4(w1, 3);
+            step();
+            scores4(w0, 2);
+            step();
+            v4(w0, 0);
+            step();
+            scores4(w1, 3);
+            step();
+        } else {
+#pragma unroll
+            for (int kt = 0; kt < 4; ++kt) {
+                k4(w0, kt);
+                scores4(w0, kt);
+            }
+        }
         if ((page + 1) * kPage > lo) {
             const int key0 = page * kPage + g4 * 4;
 #pragma unroll
@@ -633,16 +648,15 @@ struct Rows {
             prob[r][0] = w.v[0];
             prob[r][1] = w.v[1];
         }
-        auto add8 = [&](const bf16x8 (&w)[8], int g) {
+        auto add4 = [&](const bf16x8 (&w)[4], int g) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
+            for (int i = 0; i < 4; ++i)
 #pragma unroll
                 for (int r = 0; r < RT; ++r)
-                    o[4 * g + i / 2][r] = mfma_bf16(w[i], prob[r][i % 2], o[4 * g + i / 2][r]);
+                    o[2 * g + i / 2][r] = mfma_bf16(w[i], prob[r][i % 2], o[2 * g + i / 2][r]);
         };
         step();
-        if constexpr (AHEAD) v8(w1, 1);
-        else v8(w0, 0);
+        if constexpr (AHEAD) v4(w1, 1);
         step();
         // The sum of the rounded probabilities, as the product with a row of ones: it
         // takes what the numerators take, and the matrix cores have the time.
@@ -651,10 +665,25 @@ struct Rows {
         for (int h = 0; h < 2; ++h)
 #pragma unroll
             for (int r = 0; r < RT; ++r) sum[r] = mfma_bf16(one, prob[r][h], sum[r]);
-        add8(w0, 0);
-        step();
-        if constexpr (!AHEAD) v8(w1, 1);
-        add8(w1, 1);
+        if constexpr (AHEAD) {
+            add4(w0, 0);
+            step();
+            v4(w0, 2);
+            step();
+            add4(w1, 1);
+            step();
+            v4(w1, 3);
+            step();
+            add4(w0, 2);
+            step();
+            add4(w1, 3);
+        } else {
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                v4(w0, g);
+                add4(w0, g);
+            }
+        }
     }
 
     // The rows' results over dim tiles d0 .. d0+nd-1, held in o[0 .. nd): to out
@@ -809,8 +838,8 @@ __device__ __forceinline__ void attend_narrow(const AttnArgs& a, const Unit& u, 
 // Up to 128 rows, 32 a wave. Bound by the matrix cores and the VALU's share beside
 // them (exp2, maxima, conversions), so each wave converts a quarter of a page's codes
 // to bf16 for all four, into one of two buffers in LDS in the operands' lane order
-// (linear: free of bank conflicts), while the other is worked on; the codes of the
-// page after that are on their way in registers.
+// (linear: free of bank conflicts), while the other is worked on; the codes of the two
+// pages after that are on their way in registers.
 constexpr int kWidePage = 2 * 2 * kPageBytes;      // K and V as bf16
 
 // LDS accesses of the workgroup before and behind it are ordered; loads from
@@ -842,37 +871,36 @@ __device__ __forceinline__ void attend_wide(const AttnArgs& a, const Unit& u, in
         const int last = min(first + 64, end), ids = page_ids(a, u, first);
         wait_vm<0>();           // (nothing but pages on its way below)
         auto id_of = [&](int n) { return __builtin_amdgcn_readlane(ids, n - first); };
-        i32x4 w[4];
-        auto load = [&](int n) {
-            const int id = id_of(n), at = id >= 0 && id < a.n_pages ? id : 0;
+        struct Codes {
+            i32x4 w[4];
+        } c0, c1;
+        // (past the run its last page again, so that the waits count the same loads always)
+        auto load = [&](Codes& x, int n) {
+            const int id = id_of(min(n, last - 1)), at = id >= 0 && id < a.n_pages ? id : 0;
             const uint8_t* p = pool + ((size_t)at * n_kv + head) * kPageBytes;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) w[i] = ldg16(p + i * 1024);
+            for (int i = 0; i < 4; ++i) x.w[i] = ldg16(p + i * 1024);
         };
         auto buffer = [&](int n) { return lds + ((n - first) & 1) * kWidePage + l * 16; };
-        auto convert = [&](int n) {
+        auto convert = [&](Codes& x, int n) {
             uint8_t* to = buffer(n) + wave * 8192;
             if (wave >= 2 && (n + 1) * kPage > lo) {
                 bool any = false;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) any |= clear_nan(w[i]);
+                for (int i = 0; i < 4; ++i) any |= clear_nan(x.w[i]);
                 if (__any(any) && l == 0) nan_page[(n - first) & 1] = n;
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                *reinterpret_cast<bf16x8*>(to + i * 2048) = bf16_of_codes(w[i][0], w[i][1]);
-                *reinterpret_cast<bf16x8*>(to + i * 2048 + 1024) = bf16_of_codes(w[i][2], w[i][3]);
+                *reinterpret_cast<bf16x8*>(to + i * 2048) = bf16_of_codes(x.w[i][0], x.w[i][1]);
+                *reinterpret_cast<bf16x8*>(to + i * 2048 + 1024) = bf16_of_codes(x.w[i][2], x.w[i][3]);
             }
         };
-        load(first);
-        if (threadIdx.x < 2) nan_page[threadIdx.x] = -1;
-        lds_barrier();          // (the last block's pages are read)
-        convert(first);
-        if (first + 1 < last) load(first + 1);
-        lds_barrier();
-        for (int n = first; n < last; ++n) {
-            if (n + 1 < last) convert(n + 1);
-            if (n + 2 < last) load(n + 2);
+        // Page n, while the next one's codes (in c) go to the other buffer and the one
+        // after next's are on their way: c takes the third.
+        auto step = [&](Codes& codes, int n) {
+            if (n + 1 < last) convert(codes, n + 1);
+            load(codes, n + 3);
             const int id = id_of(n);
             if (id >= 0 && id < a.n_pages && n * kPage < x.hi) {
                 const uint8_t* base = buffer(n);
@@ -883,6 +911,18 @@ __device__ __forceinline__ void attend_wide(const AttnArgs& a, const Unit& u, in
                              a.v_pages + ((size_t)id * n_kv + head) * kPageBytes + c * 64 + g4 * 16);
             }
             lds_barrier();
+        };
+        load(c0, first);
+        if (threadIdx.x < 2) nan_page[threadIdx.x] = -1;
+        lds_barrier();          // (the last block's pages are read)
+        convert(c0, first);
+        load(c0, first + 1);
+        load(c1, first + 2);
+        lds_barrier();
+        for (int n = first; n < last; n += 2) {
+            step(c0, n);
+            if (n + 1 >= last) break;
+            step(c1, n + 1);
         }
     }
     x.store(a, u, head, 0, 8);
