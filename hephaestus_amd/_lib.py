@@ -110,6 +110,7 @@ SIGNATURES = {
 
 ATTN_MAX_KEYS = 262144
 PAGE_KEYS = 64
+PAGES_MAX_SEQS = 1024
 # HEPH_ABI_VERSION of include/hephfp8.h that these signatures follow
 ABI_VERSION = 6
 

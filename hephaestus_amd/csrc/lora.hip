@@ -445,7 +445,8 @@ __global__ __launch_bounds__(256) void expand_kernel(LoraArgs g)
         for (int e = 0; e < 8; ++e) {
             const float v = there ? s[e / 4][e % 4] * scale : 0.0f;
             hi[e] = (__bf16)v;
-            lo[e] = (__bf16)(v - (float)hi[e]);
+            // (an infinity has no remainder: inf - inf would make it NaN)
+            lo[e] = (__bf16)(__builtin_isinf((float)hi[e]) ? 0.0f : v - (float)hi[e]);
         }
         if constexpr (F == 0) {
             lds[i][0][0][ul] = ul < 32 ? hi : lo;

@@ -337,7 +337,7 @@ __global__ __launch_bounds__(kMaxSeqs) void plan_kernel(PlanArgs a)
         for (int r = x.tiles - 1; r >= 0; --r) {
             const Cut c = cut_tile(x, rounds, G, r);
             for (int k = 0; k < c.chunks; ++k, ++u)
-                if (u < max_units)
+                if ((unsigned)u < (unsigned)max_units)     // (wrapped where q_start falls)
                     units[u] = Unit{x.seq, x.tok0, r * x.tile, rows_in(x, r),
                                     x.page0 + k * c.per, min(c.per, x.pages - k * c.per), k, prefix};
         }
@@ -714,7 +714,8 @@ struct Rows {
             } else {
                 const long part = (u.prefix ? tk.prefix + u.part * tk.prefix_step : tk.own + u.part * tk.own_step) +
                                   (hd[r] - head * a.s.group());
-                if (part >= a.s.max_parts()) continue;          // (a plan never asks for it)
+                // (only where a falling q_start made the plan's counts wrap)
+                if ((unsigned long)part >= (unsigned long)a.s.max_parts()) continue;
                 const size_t slot = (size_t)head * a.s.max_parts() + part;
                 if (g4 == 0 && d0 == 0) a.part_ml[slot] = make_float2(m[r], sum[r][0]);
 #pragma unroll
@@ -862,8 +863,10 @@ __device__ __forceinline__ void attend_wide(const AttnArgs& a, const Unit& u, in
     end = __builtin_amdgcn_readfirstlane(end);
     if (l == 0) lows[wave] = x.lo;
     __syncthreads();
-    // pages that some row does not see all of: their V goes to LDS without NaN
+    // Pages that some row of any wave does not see all of: their V goes to LDS without NaN,
+    // and every wave has to look for those that its rows see.
     const int lo = __builtin_amdgcn_readfirstlane(min(min(lows[0], lows[1]), min(lows[2], lows[3])));
+    x.lo = lo;
     const float sc = a.kv_scale[head] * (0.08838834764831845f * 1.4426950408889634f);
     // waves 0, 1: K's 1 KB tiles 0..3, 4..7; waves 2, 3: V's
     const uint8_t* pool = (wave < 2 ? a.k_pages : a.v_pages) + (wave & 1) * 4096 + c * 64 + g4 * 16;
@@ -951,7 +954,7 @@ __device__ __forceinline__ void merge_row(const AttnArgs& a, long row, int l)
     auto slot = [&](int k) {
         const long part = (k < tk.n_prefix ? tk.prefix + k * tk.prefix_step
                                            : tk.own + (k - tk.n_prefix) * tk.own_step) + h % G;
-        return (size_t)(h / G) * max_parts + (part < max_parts ? part : 0);
+        return (size_t)(h / G) * max_parts + ((unsigned long)part < (unsigned long)max_parts ? part : 0);
     };
     float2 ml[2];
     float top = -INFINITY;

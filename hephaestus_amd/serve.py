@@ -177,6 +177,8 @@ def attention_pages(out, q, k_pages, v_pages, kv_scale, page_table, plan: Attent
     table_pages]."""
     p = plan
     dev, stream = _at(ctx)
+    if k_pages.dim() != 5:
+        raise ValueError(f"k_pages of shape {tuple(k_pages.shape)} is not one layer's pool")
     if page_table.shape != (p.n_seqs, p.table_pages):
         raise ValueError(f"page_table of shape {tuple(page_table.shape)} is not "
                          f"[{p.n_seqs}, {p.table_pages}] as planned")
@@ -241,6 +243,9 @@ def lora_add(c, base, x, a, b, scale, plan: LoraPlan, ctx=None) -> None:
     if c.dtype not in HK._OUT or base.dtype != c.dtype:
         raise TypeError(f"lora_add: c {c.dtype} and base {base.dtype} not supported")
     rank, k, n, dt = sa[1], sa[2], sb[1], (c.dtype,)
+    for t, name, width in ((c, "c", n), (base, "base", n), (x, "x", k)):
+        if t.dim() > 1 and t.shape[-1] != width:
+            raise ValueError(f"{name} of shape {tuple(t.shape)} has no rows of {width}")
     dev, stream = _at(ctx)
     _call("heph_lora_add", _dev(c, "c", dt, m * n, dev), HK._OUT[c.dtype],
           _dev(base, "base", dt, m * n, dev), _dev(x, "x", _BF16, m * k, dev),
@@ -266,7 +271,8 @@ class PagedKVCache:
     2, 64, 64] and v [n_layers, n_pages, n_kv, 128, 64], f32 scales [n_layers,
     2*n_kv] and their reciprocals, and which sequence holds which page. A page
     may belong to several sequences (a shared prefix): it is freed with the
-    last of them."""
+    last of them. Page copies run on the current stream (or ctx's); steps on other
+    streams are ordered by the caller."""
 
     def __init__(self, cfg: Qwen3Config, n_pages: int, device="cuda"):
         if cfg.head_dim != 128:
@@ -332,6 +338,13 @@ class PagedKVCache:
             raise ValueError(f"{n} forks")
         full = seq.length // PAGE
         tails = self._take(n if seq.length % PAGE else 0)
+        if tails:
+            try:
+                copy_pages(self.k, self.v, [seq.pages[full]] * n, tails, ctx)
+            except Exception:
+                for p in tails:
+                    self._drop(p)
+                raise
         made = []
         for i in range(n):
             s = self.new()
@@ -339,8 +352,6 @@ class PagedKVCache:
             for p in seq.pages[:full]:
                 self._users[p] += 1
             made.append(s)
-        if tails:
-            copy_pages(self.k, self.v, [seq.pages[full]] * n, tails, ctx)
         return made
 
     def free(self, seq: Sequence) -> None:
@@ -432,14 +443,21 @@ class Qwen3BatchDecoder:
              adapters: list[int] | None = None) -> torch.Tensor:
         """tokens[i] (one or more) enter sequence seqs[i], with adapter
         adapters[i] (-1: none). Returns the f32 logits [len(seqs), vocab] after
-        each sequence's last token."""
-        cfg, w, kv = self.w.cfg, self.w, self.kv
+        each sequence's last token. A step that raises leaves the sequences as
+        they were."""
+        cfg, kv = self.w.cfg, self.kv
         if len(tokens) != len(seqs) or not seqs or any(len(t) < 1 for t in tokens):
             raise ValueError("every sequence brings one token or more")
         if len({id(s) for s in seqs}) != len(seqs):
             raise ValueError("a sequence appears twice")
         if adapters is not None and (self.lora is None or len(adapters) != len(seqs)):
             raise ValueError("adapters without weights, or not one a sequence")
+        if len(seqs) > L.PAGES_MAX_SEQS:
+            raise ValueError(f"{len(seqs)} sequences > {L.PAGES_MAX_SEQS}")
+        if any(not 0 <= i < cfg.vocab for t in tokens for i in t):
+            raise ValueError(f"a token outside the vocabulary of {cfg.vocab}")
+        if adapters is not None and any(not -1 <= a < self.lora.n_adapters for a in adapters):
+            raise ValueError(f"an adapter outside the {self.lora.n_adapters} that there are")
         need = 0
         for t, s in zip(tokens, seqs):
             kv._own(s)
@@ -449,6 +467,18 @@ class Qwen3BatchDecoder:
             need += -(-(s.length + len(t)) // PAGE) - len(s.pages)
         if need > kv.free_pages:
             raise MemoryError(f"{need} pages wanted, {kv.free_pages} free")
+        before = [(s, s.length, len(s.pages)) for s in seqs]
+        try:
+            return self._run(tokens, seqs, adapters)
+        except Exception:
+            for s, length, pages in before:
+                for p in s.pages[pages:]:
+                    kv._drop(p)
+                s.length, s.pages = length, s.pages[:pages]
+            raise
+
+    def _run(self, tokens, seqs, adapters) -> torch.Tensor:
+        cfg, w, kv = self.w.cfg, self.w, self.kv
         flat = [i for t in tokens for i in t]
         positions = [s.length + i for t, s in zip(tokens, seqs) for i in range(len(t))]
         slots = [i for t, s in zip(tokens, seqs) for i in kv.extend(s, len(t))]

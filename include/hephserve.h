@@ -53,12 +53,13 @@ int heph_rope_table_f32(float* table, int n_pos, int head_dim, double theta, voi
  * multiples of 8): per-head RMSNorm of q (q_gamma) and k (k_gamma) and the
  * rotation of both by rope_table's row positions[t], q to q_out + t * q_stride
  * ([n_heads, 128] bf16); k and v as e4m3(clamp(x * kv_inv_scale[h], +-448))
- * into slot slots[t] of the pools (kv_inv_scale: n_kv_heads K entries, then V).
+ * into slot slots[t] of the pools (kv_inv_scale: n_kv_heads K entries, then V; a
+ * NaN is clamped to -448, as heph_qk_norm_rope_kv does).
  * Norm and rotation are computed in f32 and rounded once (heph_qk_norm_rope_kv
  * rounds every step to bf16, as the reference's single-token path does).
  * A token whose position is outside [0, n_rope_pos) is skipped: its q and its
  * slot stay as they were (padding rows: position -1). A slot outside
- * [0, 64 * n_pages) is not written; q is. The slots of a call's tokens are
+ * [0, 64 * n_pages) is not written; q is. n_pages < 2^25. The slots of a call's tokens are
  * distinct. q_out may be qkv itself with the same stride (q in place), and
  * overlaps it in no other way.
  * Replaces, for a batch, the q/k norms, rotation and cache write of the

@@ -254,7 +254,8 @@ def run_attention(b, plan=None, fill=7.0):
     return out
 
 
-def check_attention(b, out):
+def check_attention(b, out, tokens=None):
+    """All rows of out, or those of some tokens."""
     H, KV, G = b["H"], b["KV"], b["H"] // b["KV"]
     table, n_pages = b["table"].cpu(), b["k"].shape[0]
     sk, sv = f64(b["scale"])[:KV], f64(b["scale"])[KV:]
@@ -267,6 +268,9 @@ def check_attention(b, out):
         ks = k_rows(b["k"][ids])[:total] * sk[:, None]
         vs = v_rows(b["v"][ids])[:total] * sv[:, None]
         for i in range(n):
+            if tokens is not None and t not in tokens:
+                t += 1
+                continue
             see = ok & (torch.arange(total) <= total - n + i)
             q = f64(b["q"][t]).view(KV, G, D)
             x = torch.einsum("kgd,jkd->kgj", q, ks[see]) / math.sqrt(D)
@@ -369,6 +373,165 @@ def test_attention_bad_metadata():
     plan = make_plan(b)
     run_attention(b, plan)
     torch.cuda.synchronize()
+
+
+def same_pages(n_seqs, new, keys, H, KV, seed):
+    """n_seqs sequences on the same pages, each with `new` tokens: long runs in a small pool."""
+    b = batch([new], [keys], seed=seed, H=H, KV=KV, garbage=False)
+    g = torch.Generator(device="cuda").manual_seed(seed + 1)
+    T = n_seqs * new
+    b.update(new=[new] * n_seqs, kv_len=[keys] * n_seqs, table=b["table"].repeat(n_seqs, 1), T=T,
+             q=torch.randn(T, H, D, generator=g, device="cuda").to(torch.bfloat16),
+             q_start=(torch.arange(n_seqs + 1) * new).int().cuda(),
+             lens=torch.full((n_seqs,), keys, dtype=torch.int32, device="cuda"))
+    return b
+
+
+def test_attention_units_of_more_than_64_pages():
+    # narrow: 40 sequences in the 64 slots of a kv head, 130 pages each
+    b = same_pages(40, 1, 64 * 130 - 7, 8, 8, seed=30)
+    b["table"][3, 70] = -1                               # a page left out behind the first 64
+    check_attention(b, run_attention(b), tokens=[0, 3, 39])
+    # wide: nine tiles in the eight slots, eight whole and the last one cut
+    b = same_pages(3, 300, 64 * 150 - 20, 64, 64, seed=31)
+    b["table"][1, [0, 65, 149]] = torch.tensor([-1, 10 ** 6, -7], dtype=torch.int32, device="cuda")
+    check_attention(b, run_attention(b), tokens=[0, 127, 128, 299, 300, 555, 599, 600, 899])
+
+
+def test_attention_wide_tiles_split_over_pages():
+    # few tiles, long runs: units of a tile meet again in the merge
+    for new, keys, H, KV in ((128, 64 * 40, 8, 2), (65, 64 * 33 + 1, 4, 4), (40, 5000, 28, 4)):
+        b = batch([new, 1], [keys, 700], seed=new, H=H, KV=KV)
+        check_attention(b, run_attention(b), tokens=[0, 1, new // 2, new - 1, new])
+
+
+def test_attention_nan_and_bad_pages_in_wide_tiles():
+    # a NaN in V behind one tile's edge, in a page that the run's other rows see, and
+    # beside pages left out
+    b = batch([150], [64 * 80], seed=33, H=8, KV=2)
+    edges = []
+    for key, dim in ((64 * 80 - 149, 5), (64 * 80 - 100, 77), (64 * 80 - 2, 127)):
+        page = int(b["table"][0, key // PAGE])
+        b["v"][page, 1, dim, S.v_place(key % PAGE)] = 0xFF
+        edges.append((key - (64 * 80 - 150), dim))
+    for p in (2, 66):
+        b["table"][0, p] = -1
+    out = run_attention(b).float()
+    t = torch.arange(150, device="cuda")
+    nan = torch.zeros(150, 8, D, dtype=torch.bool, device="cuda")
+    for first, dim in edges:
+        nan[t >= first, 4:, dim] = True
+    assert torch.equal(torch.isnan(out), nan)
+    for key, dim in ((64 * 80 - 149, 5), (64 * 80 - 100, 77), (64 * 80 - 2, 127)):
+        b["v"][int(b["table"][0, key // PAGE]), 1, dim, S.v_place(key % PAGE)] = 0
+    # (a code in place of the NaN: only rows that do not see it are compared)
+    want = run_attention(b).float()
+    assert torch.equal(out[~nan], want[~nan])
+    check_attention(b, run_attention(b), tokens=[0, 60, 149])
+    # a NaN key reaches all dims of the heads of its kv head, where it is seen
+    key = 64 * 80 - 50
+    b["k"][int(b["table"][0, key // PAGE]), 0, 1, key % PAGE, 3] = 0x7F
+    out = run_attention(b)
+    assert torch.isnan(out[100:, :4]).all() and torch.isfinite(out[:100]).all()
+    assert torch.isfinite(out[100:, 4:]).all()
+
+
+@pytest.mark.parametrize("n,G", [(1024, 1), (1024, 1024), (333, 70)])
+def test_attention_many_sequences(n, G):
+    rng = np.random.default_rng(n + G)
+    own = [int(x) for x in rng.integers(1, 90, n)]
+    cuts = sorted(int(x) for x in rng.integers(0, n + 1, G - 1))
+    group_start = [0] + cuts + [n]
+    shared = [int(x) for x in rng.integers(0, 4, G)]
+    new = [min(o, int(x)) for o, x in zip(own, rng.integers(1, 4, n))]
+    b = batch(new, own, shared, group_start, seed=n, H=4, KV=1)
+    check_attention(b, run_attention(b), tokens=set(rng.integers(0, b["T"], 150).tolist()))
+
+
+def test_attention_falling_starts_stay_in_bounds():
+    # every second sequence has all the tokens, many times the rows that the plan was sized for
+    b = batch([1] * 64 + [0] * 64, [64 * 3] * 128, seed=35, H=64, KV=1, garbage=False)
+    b["q_start"] = torch.tensor([0, 64] * 64 + [0], dtype=torch.int32).cuda()
+    plan = make_plan(b)
+    guard = plan.ws.clone()
+    extra = torch.full((1 << 20,), 0x5A, dtype=torch.uint8, device="cuda")
+    plan.ws = torch.cat([guard, extra])
+    kept, plan.plan = plan.plan, torch.cat([plan.plan, extra])
+    plan.update(b["q_start"], b["lens"])
+    run_attention(b, plan)
+    torch.cuda.synchronize()
+    assert (plan.ws[guard.numel():] == 0x5A).all() and (plan.plan[kept.numel():] == 0x5A).all()
+
+
+def test_attention_pools_past_32_bits():
+    # the last pages of pools of 5 GiB each, through all the ops that address them
+    KV, n_pages = 8, (5 << 30) // (8 * 8192)
+    k = torch.empty(1, n_pages, KV, 2, PAGE, 64, dtype=torch.uint8, device="cuda")
+    v = torch.empty(1, n_pages, KV, D, PAGE, dtype=torch.uint8, device="cuda")
+    small = batch([1, 40], [300, 200], seed=36, H=32, KV=KV, garbage=False)
+    used = small["k"].shape[0]
+    at = n_pages - used
+    k[0, at:], v[0, at:] = small["k"], small["v"]
+    far = dict(small, k=k[0], v=v[0], table=torch.where(small["table"] < 0, small["table"], small["table"] + at))
+    assert torch.equal(run_attention(far), run_attention(small))
+    S.copy_pages(k, v, list(range(at, n_pages)), list(range(used)))
+    assert torch.equal(k[0, :used], small["k"]) and torch.equal(v[0, :used], small["v"])
+    S.copy_pages(k, v, list(range(used)), list(range(at - used, at)))
+    assert torch.equal(k[0, at - used:at], small["k"]) and torch.equal(v[0, at - used:at], small["v"])
+    for T in (5, 600):
+        c = qk_case(T, 32, KV, seed=37)
+        lo = c["k"].shape[0]
+        rope = S.rope_table_f32(c["n_pos"])
+        for kk, vv, base in ((c["k"], c["v"], 0), (k[0], v[0], n_pages - lo)):
+            kk[base:base + lo], vv[base:base + lo] = 0, 0
+            S.qk_norm_rope_pages(c["q"], c["qkv"], *c["gam"], kk, vv, c["inv"], rope, c["pos"],
+                                 c["slot"] + base * PAGE)
+        assert torch.equal(k[0, -lo:], c["k"]) and torch.equal(v[0, -lo:], c["v"])
+
+
+def test_two_plans_on_two_streams_at_once():
+    bs = [batch([1] * 30, [100 * i + 1 for i in range(30)], [12], [0, 30], seed=38),
+          batch([200, 3], [2000, 64], seed=39)]
+    want = [run_attention(b) for b in bs]
+    plans = [make_plan(b) for b in bs]
+    outs = [[torch.zeros_like(w) for _ in range(8)] for w in want]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in bs]
+    for i in range(8):
+        for b, p, o, s in zip(bs, plans, outs, streams):
+            with torch.cuda.stream(s):
+                p.update(b["q_start"], b["lens"], b["group_start"], b["shared"])
+                S.attention_pages(o[i], b["q"], b["k"], b["v"], b["scale"], b["table"], p)
+    torch.cuda.synchronize()
+    for w, os in zip(want, outs):
+        for o in os:
+            assert torch.equal(o, w)
+
+
+def test_two_graphs_share_a_plan():
+    # captured apart, replayed in turn on one stream, with eager calls of the same plan between
+    bs = [batch([1] * 6, own, [5], [0, 6], seed=40) for own in ([1, 64, 200, 7, 900, 65], [3] * 6)]
+    bs[1]["table"] = torch.nn.functional.pad(
+        bs[1]["table"], (0, bs[0]["table"].shape[1] - bs[1]["table"].shape[1]), value=-1)
+    want = [run_attention(b) for b in bs]
+    plan, graphs, outs = make_plan(bs[0]), [], [torch.zeros_like(w) for w in want]
+    torch.cuda.synchronize()
+    for b, o in zip(bs, outs):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            plan.update(b["q_start"], b["lens"], b["group_start"], b["shared"])
+            S.attention_pages(o, b["q"], b["k"], b["v"], b["scale"], b["table"], plan)
+    for i in range(6):
+        for o in outs:
+            o.zero_()
+        graphs[i % 2].replay()
+        graphs[1 - i % 2].replay()
+        if i % 3 == 0:
+            plan.update(bs[0]["q_start"], bs[0]["lens"], bs[0]["group_start"], bs[0]["shared"])
+            assert torch.equal(run_attention(bs[0], plan), want[0])
+        torch.cuda.synchronize()
+        for o, w in zip(outs, want):
+            assert torch.equal(o, w)
 
 
 def test_attention_rows_behind_the_last_sequence():
@@ -570,6 +733,62 @@ def check_lora(c, in_place=False, plan=None):
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_lora_add(M, N, K, r, A, dtype):
     check_lora(lora_case(M, N, K, r, A, seed=M + N, dtype=dtype))
+
+
+@pytest.mark.parametrize("M,N,K,r,A", [
+    (2200, 48, 272, 16, 3), (1030, 1040, 976, 24, 4096), (700, 4096, 64, 128, 1), (4096, 16, 48, 40, 2),
+    (256, 528, 976, 64, 2000), (513, 6144, 4112, 8, 2),
+])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_lora_long_batches_and_many_adapters(M, N, K, r, A, dtype):
+    if A > 1000:                      # (adapters beyond the few that are used need no values)
+        c = lora_case(M, 16, 16, 8, A, seed=M, dtype=dtype)
+        few = lora_case(M, N, K, r, 5, seed=M, dtype=dtype)
+        far = torch.tensor([0, 17, 1000, A - 2, A - 1], device="cuda")
+        c["a"] = torch.zeros(A, r, K, dtype=torch.bfloat16, device="cuda").index_copy_(0, far, few["a"])
+        c["b"] = torch.zeros(A, N, r, dtype=torch.bfloat16, device="cuda").index_copy_(0, far, few["b"])
+        c["ids"] = torch.where(few["ids"] < 0, -1, far[few["ids"].clamp(min=0).long()].int()).contiguous()
+        c["x"], c["base"] = few["x"], few["base"]
+        check_lora(c)
+    else:
+        check_lora(lora_case(M, N, K, r, A, seed=M, dtype=dtype), in_place=True)
+
+
+def test_lora_infinite_products():
+    # t of one rank overflows: an infinity of b's sign there, no NaN
+    c = lora_case(20, 96, 256, 16, 2, seed=9, ids=[0] * 20)
+    c["x"].zero_()
+    c["a"].zero_()
+    c["x"][4, 9], c["a"][0, 3, 9] = 3e38, 8.0
+    plan = S.LoraPlan(20, 2, 16, 256)
+    plan.update(c["ids"])
+    out = torch.empty_like(c["base"])
+    S.lora_add(out, c["base"], c["x"], c["a"], c["b"], c["scale"], plan)
+    assert torch.equal(out[4].float(), torch.sign(c["b"][0, :, 3].float()) * float("inf"))
+    rest = torch.arange(20) != 4
+    assert torch.equal(out[rest], c["base"][rest])
+
+
+def test_lora_on_two_streams_at_once():
+    cs = [lora_case(500, 512, 1024, 16, 4, seed=10), lora_case(9, 2560, 4096, 64, 3, seed=11)]
+    plans, outs, want = [], [], []
+    for c in cs:
+        M, K = c["x"].shape
+        A, N, r = c["b"].shape
+        plans.append(S.LoraPlan(M, A, r, K))
+        want.append(check_lora(c))
+        outs.append([torch.zeros_like(want[-1]) for _ in range(8)])
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cs]
+    for i in range(8):
+        for c, p, o, s in zip(cs, plans, outs, streams):
+            with torch.cuda.stream(s):
+                p.update(c["ids"])
+                S.lora_add(o[i], c["base"], c["x"], c["a"], c["b"], c["scale"], p)
+    torch.cuda.synchronize()
+    for w, os in zip(want, outs):
+        for o in os:
+            assert torch.equal(o, w)
 
 
 @pytest.mark.parametrize("ids", [[-1] * 20, [0] * 20, [3, -1, 7, 2 ** 31 - 1, -2 ** 31] * 4,

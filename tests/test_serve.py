@@ -1,5 +1,6 @@
 """The serving ops' argument checks and the page bookkeeping, without a GPU."""
 import ctypes
+from types import SimpleNamespace
 
 import numpy as np
 import pytest
@@ -152,11 +153,28 @@ def test_python_rejects_host_tensors(monkeypatch):
                              torch.ones(4), torch.zeros(4, 64, 2), i, i)
     with pytest.raises(ValueError):
         S.copy_pages(k[None], v[None], [0], [1])
+    with pytest.raises(ValueError, match="one layer"):
+        S.attention_pages(t, t, k[None], v[None], torch.ones(4), i, SimpleNamespace())
     with pytest.raises(ValueError):
         plan = S.LoraPlan.__new__(S.LoraPlan)                  # (without its device buffers)
         plan.m, plan.n_adapters = 2, 2
         S.lora_add(t[0], t[0], t[0], torch.zeros(2, 8, 128, dtype=torch.bfloat16),
                    torch.zeros(2, 128, 8, dtype=torch.bfloat16), torch.ones(2), plan)
+    for n, k in ((64, 128), (128, 64)):                        # rows of another width than c's, x's
+        with pytest.raises(ValueError, match="no rows of"):
+            S.lora_add(t[0], t[0], t[0], torch.zeros(2, 8, k, dtype=torch.bfloat16),
+                       torch.zeros(2, n, 8, dtype=torch.bfloat16), torch.ones(2), plan)
+
+
+def test_attention_buffers_of_extreme_batches(lib):
+    plan, ws = lib.heph_pages_attention_plan_bytes, lib.heph_pages_attention_ws_bytes
+    for sizes in ((1, 1, 0, 1, 1), (1024, 1024, 1024, 64, 1), (1 << 20, 1024, 3, 4096, 64), (7, 3, 1, 96, 96)):
+        T, n_seqs, G, H, KV = sizes
+        # at least a token's entry, a row's partial result behind a prefix and its own
+        assert plan(*sizes) > 32 * T and ws(*sizes) >= 2 * T * H * (128 * 4 + 8)
+    for sizes in ((0, 1, 0, 8, 8), (1, 0, 0, 8, 8), (1, 1025, 0, 8, 8), (1, 1, 2, 8, 8), (1, 1, -1, 8, 8),
+                  ((1 << 20) + 1, 1, 0, 8, 8), (1, 1, 0, 130, 2), (1, 1, 0, 4160, 65), (1, 1, 0, 7, 2)):
+        assert plan(*sizes) == 0 and ws(*sizes) == 0
 
 
 def test_v_place_is_a_permutation_that_keeps_runs_of_four():
@@ -264,6 +282,51 @@ def test_bookkeeping_refusals(cache):
             f(a)
     with pytest.raises(ValueError):
         S.PagedKVCache(CFG, 0, device="cpu")
+
+
+def test_a_fork_whose_copy_fails_changes_nothing(cache, monkeypatch):
+    c = cache
+    a = c.new()
+    c.extend(a, 70)
+
+    def fails(*args):
+        raise S.HephError(L.HEPH_ERR_LAUNCH, "heph_copy_pages")
+    monkeypatch.setattr(S, "copy_pages", fails)
+    with pytest.raises(S.HephError):
+        c.fork(a, 3)
+    assert len(c._seqs) == 1 and c.free_pages == 10
+    check_counts(c)
+
+
+def test_step_refusals_leave_the_sequences(cache, monkeypatch):
+    c = cache
+    w = SimpleNamespace(cfg=CFG, embed=SimpleNamespace(block=True, w=torch.zeros(1)),
+                        layers=[None] * CFG.n_layers)
+    monkeypatch.setattr(S, "rope_table_f32", lambda n, theta, device: torch.zeros(n, 64, 2))
+    lora = S.LoraWeights(torch.ones(3), [{}] * CFG.n_layers)
+    d = S.Qwen3BatchDecoder(w, c, n_pos=300, lora=lora)
+    a, b, other = c.new(), c.new(), S.PagedKVCache(CFG, 2, device="cpu").new()
+    c.extend(a, 70)
+    for tokens, seqs, adapters, error in (
+            ([], [], None, ValueError), ([[1]], [a, b], None, ValueError),
+            ([[1], []], [a, b], None, ValueError), ([[1], [2]], [a, a], None, ValueError),
+            ([[1]], [other], None, ValueError), ([[512]], [a], None, ValueError),
+            ([[1, -1]], [a], None, ValueError), ([[1]], [a], [0, 1], ValueError),
+            ([[1]], [a], [3], ValueError), ([[1]], [a], [-2], ValueError),
+            ([[0] * 231], [a], None, ValueError),                     # past the rotation table
+            ([[0] * 230, [0] * 290], [a, b], [0, -1], None)):         # fails in its first launch
+        def launches(*args):
+            raise S.HephError(L.HEPH_ERR_LAUNCH, "step")
+        monkeypatch.setattr(d, "_run", lambda t, s, ad: ([c.extend(i, len(j)) for i, j in zip(s, t)],
+                                                         launches()))
+        with pytest.raises(error or S.HephError):
+            d.step(tokens, seqs, adapters)
+        assert (a.length, b.length, len(a.pages), b.pages, c.free_pages) == (70, 0, 2, [], 10)
+        check_counts(c)
+    c.extend(b, 10 * 64)
+    with pytest.raises(MemoryError):
+        d.step([[0] * 100], [a])
+    check_counts(c)
 
 
 def test_random_use_keeps_every_sequence(cache):
