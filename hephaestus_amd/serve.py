@@ -33,6 +33,9 @@ _U8 = (torch.uint8, torch.float8_e4m3fn)
 _I32, _BF16, _F32 = (torch.int32,), (torch.bfloat16,), (torch.float32,)
 
 
+# The checks run before every call of a decode step: one look at each property, and the
+# words of a refusal only where there is one.
+
 def _dev(t, name: str, dtypes, numel: int, dev: int) -> int:
     """Pointer of a contiguous tensor on device dev with at least numel elements."""
     if isinstance(t, torch.Tensor) and t.dtype in dtypes and t.get_device() == dev and \
@@ -53,14 +56,32 @@ def _rows(t, name: str, n: int, width: int, dev: int) -> tuple[int, int]:
         raise ValueError(f"{name} must be in the current device's memory (got {t.device})")
     if t.dtype != torch.bfloat16:
         raise TypeError(f"{name} has dtype {t.dtype}, expected torch.bfloat16")
-    if t.dim() >= 2 and t.shape[0] >= n:
+    shape = t.shape
+    if len(shape) >= 2 and shape[0] >= n:
         if t.is_contiguous():
-            if t.numel() == t.shape[0] * width:
+            if t.numel() == shape[0] * width:
                 return t.data_ptr(), width
-        elif t[0].numel() == width and t[0].is_contiguous():
-            return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else width
-    raise ValueError(f"{name} of shape {tuple(t.shape)} is not {n} rows of {width} "
+        else:
+            strides, run = t.stride(), 1
+            for i in range(len(shape) - 1, 0, -1):
+                if strides[i] != run and shape[i] != 1:
+                    break
+                run *= shape[i]
+            else:
+                if run == width:
+                    return t.data_ptr(), strides[0] if shape[0] > 1 else width
+    raise ValueError(f"{name} of shape {tuple(shape)} is not {n} rows of {width} "
                      "consecutive values")
+
+
+def _matrix(t, name: str, dtypes, m: int, n: int, dev: int) -> int:
+    """Pointer of a contiguous [m, n] tensor, or of a larger or flat buffer in its place."""
+    if isinstance(t, torch.Tensor) and t.shape == (m, n) and t.dtype in dtypes and \
+            t.get_device() == dev and t.is_contiguous():
+        return t.data_ptr()
+    if isinstance(t, torch.Tensor) and t.dim() > 1 and t.shape[-1] != n:
+        raise ValueError(f"{name} of shape {tuple(t.shape)} has no rows of {n}")
+    return _dev(t, name, dtypes, m * n, dev)
 
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
@@ -96,13 +117,12 @@ def rope_table_f32(n_pos: int, theta: float = 1e6, device="cuda", ctx=None) -> t
     return t
 
 
-def _pools(k_pages, v_pages, n_kv: int, dev: int) -> tuple[int, int, int]:
-    """Pointers of the K and V pools and how many pages a layer of them has."""
-    ks = k_pages.shape
-    if len(ks) < 5 or ks[-4:] != (n_kv, 2, PAGE, 64) or v_pages.shape != ks[:-3] + (128, PAGE):
+def _pools(k_pages, v_pages, lead: tuple, dev: int) -> tuple[int, int]:
+    """Pointers of the K and V pools [*lead, ...], lead ending with n_pages and n_kv."""
+    if k_pages.shape != lead + (2, PAGE, 64) or v_pages.shape != lead + (128, PAGE):
         raise ValueError(f"pools of shapes {tuple(k_pages.shape)} and {tuple(v_pages.shape)} are "
-                         f"not [n_pages, {n_kv}, 2, 64, 64] and [n_pages, {n_kv}, 128, 64]")
-    return _dev(k_pages, "k_pages", _U8, 0, dev), _dev(v_pages, "v_pages", _U8, 0, dev), ks[-5]
+                         f"not {list(lead)} pages and heads of [2, 64, 64] and [128, 64]")
+    return _dev(k_pages, "k_pages", _U8, 0, dev), _dev(v_pages, "v_pages", _U8, 0, dev)
 
 
 def qk_norm_rope_pages(q_out, qkv, q_gamma, k_gamma, k_pages, v_pages, kv_inv, rope, positions,
@@ -114,23 +134,35 @@ def qk_norm_rope_pages(q_out, qkv, q_gamma, k_gamma, k_pages, v_pages, kv_inv, r
     rows may lie apart; q_out may be qkv[:, :n_heads]. A position outside
     rope skips the token, a slot outside the pools the cache write."""
     dev, stream = _at(ctx)
-    if q_out.dim() != 3 or q_out.shape[2] != 128 or k_pages.dim() != 5:
-        raise ValueError(f"q_out of shape {tuple(q_out.shape)} and k_pages of shape "
-                         f"{tuple(k_pages.shape)} are not [n_tok, n_heads, 128] and one layer's pool")
-    n_tok, n_heads = q_out.shape[0], q_out.shape[1]
-    n_kv = k_pages.shape[1]
+    qs, ks, rs = q_out.shape, k_pages.shape, rope.shape
+    if len(qs) != 3 or qs[2] != 128 or len(ks) != 5:
+        raise ValueError(f"q_out of shape {tuple(qs)} and k_pages of shape {tuple(ks)} are not "
+                         "[n_tok, n_heads, 128] and one layer's pool")
+    n_tok, n_heads, n_pages, n_kv = qs[0], qs[1], ks[0], ks[1]
     qp, qs = _rows(q_out, "q_out", n_tok, n_heads * 128, dev)
     xp, xs = _rows(qkv, "qkv", n_tok, (n_heads + 2 * n_kv) * 128, dev)
     if n_tok == 1 and qp == xp:
         qs = xs                   # (one row has no stride of its own)
-    kp, vp, n_pages = _pools(k_pages, v_pages, n_kv, dev)
-    if rope.dim() != 3 or rope.shape[1:] != (64, 2):
-        raise ValueError(f"rope of shape {tuple(rope.shape)} is not [n_pos, 64, 2]")
+    kp, vp = _pools(k_pages, v_pages, (n_pages, n_kv), dev)
+    if len(rs) != 3 or rs[1] != 64 or rs[2] != 2:
+        raise ValueError(f"rope of shape {tuple(rs)} is not [n_pos, 64, 2]")
     _call("heph_qk_norm_rope_pages", qp, qs, xp, xs, _dev(q_gamma, "q_gamma", _BF16, 128, dev),
           _dev(k_gamma, "k_gamma", _BF16, 128, dev), kp, vp, n_pages,
           _dev(kv_inv, "kv_inv", _F32, 2 * n_kv, dev), _dev(rope, "rope", _F32, 0, dev),
-          rope.shape[0], _dev(positions, "positions", _I32, n_tok, dev),
+          rs[0], _dev(positions, "positions", _I32, n_tok, dev),
           _dev(slots, "slots", _I32, n_tok, dev), n_tok, n_heads, n_kv, 128, eps, stream)
+
+
+def _bind(p) -> None:
+    """Keeps where a plan's own buffers are."""
+    p._bound = (p.plan.data_ptr(), p.plan.numel(), p.ws.data_ptr(), p.ws.numel())
+    p._dev = p.plan.get_device()
+
+
+def _bound(p, dev: int) -> tuple:
+    if p._dev != dev:
+        raise ValueError(f"the plan is on {p.plan.device}, not on the current device")
+    return p._bound
 
 
 class AttentionPlan:
@@ -151,6 +183,7 @@ class AttentionPlan:
         self.plan = torch.zeros(nb, dtype=torch.uint8, device=device)
         self.ws = torch.empty(L.lib().heph_pages_attention_ws_bytes(*sizes), dtype=torch.uint8,
                               device=device)
+        _bind(self)
 
     def update(self, q_start, kv_len, group_start=None, shared_pages=None, ctx=None) -> None:
         """q_start int32 [n_seqs + 1], kv_len int32 [n_seqs]; with groups
@@ -160,7 +193,8 @@ class AttentionPlan:
             raise ValueError(f"a plan of {self.n_groups} groups "
                              + ("needs" if g else "takes no") + " group_start and shared_pages")
         dev, stream = _at(ctx)
-        _call("heph_pages_attention_plan", _dev(self.plan, "plan", _U8, 0, dev), self.plan.numel(),
+        plan, plan_bytes, _, _ = _bound(self, dev)
+        _call("heph_pages_attention_plan", plan, plan_bytes,
               _dev(q_start, "q_start", _I32, self.n_seqs + 1, dev),
               _dev(kv_len, "kv_len", _I32, self.n_seqs, dev),
               _dev(group_start, "group_start", _I32, self.n_groups + 1, dev) if g else None,
@@ -177,33 +211,32 @@ def attention_pages(out, q, k_pages, v_pages, kv_scale, page_table, plan: Attent
     table_pages]."""
     p = plan
     dev, stream = _at(ctx)
-    if k_pages.dim() != 5:
-        raise ValueError(f"k_pages of shape {tuple(k_pages.shape)} is not one layer's pool")
+    n_pages = len(k_pages)
+    kp, vp = _pools(k_pages, v_pages, (n_pages, p.n_kv), dev)
     if page_table.shape != (p.n_seqs, p.table_pages):
         raise ValueError(f"page_table of shape {tuple(page_table.shape)} is not "
                          f"[{p.n_seqs}, {p.table_pages}] as planned")
     qp, qs = _rows(q, "q", p.n_tok, p.n_heads * 128, dev)
-    kp, vp, n_pages = _pools(k_pages, v_pages, p.n_kv, dev)
     _call("heph_pages_attention", _dev(out, "out", _BF16, p.n_tok * p.n_heads * 128, dev), qp, qs,
           kp, vp, n_pages, _dev(kv_scale, "kv_scale", _F32, 2 * p.n_kv, dev),
           _dev(page_table, "page_table", _I32, 0, dev), p.table_pages,
-          _dev(p.plan, "plan", _U8, 0, dev), p.plan.numel(), _dev(p.ws, "ws", _U8, 0, dev),
-          p.ws.numel(), p.n_tok, p.n_seqs, p.n_groups, p.n_heads, p.n_kv, 128, stream)
+          *_bound(p, dev), p.n_tok, p.n_seqs, p.n_groups, p.n_heads, p.n_kv, 128, stream)
 
 
 def copy_pages(k_pools, v_pools, src, dst, ctx=None) -> None:
     """Page src[i] of every layer copied to page dst[i] in both pools
     [n_layers, n_pages, ...]; src and dst are host lists. A destination may
     neither repeat nor be a source."""
-    if k_pools.dim() != 6:
-        raise ValueError(f"k_pools of shape {tuple(k_pools.shape)} has no layers")
+    ks = k_pools.shape
+    if len(ks) != 6:
+        raise ValueError(f"k_pools of shape {tuple(ks)} has no layers")
     dev, stream = _at(ctx)
-    kp, vp, n_pages = _pools(k_pools, v_pools, k_pools.shape[2], dev)
+    kp, vp = _pools(k_pools, v_pools, tuple(ks[:3]), dev)
     s, d = np.asarray(src, dtype=np.int32).reshape(-1), np.asarray(dst, dtype=np.int32).reshape(-1)
     if s.size != d.size:
         raise ValueError(f"{s.size} sources and {d.size} destinations")
     s, d = np.ascontiguousarray(s), np.ascontiguousarray(d)
-    _call("heph_copy_pages", kp, vp, k_pools.shape[0], n_pages, k_pools.shape[2], s.ctypes.data,
+    _call("heph_copy_pages", kp, vp, *ks[:3], s.ctypes.data,
           d.ctypes.data, s.size, stream)
 
 
@@ -222,11 +255,12 @@ class LoraPlan:
             raise HephError(L.HEPH_ERR_SHAPE, "LoraPlan")
         self.plan = torch.zeros(nb, dtype=torch.uint8, device=device)
         self.ws = torch.empty(wb, dtype=torch.uint8, device=device)
+        _bind(self)
 
     def update(self, ids, ctx=None) -> None:
         dev, stream = _at(ctx)
-        _call("heph_lora_plan", _dev(self.plan, "plan", _U8, 0, dev), self.plan.numel(),
-              _dev(ids, "ids", _I32, self.m, dev), self.m, self.n_adapters, stream)
+        plan, plan_bytes, _, _ = _bound(self, dev)
+        _call("heph_lora_plan", plan, plan_bytes, _dev(ids, "ids", _I32, self.m, dev), self.m, self.n_adapters, stream)
 
 
 def lora_add(c, base, x, a, b, scale, plan: LoraPlan, ctx=None) -> None:
@@ -243,16 +277,11 @@ def lora_add(c, base, x, a, b, scale, plan: LoraPlan, ctx=None) -> None:
     if c.dtype not in HK._OUT or base.dtype != c.dtype:
         raise TypeError(f"lora_add: c {c.dtype} and base {base.dtype} not supported")
     rank, k, n, dt = sa[1], sa[2], sb[1], (c.dtype,)
-    for t, name, width in ((c, "c", n), (base, "base", n), (x, "x", k)):
-        if t.dim() > 1 and t.shape[-1] != width:
-            raise ValueError(f"{name} of shape {tuple(t.shape)} has no rows of {width}")
     dev, stream = _at(ctx)
-    _call("heph_lora_add", _dev(c, "c", dt, m * n, dev), HK._OUT[c.dtype],
-          _dev(base, "base", dt, m * n, dev), _dev(x, "x", _BF16, m * k, dev),
+    _call("heph_lora_add", _matrix(c, "c", dt, m, n, dev), HK._OUT[c.dtype],
+          _matrix(base, "base", dt, m, n, dev), _matrix(x, "x", _BF16, m, k, dev),
           _dev(a, "a", _BF16, 0, dev), _dev(b, "b", _BF16, 0, dev),
-          _dev(scale, "scale", _F32, plan.n_adapters, dev),
-          _dev(plan.plan, "plan", _U8, 0, dev), plan.plan.numel(),
-          _dev(plan.ws, "ws", _U8, 0, dev), plan.ws.numel(), m, n, k, rank, plan.n_adapters,
+          _dev(scale, "scale", _F32, plan.n_adapters, dev), *_bound(plan, dev), m, n, k, rank, plan.n_adapters,
           stream)
 
 

@@ -457,6 +457,7 @@ def test_attention_falling_starts_stay_in_bounds():
     extra = torch.full((1 << 20,), 0x5A, dtype=torch.uint8, device="cuda")
     plan.ws = torch.cat([guard, extra])
     kept, plan.plan = plan.plan, torch.cat([plan.plan, extra])
+    S._bind(plan)
     plan.update(b["q_start"], b["lens"])
     run_attention(b, plan)
     torch.cuda.synchronize()
@@ -1038,3 +1039,14 @@ def test_host_refusals_on_device_tensors():
         S.lora_add(c["base"], c["base"], c["x"], c["a"][:1], c["b"][:1], c["scale"], plan)
     with pytest.raises(TypeError):
         S.lora_add(c["base"], c["base"].float(), c["x"], c["a"], c["b"], c["scale"], plan)
+    with pytest.raises(ValueError, match="x of shape"):
+        S.lora_add(c["base"], c["base"], torch.cat([c["x"], c["x"]], 1), c["a"], c["b"], c["scale"], plan)
+    with pytest.raises(ValueError, match="c of shape"):
+        S.lora_add(c["base"].t().contiguous(), c["base"], c["x"], c["a"], c["b"], c["scale"], plan)
+    plan = make_plan(b)
+    for q in (b["q"].transpose(1, 2).contiguous().transpose(1, 2), b["q"][:, ::2], b["q"][:, :, :64],
+              b["q"].flatten(), b["q"][:1].expand(2, 32, D)):
+        with pytest.raises((ValueError, HephError)):
+            S.attention_pages(out, q, b["k"], b["v"], b["scale"], b["table"], plan)
+    with pytest.raises(ValueError):                       # a pool with a layer dimension
+        S.attention_pages(out, b["q"], k, v, b["scale"], b["table"], plan)

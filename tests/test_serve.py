@@ -153,17 +153,18 @@ def test_python_rejects_host_tensors(monkeypatch):
                              torch.ones(4), torch.zeros(4, 64, 2), i, i)
     with pytest.raises(ValueError):
         S.copy_pages(k[None], v[None], [0], [1])
-    with pytest.raises(ValueError, match="one layer"):
-        S.attention_pages(t, t, k[None], v[None], torch.ones(4), i, SimpleNamespace())
+    with pytest.raises(ValueError, match="pools of shapes"):
+        S.attention_pages(t, t, k[None], v[None], torch.ones(4), i[None], SimpleNamespace(
+            n_seqs=1, table_pages=2, n_tok=2, n_heads=8, n_kv=2))
     with pytest.raises(ValueError):
         plan = S.LoraPlan.__new__(S.LoraPlan)                  # (without its device buffers)
         plan.m, plan.n_adapters = 2, 2
+        plan._dev, plan._bound = 0, (0, 0, 0, 0)
         S.lora_add(t[0], t[0], t[0], torch.zeros(2, 8, 128, dtype=torch.bfloat16),
                    torch.zeros(2, 128, 8, dtype=torch.bfloat16), torch.ones(2), plan)
-    for n, k in ((64, 128), (128, 64)):                        # rows of another width than c's, x's
-        with pytest.raises(ValueError, match="no rows of"):
-            S.lora_add(t[0], t[0], t[0], torch.zeros(2, 8, k, dtype=torch.bfloat16),
-                       torch.zeros(2, n, 8, dtype=torch.bfloat16), torch.ones(2), plan)
+    with pytest.raises(ValueError, match="no rows of 64"):
+        S.lora_add(t[0], t[0], t[0], torch.zeros(2, 8, 128, dtype=torch.bfloat16),
+                   torch.zeros(2, 64, 8, dtype=torch.bfloat16), torch.ones(2), plan)
 
 
 def test_attention_buffers_of_extreme_batches(lib):
