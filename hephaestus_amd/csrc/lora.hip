@@ -615,14 +615,19 @@ int heph_lora_add(void* c, int c_dtype, const void* base, const uint16_t* x_bf16
         ws_bytes < heph_lora_ws_bytes(M, n_adapters, K, rank))
         return HEPH_ERR_WORKSPACE;
     const int tiles = max_tiles(M, n_adapters), splits = k_splits(M, n_adapters, K);
-    // Columns a workgroup: few enough for two workgroups a CU, each of which joins the
-    // parts of t for itself; whole rounds of its four waves.
+    // Columns a workgroup, each of which joins the parts of t for itself: for four workgroups
+    // a CU of decode tiles (two: 64 rows of 40 adapters, 2560 -> 19456, 13.7 us instead of
+    // 12.3), six of a prompt's, but then 256 columns each while these fill half of the device
+    // (two: 4090 rows -> 19456 111 us, 96; 128 columns: 1000 rows of rank 128 49 us, 39). A
+    // wave takes all its steps at once where there are rounds of them, in a prompt two.
     const bool f32 = c_dtype == HEPH_DTYPE_F32, decode = tile_rows(M) == 16;
     const int round = 128 * (decode ? (f32 ? expand_steps<1, true>(rank) : expand_steps<1, false>(rank))
                                     : expand_steps<4, false>(rank));
-    const int chunks = std::max(1, std::min((2 * kPlanCUs + tiles - 1) / tiles, (N + 127) / 128));
+    const int least = !decode && (int64_t)tiles * (N / 256) >= kPlanCUs / 2 ? 256 : 128;
+    const int chunks = std::max(1, std::min(((decode ? 4 : 6) * kPlanCUs + tiles - 1) / tiles,
+                                            (N + least - 1) / least));
     const int want = (N + chunks - 1) / chunks;
-    const bool big = want >= round;
+    const bool big = want >= (decode ? round : 2 * round);
     const int n_chunk = big ? (want + round - 1) / round * round : (want + 127) / 128 * 128;
     const int64_t expand = blocks_for(tiles, (N + n_chunk - 1) / n_chunk);
     if (expand > INT32_MAX) return HEPH_ERR_UNSUPPORTED;
