@@ -8,6 +8,12 @@
 // both on v_mfma_f32_16x16x32_bf16. t enters the second product as a bf16 and the
 // bf16 of its remainder (16 bits of mantissa): the product has matrix cores to
 // spare, as both launches are bound by what they stream.
+//
+// Measured (rank 16 unless said, graph replays): 5 rows of 3 adapters, 2560 -> 6144
+// 6.9 us, two launches of a chain of four loads each; 64 rows of 40 adapters, 2560 ->
+// 19456 12.2 us (33 MB, 2.7 TB/s); 4090 rows, 9728 -> 2560, rank 64, 40 us (129 MB,
+// 3.2 TB/s). One launch for both products, each workgroup with all of t for itself,
+// was slower throughout.
 #include <algorithm>
 #include <type_traits>
 
@@ -41,8 +47,9 @@ __host__ __device__ inline int* plan_rows(PlanHeader* p, int M, int n_adapters)
     return reinterpret_cast<int*>(plan_tiles(p) + max_tiles(M, n_adapters));
 }
 
-// Counting sort of the rows by adapter. Rows of one adapter come in no fixed
-// order; no result depends on it.
+// Counting sort of the rows by adapter in one workgroup, once a step: 2.4 us for 64 rows,
+// 7.2 for 4090 (two passes over the ids). Rows of one adapter come in no fixed order; no
+// result depends on it.
 __global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanHeader* plan, const int32_t* ids, int M,
                                                             int n_adapters)
 {
