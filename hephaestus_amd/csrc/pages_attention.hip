@@ -65,8 +65,9 @@ __host__ __device__ __forceinline__ int wide_rows(int G) { return 128 / G * G; }
 // Pages a unit has at least: fewer would not keep the four waves of a narrow one
 // busy, and writing and joining a wide one's 128 rows would outweigh its pages (4 pages
 // instead of 8: two prefixes of 64 pages, 32 sequences each, beside 1000 keys a sequence,
-// four layers 153 us instead of 141; alone, a prefix of 48 pages for 32 sequences gained,
-// 23.7 us -> 19.2).
+// four layers 163 us instead of 140, 16 pages 167; alone, a prefix of 48 pages for 32
+// sequences gained from 4, 22.5 us -> 18.3. Narrow units of 8 pages: four sequences of 512
+// keys, four layers, 48.7 us instead of 45.0).
 constexpr int kMinNarrow = 4, kMinWide = 8;
 
 struct Sizes {
