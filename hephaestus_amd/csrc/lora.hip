@@ -11,7 +11,7 @@
 //
 // Measured (rank 16 unless said, graph replays): 5 rows of 3 adapters, 2560 -> 6144
 // 6.9 us, two launches of a chain of four loads each; 64 rows of 40 adapters, 2560 ->
-// 19456 12.2 us (33 MB, 2.7 TB/s); 4090 rows, 9728 -> 2560, rank 64, 40 us (129 MB,
+// 19456 11.1 us (33 MB, 3.0 TB/s); 4090 rows, 9728 -> 2560, rank 64, 40 us (129 MB,
 // 3.2 TB/s). One launch for both products, each workgroup with all of t for itself,
 // was slower throughout.
 #include <algorithm>
@@ -558,11 +558,11 @@ void launch_shrink_ring(const LoraArgs& g, unsigned blocks, hipStream_t s)
 }
 
 // Steps of 32 columns a wave loads at once (of `big` launches, whose workgroups have them
-// for all four waves).
-template <int RT, bool F32>
+// for all four waves; 8, 4 or 6 steps for few ranks gained nothing).
+template <int RT>
 constexpr int expand_steps(int r)
 {
-    return RT > 1 ? (r <= 64 ? 2 : 1) : r <= 16 ? (F32 ? 6 : 8) : r <= 64 ? 4 : 2;
+    return RT == 1 || r <= 64 ? 2 : 1;
 }
 
 template <int RT, bool F32>
@@ -573,10 +573,10 @@ void launch_expand(const LoraArgs& g, bool big, unsigned blocks, hipStream_t s)
         if (big) expand_kernel<RT, F, F32, U><<<blocks, 256, 0, s>>>(g);
         else expand_kernel<RT, F, F32, 1><<<blocks, 256, 0, s>>>(g);
     };
-    if (g.r <= 16) go(std::integral_constant<int, 0>{}, std::integral_constant<int, expand_steps<RT, F32>(16)>{});
-    else if (g.r <= 32) go(std::integral_constant<int, 1>{}, std::integral_constant<int, expand_steps<RT, F32>(32)>{});
-    else if (g.r <= 64) go(std::integral_constant<int, 2>{}, std::integral_constant<int, expand_steps<RT, F32>(64)>{});
-    else go(std::integral_constant<int, 4>{}, std::integral_constant<int, expand_steps<RT, F32>(128)>{});
+    if (g.r <= 16) go(std::integral_constant<int, 0>{}, std::integral_constant<int, expand_steps<RT>(16)>{});
+    else if (g.r <= 32) go(std::integral_constant<int, 1>{}, std::integral_constant<int, expand_steps<RT>(32)>{});
+    else if (g.r <= 64) go(std::integral_constant<int, 2>{}, std::integral_constant<int, expand_steps<RT>(64)>{});
+    else go(std::integral_constant<int, 4>{}, std::integral_constant<int, expand_steps<RT>(128)>{});
 }
 
 }  // namespace
@@ -631,18 +631,18 @@ int heph_lora_add(void* c, int c_dtype, const void* base, const uint16_t* x_bf16
     const int tiles = max_tiles(M, n_adapters), splits = k_splits(M, n_adapters, K);
     // Columns a workgroup, each of which joins the parts of t for itself: for four workgroups
     // a CU of decode tiles (two: 64 rows of 40 adapters, 2560 -> 19456, 13.7 us instead of
-    // 12.3), six of a prompt's, but then 256 columns each while these fill half of the device
+    // 11.1), six of a prompt's, but then 256 columns each while these fill half of the device
     // (two: 4090 rows -> 19456 111 us, 96; 128 columns: 1000 rows of rank 128 49 us, 39). A
-    // wave takes all its steps at once where there are rounds of them, in a prompt two.
+    // wave takes its steps together where there are two rounds of them or more; the columns
+    // are then whole rounds, in decode rather fewer (more: 12.1 us in the case above).
     const bool f32 = c_dtype == HEPH_DTYPE_F32, decode = tile_rows(M) == 16;
-    const int round = 128 * (decode ? (f32 ? expand_steps<1, true>(rank) : expand_steps<1, false>(rank))
-                                    : expand_steps<4, false>(rank));
+    const int round = 128 * (decode ? expand_steps<1>(rank) : expand_steps<4>(rank));
     const int least = !decode && (int64_t)tiles * (N / 256) >= kPlanCUs / 2 ? 256 : 128;
     const int chunks = std::max(1, std::min(((decode ? 4 : 6) * kPlanCUs + tiles - 1) / tiles,
                                             (N + least - 1) / least));
     const int want = (N + chunks - 1) / chunks;
-    const bool big = want >= (decode ? round : 2 * round);
-    const int n_chunk = big ? (want + round - 1) / round * round : (want + 127) / 128 * 128;
+    const bool big = want >= 2 * round;
+    const int n_chunk = big ? (decode ? want : want + round - 1) / round * round : (want + 127) / 128 * 128;
     const int64_t expand = blocks_for(tiles, (N + n_chunk - 1) / n_chunk);
     if (expand > INT32_MAX) return HEPH_ERR_UNSUPPORTED;
     if (int st = check_device()) return st;
