@@ -126,7 +126,7 @@ struct Source {
     int seq, tok0, n_tok, page0, pages, kv;     // kv: 0 for a group
     int tile, tiles, base;
     int chunks;                                 // a tile's units before the last round
-    int parts;                                  // where its partial results start
+    int parts, units;                           // where its partial results and units start
 };
 
 struct SeqTokens {
@@ -274,11 +274,26 @@ __global__ __launch_bounds__(kMaxSeqs) void plan_kernel(PlanArgs a)
     constexpr int cap = 64;                    // (merge_row takes two lanes' worth)
     Token* tokens = plan_tokens(a.plan);
     Unit* units = plan_units(a.plan, a.s.n_tok);
-    for (int i = t; i <= a.s.n_seqs; i += nt) in.q_start[i] = a.q_start[i];
-    if (t < a.s.n_seqs) in.kv_len[t] = a.kv_len[t];
-    if (a.s.n_groups) {
-        for (int i = t; i <= a.s.n_groups; i += nt) in.group_start[i] = a.group_start[i];
-        if (t < a.s.n_groups) in.shared[t] = a.shared[t];
+    {
+        // (all loads at once; the threads behind the last sequence or group repeat its entry)
+        const int s = min(t, a.s.n_seqs - 1), g = min(t, a.s.n_groups - 1);
+        const int start = a.q_start[s], end = a.q_start[a.s.n_seqs], kv = a.kv_len[s];
+        int group_start = 0, group_end = 0, shared = 0;
+        if (a.s.n_groups) {
+            group_start = a.group_start[g];
+            group_end = a.group_start[a.s.n_groups];
+            shared = a.shared[g];
+        }
+        in.q_start[s] = start;
+        in.kv_len[s] = kv;
+        if (a.s.n_groups) {
+            in.group_start[g] = group_start;
+            in.shared[g] = shared;
+        }
+        if (t == 0) {
+            in.q_start[a.s.n_seqs] = end;
+            in.group_start[a.s.n_groups] = group_end;
+        }
     }
     if (t == 0) merges = 0;
     __syncthreads();
@@ -337,30 +352,43 @@ __global__ __launch_bounds__(kMaxSeqs) void plan_kernel(PlanArgs a)
     xg.parts = parts(xg);
     xs.parts = parts(xs);
     scan_block(xg.parts, xs.parts, red_i);
-    if (t < a.s.n_groups) groups[t] = xg;
-    int at_g = count(xg), at_s = count(xs);
+    xg.units = count(xg);
+    xs.units = count(xs);
     // a row of another number of units than one: behind a prefix, in a split run, without keys
-    if (xg.tiles > 0 || (xs.n_tok > 0 && (xs.kv < xs.n_tok || xs.tiles == 0 || at_s > xs.tiles)))
+    if (xg.tiles > 0 || (xs.n_tok > 0 && (xs.kv < xs.n_tok || xs.tiles == 0 || xs.units > xs.tiles)))
         merges = 1;
-    const int all_units = scan_block(at_g, at_s, red_i);
+    const int all_units = scan_block(xg.units, xs.units, red_i);
     const int max_units = (int)min(a.s.max_units(), (long)INT32_MAX);
-    auto emit = [&](const Source& x, int u, int prefix) {
-        for (int r = x.tiles - 1; r >= 0; --r) {
-            const Cut c = cut_tile(x, rounds, G, r);
-            for (int k = 0; k < c.chunks; ++k, ++u)
-                if ((unsigned)u < (unsigned)max_units)     // (wrapped where q_start falls)
-                    units[u] = Unit{x.seq, x.tok0, r * x.tile, rows_in(x, r),
-                                    x.page0 + k * c.per, min(c.per, x.pages - k * c.per), k, prefix};
-        }
-    };
+    if (t < a.s.n_groups) groups[t] = xg;
     if (t < a.s.n_seqs) seqs[t] = SeqTokens{xs, group};
     __syncthreads();
-    if (blockIdx.x == 0) {
-        emit(xg, at_g, 1);
-        emit(xs, at_s, 0);
-        if (t == 0)
-            *a.plan = PlanHeader{kMagic, a.s.n_tok, a.s.n_seqs, a.s.n_groups, a.table_pages, a.s.n_heads,
-                                 a.s.n_kv, min(all_units, max_units), merges, {}};
+    const int n_units = min(all_units, max_units);
+    if (blockIdx.x == 0 && t == 0)
+        *a.plan = PlanHeader{kMagic, a.s.n_tok, a.s.n_seqs, a.s.n_groups, a.table_pages, a.s.n_heads,
+                             a.s.n_kv, n_units, merges, {}};
+    // Units: a source's tiles from its last on, each one's runs in order.
+    for (int u = blockIdx.x * nt + t; u < n_units; u += gridDim.x * nt) {
+        auto source = [&](int i) -> const Source& {
+            return i < a.s.n_groups ? groups[i] : seqs[i - a.s.n_groups].x;
+        };
+        int lo = 0, hi = a.s.n_groups + a.s.n_seqs;   // the last source that starts at u or before
+        while (lo < hi) {
+            const int mid = (lo + hi) / 2;
+            if (source(mid).units <= u) lo = mid + 1;
+            else hi = mid;
+        }
+        const Source x = source(max(lo - 1, 0));
+        const int at = u - x.units, last = last_round(x, rounds), whole = (x.tiles - last) * x.chunks;
+        // (none of the source's where the counts wrapped: q_start falls)
+        Unit unit{x.seq, x.tok0, 0, 0, 0, 0, 0, 0};
+        if ((unsigned)at < (unsigned)count(x)) {
+            const int in_last = max(at - whole, 0), k = at < whole ? at % x.chunks : in_last % rounds.chunks;
+            const int r = at < whole ? x.tiles - 1 - at / x.chunks : last - 1 - in_last / rounds.chunks;
+            const int per = cut_tile(x, rounds, G, r).per;
+            unit = Unit{x.seq, x.tok0, r * x.tile, rows_in(x, r), x.page0 + k * per,
+                        min(per, x.pages - k * per), k, lo <= a.s.n_groups};
+        }
+        units[u] = unit;
     }
     for (int i = blockIdx.x * kPlanTokens + t; i < min(a.s.n_tok, ((int)blockIdx.x + 1) * kPlanTokens); i += nt) {
         int lo = 0, hi = a.s.n_seqs;              // the last sequence that starts at i or before
