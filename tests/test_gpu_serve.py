@@ -1009,6 +1009,84 @@ def test_batch_decoder_rows_do_not_depend_on_their_batch():
     assert a.length == 101 and d.kv.free_pages == 40 - len(set(a.pages + b.pages + alone.pages))
 
 
+def test_captured_step_of_all_ops():
+    # adapters -> q/k norm, rotation, pages -> attention -> adapters as one graph, replayed over
+    # growing sequences, a padding row among them, with the same step run eagerly in between
+    H, KV, K, T = 8, 2, 256, 6
+    N, g = (H + 2 * KV) * D, torch.Generator(device="cuda").manual_seed(50)
+    up, down = lora_case(T, N, K, 16, 3, seed=51), lora_case(T, K, H * D, 16, 3, seed=52)
+    gam = torch.ones(2, D, dtype=torch.bfloat16, device="cuda")
+    rope, inv = S.rope_table_f32(1000), torch.full((2 * KV,), 30.0, device="cuda")
+    scale, table = 1 / inv, torch.arange(T * 4, dtype=torch.int32, device="cuda").view(T, 4).clone()
+    table[1:4, 0] = 0                                    # a shared first page
+    sides = []
+    for _ in range(2):
+        k, v = codes(g, T * 4, KV, 2, PAGE, 64), codes(g, T * 4, KV, D, PAGE)
+        sides.append(dict(k=k, v=v, qkv=torch.zeros(T, N, dtype=torch.bfloat16, device="cuda"),
+                          att=torch.zeros(T, H, D, dtype=torch.bfloat16, device="cuda"),
+                          o=torch.zeros(T, K, dtype=torch.bfloat16, device="cuda"),
+                          plan=S.AttentionPlan(T - 1, T, H, KV, 4, n_groups=2),
+                          lplan=S.LoraPlan(T, 3, 16, H * D)))
+    sides[1]["k"], sides[1]["v"] = sides[0]["k"].clone(), sides[0]["v"].clone()
+    meta = {n: torch.zeros(m, dtype=torch.int32, device="cuda") for n, m in
+            (("pos", T), ("slot", T), ("start", T), ("lens", T - 1), ("group", 3), ("shared", 2), ("ids", T))}
+
+    def step(s):
+        s["plan"].update(meta["start"], meta["lens"], meta["group"], meta["shared"])
+        s["lplan"].update(meta["ids"])
+        S.lora_add(s["qkv"], up["base"], up["x"], up["a"], up["b"], up["scale"], s["lplan"])
+        x = s["qkv"].view(T, H + 2 * KV, D)
+        S.qk_norm_rope_pages(x[:, :H], x, gam[0], gam[1], s["k"], s["v"], inv, rope, meta["pos"], meta["slot"])
+        S.attention_pages(s["att"], x[:, :H], s["k"], s["v"], scale, table[:T - 1], s["plan"])
+        S.lora_add(s["o"], down["base"], s["att"].view(T, H * D), down["a"], down["b"], down["scale"],
+                   s["lplan"])
+
+    def put(i):
+        lens = [70 + i, 65 + i, 66 + 3 * i, 130 + i, 1 + i]
+        own = [n - 1 for n in lens]                     # the new key of each sequence
+        rows = dict(pos=own + [-1], lens=lens, start=list(range(T)), group=[0, 1, 4], shared=[0, 1],
+                    slot=[int(table[s, j // PAGE]) * PAGE + j % PAGE for s, j in enumerate(own)] + [-1],
+                    ids=[(i + s) % 4 - 1 for s in range(T)])
+        for n, values in rows.items():
+            meta[n].copy_(torch.tensor(values, dtype=torch.int32))
+        up["x"].normal_(generator=g)
+
+    put(0)
+    for s in sides:
+        step(s)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step(sides[0])
+    for i in range(1, 8):
+        put(i)
+        graph.replay()
+        step(sides[1])
+        torch.cuda.synchronize()
+        for n in ("qkv", "k", "v", "att", "o"):
+            assert torch.equal(sides[0][n], sides[1][n]), (i, n)
+    assert torch.isfinite(sides[0]["o"].float()).all()
+
+
+def test_batch_decoder_on_another_stream():
+    rng = np.random.default_rng(2)
+    prompts = [rng.integers(0, CFG.vocab, n).tolist() for n in (130, 70, 3)]
+    got = []
+    for stream in (torch.cuda.current_stream(), torch.cuda.Stream()):
+        d = decoder(seed=2)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            root = d.kv.new()
+            d.step([prompts[0]], [root])
+            seqs = d.kv.fork(root, 2) + [d.kv.new()]
+            d.step([[5], prompts[1], prompts[2]], seqs)
+            d.kv.free(seqs[0])
+            d.kv.compact()
+            got.append(d.step([[7], [8]], seqs[1:]))
+        torch.cuda.synchronize()
+    assert torch.equal(got[0], got[1])
+
+
 def test_host_refusals_on_device_tensors():
     b = batch([1, 1], [64, 70], seed=1)
     plan = make_plan(b)
