@@ -380,7 +380,7 @@ __global__ __launch_bounds__(kMaxSeqs) void plan_kernel(PlanArgs a)
         const Source x = source(max(lo - 1, 0));
         const int at = u - x.units, last = last_round(x, rounds), whole = (x.tiles - last) * x.chunks;
         // (none of the source's where the counts wrapped: q_start falls)
-        Unit unit{x.seq, x.tok0, 0, 0, 0, 0, 0, 0};
+        Unit unit{0, 0, 0, 0, 0, 0, 0, 0};
         if ((unsigned)at < (unsigned)count(x)) {
             const int in_last = max(at - whole, 0), k = at < whole ? at % x.chunks : in_last % rounds.chunks;
             const int r = at < whole ? x.tiles - 1 - at / x.chunks : last - 1 - in_last / rounds.chunks;
@@ -436,9 +436,10 @@ struct AttnArgs {
 
 __device__ __forceinline__ bool plan_fits(const PlanHeader& h, const AttnArgs& a)
 {
-    return h.magic == kMagic && h.n_tok == a.s.n_tok && h.n_seqs == a.s.n_seqs &&
-           h.n_groups == a.s.n_groups && h.table_pages == a.table_pages &&
-           h.n_heads == a.s.n_heads && h.n_kv == a.s.n_kv;
+    // (no branches: they would load it piece by piece)
+    return ((h.magic ^ kMagic) | (h.n_tok ^ a.s.n_tok) | (h.n_seqs ^ a.s.n_seqs) |
+            (h.n_groups ^ a.s.n_groups) | (h.table_pages ^ a.table_pages) |
+            (h.n_heads ^ a.s.n_heads) | (h.n_kv ^ a.s.n_kv)) == 0;
 }
 
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
@@ -541,11 +542,10 @@ struct Rows {
             const int at = u.row0 + (live ? row : 0);
             tok[r] = live ? u.tok0 + at / G : -1;
             hd[r] = head * G + at % G;
-            limit[r] = live ? tokens[tok[r]].limit : 0;
-            if (live) {
-                lo = min(lo, limit[r]);
-                hi = max(hi, limit[r]);
-            }
+            const int keys = tokens[u.tok0 + at / G].limit;    // (no branch: all loads at once)
+            limit[r] = keys & (live ? -1 : 0);
+            lo = min(lo, keys | (live ? 0 : INT32_MAX));
+            hi = max(hi, limit[r]);
             const uint16_t* p = a.q + (size_t)(live ? tok[r] : u.tok0) * a.q_stride + (size_t)hd[r] * kHeadDim;
 #pragma unroll
             for (int f = 0; f < 4; ++f)
@@ -787,7 +787,7 @@ __device__ __forceinline__ void wait_vm()
 // a wave are on their way into registers while one is worked on. (64 sequences, each
 // 1024 keys 28 us, 4.8 TB/s; 64 keys 9 us, where a chain of four loads counts: unit,
 // limits and page ids, q, pages.)
-__device__ __forceinline__ void attend_narrow(const AttnArgs& a, const Unit& u, int head, uint8_t* lds)
+__device__ __forceinline__ void attend_narrow(const AttnArgs& a, const Unit& u, int head, int ids0, uint8_t* lds)
 {
     const int l = threadIdx.x & 63, c = l & 15, g4 = l >> 4, n_kv = a.s.n_kv;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -831,7 +831,7 @@ __device__ __forceinline__ void attend_narrow(const AttnArgs& a, const Unit& u, 
     };
     for (first = u.page0; first < end; first += 64) {
         last = min(first + 64, end);
-        ids = page_ids(a, u, first);
+        ids = first == u.page0 ? ids0 : page_ids(a, u, first);
         wait_vm<0>();           // (nothing but pages on its way below)
         int n = first + kw;
         load(p0, n);
@@ -891,7 +891,7 @@ constexpr int kWidePage = 2 * 2 * kPageBytes;      // K and V as bf16
 // memory stay in flight (__syncthreads would wait for them).
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
-__device__ __forceinline__ void attend_wide(const AttnArgs& a, const Unit& u, int head, uint8_t* lds)
+__device__ __forceinline__ void attend_wide(const AttnArgs& a, const Unit& u, int head, int ids0, uint8_t* lds)
 {
     __shared__ int nan_page[2], lows[4];       // of each buffer's page; each wave's smallest limit
     const int l = threadIdx.x & 63, c = l & 15, g4 = l >> 4, n_kv = a.s.n_kv;
@@ -915,7 +915,7 @@ __device__ __forceinline__ void attend_wide(const AttnArgs& a, const Unit& u, in
     // waves 0, 1: K's 1 KB tiles 0..3, 4..7; waves 2, 3: V's
     const uint8_t* pool = (wave < 2 ? a.k_pages : a.v_pages) + (wave & 1) * 4096 + c * 64 + g4 * 16;
     for (int first = u.page0; first < end; first += 64) {
-        const int last = min(first + 64, end), ids = page_ids(a, u, first);
+        const int last = min(first + 64, end), ids = first == u.page0 ? ids0 : page_ids(a, u, first);
         wait_vm<0>();           // (nothing but pages on its way below)
         auto id_of = [&](int n) { return __builtin_amdgcn_readlane(ids, n - first); };
         struct Codes {
@@ -978,12 +978,20 @@ __device__ __forceinline__ void attend_wide(const AttnArgs& a, const Unit& u, in
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void attention_kernel(AttnArgs a)
 {
     __shared__ __attribute__((aligned(16))) uint8_t lds[2 * kWidePage];
-    const PlanHeader h = *a.plan;
+    PlanHeader h = *a.plan;
     const int n_kv = a.s.n_kv, unit = blockIdx.x / n_kv, head = blockIdx.x % n_kv;
-    const Unit u = plan_units(a.plan, a.s.n_tok)[unit];        // (the plan has room for all of the grid's)
+    // Loaded beside the header, not behind its check (the plan has room for all of the
+    // grid's): the start of a unit is a chain of loads, this one then its rows' limits, q
+    // and page ids, then pages.
+    const Unit u = plan_units(a.plan, a.s.n_tok)[unit];
+    asm volatile("" : "+s"(h.magic), "+s"(h.n_tok), "+s"(h.n_seqs), "+s"(h.n_groups), "+s"(h.table_pages),
+                 "+s"(h.n_heads), "+s"(h.n_kv), "+s"(h.n_units)
+                 : "s"(u.seq), "s"(u.tok0), "s"(u.row0), "s"(u.rows), "s"(u.page0), "s"(u.pages), "s"(u.part),
+                   "s"(u.prefix));
     if (!plan_fits(h, a) || unit >= h.n_units) return;
-    if (u.rows <= kNarrow) attend_narrow(a, u, head, lds);
-    else attend_wide(a, u, head, lds);
+    const int ids = page_ids(a, u, u.page0);        // (on its way while the rows are looked at)
+    if (u.rows <= kNarrow) attend_narrow(a, u, head, ids, lds);
+    else attend_wide(a, u, head, ids, lds);
 }
 
 // Joins the partial results of a row, two dims a lane. A row of one unit is
