@@ -978,16 +978,11 @@ __device__ __forceinline__ void attend_wide(const AttnArgs& a, const Unit& u, in
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void attention_kernel(AttnArgs a)
 {
     __shared__ __attribute__((aligned(16))) uint8_t lds[2 * kWidePage];
-    PlanHeader h = *a.plan;
+    const PlanHeader h = *a.plan;
     const int n_kv = a.s.n_kv, unit = blockIdx.x / n_kv, head = blockIdx.x % n_kv;
-    // Loaded beside the header, not behind its check (the plan has room for all of the
-    // grid's): the start of a unit is a chain of loads, this one then its rows' limits, q
-    // and page ids, then pages.
-    const Unit u = plan_units(a.plan, a.s.n_tok)[unit];
-    asm volatile("" : "+s"(h.magic), "+s"(h.n_tok), "+s"(h.n_seqs), "+s"(h.n_groups), "+s"(h.table_pages),
-                 "+s"(h.n_heads), "+s"(h.n_kv), "+s"(h.n_units)
-                 : "s"(u.seq), "s"(u.tok0), "s"(u.row0), "s"(u.rows), "s"(u.page0), "s"(u.pages), "s"(u.part),
-                   "s"(u.prefix));
+    // The start of a unit is a chain of loads: header, unit, then its rows' limits, q and
+    // page ids together, then pages.
+    const Unit u = plan_units(a.plan, a.s.n_tok)[unit];        // (the plan has room for all of the grid's)
     if (!plan_fits(h, a) || unit >= h.n_units) return;
     const int ids = page_ids(a, u, u.page0);        // (on its way while the rows are looked at)
     if (u.rows <= kNarrow) attend_narrow(a, u, head, ids, lds);
@@ -996,12 +991,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 
 // Joins the partial results of a row, two dims a lane. A row of one unit is
 // finished already.
-__device__ __forceinline__ void merge_row(const AttnArgs& a, long row, int l)
+__device__ __forceinline__ void merge_row(const AttnArgs& a, const Token& tk, long row, int l)
 {
-    const int t = (int)(row / a.s.n_heads), h = (int)(row % a.s.n_heads);
-    const Token tk = plan_tokens(a.plan)[t];
-    const int n = min(tk.n_prefix + tk.n_own, 128), G = a.s.group();
-    if (tk.limit < 0 || n == 1) return;
+    const int h = (int)(row % a.s.n_heads), n = min(tk.n_prefix + tk.n_own, 128), G = a.s.group();
     const long max_parts = a.s.max_parts();
     auto slot = [&](int k) {
         const long part = (k < tk.n_prefix ? tk.prefix + k * tk.prefix_step
@@ -1044,19 +1036,23 @@ __device__ __forceinline__ void merge_row(const AttnArgs& a, long row, int l)
 constexpr int kMergeBlocks = 2048;
 __global__ __launch_bounds__(256) void merge_kernel(AttnArgs a)
 {
-    const PlanHeader head = *a.plan;
-    if (!plan_fits(head, a) || !head.merges) return;
+    PlanHeader head = *a.plan;
     // each lane looks at one of the wave's next 64 rows
     const long step = (long)gridDim.x * 4, rows = a.s.rows();
     for (long row0 = (long)blockIdx.x * 4 + (threadIdx.x >> 6); row0 < rows; row0 += 64 * step) {
         const long row = row0 + (threadIdx.x & 63) * step;
-        bool todo = false;
-        if (row < rows) {
-            const Token tk = plan_tokens(a.plan)[row / a.s.n_heads];
-            todo = tk.limit >= 0 && tk.n_prefix + tk.n_own != 1;
+        const Token tk = plan_tokens(a.plan)[min(row, rows - 1) / a.s.n_heads];
+        // (loaded beside the header, not behind its check)
+        asm volatile("" : "+s"(head.magic) : "v"(tk.limit), "v"(tk.n_own), "v"(tk.own_step));
+        if (!plan_fits(head, a) || !head.merges) return;
+        const bool todo = row < rows && tk.limit >= 0 && tk.n_prefix + tk.n_own != 1;
+        for (unsigned long long m = __ballot(todo); m; m &= m - 1) {
+            const int k = __ffsll((long long)m) - 1;
+            auto of = [&](int v) { return __builtin_amdgcn_readlane(v, k); };
+            const Token t{of(tk.limit), of(tk.n_prefix), of(tk.n_own), of(tk.prefix), of(tk.prefix_step),
+                          of(tk.own), of(tk.own_step), 0};
+            merge_row(a, t, row0 + k * step, threadIdx.x & 63);
         }
-        for (unsigned long long m = __ballot(todo); m; m &= m - 1)
-            merge_row(a, row0 + (__ffsll((long long)m) - 1) * step, threadIdx.x & 63);
     }
 }
 
