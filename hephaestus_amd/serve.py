@@ -177,7 +177,7 @@ class AttentionPlan:
         self.n_heads, self.n_kv, self.table_pages = n_heads, n_kv, table_pages
         sizes = (n_tok, n_seqs, n_groups, n_heads, n_kv)
         nb = L.lib().heph_pages_attention_plan_bytes(*sizes)
-        if nb == 0:
+        if nb == 0 or not 1 <= table_pages <= L.ATTN_MAX_KEYS // PAGE:
             raise HephError(L.HEPH_ERR_SHAPE, "AttentionPlan")
         # (zeros: no plan until the first update)
         self.plan = torch.zeros(nb, dtype=torch.uint8, device=device)

@@ -398,6 +398,15 @@ def test_attention_units_of_more_than_64_pages():
     check_attention(b, run_attention(b), tokens=[0, 127, 128, 299, 300, 555, 599, 600, 899])
 
 
+@pytest.mark.parametrize("new,H", [(1, 2), (1, 40), (90, 2)])
+def test_attention_longest_sequences(new, H):
+    # as many keys as an op takes: units of 64 pages and more, 64 of them a row
+    keys = L.ATTN_MAX_KEYS
+    b = batch([new, 1], [keys, 2], seed=41 + new, H=H, KV=1, garbage=False)
+    b["table"] = b["table"][:, :keys // PAGE].contiguous()
+    check_attention(b, run_attention(b), tokens=[0, new - 1, new])
+
+
 def test_attention_wide_tiles_split_over_pages():
     # few tiles, long runs: units of a tile meet again in the merge
     for new, keys, H, KV in ((128, 64 * 40, 8, 2), (65, 64 * 33 + 1, 4, 4), (40, 5000, 28, 4)):

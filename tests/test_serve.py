@@ -167,6 +167,20 @@ def test_python_rejects_host_tensors(monkeypatch):
                    torch.zeros(2, 64, 8, dtype=torch.bfloat16), torch.ones(2), plan)
 
 
+def test_plan_refusals(lib):
+    for args in ((1, 1, 8, 8, 0), (1, 1, 8, 8, 4097), (0, 1, 8, 8, 4), (1, 0, 8, 8, 4), (1025, 1, 8, 8, 4),
+                 (1, 1, 8, 3, 4)):
+        with pytest.raises(S.HephError) as e:
+            S.AttentionPlan(*args, device="cpu")
+        assert e.value.status == L.HEPH_ERR_SHAPE
+    for args in ((0, 1, 8, 128), (1, 0, 8, 128), (1, 4097, 8, 128), (1, 1, 12, 128), (1, 1, 136, 128), (1, 1, 8, 8)):
+        with pytest.raises(S.HephError):
+            S.LoraPlan(*args, device="cpu")
+    p = S.AttentionPlan(2, 3, 8, 8, 4, n_groups=1, device="cpu")
+    with pytest.raises(ValueError, match="needs group_start"):
+        p.update(torch.zeros(3, dtype=torch.int32), torch.zeros(2, dtype=torch.int32))
+
+
 def test_attention_buffers_of_extreme_batches(lib):
     plan, ws = lib.heph_pages_attention_plan_bytes, lib.heph_pages_attention_ws_bytes
     for sizes in ((1, 1, 0, 1, 1), (1024, 1024, 1024, 64, 1), (1 << 20, 1024, 3, 4096, 64), (7, 3, 1, 96, 96)):
