@@ -117,6 +117,7 @@ struct PlanArgs {
 // in chains.
 struct PlanLds {
     int32_t q_start[kMaxSeqs + 1], kv_len[kMaxSeqs], group_start[kMaxSeqs + 1], shared[kMaxSeqs];
+    int32_t few[kMaxSeqs + 1], few_tokens[kMaxSeqs + 1];   // before each sequence: those of less than 64 rows
 };
 
 // Rows that work on the same pages: a group's on its shared ones, or one
@@ -146,17 +147,22 @@ __device__ __forceinline__ void set_tiles(Source& x, int G)
     x.tiles = x.pages > 0 ? ceil_div(rows, x.tile) : 0;
 }
 
-// The group's sequences and shared pages; none where sharing gains nothing: a
-// single sequence, or sequences that bring 64 rows or more each, whose own
-// units are bound by the matrix cores and re-read a prefix from the caches.
+// The group's sequences and shared pages; none where sharing gains nothing. Sequences of
+// 64 rows or more are bound by the matrix cores and re-read a prefix from the caches; in a
+// shared one each of their rows pays another partial result, 1.5 KB written and read. It is
+// shared for the others, two or more, if the pages that they need not stream again, 16 KB
+// each, outweigh that (64 single tokens and a prompt of 1100 behind 64 pages 199 us -> 170,
+// 16 and 500 behind 32 pages 57 -> 49; by the mean of all, as it was, one long prompt could
+// take the sharing from all others).
 __device__ Source group_source(const PlanLds& in, const PlanArgs& a, int g)
 {
     const int s0 = clampi(in.group_start[g], 0, a.s.n_seqs);
     const int s1 = clampi(in.group_start[g + 1], s0, a.s.n_seqs);
     const int t0 = clampi(in.q_start[s0], 0, a.s.n_tok), t1 = clampi(in.q_start[s1], t0, a.s.n_tok);
-    const int n = s1 - s0;
     int pages = clampi(in.shared[g], 0, a.table_pages);
-    if (n < 2 || (long)(t1 - t0) * a.s.group() >= 64L * n) pages = 0;
+    const int few = in.few[s1] - in.few[s0];
+    const long many_rows = (long)(t1 - t0 - (in.few_tokens[s1] - in.few_tokens[s0])) * a.s.group();
+    if (few < 2 || many_rows > 10L * (few - 1) * pages) pages = 0;
     Source x{s0, t0, t1 - t0, 0, pages, 0};
     set_tiles(x, a.s.group());
     return x;
@@ -297,6 +303,25 @@ __global__ __launch_bounds__(kMaxSeqs) void plan_kernel(PlanArgs a)
     }
     if (t == 0) merges = 0;
     __syncthreads();
+    {
+        int n = 0;
+        if (t < a.s.n_seqs) {
+            const int t0 = clampi(in.q_start[t], 0, a.s.n_tok);
+            n = clampi(in.q_start[t + 1], t0, a.s.n_tok) - t0;
+            if (n * G >= 64) n = 0;
+        }
+        int few = n > 0, few_tokens = n;
+        scan_block(few, few_tokens, red_i);         // (few_tokens: behind few's total, in all of them)
+        if (t == 0) {
+            in.few[0] = few;
+            in.few_tokens[0] = few_tokens;
+        }
+        if (t < a.s.n_seqs) {
+            in.few[t + 1] = few + (n > 0);
+            in.few_tokens[t + 1] = few_tokens + n;
+        }
+        __syncthreads();
+    }
     Source xg{}, xs{};
     int group = -1;
     if (t < a.s.n_groups) xg = group_source(in, a, t);

@@ -318,6 +318,8 @@ def test_attention_head_layouts(H, KV):
     ([1, 1], [5, 6], [0, 3], [0, 1, 2]),                           # a group that shares nothing
     ([1, 1], [5, 6], [3, 2], [0, 0, 2]),                           # a group of no sequence
     ([2, 1], [5, 6], [40], [0, 2]),
+    ([1, 100, 1, 1], [3, 120, 70, 5], [25], [0, 4]),               # shared beside a long prompt
+    ([1, 100, 1, 90], [3, 120, 70, 95], [4], [0, 4]),              # not shared for two prompts' sake
 ])
 def test_attention_shared_prefix(new, own, shared, group_start):
     b = batch(new, own, shared, group_start, seed=sum(own))
