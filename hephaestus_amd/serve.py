@@ -18,6 +18,7 @@ sequence and calls attention per sequence.
 from __future__ import annotations
 
 import heapq
+from array import array
 
 import numpy as np
 import torch
@@ -211,7 +212,7 @@ def attention_pages(out, q, k_pages, v_pages, kv_scale, page_table, plan: Attent
     table_pages]."""
     p = plan
     dev, stream = _at(ctx)
-    n_pages = len(k_pages)
+    n_pages = k_pages.shape[0]
     kp, vp = _pools(k_pages, v_pages, (n_pages, p.n_kv), dev)
     if page_table.shape != (p.n_seqs, p.table_pages):
         raise ValueError(f"page_table of shape {tuple(page_table.shape)} is not "
@@ -225,19 +226,17 @@ def attention_pages(out, q, k_pages, v_pages, kv_scale, page_table, plan: Attent
 
 def copy_pages(k_pools, v_pools, src, dst, ctx=None) -> None:
     """Page src[i] of every layer copied to page dst[i] in both pools
-    [n_layers, n_pages, ...]; src and dst are host lists. A destination may
+    [n_layers, n_pages, ...]; src and dst are host lists of ints. A destination may
     neither repeat nor be a source."""
     ks = k_pools.shape
     if len(ks) != 6:
         raise ValueError(f"k_pools of shape {tuple(ks)} has no layers")
     dev, stream = _at(ctx)
     kp, vp = _pools(k_pools, v_pools, tuple(ks[:3]), dev)
-    s, d = np.asarray(src, dtype=np.int32).reshape(-1), np.asarray(dst, dtype=np.int32).reshape(-1)
-    if s.size != d.size:
-        raise ValueError(f"{s.size} sources and {d.size} destinations")
-    s, d = np.ascontiguousarray(s), np.ascontiguousarray(d)
-    _call("heph_copy_pages", kp, vp, *ks[:3], s.ctypes.data,
-          d.ctypes.data, s.size, stream)
+    s, d = array("i", src), array("i", dst)
+    if len(s) != len(d):
+        raise ValueError(f"{len(s)} sources and {len(d)} destinations")
+    _call("heph_copy_pages", kp, vp, *ks[:3], s.buffer_info()[0], d.buffer_info()[0], len(s), stream)
 
 
 class LoraPlan:

@@ -1119,6 +1119,12 @@ def test_host_refusals_on_device_tensors():
             S.copy_pages(k, v, src, dst)
         assert e.value.status == L.HEPH_ERR_SHAPE
     S.copy_pages(k, v, [], [])
+    with pytest.raises(ValueError):
+        S.copy_pages(k, v, [0, 1], [2])
+    with pytest.raises(TypeError):
+        S.copy_pages(k, v, [0.0], [1])
+    with pytest.raises(OverflowError):
+        S.copy_pages(k, v, [2 ** 31], [1])
     c = lora_case(4, 96, 256, 16, 2, seed=1)
     plan = S.LoraPlan(4, 2, 16, 256)
     with pytest.raises(HephError):                        # a workspace planned for less
