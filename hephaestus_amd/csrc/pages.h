@@ -21,8 +21,6 @@ __host__ __device__ __forceinline__ int v_place(int j)
 __host__ __device__ __forceinline__ int k_byte(int j, int d) { return d / 64 * 4096 + j * 64 + d % 64; }
 __host__ __device__ __forceinline__ int v_byte(int j, int d) { return d * 64 + v_place(j); }
 
-__device__ __forceinline__ float bf16_value(uint16_t h) { return __uint_as_float((uint32_t)h << 16); }
-
 inline bool aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 inline int status_of(hipError_t e) { return e == hipSuccess ? HEPH_OK : HEPH_ERR_LAUNCH; }
 

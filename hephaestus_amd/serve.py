@@ -241,7 +241,7 @@ def copy_pages(k_pools, v_pools, src, dst, ctx=None) -> None:
 
 class LoraPlan:
     """The rows of a step grouped by adapter, and the workspace of lora_add for
-    projections of up to rank x k -> n: update() it from the rows' adapter ids
+    projections k -> n of up to this rank and k (of any n): update() it from the rows' adapter ids
     in device memory (an id outside [0, n_adapters): no adapter). Calls that
     share a plan are ordered by the caller."""
 
