@@ -1149,7 +1149,7 @@ int heph_pages_attention(void* out_bf16, const void* q_bf16, int64_t q_stride,
         return HEPH_ERR_NULL;
     if (head_dim != kHeadDim || !sizes_ok(n_tok, n_seqs, n_groups, n_heads, n_kv_heads) ||
         n_pages < 1 || table_pages < 1 || table_pages > HEPH_ATTN_MAX_KEYS / kPage ||
-        q_stride < (int64_t)n_heads * kHeadDim)
+        q_stride < (int64_t)n_heads * kHeadDim || out_bf16 == q_bf16)
         return HEPH_ERR_SHAPE;
     if (!aligned(out_bf16, 16) || !aligned(q_bf16, 16) || !aligned(k_pages, 16) ||
         !aligned(v_pages, 16) || !aligned(plan, 16) || !aligned(ws, 16) || q_stride % 8)

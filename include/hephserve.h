@@ -106,7 +106,7 @@ int heph_qk_norm_rope_pages(void* q_out_bf16, int64_t q_stride, const void* qkv_
  * q_start gives to two sequences, or that a decreasing group_start gives to two
  * groups, are undefined.
  * q + t * q_stride: [n_heads, 128] (q_stride in elements, a multiple of 8);
- * out: [n_tok, n_heads, 128], not overlapping q.
+ * out: [n_tok, n_heads, 128], not overlapping q (q's own address: HEPH_ERR_SHAPE).
  * Replaces, for a batch, attention (src/hephaestus/kernels.mojo:923-1240) as
  * forward_fp8_batched_decode calls it per sequence
  * (src/hephaestus/forward.mojo:618-871).

@@ -58,6 +58,7 @@ def attn(lib, **kw):
     *[({f: None}, L.HEPH_ERR_NULL) for f in ("out", "q", "k", "v", "sc", "table", "plan", "ws")],
     *[({f: ODD}, L.HEPH_ERR_ALIGN) for f in ("out", "q", "k", "v", "plan", "ws")],
     (dict(qs=4088), L.HEPH_ERR_SHAPE), (dict(qs=4100), L.HEPH_ERR_ALIGN),
+    (dict(out=FAKE * 4), L.HEPH_ERR_SHAPE),                     # q's own buffer
     (dict(T=0), L.HEPH_ERR_SHAPE), (dict(S=0), L.HEPH_ERR_SHAPE),
     (dict(S=1025, T=2000), L.HEPH_ERR_SHAPE), (dict(G=3), L.HEPH_ERR_SHAPE),
     (dict(G=-1), L.HEPH_ERR_SHAPE), (dict(np=0), L.HEPH_ERR_SHAPE), (dict(tp=0), L.HEPH_ERR_SHAPE),
