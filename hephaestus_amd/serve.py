@@ -417,9 +417,25 @@ class LoraWeights:
     def __init__(self, scale: torch.Tensor, layers: list[dict]):
         self.scale, self.layers = scale, layers
         self.n_adapters = scale.numel()
+        for i, d in enumerate(layers):
+            for name, (a, b) in d.items():
+                if name not in _PROJECTIONS:
+                    raise ValueError(f"layer {i}: no projection is named {name!r}")
+                if a.dim() != 3 or b.dim() != 3 or a.shape[:2] != (b.shape[0], b.shape[2]) or \
+                        a.shape[0] != self.n_adapters or not _rank_ok(a.shape[1]):
+                    raise ValueError(f"layer {i}, {name}: a {tuple(a.shape)} and b {tuple(b.shape)} "
+                                     f"are not [{self.n_adapters}, rank, k] and "
+                                     f"[{self.n_adapters}, n, rank], rank a multiple of 8 up to 128")
         pairs = [p for d in layers for p in d.values()]
         self.max_rank = max((a.shape[1] for a, _ in pairs), default=8)
         self.max_k = max((a.shape[2] for a, _ in pairs), default=128)
+
+
+_PROJECTIONS = ("qkv", "o", "gate_up", "down")
+
+
+def _rank_ok(rank: int) -> bool:
+    return 8 <= rank <= 128 and rank % 8 == 0
 
 
 def _groups(seqs: list[Sequence]) -> tuple[list[int], list[int]]:
@@ -458,6 +474,12 @@ class Qwen3BatchDecoder:
         if lora is not None and len(lora.layers) != weights.cfg.n_layers:
             raise ValueError(f"adapters of {len(lora.layers)} layers, "
                              f"{weights.cfg.n_layers} in the model")
+        for i, d in enumerate(lora.layers if lora is not None else []):
+            for name, (a, b) in d.items():
+                fw = getattr(weights.layers[i], name)
+                if (b.shape[1], a.shape[2]) != (fw.N, fw.K):
+                    raise ValueError(f"layer {i}, {name}: adapters {a.shape[2]} -> {b.shape[1]} "
+                                     f"beside a projection {fw.K} -> {fw.N}")
         self.w, self.kv, self.lora = weights, kv, lora
         self.n_pos = min(n_pos, L.ATTN_MAX_KEYS)
         self.rope = rope_table_f32(self.n_pos, weights.cfg.theta, device=weights.embed.w.device)

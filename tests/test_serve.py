@@ -410,3 +410,47 @@ def test_ctypes_signatures_of_the_serving_ops():
                         ("heph_lora_add", 17)):
         assert len(L.SIGNATURES[name][1]) == nargs
         assert getattr(L.lib(), name).restype is ctypes.c_int
+
+
+# --------------------------------------------------------- the decoder's host side ----
+
+def host_decoder(cache, monkeypatch, lora=None, n_pos=300):
+    """A decoder without device memory: what a step does before its first launch."""
+    H, I, Q, KV = CFG.hidden, CFG.inter, CFG.q_out, CFG.kv_out
+
+    def weight(n, k):
+        return SimpleNamespace(N=n, K=k)
+    layer = SimpleNamespace(qkv=weight(Q + 2 * KV, H), o=weight(H, Q), gate_up=weight(2 * I, H),
+                            down=weight(H, I))
+    w = SimpleNamespace(cfg=CFG, embed=SimpleNamespace(block=True, w=torch.zeros(1)),
+                        layers=[layer] * CFG.n_layers)
+    monkeypatch.setattr(S, "rope_table_f32", lambda n, theta, device: torch.zeros(n, 64, 2))
+    return S.Qwen3BatchDecoder(w, cache, n_pos=n_pos, lora=lora)
+
+
+def pair(n, k, rank=16, n_adapters=3):
+    return (torch.zeros(n_adapters, rank, k, dtype=torch.bfloat16),
+            torch.zeros(n_adapters, n, rank, dtype=torch.bfloat16))
+
+
+def test_lora_weights_that_no_projection_takes_are_refused(cache, monkeypatch):
+    H, I, Q, KV = CFG.hidden, CFG.inter, CFG.q_out, CFG.kv_out
+    good = {"qkv": pair(Q + 2 * KV, H), "o": pair(H, Q), "gate_up": pair(2 * I, H, rank=8),
+            "down": pair(H, I)}
+    scale = torch.ones(3)
+    lora = S.LoraWeights(scale, [good, {}])
+    assert (lora.n_adapters, lora.max_rank, lora.max_k) == (3, 16, max(Q, I))
+    host_decoder(cache, monkeypatch, lora)
+    for name in ("q", "q_proj", "gate", "up_proj", "Down", ""):
+        with pytest.raises(ValueError, match="no projection"):
+            S.LoraWeights(scale, [{}, {name: pair(H, I)}])
+    a, b = pair(H, I)
+    for bad in (pair(H, I, n_adapters=2), (a, b[:2]), (a[:, :8], b), pair(H, I, rank=12), pair(H, I, rank=136), (a[0], b), (a, b[0]), (b, a)):
+        with pytest.raises(ValueError, match="layer 1, down"):
+            S.LoraWeights(scale, [good, {"down": bad}])
+    # sizes of another projection or of another model, before any step
+    for name, wrong in (("qkv", pair(H, Q)), ("qkv", pair(Q, H)), ("o", pair(Q, H)),
+                        ("gate_up", pair(I, H)), ("down", pair(H, I // 2))):
+        lora = S.LoraWeights(scale, [good, dict(good, **{name: wrong})])
+        with pytest.raises(ValueError, match=f"layer 1, {name}"):
+            host_decoder(cache, monkeypatch, lora)
