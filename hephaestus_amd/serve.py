@@ -443,7 +443,7 @@ def _groups(seqs: list[Sequence]) -> tuple[list[int], list[int]]:
     group_start and shared_pages. A run grows while its common prefix keeps
     at least half of the pages its first two share."""
     start, shared = [0], []
-    n = None
+    n = first = None
     for i in range(1, len(seqs) + 1):
         if i < len(seqs):
             a, b = seqs[start[-1]].pages, seqs[i].pages
@@ -452,9 +452,9 @@ def _groups(seqs: list[Sequence]) -> tuple[list[int], list[int]]:
                 m += 1
             if n is None:
                 if m > 0:
-                    n = m
+                    n = first = m
                     continue
-            elif 2 * min(n, m) >= n:
+            elif 2 * min(n, m) >= first:
                 n = min(n, m)
                 continue
         shared.append(n or 0)

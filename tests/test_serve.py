@@ -454,3 +454,29 @@ def test_lora_weights_that_no_projection_takes_are_refused(cache, monkeypatch):
         lora = S.LoraWeights(scale, [good, dict(good, **{name: wrong})])
         with pytest.raises(ValueError, match=f"layer 1, {name}"):
             host_decoder(cache, monkeypatch, lora)
+
+
+def chain(*shared_with_the_first):
+    """Sequences of 64 pages; number i shares that many with the first one."""
+    out = []
+    for i, n in enumerate(shared_with_the_first):
+        s = S.Sequence()
+        s.pages = list(range(n)) + [1000 * (i + 1) + j for j in range(64 - n)]
+        out.append(s)
+    return out
+
+
+def test_groups_do_not_shrink_step_by_step():
+    # every neighbour halves the common prefix: the group ends at half of its first two's pages
+    start, shared = S._groups(chain(*[64] * 32, 32, 16, 8, 4, 2, 1))
+    assert start[:2] == [0, 33] and shared[0] == 32
+    assert S._groups(chain(64, 40, 20, 19, 64)) == ([0, 3, 5], [20, 19])
+    assert S._groups(chain(64, 41, 20)) == ([0, 2, 3], [41, 0])
+    rng = np.random.default_rng(2)
+    for _ in range(50):
+        seqs = chain(*(int(n) for n in rng.integers(0, 65, 12)))
+        start, shared = S._groups(seqs)
+        for a, b, n in zip(start, start[1:], shared):
+            rows = [s.pages for s in seqs[a:b]]
+            first_two = next(i for i in range(65) if i == 64 or rows[0][i] != rows[1][i]) if b - a > 1 else 0
+            assert all(r[:n] == rows[0][:n] for r in rows) and 2 * n >= first_two
