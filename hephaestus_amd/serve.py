@@ -369,7 +369,7 @@ class PagedKVCache:
         if tails:
             try:
                 copy_pages(self.k, self.v, [seq.pages[full]] * n, tails, ctx)
-            except Exception:
+            except BaseException:
                 for p in tails:
                     self._drop(p)
                 raise
@@ -520,7 +520,7 @@ class Qwen3BatchDecoder:
         before = [(s, s.length, len(s.pages)) for s in seqs]
         try:
             return self._run(tokens, seqs, adapters)
-        except Exception:
+        except BaseException:
             for s, length, pages in before:
                 for p in s.pages[pages:]:
                     kv._drop(p)

@@ -480,3 +480,22 @@ def test_groups_do_not_shrink_step_by_step():
             rows = [s.pages for s in seqs[a:b]]
             first_two = next(i for i in range(65) if i == 64 or rows[0][i] != rows[1][i]) if b - a > 1 else 0
             assert all(r[:n] == rows[0][:n] for r in rows) and 2 * n >= first_two
+
+
+@pytest.mark.parametrize("error", [KeyboardInterrupt, MemoryError])
+def test_an_interrupted_step_or_fork_changes_nothing(cache, monkeypatch, error):
+    c = cache
+    d = host_decoder(c, monkeypatch)
+    a, b = c.new(), c.new()
+    c.extend(a, 70)
+
+    def stops(*args):
+        raise error()
+    monkeypatch.setattr(d, "_run", lambda t, s, ad: ([c.extend(i, len(j)) for i, j in zip(s, t)], stops()))
+    with pytest.raises(error):
+        d.step([[1] * 100, [2]], [a, b])
+    monkeypatch.setattr(S, "copy_pages", stops)
+    with pytest.raises(error):
+        c.fork(a, 2)
+    assert (a.length, b.length, len(c._seqs), c.free_pages) == (70, 0, 2, 10)
+    check_counts(c)
