@@ -316,7 +316,7 @@ class PagedKVCache:
         self.inv = torch.ones_like(self.scale)
         self._free = list(range(n_pages))          # a heap: the lowest page first
         self._users = [0] * n_pages
-        self._seqs: list[Sequence] = []
+        self._seqs: dict[Sequence, None] = {}      # in the order of their making
 
     @property
     def free_pages(self) -> int:
@@ -336,14 +336,15 @@ class PagedKVCache:
             heapq.heappush(self._free, page)
 
     def _own(self, seq: Sequence) -> Sequence:
-        if not any(s is seq for s in self._seqs):
+        if not isinstance(seq, Sequence) or seq not in self._seqs:
             raise ValueError("the sequence is not in this cache")
         return seq
 
     def new(self) -> Sequence:
         """An empty sequence."""
-        self._seqs.append(Sequence())
-        return self._seqs[-1]
+        seq = Sequence()
+        self._seqs[seq] = None
+        return seq
 
     def extend(self, seq: Sequence, n: int) -> list[int]:
         """Room for n more keys; their slots. Nothing changes if the pages do
@@ -387,7 +388,7 @@ class PagedKVCache:
         self._own(seq)
         for p in seq.pages:
             self._drop(p)
-        self._seqs = [s for s in self._seqs if s is not seq]
+        del self._seqs[seq]
         seq.pages, seq.length = [], 0
 
     def compact(self, ctx=None) -> int:
@@ -438,6 +439,18 @@ def _rank_ok(rank: int) -> bool:
     return 8 <= rank <= 128 and rank % 8 == 0
 
 
+def _common(a: list[int], b: list[int]) -> int:
+    """How many first entries two lists share, halving a range that holds the end."""
+    m, end = 0, min(len(a), len(b))
+    while m < end:
+        mid = (m + end + 1) // 2
+        if a[m:mid] == b[m:mid]:
+            m = mid
+        else:
+            end = mid - 1
+    return m
+
+
 def _groups(seqs: list[Sequence]) -> tuple[list[int], list[int]]:
     """Runs of neighbouring sequences that share their first pages:
     group_start and shared_pages. A run grows while its common prefix keeps
@@ -446,10 +459,7 @@ def _groups(seqs: list[Sequence]) -> tuple[list[int], list[int]]:
     n = first = None
     for i in range(1, len(seqs) + 1):
         if i < len(seqs):
-            a, b = seqs[start[-1]].pages, seqs[i].pages
-            m = 0
-            while m < min(len(a), len(b)) and a[m] == b[m]:
-                m += 1
+            m = _common(seqs[start[-1]].pages, seqs[i].pages)
             if n is None:
                 if m > 0:
                     n = first = m
@@ -527,23 +537,28 @@ class Qwen3BatchDecoder:
                 s.length, s.pages = length, s.pages[:pages]
             raise
 
-    def _run(self, tokens, seqs, adapters) -> torch.Tensor:
-        cfg, w, kv = self.w.cfg, self.w, self.kv
+    def _layout(self, tokens, seqs, adapters) -> list:
+        """The sequences take their tokens; the int32 values that the step's ops read: tokens,
+        positions, slots, q_start, kv_len, group_start, shared_pages, adapter ids and the page
+        table [len(seqs), most pages]."""
         flat = [i for t in tokens for i in t]
         positions = [s.length + i for t, s in zip(tokens, seqs) for i in range(len(t))]
-        slots = [i for t, s in zip(tokens, seqs) for i in kv.extend(s, len(t))]
+        slots = [i for t, s in zip(tokens, seqs) for i in self.kv.extend(s, len(t))]
         q_start = np.concatenate([[0], np.cumsum([len(t) for t in tokens])])
-        group_start, shared = _groups(seqs)
-        T, S, G = len(flat), len(seqs), len(shared)
-        width = max(len(s.pages) for s in seqs)
-        ids = [-1] * T if adapters is None else [a for t, a in zip(tokens, adapters) for _ in t]
-        table = [s.pages + [-1] * (width - len(s.pages)) for s in seqs]
-        parts = [flat, positions, slots, q_start, [s.length for s in seqs], group_start, shared,
-                 ids, sum(table, [])]
+        ids = [-1] * len(flat) if adapters is None else [a for t, a in zip(tokens, adapters) for _ in t]
+        table = np.full((len(seqs), max(len(s.pages) for s in seqs)), -1, dtype=np.int32)
+        for row, s in zip(table, seqs):
+            row[:len(s.pages)] = s.pages
+        return [flat, positions, slots, q_start, [s.length for s in seqs], *_groups(seqs), ids, table]
+
+    def _run(self, tokens, seqs, adapters) -> torch.Tensor:
+        cfg, w, kv = self.w.cfg, self.w, self.kv
+        parts = [np.asarray(p, dtype=np.int32) for p in self._layout(tokens, seqs, adapters)]
         # one upload for everything the step's ops read
-        meta = torch.from_numpy(np.concatenate(parts).astype(np.int32)).to(w.embed.w.device)
+        meta = torch.from_numpy(np.concatenate([p.ravel() for p in parts])).to(w.embed.w.device)
         (tok, pos, slot, q_start, kv_len, group_start, shared, ids,
-         table) = meta.split([len(p) for p in parts])
+         table) = meta.split([p.size for p in parts])
+        T, S, G, width = tok.numel(), len(seqs), shared.numel(), parts[-1].shape[1]
 
         H, I, Q, KV = cfg.hidden, cfg.inter, cfg.q_out, cfg.kv_out
         dev = w.embed.w.device
