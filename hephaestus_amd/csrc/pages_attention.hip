@@ -117,7 +117,9 @@ struct PlanArgs {
 // in chains.
 struct PlanLds {
     int32_t q_start[kMaxSeqs + 1], kv_len[kMaxSeqs], group_start[kMaxSeqs + 1], shared[kMaxSeqs];
-    int32_t few[kMaxSeqs + 1], few_tokens[kMaxSeqs + 1];   // before each sequence: those of less than 64 rows
+    // before each sequence: how many have less than 64 rows, with 2^16 times how many have
+    // 64, and the tokens of the former
+    int32_t few[kMaxSeqs + 1], few_tokens[kMaxSeqs + 1];
 };
 
 // Rows that work on the same pages: a group's on its shared ones, or one
@@ -148,19 +150,26 @@ __device__ __forceinline__ void set_tiles(Source& x, int G)
 }
 
 // The group's sequences and shared pages; none where sharing gains nothing. Sequences of
-// 64 rows or more are bound by the matrix cores and re-read a prefix from the caches; in a
+// more than 64 rows are bound by the matrix cores and re-read a prefix from the caches; in a
 // shared one each of their rows pays another partial result, 1.5 KB written and read. It is
 // shared for the others, two or more, if the pages that they need not stream again, 16 KB
 // each, outweigh that (64 single tokens and a prompt of 1100 behind 64 pages 199 us -> 170,
 // 16 and 500 behind 32 pages 57 -> 49; by the mean of all, as it was, one long prompt could
-// take the sharing from all others).
+// take the sharing from all others). Sequences of 64 rows stream too (attend_narrow), but
+// pay for 64 rows each: they count where the prefix is long and what they stream of it
+// again is 16 MB or more (100 own keys each; 64 of 16 tokens, 32 + 8 heads: 256 pages
+// 479 us -> 288, 64 pages 135 -> 98, but 16 pages 47 -> 56; 16 of one token, 64 + 1 heads:
+// 256 pages 39 -> 35; four of them 22 -> 27).
+constexpr int kLongPrefix = 32;
 __device__ Source group_source(const PlanLds& in, const PlanArgs& a, int g)
 {
     const int s0 = clampi(in.group_start[g], 0, a.s.n_seqs);
     const int s1 = clampi(in.group_start[g + 1], s0, a.s.n_seqs);
     const int t0 = clampi(in.q_start[s0], 0, a.s.n_tok), t1 = clampi(in.q_start[s1], t0, a.s.n_tok);
     int pages = clampi(in.shared[g], 0, a.table_pages);
-    const int few = in.few[s1] - in.few[s0];
+    const int counts = in.few[s1] - in.few[s0], full = counts >> 16;
+    const bool again = pages >= kLongPrefix && (long)(full - 1) * pages * a.s.n_kv >= 1024;
+    const int few = (counts & 0xFFFF) + (again ? full : 0);
     const long many_rows = (long)(t1 - t0 - (in.few_tokens[s1] - in.few_tokens[s0])) * a.s.group();
     if (few < 2 || many_rows > 10L * (few - 1) * pages) pages = 0;
     Source x{s0, t0, t1 - t0, 0, pages, 0};
@@ -304,20 +313,21 @@ __global__ __launch_bounds__(kMaxSeqs) void plan_kernel(PlanArgs a)
     if (t == 0) merges = 0;
     __syncthreads();
     {
-        int n = 0;
+        int n = 0, mine = 0;
         if (t < a.s.n_seqs) {
             const int t0 = clampi(in.q_start[t], 0, a.s.n_tok);
             n = clampi(in.q_start[t + 1], t0, a.s.n_tok) - t0;
-            if (n * G >= 64) n = 0;
+            mine = n * G == kNarrow ? 1 << 16 : n > 0 && n * G < kNarrow;
+            if (n * G >= kNarrow) n = 0;
         }
-        int few = n > 0, few_tokens = n;
+        int few = mine, few_tokens = n;
         scan_block(few, few_tokens, red_i);         // (few_tokens: behind few's total, in all of them)
         if (t == 0) {
             in.few[0] = few;
             in.few_tokens[0] = few_tokens;
         }
         if (t < a.s.n_seqs) {
-            in.few[t + 1] = few + (n > 0);
+            in.few[t + 1] = few + mine;
             in.few_tokens[t + 1] = few_tokens + n;
         }
         __syncthreads();

@@ -90,8 +90,12 @@ int heph_qk_norm_rope_pages(void* q_out_bf16, int64_t q_stride, const void* qkv_
  * group_start[g+1]-1 (n_groups + 1 entries, not decreasing), whose first
  * shared_pages[g] page-table entries are the same pages. Their keys are read
  * once for the group's rows together, from the table row of the group's first
- * sequence. Sequences in no group, or n_groups = 0 with both NULL: nothing
- * shared. A shared_pages beyond a sequence's own keys is allowed.
+ * sequence, if two or more of its sequences have less than 64 rows (tokens x
+ * heads a kv head), or enough of them 64 behind a long prefix, and longer
+ * prompts' rows would not pay more for it than that saves; else for each sequence
+ * from its own table row, with the same answer up to the order of sums. Sequences in no
+ * group, or n_groups = 0 with both NULL: nothing shared. A shared_pages beyond a
+ * sequence's own keys is allowed.
  *
  * heph_pages_attention_plan (one small launch) lays out a step's work from
  * the lengths in device memory; one plan serves the attention of every layer

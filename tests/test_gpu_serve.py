@@ -327,6 +327,29 @@ def test_attention_shared_prefix(new, own, shared, group_start):
     check_attention(b, run_attention(b))
 
 
+def prefix_rows(plan):
+    """Rows of the plan's units that work on a shared prefix."""
+    words = plan.plan.cpu().numpy().view(np.int32)
+    n_units, first = int(words[7]), 12 + 8 * plan.n_tok
+    units = words[first:first + 8 * n_units].reshape(n_units, 8)      # rows: 3, prefix: 7
+    return int(units[units[:, 7] != 0, 3].sum()) if n_units else 0
+
+
+@pytest.mark.parametrize("n,new,H,KV,shared,planned", [
+    (30, 1, 64, 1, 40, True),          # one token of 64 heads a kv head
+    (6, 16, 32, 8, 40, True), (9, 8, 16, 2, 70, True),
+    (30, 1, 64, 1, 31, False), (4, 16, 32, 8, 40, False),       # too short, too few
+    (9, 4, 32, 8, 3, True),            # less than 64 rows: always
+    (30, 17, 16, 4, 40, False),        # more than 64
+])
+def test_attention_sequences_of_64_rows_share_a_long_prefix(n, new, H, KV, shared, planned):
+    b = batch([new] * n, [new + 7 * i % 90 for i in range(n)], [shared], [0, n], seed=n + new, H=H, KV=KV)
+    plan = make_plan(b)
+    assert prefix_rows(plan) % (n * new * H // KV) == 0 and (prefix_rows(plan) > 0) == planned
+    rng = np.random.default_rng(n)
+    check_attention(b, run_attention(b, plan), tokens=set(rng.integers(0, b["T"], 25).tolist()))
+
+
 def test_attention_shared_equals_unshared():
     # what is shared changes where keys are summed, not what is summed
     b = batch([1] * 12, [30 * i + 1 for i in range(12)], [9], [0, 12], seed=77)
