@@ -5,6 +5,7 @@ Tolerances are counted from the roundings each op documents (half a step is
 summed in f32 in any order are within n * 2^-24 of the sum of magnitudes.
 """
 import math
+from types import SimpleNamespace
 
 import numpy as np
 import pytest
@@ -189,6 +190,32 @@ def test_qk_far_positions_and_extreme_values():
     c = qk_case(9, 8, 4, seed=8)
     c["qkv"][2] = 0
     check_qk(c, 8, 4)
+
+
+def test_qk_nan_and_infinities():
+    # a NaN of k or v becomes the code of -448 in the cache, an infinite v the largest code;
+    # a NaN in a head of k reaches all of it (its norm), one in v no other element
+    for T in (9, 600):                                     # both windows of V
+        c = qk_case(T, 8, 4, seed=T)
+        x = c["qkv"]
+        x[1, 8 + 2, 77] = float("nan")
+        x[2, 12 + 1, 5], x[2, 12 + 1, 6], x[2, 12 + 1, 7] = float("nan"), float("inf"), -float("inf")
+        x[3, 4, 0] = float("nan")
+        rope = S.rope_table_f32(c["n_pos"])
+        clean = dict(c, k=c["k"].clone(), v=c["v"].clone(), q=c["q"].clone(), qkv=x.nan_to_num(0, 1, -1))
+        for d in (c, clean):
+            S.qk_norm_rope_pages(d["q"], d["qkv"], *d["gam"], d["k"], d["v"], d["inv"], rope, d["pos"],
+                                 d["slot"])
+        torch.cuda.synchronize()
+        want_k, want_v, want_q = k_rows(clean["k"]), v_rows(clean["v"]), f64(clean["q"])
+        slot = c["slot"].cpu().long()
+        want_k[slot[1], 2] = -448
+        want_v[slot[2], 1, 5:8] = torch.tensor([-448.0, 448.0, -448.0]).double()
+        assert torch.equal(k_rows(c["k"]), want_k) and torch.equal(v_rows(c["v"]), want_v)
+        got = f64(c["q"])
+        assert torch.isnan(got[3, 4]).all()
+        got[3, 4] = want_q[3, 4]
+        assert torch.equal(got, want_q)
 
 
 def test_rope_table_f32():
@@ -1041,6 +1068,36 @@ def test_batch_decoder_rows_do_not_depend_on_their_batch():
     with pytest.raises(MemoryError):
         d.step([[1] * 1900, [1] * 1900], [a, b])
     assert a.length == 101 and d.kv.free_pages == 40 - len(set(a.pages + b.pages + alone.pages))
+
+
+def test_batch_decoder_gate_notices_mistakes():
+    # the bound that the steps above are held to is one that a mistake breaks: each is planted in
+    # the restatement (adapters of the feed-forward four times as strong, so that each counts)
+    lora = lora_weights(seed=6)
+    for layer in lora.layers:
+        for op in ("gate_up", "down"):
+            if op in layer:
+                layer[op] = (layer[op][0], layer[op][1] * 4)
+    d = decoder(seed=3, lora=lora)
+    rng = np.random.default_rng(3)
+    hist = [rng.integers(0, CFG.vocab, n).tolist() for n in (6, 70)]
+    seqs, adapters = [d.kv.new() for _ in hist], [2, 1]
+    d.step([h[:-1] for h in hist], seqs, adapters)
+    got = d.step([h[-1:] for h in hist], seqs, adapters)
+
+    def off(i, history=None, adapter=adapters, layers=lora.layers):
+        other = SimpleNamespace(w=d.w, kv=d.kv, lora=SimpleNamespace(scale=lora.scale, layers=layers))
+        return near(got[i], step_reference(other, history or hist[i], adapter[i]))
+    assert off(0) < 0.1 and off(1) < 0.1
+    for li, layer in enumerate(lora.layers):
+        for op in layer:
+            without = [dict(x) for x in lora.layers]
+            del without[li][op]
+            assert off(0, layers=without) > 0.1 and off(1, layers=without) > 0.1, (li, op)
+    assert off(0, adapter=[1, 0]) > 0.1 and off(1, adapter=[1, 0]) > 0.1
+    h = hist[0]
+    for history in (h[1:], h[:-2] + h[-1:], [h[1], h[0]] + h[2:], h[:-1] + [(h[-1] + 1) % CFG.vocab]):
+        assert off(0, history=history) > 0.1, history            # a key lost, two slots swapped
 
 
 def test_captured_step_of_all_ops():
