@@ -9,11 +9,11 @@
 // bf16 of its remainder (16 bits of mantissa): the product has matrix cores to
 // spare, as both launches are bound by what they stream.
 //
-// Measured (rank 16 unless said, graph replays): 5 rows of 3 adapters, 2560 -> 6144
-// 6.9 us, two launches of a chain of four loads each; 64 rows of 40 adapters, 2560 ->
-// 19456 11.1 us (33 MB, 3.0 TB/s); 4090 rows, 9728 -> 2560, rank 64, 40 us (129 MB,
-// 3.2 TB/s). One launch for both products, each workgroup with all of t for itself,
-// was slower throughout.
+// Measured (rank 16 unless said): 5 rows of 3 adapters, 2560 -> 6144 6.9 us, two launches
+// of a chain of four loads each; 64 rows that use 32 of 40 adapters, 2560 -> 19456, 28 MB,
+// 14.6 us (1.9 TB/s), 11.4 replayed on the same buffers, which the last-level cache holds;
+// 4090 rows, 9728 -> 2560, rank 64, 41 us (123 MB, 3.0 TB/s), in f32 46. One launch for both
+// products, each workgroup with all of t for itself, was slower throughout.
 #include <algorithm>
 #include <type_traits>
 
@@ -34,7 +34,12 @@ struct Tile {
     int adapter, start, count, pad;
 };
 
-// Rows of a tile: a decode batch has few of each adapter, a prompt's rows fill 64.
+// Rows of a tile: a decode batch has few of each adapter, a prompt's rows fill 64. Tiles of
+// 16 and of 64 rows, us (2560 -> 6144 of rank 16; 9728 -> 2560 of rank 64): 128 rows of 8
+// adapters 8.2, 9.3; 12, 14. 256 of 40 9.8, 15; 21, 24. 512 of 8 9.4, 12; 20, 24. 1000 of 8
+// 15, 16; 29, 25. 2000 of 40 26, 21; 62, 31. 2000 of 200 25, 32; 82, 83. The tiles of
+// 16 win up to about 700 rows, with few rows of each adapter further still: the line lies
+// lower than it could, at the longest decode batch that they were built for.
 __host__ __device__ __forceinline__ int tile_rows(int M) { return M <= 256 ? 16 : 64; }
 __host__ __device__ __forceinline__ int max_tiles(int M, int n_adapters)
 {
@@ -47,8 +52,8 @@ __host__ __device__ inline int* plan_rows(PlanHeader* p, int M, int n_adapters)
     return reinterpret_cast<int*>(plan_tiles(p) + max_tiles(M, n_adapters));
 }
 
-// Counting sort of the rows by adapter in one workgroup, once a step: 2.4 us for 64 rows,
-// 6.3 for 4090 (two passes over the ids). Rows of one adapter come in no fixed order; no
+// Counting sort of the rows by adapter in one workgroup, once a step: 2.8 us for 64 rows,
+// 6.2 for 4090 (two passes over the ids). Rows of one adapter come in no fixed order; no
 // result depends on it.
 __global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanHeader* plan, const int32_t* ids, int M,
                                                             int n_adapters)
@@ -630,11 +635,11 @@ int heph_lora_add(void* c, int c_dtype, const void* base, const uint16_t* x_bf16
         return HEPH_ERR_WORKSPACE;
     const int tiles = max_tiles(M, n_adapters), splits = k_splits(M, n_adapters, K);
     // Columns a workgroup, each of which joins the parts of t for itself: for four workgroups
-    // a CU of decode tiles (two: 64 rows of 40 adapters, 2560 -> 19456, 13.7 us instead of
-    // 11.1), six of a prompt's, but then 256 columns each while these fill half of the device
-    // (two: 4090 rows -> 19456 111 us, 96; 128 columns: 1000 rows of rank 128 49 us, 39). A
+    // a CU of decode tiles (two: 64 rows of 40 adapters, 2560 -> 19456, 13.6 us instead of
+    // 11.4, replayed), six of a prompt's, but then 256 columns each while these fill half of the device
+    // (two: 4090 rows -> 19456 111 us, 96; 128 columns: 1000 rows of rank 128 47 us, 37). A
     // wave takes its steps together where there are two rounds of them or more; the columns
-    // are then whole rounds, in decode rather fewer (more: 12.1 us in the case above).
+    // are then whole rounds, in decode rather fewer (more: 12.3 us in the case above).
     const bool f32 = c_dtype == HEPH_DTYPE_F32, decode = tile_rows(M) == 16;
     const int round = 128 * (decode ? expand_steps<1>(rank) : expand_steps<4>(rank));
     const int least = !decode && (int64_t)tiles * (N / 256) >= kPlanCUs / 2 ? 256 : 128;

@@ -23,9 +23,9 @@
 // the workspace and merge_kernel joins them.
 //
 // Measured (8 kv heads, 32 heads, graph replays): 64 sequences x 4096 keys of their
-// own 101 us, 5.3 TB/s of K and V; 16 prompts of 128 tokens behind 20000 keys 694 us,
-// 964 TFLOP/s (a library product of 8192^3 in bf16 reaches 1240); one sequence of
-// 32768 keys 24.5 us.
+// own 102 us, 5.3 TB/s of K and V; 16 prompts of 128 tokens behind 20000 keys 706 us,
+// 948 TFLOP/s (a library product of 8192^3 in bf16 reaches 1240); one sequence of
+// 32768 keys 24.3 us.
 #include <algorithm>
 #include <type_traits>
 
@@ -65,9 +65,9 @@ __host__ __device__ __forceinline__ int wide_rows(int G) { return 128 / G * G; }
 // Pages a unit has at least: fewer would not keep the four waves of a narrow one
 // busy, and writing and joining a wide one's 128 rows would outweigh its pages (4 pages
 // instead of 8: two prefixes of 64 pages, 32 sequences each, beside 1000 keys a sequence,
-// four layers 163 us instead of 140, 16 pages 167; alone, a prefix of 48 pages for 32
-// sequences gained from 4, 22.5 us -> 18.3. Narrow units of 8 pages: four sequences of 512
-// keys, four layers, 48.7 us instead of 45.0).
+// four layers 156 us instead of 134, 16 pages 158; alone, a prefix of 48 pages for 32
+// sequences gained from 4, 21.2 us -> 17.2. Narrow units of 8 pages: four sequences behind
+// 512 shared keys, four layers, 45.2 us instead of 41.6).
 constexpr int kMinNarrow = 4, kMinWide = 8;
 
 struct Sizes {
@@ -153,9 +153,8 @@ __device__ __forceinline__ void set_tiles(Source& x, int G)
 // more than 64 rows are bound by the matrix cores and re-read a prefix from the caches; in a
 // shared one each of their rows pays another partial result, 1.5 KB written and read. It is
 // shared for the others, two or more, if the pages that they need not stream again, 16 KB
-// each, outweigh that (64 single tokens and a prompt of 1100 behind 64 pages 199 us -> 170,
-// 16 and 500 behind 32 pages 57 -> 49; by the mean of all, as it was, one long prompt could
-// take the sharing from all others). Sequences of 64 rows stream too (attend_narrow), but
+// each, outweigh that (not shared and shared: 64 single tokens and a prompt of 1100 behind 64
+// pages 185 us, 171; 16 and 500 behind 32 pages 53, 47). Sequences of 64 rows stream too (attend_narrow), but
 // pay for 64 rows each: they count where the prefix is long and what they stream of it
 // again is 16 MB or more (100 own keys each; 64 of 16 tokens, 32 + 8 heads: 256 pages
 // 479 us -> 288, 64 pages 135 -> 98, but 16 pages 47 -> 56; 16 of one token, 64 + 1 heads:
@@ -356,7 +355,9 @@ __global__ __launch_bounds__(kMaxSeqs) void plan_kernel(PlanArgs a)
         work_w += red_f[i].y;
     }
 
-    // Narrow runs are split so that the units fill the slots of a kv head. Wide tiles get
+    // Narrow runs are split so that the units fill the slots of a kv head, into `cap` units
+    // at most (262144 keys of one sequence, 4 heads a kv head: with one kv head, 64 of 512
+    // slots, 28 us; with two, 64 of 256, 32; with eight, all 64, 107). Wide tiles get
     // their share of the slots, of half of them where narrow units are a good part of the
     // work: a CU then streams for one while it multiplies for the other. Wide tiles that
     // fill the slots by themselves stay whole, but for those of a last round that would
@@ -820,7 +821,7 @@ __device__ __forceinline__ void wait_vm()
 // Up to 64 rows: a wave takes 16 of them and, where that leaves waves, every
 // KW-th page of the run. Bound by the stream of K and V: the next page's 16 KB
 // a wave are on their way into registers while one is worked on. (64 sequences, each
-// 1024 keys 28 us, 4.8 TB/s; 64 keys 9 us, where a chain of four loads counts: unit,
+// 1024 keys 27 us, 4.9 TB/s; 64 keys 8.3 us, where a chain of four loads counts: unit,
 // limits and page ids, q, pages.)
 __device__ __forceinline__ void attend_narrow(const AttnArgs& a, const Unit& u, int head, int ids0, uint8_t* lds)
 {
@@ -1063,7 +1064,7 @@ __device__ __forceinline__ void merge_row(const AttnArgs& a, const Token& tk, lo
         }
     };
     // (as many loads on their way as there are parts, up to 16: one sequence of 32768 keys
-    // 25.8 -> 24.4 us against eight always, four tokens behind 512 keys, four layers, 43 -> 42)
+    // 24.3 us, 25.7 with eight always; four tokens behind 512 keys, four layers, 42.0 and 42.6)
     if (n <= 4) add(std::integral_constant<int, 4>{}, 0);
     else if (n <= 8) add(std::integral_constant<int, 8>{}, 0);
     else

@@ -118,8 +118,8 @@ __device__ __forceinline__ void qk_heads(const QkArgs& a, long unit)
 // are single bytes 64 apart; where four tokens fill an aligned run of four slots (a
 // prompt's do) their bytes are neighbours. The codes meet in LDS; then sixteen lanes write
 // the dwords of up to sixteen such runs, a whole 64-byte line of a dim where the window
-// fills a page, and the tokens left over go as bytes. (4096 tokens, 32 + 8 heads: in
-// runs 18.5 us, all scattered 41.5; without any cache write 15.1.)
+// fills a page, and the tokens left over go as bytes. (4096 tokens, 32 + 8 heads, replayed on
+// the same rows: in runs 16.4 us, all scattered 45; without any cache write 14.9.)
 template <int W>
 __device__ __forceinline__ void v_window(const QkArgs& a, long unit)
 {
@@ -202,10 +202,14 @@ __device__ __forceinline__ void v_window(const QkArgs& a, long unit)
     }
 }
 
-// Bound by the stream of qkv and q: 4090 tokens, 32 + 8 heads (94 MB) 19.5 us, 4.8 TB/s;
-// 128 tokens 5.1, 3 tokens 3.8, where a chain of three loads counts. The first v_blocks workgroups take v, W tokens each,
-// the others four waves of q and k. A short batch is tokens of many sequences, whose
-// bytes are spread over many workgroups.
+// Bound by the stream of qkv and q: 4090 tokens, 32 + 8 heads (94 MB) 19 us, 4.9 TB/s;
+// 128 tokens 5.4, 3 tokens 3.8, where a chain of three loads counts. The first v_blocks
+// workgroups take v, W tokens each, the others four waves of q and k. A short batch is
+// tokens of many sequences, whose bytes are spread over many workgroups. Windows of 4 and
+// of 64 tokens, us: 128 scattered tokens 4.1, 7.7, in runs 3.7, 4.1; 512 scattered 7.9, 9.7,
+// in runs 5.3, 4.9; 1024 scattered 11.8, 13.6, in runs 8.3, 6.6; 4096 scattered 48, 45, in
+// runs 24, 16. Up to 512 tokens the windows of 4 lose no more than 8 %, behind it they lose
+// a prompt's runs more and more.
 template <int W>
 __global__ __launch_bounds__(256) void qk_pages_kernel(QkArgs a, long v_blocks)
 {

@@ -170,7 +170,8 @@ class AttentionPlan:
     """The layout of one step's attention and its workspace: update() it from
     the step's lengths in device memory, then call attention_pages for every
     layer. All sizes are fixed, so a captured step can be replayed with other
-    lengths. Calls that share a plan are ordered by the caller."""
+    lengths. Calls that share a plan are ordered by the caller, its making (a
+    fill on the current stream) and its first use on another stream too."""
 
     def __init__(self, n_seqs: int, n_tok: int, n_heads: int, n_kv: int, table_pages: int,
                  n_groups: int = 0, device="cuda"):
@@ -243,7 +244,8 @@ class LoraPlan:
     """The rows of a step grouped by adapter, and the workspace of lora_add for
     projections k -> n of up to this rank and k (of any n): update() it from the rows' adapter ids
     in device memory (an id outside [0, n_adapters): no adapter). Calls that
-    share a plan are ordered by the caller."""
+    share a plan are ordered by the caller, its making (a fill on the current
+    stream) and its first use on another stream too."""
 
     def __init__(self, m: int, n_adapters: int, rank: int, k: int, n: int | None = None,
                  device="cuda"):
