@@ -19,6 +19,7 @@ from __future__ import annotations
 
 import heapq
 from array import array
+from itertools import accumulate
 
 import numpy as np
 import torch
@@ -546,16 +547,18 @@ class Qwen3BatchDecoder:
         flat = [i for t in tokens for i in t]
         positions = [s.length + i for t, s in zip(tokens, seqs) for i in range(len(t))]
         slots = [i for t, s in zip(tokens, seqs) for i in self.kv.extend(s, len(t))]
-        q_start = np.concatenate([[0], np.cumsum([len(t) for t in tokens])])
+        q_start = [0, *accumulate(len(t) for t in tokens)]
         ids = [-1] * len(flat) if adapters is None else [a for t, a in zip(tokens, adapters) for _ in t]
         table = np.full((len(seqs), max(len(s.pages) for s in seqs)), -1, dtype=np.int32)
         for row, s in zip(table, seqs):
             row[:len(s.pages)] = s.pages
-        return [flat, positions, slots, q_start, [s.length for s in seqs], *_groups(seqs), ids, table]
+        rows = [flat, positions, slots, q_start, [s.length for s in seqs], *_groups(seqs), ids]
+        # (array: what is no whole number is refused, not rounded)
+        return [np.frombuffer(array("i", r), dtype=np.int32) for r in rows] + [table]
 
     def _run(self, tokens, seqs, adapters) -> torch.Tensor:
         cfg, w, kv = self.w.cfg, self.w, self.kv
-        parts = [np.asarray(p, dtype=np.int32) for p in self._layout(tokens, seqs, adapters)]
+        parts = self._layout(tokens, seqs, adapters)
         # one upload for everything the step's ops read
         meta = torch.from_numpy(np.concatenate([p.ravel() for p in parts])).to(w.embed.w.device)
         (tok, pos, slot, q_start, kv_len, group_start, shared, ids,

@@ -547,3 +547,18 @@ def test_common_pages():
         x, y = list(range(n)) + [100] * a, list(range(n)) + [200] * b
         assert S._common(x, y) == n
         assert S._common(x, x[:n]) == n and S._common(x, x + y) == len(x)
+
+
+@pytest.mark.parametrize("tokens,adapters", [([[1.5]], None), ([[1, 2.0]], None), ([[3]], [0.5]), ([["1"]], None)])
+def test_a_step_takes_whole_numbers_only(cache, monkeypatch, tokens, adapters):
+    c = cache
+    d = host_decoder(c, monkeypatch, lora=S.LoraWeights(torch.ones(3), [{}] * CFG.n_layers))
+    monkeypatch.setattr(d, "_run", lambda *a: [np.asarray(p) for p in d._layout(*a)])
+    a = c.new()
+    c.extend(a, 70)
+    with pytest.raises(TypeError):
+        d.step(tokens, [a], adapters)
+    assert (a.length, len(a.pages), c.free_pages) == (70, 2, 10)
+    check_counts(c)
+    tok, *_, ids, table = d.step([[np.int64(5), torch.tensor(6)]], [a], [np.int32(2)])
+    assert tok.tolist() == [5, 6] and ids.tolist() == [2, 2] and tok.dtype == ids.dtype == table.dtype == np.int32
