@@ -36,6 +36,8 @@ FLAG_ADD_RESIDUAL = 0x1
 FLAG_SKIP_QUANT = 0x2
 FLAG_FORCE_GEMM = 0x8
 FLAG_NO_FUSE = 0x10
+PICK_APPEND = 0x1
+PICK_MAX_BIAS = 4095
 
 SKINNY_MAX_M = 32
 
@@ -48,6 +50,15 @@ class LaunchOverrides(ctypes.Structure):
                 ("batch_split", ctypes.c_int), ("wide_tiles", ctypes.c_int),
                 ("wide_waves", ctypes.c_int), ("split_spin_limit", ctypes.c_int),
                 ("gemv_groups", ctypes.c_int), ("gemm_bn", ctypes.c_int)]
+
+
+class TokenRulesArgs(ctypes.Structure):
+    """heph_token_rules: sizes and device pointers of the requests' rules."""
+    _fields_ = [("n_slots", ctypes.c_int), ("max_tokens", ctypes.c_int),
+                ("max_bias", ctypes.c_int), ("history", ctypes.c_void_p),
+                ("length", ctypes.c_void_p), ("n_prompt", ctypes.c_void_p),
+                ("penalties", ctypes.c_void_p), ("bias_ids", ctypes.c_void_p),
+                ("bias", ctypes.c_void_p), ("n_bias", ctypes.c_void_p)]
 
 
 _vp = ctypes.c_void_p
@@ -101,6 +112,15 @@ SIGNATURES = {
     "heph_pages_attention": (_i, [_vp, _vp, _i64, _vp, _vp, _i, _vp, _vp, _i, _vp, _sz, _vp, _sz,
                                   _i, _i, _i, _i, _i, _i, _vp]),
     "heph_copy_pages": (_i, [_vp, _vp, _i, _i, _i, _vp, _vp, _i, _vp]),
+    "heph_qk_norm_rope_pages_scaled": (_i, [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _i, _vp, _vp,
+                                            _i, _vp, _vp, _i, _i, _i, _i, ctypes.c_float, _vp]),
+    "heph_pages_attention_scaled": (_i, [_vp, _vp, _i64, _vp, _vp, _i, _vp, _vp, _i, _vp, _sz, _vp,
+                                         _sz, _i, _i, _i, _i, _i, _i, _vp]),
+    "heph_copy_pages_scaled": (_i, [_vp, _vp, _vp, _i, _i, _i, _vp, _vp, _i, _vp]),
+    "heph_read_pages": (_i, [_vp, _vp, _vp, _vp, _i, _vp, _vp, _vp, _i, _i, _i, _vp]),
+    "heph_pick_ws_bytes": (_sz, [_i, _i]),
+    "heph_pick_tokens": (_i, [_vp, _vp, _vp, _i64, _vp, _i64, _i, _i, _i,
+                              ctypes.POINTER(TokenRulesArgs), _vp, _vp, _i, _vp, _i, _vp, _sz, _vp]),
     "heph_lora_plan_bytes": (_sz, [_i, _i]),
     "heph_lora_ws_bytes": (_sz, [_i, _i, _i, _i]),
     "heph_lora_plan": (_i, [_vp, _sz, _vp, _i, _i, _vp]),

@@ -461,7 +461,7 @@ struct AttnArgs {
     int64_t q_stride;
     const uint8_t* k_pages;
     const uint8_t* v_pages;
-    const float* kv_scale;
+    const float* kv_scale;  // the layer's, 2 * n_kv; or of each page (BLOCK), powers of two
     const int32_t* table;
     PlanHeader* plan;
     float* part_o;          // [n_kv][max_parts][128], unnormalized
@@ -481,17 +481,18 @@ __device__ __forceinline__ bool plan_fits(const PlanHeader& h, const AttnArgs& a
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 
-// Eight codes -> eight bf16 (exact).
-__device__ __forceinline__ bf16x8 bf16_of_codes(int lo, int hi)
+// Eight codes times scale, a power of two, -> eight bf16 (exact: the conversion multiplies by
+// 2^e of the scale's exponent e).
+__device__ __forceinline__ bf16x8 bf16_of_codes(int lo, int hi, float scale)
 {
     union {
         bf16x2 p[4];
         bf16x8 v;
     } r;
-    r.p[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)lo, 1.0f, false);
-    r.p[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)lo, 1.0f, true);
-    r.p[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)hi, 1.0f, false);
-    r.p[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)hi, 1.0f, true);
+    r.p[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)lo, scale, false);
+    r.p[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)lo, scale, true);
+    r.p[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)hi, scale, false);
+    r.p[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)hi, scale, true);
     return r.v;
 }
 
@@ -553,6 +554,29 @@ __device__ __forceinline__ void nan_seen(const uint8_t* vp, int key0, const int 
             for (int i = 0; i < 4; ++i) hit[r] |= n[i] > 0.0f ? 1u << (4 * d + i) : 0u;
         }
     }
+}
+
+// Scales of the cache. BLOCK: one for each page, K or V (index n_kv + head), applied where
+// codes become operands; else the layer's, applied to scores and outputs.
+constexpr float kScoreScale = 0.08838834764831845f * 1.4426950408889634f;     // 1/sqrt(128), log2(e)
+template <bool BLOCK>
+__device__ __forceinline__ float score_scale(const AttnArgs& a, int head)
+{
+    return BLOCK ? kScoreScale : a.kv_scale[head] * kScoreScale;
+}
+template <bool BLOCK>
+__device__ __forceinline__ float out_scale(const AttnArgs& a, int head)
+{
+    return BLOCK ? 1.0f : a.kv_scale[a.s.n_kv + head];
+}
+__device__ __forceinline__ float page_scale(const AttnArgs& a, int id, int index)
+{
+    // (a page that is not there is not used: any entry of the table)
+    return a.kv_scale[(size_t)(id >= 0 && id < a.n_pages ? id : 0) * 2 * a.s.n_kv + index];
+}
+__device__ __forceinline__ float lane_of(float v, int lane)
+{
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), lane));
 }
 
 // One wave's query rows: RT tiles of 16, column c of each in lane c, c+16, c+32, c+48.
@@ -763,11 +787,12 @@ struct Rows {
 
     // The rows' results over dim tiles d0 .. d0+nd-1, held in o[0 .. nd): to out
     // where the unit is the row's only one, else to its slot in the workspace.
+    template <bool BLOCK>
     __device__ __forceinline__ void store(const AttnArgs& a, const Unit& u, int head, int d0, int nd)
     {
         const int g4 = (threadIdx.x & 63) >> 4;
         const Token* tokens = plan_tokens(a.plan);
-        const float sv = a.kv_scale[a.s.n_kv + head];
+        const float sv = out_scale<BLOCK>(a, head);
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
             if (tok[r] < 0) continue;
@@ -823,6 +848,7 @@ __device__ __forceinline__ void wait_vm()
 // a wave are on their way into registers while one is worked on. (64 sequences, each
 // 1024 keys 27 us, 4.9 TB/s; 64 keys 8.3 us, where a chain of four loads counts: unit,
 // limits and page ids, q, pages.)
+template <bool BLOCK>
 __device__ __forceinline__ void attend_narrow(const AttnArgs& a, const Unit& u, int head, int ids0, uint8_t* lds)
 {
     const int l = threadIdx.x & 63, c = l & 15, g4 = l >> 4, n_kv = a.s.n_kv;
@@ -831,7 +857,7 @@ __device__ __forceinline__ void attend_narrow(const AttnArgs& a, const Unit& u, 
     Rows<1> x;
     x.init(a, u, head, wave / KW * 16);
     const int end = min(u.page0 + u.pages, (x.hi + kPage - 1) / kPage);
-    const float sc = a.kv_scale[head] * (0.08838834764831845f * 1.4426950408889634f);
+    const float sc = score_scale<BLOCK>(a, head);
     auto place = [&](int id) {
         // (a page that is not there is not used: any address in the pool)
         const int at = id >= 0 && id < a.n_pages ? id : 0;
@@ -840,12 +866,17 @@ __device__ __forceinline__ void attend_narrow(const AttnArgs& a, const Unit& u, 
     struct Page {
         i32x4 k[8], v[8];
         int id;
+        float sk, sv;
     } p0, p1;
     int ids = 0, first = 0, last = 0;
+    float sk = 1.0f, sv = 1.0f;            // of the pages of ids, one a lane
     // (past the run its last page again: a load that is left out on some path would make
     // the waits for the page before count without it, and hold up the one behind)
     auto load = [&](Page& p, int n) {
-        p.id = __builtin_amdgcn_readlane(ids, min(n, last - 1) - first);
+        const int i = min(n, last - 1) - first;
+        p.id = __builtin_amdgcn_readlane(ids, i);
+        p.sk = BLOCK ? lane_of(sk, i) : 1.0f;
+        p.sv = BLOCK ? lane_of(sv, i) : 1.0f;
         const size_t o = place(p.id);
 #pragma unroll
         for (int i = 0; i < 8; ++i) p.k[i] = ldg16(a.k_pages + o + i * 1024);
@@ -854,20 +885,24 @@ __device__ __forceinline__ void attend_narrow(const AttnArgs& a, const Unit& u, 
     };
     auto work = [&](Page& p, int n) {
         if (p.id < 0 || p.id >= a.n_pages) return;
-        auto half = [](const i32x4& w, int h) { return bf16_of_codes(w[2 * h], w[2 * h + 1]); };
+        auto half = [](const i32x4& w, int h, float s) { return bf16_of_codes(w[2 * h], w[2 * h + 1], s); };
         auto clear = [&] {
             bool any = false;
 #pragma unroll
             for (int i = 0; i < 8; ++i) any |= clear_nan(p.v[i]);
             return __any(any);
         };
-        x.page<false>(n, sc, [&](int i, int h) { return half(p.k[i], h); },
-                      [&](int i, int h) { return half(p.v[i], h); }, clear,
+        x.template page<false>(n, sc, [&](int i, int h) { return half(p.k[i], h, p.sk); },
+                      [&](int i, int h) { return half(p.v[i], h, p.sv); }, clear,
                       a.v_pages + place(p.id));
     };
     for (first = u.page0; first < end; first += 64) {
         last = min(first + 64, end);
         ids = first == u.page0 ? ids0 : page_ids(a, u, first);
+        if constexpr (BLOCK) {
+            sk = page_scale(a, ids, head);
+            sv = page_scale(a, ids, n_kv + head);
+        }
         wait_vm<0>();           // (nothing but pages on its way below)
         int n = first + kw;
         load(p0, n);
@@ -910,7 +945,7 @@ __device__ __forceinline__ void attend_narrow(const AttnArgs& a, const Unit& u, 
 #pragma unroll
         for (int d = 0; d < 4; ++d) x.o[d][0] = o[d];
     }
-    x.store(a, u, head, d0, nd);
+    x.template store<BLOCK>(a, u, head, d0, nd);
 }
 
 // Up to 128 rows, 32 a wave. Bound by the matrix cores and the VALU's share beside
@@ -927,6 +962,7 @@ constexpr int kWidePage = 2 * 2 * kPageBytes;      // K and V as bf16
 // memory stay in flight (__syncthreads would wait for them).
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
+template <bool BLOCK>
 __device__ __forceinline__ void attend_wide(const AttnArgs& a, const Unit& u, int head, int ids0, uint8_t* lds)
 {
     __shared__ int nan_page[2], lows[4];       // of each buffer's page; each wave's smallest limit
@@ -947,11 +983,12 @@ __device__ __forceinline__ void attend_wide(const AttnArgs& a, const Unit& u, in
     // and every wave has to look for those that its rows see.
     const int lo = __builtin_amdgcn_readfirstlane(min(min(lows[0], lows[1]), min(lows[2], lows[3])));
     x.lo = lo;
-    const float sc = a.kv_scale[head] * (0.08838834764831845f * 1.4426950408889634f);
+    const float sc = score_scale<BLOCK>(a, head);
     // waves 0, 1: K's 1 KB tiles 0..3, 4..7; waves 2, 3: V's
     const uint8_t* pool = (wave < 2 ? a.k_pages : a.v_pages) + (wave & 1) * 4096 + c * 64 + g4 * 16;
     for (int first = u.page0; first < end; first += 64) {
         const int last = min(first + 64, end), ids = first == u.page0 ? ids0 : page_ids(a, u, first);
+        const float scales = BLOCK ? page_scale(a, ids, (wave < 2 ? 0 : n_kv) + head) : 1.0f;
         wait_vm<0>();           // (nothing but pages on its way below)
         auto id_of = [&](int n) { return __builtin_amdgcn_readlane(ids, n - first); };
         struct Codes {
@@ -973,10 +1010,11 @@ __device__ __forceinline__ void attend_wide(const AttnArgs& a, const Unit& u, in
                 for (int i = 0; i < 4; ++i) any |= clear_nan(x.w[i]);
                 if (__any(any) && l == 0) nan_page[(n - first) & 1] = n;
             }
+            const float s = BLOCK ? lane_of(scales, n - first) : 1.0f;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                *reinterpret_cast<bf16x8*>(to + i * 2048) = bf16_of_codes(x.w[i][0], x.w[i][1]);
-                *reinterpret_cast<bf16x8*>(to + i * 2048 + 1024) = bf16_of_codes(x.w[i][2], x.w[i][3]);
+                *reinterpret_cast<bf16x8*>(to + i * 2048) = bf16_of_codes(x.w[i][0], x.w[i][1], s);
+                *reinterpret_cast<bf16x8*>(to + i * 2048 + 1024) = bf16_of_codes(x.w[i][2], x.w[i][3], s);
             }
         };
         // Page n, while the next one's codes (in c) go to the other buffer and the one
@@ -990,7 +1028,7 @@ __device__ __forceinline__ void attend_wide(const AttnArgs& a, const Unit& u, in
                 auto k = [&](int i, int h) { return *reinterpret_cast<const bf16x8*>(base + (2 * i + h) * 1024); };
                 auto v = [&](int i, int h) { return k(8 + i, h); };
                 auto clear = [&] { return nan_page[(n - first) & 1] == n; };
-                x.page<true>(n, sc, k, v, clear,
+                x.template page<true>(n, sc, k, v, clear,
                              a.v_pages + ((size_t)id * n_kv + head) * kPageBytes + c * 64 + g4 * 16);
             }
             lds_barrier();
@@ -1008,9 +1046,10 @@ __device__ __forceinline__ void attend_wide(const AttnArgs& a, const Unit& u, in
             step(c1, n + 1);
         }
     }
-    x.store(a, u, head, 0, 8);
+    x.template store<BLOCK>(a, u, head, 0, 8);
 }
 
+template <bool BLOCK>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void attention_kernel(AttnArgs a)
 {
     __shared__ __attribute__((aligned(16))) uint8_t lds[2 * kWidePage];
@@ -1021,12 +1060,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     const Unit u = plan_units(a.plan, a.s.n_tok)[unit];        // (the plan has room for all of the grid's)
     if (!plan_fits(h, a) || unit >= h.n_units) return;
     const int ids = page_ids(a, u, u.page0);        // (on its way while the rows are looked at)
-    if (u.rows <= kNarrow) attend_narrow(a, u, head, ids, lds);
-    else attend_wide(a, u, head, ids, lds);
+    if (u.rows <= kNarrow) attend_narrow<BLOCK>(a, u, head, ids, lds);
+    else attend_wide<BLOCK>(a, u, head, ids, lds);
 }
 
 // Joins the partial results of a row, two dims a lane. A row of one unit is
 // finished already.
+template <bool BLOCK>
 __device__ __forceinline__ void merge_row(const AttnArgs& a, const Token& tk, long row, int l)
 {
     const int h = (int)(row % a.s.n_heads), n = min(tk.n_prefix + tk.n_own, 128), G = a.s.group();
@@ -1069,14 +1109,14 @@ __device__ __forceinline__ void merge_row(const AttnArgs& a, const Token& tk, lo
     else if (n <= 8) add(std::integral_constant<int, 8>{}, 0);
     else
         for (int k = 0; k < n; k += 16) add(std::integral_constant<int, 16>{}, k);
-    const float f = sum == 0.0f && top == -INFINITY ? 0.0f
-                                                    : a.kv_scale[a.s.n_kv + h / a.s.group()] / sum;
+    const float f = sum == 0.0f && top == -INFINITY ? 0.0f : out_scale<BLOCK>(a, h / G) / sum;
     *reinterpret_cast<uint32_t*>(a.out + row * kHeadDim + 2 * l) =
         (uint32_t)f32_to_bf16(x * f) | (uint32_t)f32_to_bf16(y * f) << 16;
 }
 
 // One wave a row at a time; nothing to do where every row has one unit.
 constexpr int kMergeBlocks = 2048;
+template <bool BLOCK>
 __global__ __launch_bounds__(256) void merge_kernel(AttnArgs a)
 {
     PlanHeader head = *a.plan;
@@ -1094,7 +1134,7 @@ __global__ __launch_bounds__(256) void merge_kernel(AttnArgs a)
             auto of = [&](int v) { return __builtin_amdgcn_readlane(v, k); };
             const Token t{of(tk.limit), of(tk.n_prefix), of(tk.n_own), of(tk.prefix), of(tk.prefix_step),
                           of(tk.own), of(tk.own_step), 0};
-            merge_row(a, t, row0 + k * step, threadIdx.x & 63);
+            merge_row<BLOCK>(a, t, row0 + k * step, threadIdx.x & 63);
         }
     }
 }
@@ -1109,6 +1149,54 @@ bool sizes_ok(int n_tok, int n_seqs, int n_groups, int n_heads, int n_kv)
 }  // namespace heph
 
 using namespace heph;
+
+// scale: kv_scale, or (BLOCK) page_scale.
+template <bool BLOCK>
+static int attend(void* out_bf16, const void* q_bf16, int64_t q_stride,
+                         const uint8_t* k_pages, const uint8_t* v_pages, int n_pages,
+                         const float* scale, const int32_t* page_table, int table_pages,
+                         const void* plan, size_t plan_bytes, void* ws, size_t ws_bytes,
+                         int n_tok, int n_seqs, int n_groups, int n_heads, int n_kv_heads,
+                         int head_dim, void* stream)
+{
+    if (!out_bf16 || !q_bf16 || !k_pages || !v_pages || !scale || !page_table || !plan || !ws)
+        return HEPH_ERR_NULL;
+    if (head_dim != kHeadDim || !sizes_ok(n_tok, n_seqs, n_groups, n_heads, n_kv_heads) ||
+        n_pages < 1 || table_pages < 1 || table_pages > HEPH_ATTN_MAX_KEYS / kPage ||
+        q_stride < (int64_t)n_heads * kHeadDim || out_bf16 == q_bf16)
+        return HEPH_ERR_SHAPE;
+    if (!aligned(out_bf16, 16) || !aligned(q_bf16, 16) || !aligned(k_pages, 16) ||
+        !aligned(v_pages, 16) || !aligned(plan, 16) || !aligned(ws, 16) || q_stride % 8)
+        return HEPH_ERR_ALIGN;
+    if (plan_bytes < heph_pages_attention_plan_bytes(n_tok, n_seqs, n_groups, n_heads, n_kv_heads) ||
+        ws_bytes < heph_pages_attention_ws_bytes(n_tok, n_seqs, n_groups, n_heads, n_kv_heads))
+        return HEPH_ERR_WORKSPACE;
+    AttnArgs a;
+    a.s = Sizes{n_tok, n_seqs, n_groups, n_heads, n_kv_heads};
+    // no unit has fewer pages than kMinNarrow unless it is its rows' only one
+    const long tiles = (long)n_tok * a.s.group() / wide_rows(a.s.group()) * 2 + n_seqs + n_groups;
+    const long blocks = std::min(a.s.max_units(), tiles * ((table_pages + kMinNarrow - 1) / kMinNarrow)) *
+                        n_kv_heads;
+    const long merges = std::min((a.s.rows() + 3) / 4, (long)kMergeBlocks);
+    if (blocks > INT32_MAX) return HEPH_ERR_UNSUPPORTED;
+    if (int st = check_device()) return st;
+    a.out = static_cast<uint16_t*>(out_bf16);
+    a.q = static_cast<const uint16_t*>(q_bf16);
+    a.q_stride = q_stride;
+    a.k_pages = k_pages;
+    a.v_pages = v_pages;
+    a.kv_scale = scale;
+    a.table = page_table;
+    a.plan = static_cast<PlanHeader*>(const_cast<void*>(plan));
+    a.part_o = static_cast<float*>(ws);
+    a.part_ml = reinterpret_cast<float2*>(a.part_o + (size_t)n_kv_heads * a.s.max_parts() * kHeadDim);
+    a.n_pages = n_pages;
+    a.table_pages = table_pages;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    attention_kernel<BLOCK><<<(unsigned)blocks, 256, 0, s>>>(a);
+    merge_kernel<BLOCK><<<(unsigned)merges, 256, 0, s>>>(a);
+    return status_of(hipGetLastError());
+}
 
 extern "C" {
 
@@ -1156,43 +1244,21 @@ int heph_pages_attention(void* out_bf16, const void* q_bf16, int64_t q_stride,
                          int n_tok, int n_seqs, int n_groups, int n_heads, int n_kv_heads,
                          int head_dim, void* stream)
 {
-    if (!out_bf16 || !q_bf16 || !k_pages || !v_pages || !kv_scale || !page_table || !plan || !ws)
-        return HEPH_ERR_NULL;
-    if (head_dim != kHeadDim || !sizes_ok(n_tok, n_seqs, n_groups, n_heads, n_kv_heads) ||
-        n_pages < 1 || table_pages < 1 || table_pages > HEPH_ATTN_MAX_KEYS / kPage ||
-        q_stride < (int64_t)n_heads * kHeadDim || out_bf16 == q_bf16)
-        return HEPH_ERR_SHAPE;
-    if (!aligned(out_bf16, 16) || !aligned(q_bf16, 16) || !aligned(k_pages, 16) ||
-        !aligned(v_pages, 16) || !aligned(plan, 16) || !aligned(ws, 16) || q_stride % 8)
-        return HEPH_ERR_ALIGN;
-    if (plan_bytes < heph_pages_attention_plan_bytes(n_tok, n_seqs, n_groups, n_heads, n_kv_heads) ||
-        ws_bytes < heph_pages_attention_ws_bytes(n_tok, n_seqs, n_groups, n_heads, n_kv_heads))
-        return HEPH_ERR_WORKSPACE;
-    AttnArgs a;
-    a.s = Sizes{n_tok, n_seqs, n_groups, n_heads, n_kv_heads};
-    // no unit has fewer pages than kMinNarrow unless it is its rows' only one
-    const long tiles = (long)n_tok * a.s.group() / wide_rows(a.s.group()) * 2 + n_seqs + n_groups;
-    const long blocks = std::min(a.s.max_units(), tiles * ((table_pages + kMinNarrow - 1) / kMinNarrow)) *
-                        n_kv_heads;
-    const long merges = std::min((a.s.rows() + 3) / 4, (long)kMergeBlocks);
-    if (blocks > INT32_MAX) return HEPH_ERR_UNSUPPORTED;
-    if (int st = check_device()) return st;
-    a.out = static_cast<uint16_t*>(out_bf16);
-    a.q = static_cast<const uint16_t*>(q_bf16);
-    a.q_stride = q_stride;
-    a.k_pages = k_pages;
-    a.v_pages = v_pages;
-    a.kv_scale = kv_scale;
-    a.table = page_table;
-    a.plan = static_cast<PlanHeader*>(const_cast<void*>(plan));
-    a.part_o = static_cast<float*>(ws);
-    a.part_ml = reinterpret_cast<float2*>(a.part_o + (size_t)n_kv_heads * a.s.max_parts() * kHeadDim);
-    a.n_pages = n_pages;
-    a.table_pages = table_pages;
-    hipStream_t s = static_cast<hipStream_t>(stream);
-    attention_kernel<<<(unsigned)blocks, 256, 0, s>>>(a);
-    merge_kernel<<<(unsigned)merges, 256, 0, s>>>(a);
-    return status_of(hipGetLastError());
+    return attend<false>(out_bf16, q_bf16, q_stride, k_pages, v_pages, n_pages, kv_scale, page_table, table_pages,
+                         plan, plan_bytes, ws, ws_bytes, n_tok, n_seqs, n_groups, n_heads, n_kv_heads,
+                         head_dim, stream);
+}
+
+int heph_pages_attention_scaled(void* out_bf16, const void* q_bf16, int64_t q_stride,
+                         const uint8_t* k_pages, const uint8_t* v_pages, int n_pages,
+                         const float* page_scale, const int32_t* page_table, int table_pages,
+                         const void* plan, size_t plan_bytes, void* ws, size_t ws_bytes,
+                         int n_tok, int n_seqs, int n_groups, int n_heads, int n_kv_heads,
+                         int head_dim, void* stream)
+{
+    return attend<true>(out_bf16, q_bf16, q_stride, k_pages, v_pages, n_pages, page_scale, page_table, table_pages,
+                         plan, plan_bytes, ws, ws_bytes, n_tok, n_seqs, n_groups, n_heads, n_kv_heads,
+                         head_dim, stream);
 }
 
 }  // extern "C"

@@ -13,8 +13,9 @@ namespace {
 constexpr int kPairs = 256;
 struct CopyArgs {
     uint8_t* pool[2];
+    float* scale;                  // [n_layers][n_pages][2 * n_kv], or NULL
     size_t page_bytes, layer_bytes;
-    int n_kv;
+    int n_kv, n_pages;
     int src[kPairs], dst[kPairs];
 };
 
@@ -31,6 +32,10 @@ __global__ __launch_bounds__(256) void copy_pages_kernel(CopyArgs a)
     const uint4 x = ldg16u(from + o), y = ldg16u(from + o + 4096);
     *reinterpret_cast<uint4*>(to + o) = x;
     *reinterpret_cast<uint4*>(to + o + 4096) = y;
+    if (a.scale && threadIdx.x == 0) {             // the block's scale
+        float* s = a.scale + ((size_t)blockIdx.y * a.n_pages * 2 + blockIdx.z) * a.n_kv + head;
+        s[(size_t)a.dst[pair] * 2 * a.n_kv] = s[(size_t)a.src[pair] * 2 * a.n_kv];
+    }
 }
 
 }  // namespace
@@ -38,15 +43,14 @@ __global__ __launch_bounds__(256) void copy_pages_kernel(CopyArgs a)
 
 using namespace heph;
 
-extern "C" int heph_copy_pages(uint8_t* k_pages, uint8_t* v_pages, int n_layers, int n_pages,
-                               int n_kv_heads, const int32_t* src, const int32_t* dst, int n,
-                               void* stream)
+static int copy_pages(uint8_t* k_pages, uint8_t* v_pages, float* scale, int n_layers, int n_pages,
+                      int n_kv_heads, const int32_t* src, const int32_t* dst, int n, void* stream)
 {
     if (!k_pages || !v_pages || (n > 0 && (!src || !dst))) return HEPH_ERR_NULL;
     if (n_layers < 1 || n_layers > 65535 || n_pages < 1 || n_kv_heads < 1 || n_kv_heads > 4096 ||
         n < 0 || n > n_pages)
         return HEPH_ERR_SHAPE;
-    if (!aligned(k_pages, 16) || !aligned(v_pages, 16)) return HEPH_ERR_ALIGN;
+    if (!aligned(k_pages, 16) || !aligned(v_pages, 16) || !aligned(scale, 4)) return HEPH_ERR_ALIGN;
     if (n == 0) return HEPH_OK;
     try {
         // destinations that repeat or are read by another pair would race
@@ -69,6 +73,8 @@ extern "C" int heph_copy_pages(uint8_t* k_pages, uint8_t* v_pages, int n_layers,
     a.page_bytes = (size_t)n_kv_heads * kPageBytes;
     a.layer_bytes = (size_t)n_pages * a.page_bytes;
     a.n_kv = n_kv_heads;
+    a.n_pages = n_pages;
+    a.scale = scale;
     for (int i = 0; i < n; i += kPairs) {
         const int pairs = std::min(kPairs, n - i);
         std::copy(src + i, src + i + pairs, a.src);
@@ -78,3 +84,21 @@ extern "C" int heph_copy_pages(uint8_t* k_pages, uint8_t* v_pages, int n_layers,
     }
     return HEPH_OK;
 }
+
+extern "C" {
+
+int heph_copy_pages(uint8_t* k_pages, uint8_t* v_pages, int n_layers, int n_pages, int n_kv_heads,
+                    const int32_t* src, const int32_t* dst, int n, void* stream)
+{
+    return copy_pages(k_pages, v_pages, nullptr, n_layers, n_pages, n_kv_heads, src, dst, n, stream);
+}
+
+int heph_copy_pages_scaled(uint8_t* k_pages, uint8_t* v_pages, float* page_scale, int n_layers,
+                           int n_pages, int n_kv_heads, const int32_t* src, const int32_t* dst,
+                           int n, void* stream)
+{
+    if (!page_scale) return HEPH_ERR_NULL;
+    return copy_pages(k_pages, v_pages, page_scale, n_layers, n_pages, n_kv_heads, src, dst, n, stream);
+}
+
+}  // extern "C"

@@ -1,6 +1,6 @@
 // pages_qk.hip - q/k norm per head, rotation and the write of k and v into the
 // paged cache for a batch of tokens, and the rotation table it reads.
-#include "pages.h"
+#include "pages_norm.h"
 
 namespace heph {
 namespace {
@@ -33,21 +33,6 @@ struct QkArgs {
     float eps;
 };
 
-__device__ __forceinline__ void unpack8(const uint4& w, float* f)
-{
-    const uint32_t d[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        f[2 * i] = bf16lo(d[i]);
-        f[2 * i + 1] = bf16hi(d[i]);
-    }
-}
-
-__device__ __forceinline__ uint32_t pack2_bf16(float a, float b)
-{
-    return (uint32_t)f32_to_bf16(a) | (uint32_t)f32_to_bf16(b) << 16;
-}
-
 __device__ __forceinline__ float clamp_e4m3(float v) { return fminf(fmaxf(v, -kE4M3Max), kE4M3Max); }
 
 __device__ __forceinline__ uint2 codes8(const float* f, float inv)
@@ -77,34 +62,11 @@ __device__ __forceinline__ void qk_heads(const QkArgs& a, long unit)
     if (pos < 0 || pos >= a.n_rope) return;
     const float4* cs = reinterpret_cast<const float4*>(a.rope + (size_t)pos * kHeadDim + 16 * c);
     const float4 w[4] = {cs[0], cs[1], cs[2], cs[3]};
-    float lo[8], hi[8], g_lo[8], g_hi[8];
-    unpack8(x_lo, lo);
-    unpack8(x_hi, hi);
-    unpack8(y_lo, g_lo);
-    unpack8(y_hi, g_hi);
-    float ss = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) ss = __builtin_fmaf(lo[i], lo[i], __builtin_fmaf(hi[i], hi[i], ss));
-#pragma unroll
-    for (int m = 1; m < 8; m <<= 1) ss += __shfl_xor(ss, m);
-    const float r = 1.0f / __fsqrt_rn(ss * (1.0f / kHeadDim) + a.eps);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float cc[2] = {w[i].x, w[i].z}, sn[2] = {w[i].y, w[i].w};
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const int e = 2 * i + j;
-            const float x = g_lo[e] * (lo[e] * r), y = g_hi[e] * (hi[e] * r);
-            lo[e] = x * cc[j] - y * sn[j];
-            hi[e] = y * cc[j] + x * sn[j];
-        }
-    }
+    float lo[8], hi[8];
+    norm_rope(lo, hi, x_lo, x_hi, y_lo, y_hi, w, a.eps);
     if (is_q) {
         uint16_t* out = a.q_out + t * a.q_stride + (size_t)h * kHeadDim + 8 * c;
-        *reinterpret_cast<uint4*>(out) = make_uint4(pack2_bf16(lo[0], lo[1]), pack2_bf16(lo[2], lo[3]),
-                                                    pack2_bf16(lo[4], lo[5]), pack2_bf16(lo[6], lo[7]));
-        *reinterpret_cast<uint4*>(out + 64) = make_uint4(pack2_bf16(hi[0], hi[1]), pack2_bf16(hi[2], hi[3]),
-                                                         pack2_bf16(hi[4], hi[5]), pack2_bf16(hi[6], hi[7]));
+        store_head(out, lo, hi);
     } else if (slot >= 0 && slot < a.n_slots) {
         const int e = h - a.n_heads, key = (int)(slot % kPage);
         const float inv = a.kv_inv[e];

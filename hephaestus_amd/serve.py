@@ -1,5 +1,7 @@
 """A batched serving step of a Qwen3 model around the W8A8 linears: the paged
-E4M3 KV cache, the ops of include/hephserve.h and a batch decoder on them.
+E4M3 KV cache (one scale a layer's head, or one a page and head found while it is
+written), the ops of include/hephserve.h, a batch decoder on them and the pick of
+its next tokens.
 
     per layer, T tokens of S sequences:
         qkv = rmsnorm(x, attn_norm) @ Wqkv^T             heph_rmsnorm_quant_fp8, heph_fp8_linear
@@ -10,6 +12,9 @@ E4M3 KV cache, the ops of include/hephserve.h and a batch decoder on them.
         x  += att @ Wo^T                                 heph_fp8_linear + ADD_RESIDUAL
         act = silu(gate) * up of rmsnorm(x) @ Wgu^T      heph_silu_mul_quant_fp8
         x  += act @ Wdown^T
+    next token of each row: penalties, biases, masks     heph_pick_tokens
+
+With a scale a page the q/k op and the attention are the _scaled ones.
 
 The step is the batched form of the reference's forward_fp8_batched_decode
 (src/hephaestus/forward.mojo:618-871), which keeps one contiguous cache per
@@ -49,15 +54,15 @@ def _dev(t, name: str, dtypes, numel: int, dev: int) -> int:
     raise ValueError(f"{name} has {t.numel()} elements, {numel} are needed")
 
 
-def _rows(t, name: str, n: int, width: int, dev: int) -> tuple[int, int]:
-    """Pointer and row stride (elements) of n rows of width bf16 values; the
-    rows may lie apart (a slice of a wider buffer)."""
+def _rows(t, name: str, n: int, width: int, dev: int, dtype=torch.bfloat16) -> tuple[int, int]:
+    """Pointer and row stride (elements) of n rows of width values; the rows may
+    lie apart (a slice of a wider buffer)."""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch tensor")
     if t.get_device() != dev:
         raise ValueError(f"{name} must be in the current device's memory (got {t.device})")
-    if t.dtype != torch.bfloat16:
-        raise TypeError(f"{name} has dtype {t.dtype}, expected torch.bfloat16")
+    if t.dtype != dtype:
+        raise TypeError(f"{name} has dtype {t.dtype}, expected {dtype}")
     shape = t.shape
     if len(shape) >= 2 and shape[0] >= n:
         if t.is_contiguous():
@@ -127,14 +132,15 @@ def _pools(k_pages, v_pages, lead: tuple, dev: int) -> tuple[int, int]:
     return _dev(k_pages, "k_pages", _U8, 0, dev), _dev(v_pages, "v_pages", _U8, 0, dev)
 
 
-def qk_norm_rope_pages(q_out, qkv, q_gamma, k_gamma, k_pages, v_pages, kv_inv, rope, positions,
-                       slots, eps: float = 1e-6, ctx=None) -> None:
-    """For each token: per-head RMSNorm of q and k, rotation by rope's row
-    positions[t], q [n_tok, n_heads, 128] to q_out, k and v as E4M3 codes into
-    slots[t] (page * 64 + key) of k_pages [n_pages, n_kv, 2, 64, 64] and
-    v_pages [n_pages, n_kv, 128, 64]. qkv: [n_tok, n_heads + 2 n_kv, 128], its
-    rows may lie apart; q_out may be qkv[:, :n_heads]. A position outside
-    rope skips the token, a slot outside the pools the cache write."""
+def _page_scale(t, lead: tuple, n_kv: int, dev: int) -> int:
+    """Pointer of the pages' scales [*lead, 2 n_kv], lead ending with n_pages."""
+    if t.shape != lead + (2 * n_kv,):
+        raise ValueError(f"page_scale of shape {tuple(t.shape)} is not {list(lead + (2 * n_kv,))}")
+    return _dev(t, "page_scale", _F32, 0, dev)
+
+
+def _qk(name: str, q_out, qkv, q_gamma, k_gamma, k_pages, v_pages, scale_name: str, scale, rope,
+        positions, slots, eps, ctx) -> None:
     dev, stream = _at(ctx)
     qs, ks, rs = q_out.shape, k_pages.shape, rope.shape
     if len(qs) != 3 or qs[2] != 128 or len(ks) != 5:
@@ -148,11 +154,58 @@ def qk_norm_rope_pages(q_out, qkv, q_gamma, k_gamma, k_pages, v_pages, kv_inv, r
     kp, vp = _pools(k_pages, v_pages, (n_pages, n_kv), dev)
     if len(rs) != 3 or rs[1] != 64 or rs[2] != 2:
         raise ValueError(f"rope of shape {tuple(rs)} is not [n_pos, 64, 2]")
-    _call("heph_qk_norm_rope_pages", qp, qs, xp, xs, _dev(q_gamma, "q_gamma", _BF16, 128, dev),
-          _dev(k_gamma, "k_gamma", _BF16, 128, dev), kp, vp, n_pages,
-          _dev(kv_inv, "kv_inv", _F32, 2 * n_kv, dev), _dev(rope, "rope", _F32, 0, dev),
-          rs[0], _dev(positions, "positions", _I32, n_tok, dev),
+    if scale_name == "kv_inv":
+        sp = _dev(scale, scale_name, _F32, 2 * n_kv, dev)
+    else:
+        sp = _page_scale(scale, (n_pages,), n_kv, dev)
+    _call(name, qp, qs, xp, xs, _dev(q_gamma, "q_gamma", _BF16, 128, dev),
+          _dev(k_gamma, "k_gamma", _BF16, 128, dev), kp, vp, n_pages, sp,
+          _dev(rope, "rope", _F32, 0, dev), rs[0], _dev(positions, "positions", _I32, n_tok, dev),
           _dev(slots, "slots", _I32, n_tok, dev), n_tok, n_heads, n_kv, 128, eps, stream)
+
+
+def qk_norm_rope_pages(q_out, qkv, q_gamma, k_gamma, k_pages, v_pages, kv_inv, rope, positions,
+                       slots, eps: float = 1e-6, ctx=None) -> None:
+    """For each token: per-head RMSNorm of q and k, rotation by rope's row
+    positions[t], q [n_tok, n_heads, 128] to q_out, k and v as E4M3 codes into
+    slots[t] (page * 64 + key) of k_pages [n_pages, n_kv, 2, 64, 64] and
+    v_pages [n_pages, n_kv, 128, 64]. qkv: [n_tok, n_heads + 2 n_kv, 128], its
+    rows may lie apart; q_out may be qkv[:, :n_heads]. A position outside
+    rope skips the token, a slot outside the pools the cache write."""
+    _qk("heph_qk_norm_rope_pages", q_out, qkv, q_gamma, k_gamma, k_pages, v_pages, "kv_inv", kv_inv,
+        rope, positions, slots, eps, ctx)
+
+
+def qk_norm_rope_pages_scaled(q_out, qkv, q_gamma, k_gamma, k_pages, v_pages, page_scale, rope,
+                              positions, slots, eps: float = 1e-6, ctx=None) -> None:
+    """qk_norm_rope_pages into pages with scales of their own, page_scale [n_pages, 2 n_kv]
+    (powers of two, updated): the least one that holds a block's new values and is no less
+    than the block's so far, whose codes are rescaled where it grows. Tokens that bring a
+    page's key 0 begin it anew. A page's tokens are neighbours among the rows."""
+    _qk("heph_qk_norm_rope_pages_scaled", q_out, qkv, q_gamma, k_gamma, k_pages, v_pages, "page_scale",
+        page_scale, rope, positions, slots, eps, ctx)
+
+
+def read_pages(k_out, v_out, k_pages, v_pages, slots, kv_scale=None, page_scale=None,
+               ctx=None) -> None:
+    """Row t of k_out and v_out (bf16 [n, n_kv, 128]): the key and value of slots[t], code times
+    scale. One of kv_scale [2 n_kv] (of all pages) and page_scale [n_pages, 2 n_kv]. A slot
+    outside the pools leaves its row as it was."""
+    if (kv_scale is None) == (page_scale is None):
+        raise ValueError("read_pages takes one of kv_scale and page_scale")
+    dev, stream = _at(ctx)
+    n_pages, n_kv = k_pages.shape[0], k_pages.shape[1]
+    kp, vp = _pools(k_pages, v_pages, (n_pages, n_kv), dev)
+    n = slots.numel()
+    if n == 0:
+        return
+    for t, name in ((k_out, "k_out"), (v_out, "v_out")):
+        if t.shape != (n, n_kv, 128):
+            raise ValueError(f"{name} of shape {tuple(t.shape)} is not [{n}, {n_kv}, 128]")
+    _call("heph_read_pages", _dev(k_out, "k_out", _BF16, 0, dev), _dev(v_out, "v_out", _BF16, 0, dev),
+          kp, vp, n_pages, None if kv_scale is None else _dev(kv_scale, "kv_scale", _F32, 2 * n_kv, dev),
+          None if page_scale is None else _page_scale(page_scale, (n_pages,), n_kv, dev),
+          _dev(slots, "slots", _I32, n, dev), n, n_kv, 128, stream)
 
 
 def _bind(p) -> None:
@@ -206,30 +259,41 @@ class AttentionPlan:
               stream)
 
 
-def attention_pages(out, q, k_pages, v_pages, kv_scale, page_table, plan: AttentionPlan,
-                    ctx=None) -> None:
-    """out[t] = attention of token t over its sequence's keys in the pages,
-    laid out by plan (updated with this step's lengths). q [n_tok, n_heads,
-    128] (rows may lie apart), out contiguous; page_table int32 [n_seqs,
-    table_pages]."""
-    p = plan
-    dev, stream = _at(ctx)
+def _attention(name: str, out, q, k_pages, v_pages, scale, page_table, p, dev, stream) -> None:
     n_pages = k_pages.shape[0]
     kp, vp = _pools(k_pages, v_pages, (n_pages, p.n_kv), dev)
     if page_table.shape != (p.n_seqs, p.table_pages):
         raise ValueError(f"page_table of shape {tuple(page_table.shape)} is not "
                          f"[{p.n_seqs}, {p.table_pages}] as planned")
     qp, qs = _rows(q, "q", p.n_tok, p.n_heads * 128, dev)
-    _call("heph_pages_attention", _dev(out, "out", _BF16, p.n_tok * p.n_heads * 128, dev), qp, qs,
-          kp, vp, n_pages, _dev(kv_scale, "kv_scale", _F32, 2 * p.n_kv, dev),
-          _dev(page_table, "page_table", _I32, 0, dev), p.table_pages,
+    _call(name, _dev(out, "out", _BF16, p.n_tok * p.n_heads * 128, dev), qp, qs, kp, vp, n_pages,
+          scale(n_pages), _dev(page_table, "page_table", _I32, 0, dev), p.table_pages,
           *_bound(p, dev), p.n_tok, p.n_seqs, p.n_groups, p.n_heads, p.n_kv, 128, stream)
 
 
-def copy_pages(k_pools, v_pools, src, dst, ctx=None) -> None:
+def attention_pages(out, q, k_pages, v_pages, kv_scale, page_table, plan: AttentionPlan,
+                    ctx=None) -> None:
+    """out[t] = attention of token t over its sequence's keys in the pages,
+    laid out by plan (updated with this step's lengths). q [n_tok, n_heads,
+    128] (rows may lie apart), out contiguous; page_table int32 [n_seqs,
+    table_pages]."""
+    dev, stream = _at(ctx)
+    _attention("heph_pages_attention", out, q, k_pages, v_pages,
+               lambda n: _dev(kv_scale, "kv_scale", _F32, 2 * plan.n_kv, dev), page_table, plan, dev, stream)
+
+
+def attention_pages_scaled(out, q, k_pages, v_pages, page_scale, page_table, plan: AttentionPlan,
+                           ctx=None) -> None:
+    """attention_pages over pages with scales of their own, page_scale [n_pages, 2 n_kv]."""
+    dev, stream = _at(ctx)
+    _attention("heph_pages_attention_scaled", out, q, k_pages, v_pages,
+               lambda n: _page_scale(page_scale, (n,), plan.n_kv, dev), page_table, plan, dev, stream)
+
+
+def copy_pages(k_pools, v_pools, src, dst, ctx=None, page_scale=None) -> None:
     """Page src[i] of every layer copied to page dst[i] in both pools
-    [n_layers, n_pages, ...]; src and dst are host lists of ints. A destination may
-    neither repeat nor be a source."""
+    [n_layers, n_pages, ...] (and in page_scale [n_layers, n_pages, 2 n_kv], if given); src and
+    dst are host lists of ints. A destination may neither repeat nor be a source."""
     ks = k_pools.shape
     if len(ks) != 6:
         raise ValueError(f"k_pools of shape {tuple(ks)} has no layers")
@@ -238,7 +302,12 @@ def copy_pages(k_pools, v_pools, src, dst, ctx=None) -> None:
     s, d = array("i", src), array("i", dst)
     if len(s) != len(d):
         raise ValueError(f"{len(s)} sources and {len(d)} destinations")
-    _call("heph_copy_pages", kp, vp, *ks[:3], s.buffer_info()[0], d.buffer_info()[0], len(s), stream)
+    pairs = s.buffer_info()[0], d.buffer_info()[0], len(s), stream
+    if page_scale is None:
+        _call("heph_copy_pages", kp, vp, *ks[:3], *pairs)
+    else:
+        _call("heph_copy_pages_scaled", kp, vp, _page_scale(page_scale, tuple(ks[:2]), ks[2], dev),
+              *ks[:3], *pairs)
 
 
 class LoraPlan:
@@ -287,6 +356,111 @@ def lora_add(c, base, x, a, b, scale, plan: LoraPlan, ctx=None) -> None:
           stream)
 
 
+# ---------------------------------------------------------------- the pick ----
+
+class TokenRules:
+    """What the requests of a batch ask of their next tokens, in device memory, one slot a
+    request: history int32 [n_slots, max_tokens] (prompt and answer), length and n_prompt int32
+    [n_slots], penalties f32 [n_slots, 3] (repetition, presence, frequency), bias_ids int32 and
+    bias f32 [n_slots, max_bias], n_bias int32 [n_slots]. set() fills a slot; the tensors may be
+    written directly too, but not replaced. set() runs on the current stream; picks on other
+    streams are ordered by the caller."""
+
+    def __init__(self, n_slots: int, vocab: int, max_tokens: int, max_bias: int = 0, device="cuda"):
+        if n_slots < 1 or vocab < 1 or not 1 <= max_tokens <= L.ATTN_MAX_KEYS or \
+                not 0 <= max_bias <= L.PICK_MAX_BIAS:
+            raise ValueError(f"rules of {n_slots} slots, {vocab} tokens, histories of {max_tokens} "
+                             f"and {max_bias} biases")
+        self.n_slots, self.vocab, self.max_tokens, self.max_bias = n_slots, vocab, max_tokens, max_bias
+
+        def zeros(*shape, dtype=torch.int32):
+            return torch.zeros(shape, dtype=dtype, device=device)
+        self.history, self.length, self.n_prompt = zeros(n_slots, max_tokens), zeros(n_slots), zeros(n_slots)
+        self.penalties = zeros(n_slots, 3, dtype=torch.float32)
+        self.penalties[:, 0] = 1
+        self.bias_ids, self.n_bias = zeros(n_slots, max_bias), zeros(n_slots)
+        self.bias = zeros(n_slots, max_bias, dtype=torch.float32)
+        self._dev = self.history.get_device()
+        self._args = L.TokenRulesArgs(n_slots, max_tokens, max_bias, *(t.data_ptr() for t in (
+            self.history, self.length, self.n_prompt, self.penalties, self.bias_ids, self.bias,
+            self.n_bias)))
+
+    def set(self, slot: int, prompt=(), answered=(), repetition: float = 1.0, presence: float = 0.0,
+            frequency: float = 0.0, bias: dict | None = None) -> None:
+        """A request begins in the slot: its tokens so far, its penalties (repetition above 0; 1, 0,
+        0: none) and its biases {token: added to its logit} (-inf: never that token)."""
+        if not 0 <= slot < self.n_slots:
+            raise ValueError(f"slot {slot} of {self.n_slots}")
+        tokens, bias = [*prompt, *answered], bias or {}
+        if len(tokens) > self.max_tokens or len(bias) > self.max_bias:
+            raise ValueError(f"{len(tokens)} tokens and {len(bias)} biases in a slot of "
+                             f"{self.max_tokens} and {self.max_bias}")
+        if any(not 0 <= t < self.vocab for t in (*tokens, *bias)):
+            raise ValueError(f"a token outside the vocabulary of {self.vocab}")
+        penalties = [float(repetition), float(presence), float(frequency)]
+        if not all(np.isfinite(penalties)) or not repetition > 0:
+            raise ValueError(f"penalties {penalties}")
+        if any(not float(b) < np.inf for b in bias.values()):
+            raise ValueError("a bias that is NaN or +inf")
+        # (array: what is no whole number is refused, not rounded)
+        ids = torch.from_numpy(np.frombuffer(array("i", [*tokens, *bias, len(tokens), len(prompt), len(bias)]),
+                                             dtype=np.int32).copy()).to(self.history.device)
+        n, m = len(tokens), len(bias)
+        values = torch.tensor(penalties + [float(b) for b in bias.values()], dtype=torch.float32,
+                              device=self.history.device)
+        self.history[slot, :n] = ids[:n]
+        self.bias_ids[slot, :m] = ids[n:n + m]
+        self.length[slot], self.n_prompt[slot], self.n_bias[slot] = ids[n + m:].unbind()
+        self.penalties[slot] = values[:3]
+        self.bias[slot, :m] = values[3:]
+
+
+def pick_ws(rows: int, vocab: int, device="cuda") -> torch.Tensor:
+    """Scratch for pick_tokens over [rows, vocab] logits."""
+    nb = L.lib().heph_pick_ws_bytes(rows, vocab)
+    if nb == 0:
+        raise HephError(L.HEPH_ERR_SHAPE, "pick_ws")
+    return torch.empty(nb, dtype=torch.uint8, device=device)
+
+
+def pick_tokens(tokens, logits, rules: TokenRules | None = None, slots=None, masks=None, mask_ids=None,
+                out=None, logprob=None, append: bool = False, ws=None, ctx=None) -> None:
+    """tokens[r] = the token of row r's largest logit (the lowest of equal ones; -1: none is
+    above -inf) after the rules of slots[r]: penalties for what its history holds, biases, and
+    the mask masks[mask_ids[r]]. logits [rows, vocab] f32 or bf16, its rows may lie apart; out, of
+    the same type, gets the logits after the rules (out may be logits); logprob f32 [rows] the
+    tokens' log-probabilities; tokens int32 [rows] may be None where out is wanted alone. masks int32 [n_masks,
+    (vocab + 31) // 32], bit t % 32 of word t // 32 set: token t is allowed. A slot or mask id
+    outside its range: no rules, no mask. append: the tokens are written behind their histories
+    (distinct slots)."""
+    dev, stream = _at(ctx)
+    if not isinstance(logits, torch.Tensor) or logits.dim() != 2 or logits.dtype not in HK._OUT:
+        raise TypeError("logits must be an f32 or bf16 tensor [rows, vocab]")
+    rows, vocab = logits.shape
+    if (rules is None) != (slots is None) or (masks is None) != (mask_ids is None):
+        raise ValueError("rules come with slots, masks with mask_ids")
+    lp, ls = _rows(logits, "logits", rows, vocab, dev, logits.dtype)
+    op, os_ = (None, 0) if out is None else _rows(out, "out", rows, vocab, dev, logits.dtype)
+    if rows == 1 and op == lp:
+        os_ = ls                  # (one row has no stride of its own)
+    if out is not None and out.shape != logits.shape:
+        raise ValueError(f"out of shape {tuple(out.shape)} for logits of {tuple(logits.shape)}")
+    if rules is not None and (rules.vocab != vocab or rules._dev != dev):
+        raise ValueError(f"rules of {rules.vocab} tokens on device {rules._dev} for logits of {vocab} on {dev}")
+    mp, n_masks = None, 0
+    if masks is not None:
+        n_masks = masks.shape[0]
+        mp = _matrix(masks, "masks", _I32, n_masks, (vocab + 31) // 32, dev)
+    if ws is None:
+        ws = pick_ws(rows, vocab, logits.device)
+    _call("heph_pick_tokens", None if tokens is None else _dev(tokens, "tokens", _I32, rows, dev),
+          None if logprob is None else _dev(logprob, "logprob", _F32, rows, dev), op, os_, lp, ls,
+          HK._OUT[logits.dtype], rows, vocab, None if rules is None else rules._args,
+          None if slots is None else _dev(slots, "slots", _I32, rows, dev), mp, n_masks,
+          None if mask_ids is None else _dev(mask_ids, "mask_ids", _I32, rows, dev),
+          L.PICK_APPEND if append else 0, _dev(ws, "ws", (torch.uint8,), 0, dev), ws.numel(), stream)
+
+
 # --------------------------------------------------------------- the cache ----
 
 class Sequence:
@@ -300,12 +474,13 @@ class Sequence:
 class PagedKVCache:
     """K and V pools of all layers with E4M3 codes, k [n_layers, n_pages, n_kv,
     2, 64, 64] and v [n_layers, n_pages, n_kv, 128, 64], f32 scales [n_layers,
-    2*n_kv] and their reciprocals, and which sequence holds which page. A page
-    may belong to several sequences (a shared prefix): it is freed with the
+    2*n_kv] and their reciprocals (page_scales: page_scale [n_layers, n_pages,
+    2*n_kv] instead, found while pages are written; scale and inv are None), and
+    which sequence holds which page. A page may belong to several sequences (a shared prefix): it is freed with the
     last of them. Page copies run on the current stream (or ctx's); steps on other
     streams are ordered by the caller."""
 
-    def __init__(self, cfg: Qwen3Config, n_pages: int, device="cuda"):
+    def __init__(self, cfg: Qwen3Config, n_pages: int, device="cuda", page_scales: bool = False):
         if cfg.head_dim != 128:
             raise ValueError("head_dim must be 128")
         if n_pages < 1:
@@ -314,9 +489,14 @@ class PagedKVCache:
         shape = (cfg.n_layers, n_pages, cfg.n_kv_heads)
         self.k = torch.zeros(*shape, 2, PAGE, 64, dtype=torch.uint8, device=device)
         self.v = torch.zeros(*shape, 128, PAGE, dtype=torch.uint8, device=device)
-        self.scale = torch.ones(cfg.n_layers, 2 * cfg.n_kv_heads, dtype=torch.float32,
-                                device=device)
-        self.inv = torch.ones_like(self.scale)
+        self.scale = self.inv = self.page_scale = None
+        if page_scales:
+            self.page_scale = torch.ones(cfg.n_layers, n_pages, 2 * cfg.n_kv_heads,
+                                         dtype=torch.float32, device=device)
+        else:
+            self.scale = torch.ones(cfg.n_layers, 2 * cfg.n_kv_heads, dtype=torch.float32,
+                                    device=device)
+            self.inv = torch.ones_like(self.scale)
         self._free = list(range(n_pages))          # a heap: the lowest page first
         self._users = [0] * n_pages
         self._seqs: dict[Sequence, None] = {}      # in the order of their making
@@ -324,6 +504,12 @@ class PagedKVCache:
     @property
     def free_pages(self) -> int:
         return len(self._free)
+
+    def _copy(self, src: list[int], dst: list[int], ctx) -> None:
+        if self.page_scale is None:
+            copy_pages(self.k, self.v, src, dst, ctx)
+        else:
+            copy_pages(self.k, self.v, src, dst, ctx, self.page_scale)
 
     def _take(self, n: int) -> list[int]:
         if n > len(self._free):
@@ -372,7 +558,7 @@ class PagedKVCache:
         tails = self._take(n if seq.length % PAGE else 0)
         if tails:
             try:
-                copy_pages(self.k, self.v, [seq.pages[full]] * n, tails, ctx)
+                self._copy([seq.pages[full]] * n, tails, ctx)
             except BaseException:
                 for p in tails:
                     self._drop(p)
@@ -385,6 +571,25 @@ class PagedKVCache:
                 self._users[p] += 1
             made.append(s)
         return made
+
+    def read(self, seq: Sequence, layer: int, first: int = 0, n: int | None = None, ctx=None):
+        """Keys first .. first+n-1 (n None: to the end) of one layer as bf16 rows, (k, v) of
+        [n, n_kv, 128]."""
+        self._own(seq)
+        n = seq.length - first if n is None else n
+        if not 0 <= first <= first + n <= seq.length:
+            raise ValueError(f"keys {first} .. {first + n - 1} of a sequence of {seq.length}")
+        if not 0 <= layer < self.cfg.n_layers:
+            raise ValueError(f"layer {layer} of {self.cfg.n_layers}")
+        dev = self.k.device
+        slots = torch.tensor([seq.pages[j // PAGE] * PAGE + j % PAGE for j in range(first, first + n)],
+                             dtype=torch.int32, device=dev)
+        k, v = (torch.empty(n, self.cfg.n_kv_heads, 128, dtype=torch.bfloat16, device=dev) for _ in range(2))
+        if self.page_scale is None:
+            read_pages(k, v, self.k[layer], self.v[layer], slots, kv_scale=self.scale[layer], ctx=ctx)
+        else:
+            read_pages(k, v, self.k[layer], self.v[layer], slots, page_scale=self.page_scale[layer], ctx=ctx)
+        return k, v
 
     def free(self, seq: Sequence) -> None:
         """The sequence leaves the cache; pages that no other one holds are free."""
@@ -401,7 +606,7 @@ class PagedKVCache:
         live = self.n_pages - len(self._free)
         dst = sorted(p for p in self._free if p < live)
         src = [p for p in range(live, self.n_pages) if self._users[p]]
-        copy_pages(self.k, self.v, src, dst, ctx)
+        self._copy(src, dst, ctx)
         to = dict(zip(src, dst))
         for s in self._seqs:
             s.pages = [to.get(p, p) for p in s.pages]
@@ -540,6 +745,34 @@ class Qwen3BatchDecoder:
                 s.length, s.pages = length, s.pages[:pages]
             raise
 
+    def next_tokens(self, tokens: list[list[int]], seqs: list[Sequence], adapters: list[int] | None = None,
+                    rules: TokenRules | None = None, slots: list[int] | None = None, masks=None,
+                    mask_ids: list[int] | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+        """step(), and the pick of each sequence's next token from its logits (pick_tokens: rules
+        of slots[i] and mask mask_ids[i], -1: none) as int32 [len(seqs)], with their
+        log-probabilities, both in device memory. The tokens are written behind their histories."""
+        S, dev = len(seqs), self.w.embed.w.device
+        if (rules is None) != (slots is None) or (masks is None) != (mask_ids is None):
+            raise ValueError("rules come with slots, masks with mask_ids")
+        if slots is not None:
+            used = [s for s in slots if s >= 0]
+            if len(slots) != S or len(set(used)) != len(used) or any(s >= rules.n_slots for s in used):
+                raise ValueError(f"slots {slots} are not one of {rules.n_slots} for each of {S} sequences")
+            if rules.vocab != self.w.cfg.vocab:
+                raise ValueError(f"rules of {rules.vocab} tokens, {self.w.cfg.vocab} in the model")
+        if mask_ids is not None:
+            if len(mask_ids) != S or any(m >= masks.shape[0] for m in mask_ids):
+                raise ValueError(f"mask_ids {mask_ids} are not one of {masks.shape[0]} for each of {S} sequences")
+            if masks.shape[1:] != ((self.w.cfg.vocab + 31) // 32,) or masks.dtype != torch.int32:
+                raise ValueError(f"masks {tuple(masks.shape)} for a vocabulary of {self.w.cfg.vocab}")
+        ids = [None if x is None else torch.tensor(array("i", x), dtype=torch.int32, device=dev)
+               for x in (slots, mask_ids)]
+        logits = self.step(tokens, seqs, adapters)
+        picked = torch.empty(S, dtype=torch.int32, device=dev)
+        logprob = torch.empty(S, dtype=torch.float32, device=dev)
+        pick_tokens(picked, logits, rules, ids[0], masks, ids[1], logprob=logprob, append=rules is not None)
+        return picked, logprob
+
     def _layout(self, tokens, seqs, adapters) -> list:
         """The sequences take their tokens; the int32 values that the step's ops read: tokens,
         positions, slots, q_start, kv_len, group_start, shared_pages, adapter ids and the page
@@ -602,9 +835,14 @@ class Qwen3BatchDecoder:
         qs = qkv.view(T, -1, 128)[:, :cfg.n_heads]
         for li, lw in enumerate(w.layers):
             norm_linear(li, "qkv", qkv, lw.attn_norm, lw.qkv)
-            qk_norm_rope_pages(qs, qkv.view(T, -1, 128), lw.q_norm, lw.k_norm, kv.k[li], kv.v[li],
-                               kv.inv[li], self.rope, pos, slot, cfg.eps)
-            attention_pages(q, qs, kv.k[li], kv.v[li], kv.scale[li], table, plan)
+            if kv.page_scale is None:
+                qk_norm_rope_pages(qs, qkv.view(T, -1, 128), lw.q_norm, lw.k_norm, kv.k[li], kv.v[li],
+                                   kv.inv[li], self.rope, pos, slot, cfg.eps)
+                attention_pages(q, qs, kv.k[li], kv.v[li], kv.scale[li], table, plan)
+            else:
+                qk_norm_rope_pages_scaled(qs, qkv.view(T, -1, 128), lw.q_norm, lw.k_norm, kv.k[li],
+                                          kv.v[li], kv.page_scale[li], self.rope, pos, slot, cfg.eps)
+                attention_pages_scaled(q, qs, kv.k[li], kv.v[li], kv.page_scale[li], table, plan)
             self._linear(x, att, lw.o, Q, ws, residual=True)
             adapt(li, "o", x, att)
             norm_linear(li, "gate_up", gu, lw.ffn_norm, lw.gate_up)

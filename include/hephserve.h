@@ -1,8 +1,10 @@
 /*
  * hephserve.h - the ops of a batched serving step around the W8A8 linears:
  * q/k norm + rotation into a paged KV cache, attention of a batch over that
- * cache with shared prefixes computed once, page copies, and the low-rank
- * adapters of many requests beside one projection. Same conventions as
+ * cache with shared prefixes computed once, page copies (each with one scale
+ * for a whole layer's head, or one for each page found while it is written),
+ * the low-rank adapters of many requests beside one projection, and the pick
+ * of the next tokens from a batch's logits. Same conventions as
  * hephfp8.h: device pointers unless an argument says host, a hipStream_t as
  * void* (NULL = default stream), HEPH_* status codes, no allocation, no
  * synchronization, capturable into a HIP graph.
@@ -142,6 +144,67 @@ int heph_copy_pages(uint8_t* k_pages, uint8_t* v_pages, int n_layers, int n_page
                     int n_kv_heads, const int32_t* src, const int32_t* dst, int n, void* stream);
 
 /*
+ * The same cache with a scale for each block: a page's 64 keys of one kv head,
+ * K and V apart. page_scale [n_pages][2 * n_kv_heads] (a page's K heads, then
+ * its V heads), all powers of two 2^e, -117 <= e <= 119: a code c stands for
+ * c * 2^e, a bf16 value. Nothing has to be calibrated: the ops below find the
+ * scales from what they write. Pages, slots, positions and the remaining
+ * arguments are as in the ops of the same names without _scaled.
+ *
+ * heph_qk_norm_rope_pages_scaled: a block's scale becomes the least 2^e with
+ * |x| <= 448 * 2^e for its new keys' finite values x (computed in f32; e is
+ * held to the range above and values past 448 * 2^119 are clamped), and no less
+ * than it was, unless the page's key 0 is among the call's tokens: they begin
+ * the page anew, whatever it held. Where a scale grows by 2^n, the codes of all
+ * 64 keys are divided by 2^n (exactly, but for those that leave E4M3's normal
+ * range, which are rounded to its subnormal ones); new codes are
+ * e4m3(x * 2^-e), and a NaN or an infinity, which E4M3 has not, is the code of
+ * NaN. A scale outside the range (memory that was never written) counts as the
+ * nearest one in it.
+ * The tokens of a page are neighbours among the call's rows, as a sequence's
+ * newest tokens are, and a page belongs to one sequence while it is written; a
+ * page whose tokens lie apart gets codes of more than one scale.
+ * Writes no page and no scale without a token of the call.
+ *
+ * heph_pages_attention_scaled takes a plan of heph_pages_attention_plan and the
+ * workspace of heph_pages_attention_ws_bytes. Of a page_scale only the exponent
+ * is used.
+ *
+ * heph_copy_pages_scaled copies the pages' scales with them (page_scale
+ * [n_layers][n_pages][2 * n_kv_heads]).
+ * No counterpart in the reference, whose cache is bf16.
+ */
+int heph_qk_norm_rope_pages_scaled(void* q_out_bf16, int64_t q_stride, const void* qkv_bf16,
+                                   int64_t qkv_stride, const void* q_gamma, const void* k_gamma,
+                                   uint8_t* k_pages, uint8_t* v_pages, int n_pages,
+                                   float* page_scale, const float* rope_table, int n_rope_pos,
+                                   const int32_t* positions, const int32_t* slots, int n_tok,
+                                   int n_heads, int n_kv_heads, int head_dim, float eps,
+                                   void* stream);
+int heph_pages_attention_scaled(void* out_bf16, const void* q_bf16, int64_t q_stride,
+                                const uint8_t* k_pages, const uint8_t* v_pages, int n_pages,
+                                const float* page_scale, const int32_t* page_table, int table_pages,
+                                const void* plan, size_t plan_bytes, void* ws, size_t ws_bytes,
+                                int n_tok, int n_seqs, int n_groups, int n_heads, int n_kv_heads,
+                                int head_dim, void* stream);
+int heph_copy_pages_scaled(uint8_t* k_pages, uint8_t* v_pages, float* page_scale, int n_layers,
+                           int n_pages, int n_kv_heads, const int32_t* src, const int32_t* dst,
+                           int n, void* stream);
+
+/*
+ * Keys read back: row t < n_rows of k_out and v_out ([n_rows, n_kv_heads, 128]
+ * bf16) gets the key and value of slots[t], code * scale, rounded once (exact
+ * with page_scale). One of kv_scale (2 * n_kv_heads, of all pages) and
+ * page_scale is given, the other NULL. Rows of a slot outside
+ * [0, 64 * n_pages) are left as they were; n_pages < 2^25. Slots may repeat and come
+ * in any order; consecutive ones are read together. k_out and v_out do not overlap.
+ */
+int heph_read_pages(void* k_out_bf16, void* v_out_bf16, const uint8_t* k_pages,
+                    const uint8_t* v_pages, int n_pages, const float* kv_scale,
+                    const float* page_scale, const int32_t* slots, int n_rows, int n_kv_heads,
+                    int head_dim, void* stream);
+
+/*
  * Low-rank adapters of many requests beside one projection:
  *   c[m, :] = base[m, :] + scale[i] * (x[m, :] @ a[i]^T) @ b[i]^T,  i = ids[m],
  * x bf16 [M, K], a bf16 [n_adapters, rank, K], b bf16 [n_adapters, N, rank],
@@ -170,6 +233,57 @@ int heph_lora_add(void* c, int c_dtype, const void* base, const uint16_t* x_bf16
                   const uint16_t* a_bf16, const uint16_t* b_bf16, const float* scale,
                   const void* plan, size_t plan_bytes, void* ws, size_t ws_bytes, int M, int N,
                   int K, int rank, int n_adapters, void* stream);
+
+/*
+ * The pick: each row's next token from its logits, after the rules of its
+ * request. For row r of logits ([rows, vocab], rows logits_stride elements
+ * apart, f32 or bf16) and s = slots[r], the request's place in the rules, in f32:
+ *   penalties[s] = (repetition, presence, frequency)
+ *   seen t (in history[s][0 .. length[s])):  l = l > 0 ? l / repetition
+ *                                                      : l * repetition
+ *   answered n > 0 times (from n_prompt[s] on): l = l - (n * frequency + presence)
+ *   in bias_ids[s][0 .. n_bias[s]):          l = l + bias (of an id that is
+ *                                            there twice, its last entry's)
+ *   bit t % 32 of masks[mask_ids[r]][t / 32] is 0:  l = -inf
+ * tokens[r] is the lowest index of the largest l, NaN left out; -1 if none is
+ * above -inf. logprob[r] is its log-probability under the softmax of all l:
+ * -inf where tokens[r] is -1, NaN where an l is NaN or +inf. out (the type of
+ * logits, rows out_stride apart; may be logits itself with the same stride, and
+ * overlaps it in no other way) gets the l's, rounded once. Each of tokens, logprob and
+ * out may be NULL, but not tokens and out both; with flags HEPH_PICK_APPEND (tokens not
+ * NULL) a token >= 0 is then written behind its request's history while that has
+ * room, and length[s] grows by one; the rows' slots are then distinct.
+ * A row has no rules if rules or slots is NULL or its slot is outside
+ * [0, n_slots); no mask if masks or mask_ids is NULL or its id is outside [0, n_masks).
+ *
+ * heph_token_rules: device pointers, row by row: history [n_slots][max_tokens],
+ * bias_ids and bias [n_slots][max_bias] (bias_ids, bias and n_bias may be NULL
+ * with max_bias 0), masks [n_masks][(vocab + 31) / 32]. max_tokens up to
+ * 262144, max_bias up to HEPH_PICK_MAX_BIAS. Lengths are clamped to their
+ * buffers on the device, ids outside the vocabulary are passed over.
+ * ws: heph_pick_ws_bytes(rows, vocab) bytes, 16-byte aligned; calls that share it are
+ * ordered by the caller.
+ * Replaces, for a batch with rules, argmax (src/hephaestus/kernels.mojo:1376-1433),
+ * which rounds logits to bf16 first.
+ */
+#define HEPH_PICK_APPEND 0x1
+#define HEPH_PICK_MAX_BIAS 4095
+typedef struct heph_token_rules {
+    int n_slots, max_tokens, max_bias;
+    int32_t* history;
+    int32_t* length;
+    const int32_t* n_prompt;
+    const float* penalties;
+    const int32_t* bias_ids;
+    const float* bias;
+    const int32_t* n_bias;
+} heph_token_rules;
+size_t heph_pick_ws_bytes(int rows, int vocab);
+int heph_pick_tokens(int32_t* tokens, float* logprob, void* out, int64_t out_stride,
+                     const void* logits, int64_t logits_stride, int dtype, int rows, int vocab,
+                     const heph_token_rules* rules, const int32_t* slots, const uint32_t* masks,
+                     int n_masks, const int32_t* mask_ids, int flags, void* ws, size_t ws_bytes,
+                     void* stream);
 
 #ifdef __cplusplus
 }
