@@ -21,6 +21,10 @@ __host__ __device__ __forceinline__ int v_place(int j)
 __host__ __device__ __forceinline__ int k_byte(int j, int d) { return d / 64 * 4096 + j * 64 + d % 64; }
 __host__ __device__ __forceinline__ int v_byte(int j, int d) { return d * 64 + v_place(j); }
 
+// LDS accesses of the workgroup before and behind it are ordered; loads from
+// memory stay in flight (__syncthreads would wait for them).
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
 inline bool aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 inline int status_of(hipError_t e) { return e == hipSuccess ? HEPH_OK : HEPH_ERR_LAUNCH; }
 

@@ -958,10 +958,6 @@ __device__ __forceinline__ void attend_narrow(const AttnArgs& a, const Unit& u, 
 // the other's products took 6 % fewer cycles a page at 1.7 GHz, 745 us instead of 694.
 constexpr int kWidePage = 2 * 2 * kPageBytes;      // K and V as bf16
 
-// LDS accesses of the workgroup before and behind it are ordered; loads from
-// memory stay in flight (__syncthreads would wait for them).
-__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
-
 template <bool BLOCK>
 __device__ __forceinline__ void attend_wide(const AttnArgs& a, const Unit& u, int head, int ids0, uint8_t* lds)
 {

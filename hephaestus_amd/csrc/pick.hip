@@ -13,8 +13,6 @@
 namespace heph {
 namespace {
 
-constexpr int kThreads = 512, kVecs = 8, kTile = kThreads * kVecs * 4;
-
 // A token's word: how often it was answered, whether it was seen in the prompt, and the number
 // of its bias entry from 1 on.
 constexpr uint32_t kCount = 0x7FFFFu, kPrompt = 0x80000u, kSeen = kCount | kPrompt;
@@ -61,12 +59,23 @@ __device__ __forceinline__ void store4(uint16_t* p, const f32x4& x)
 __device__ __forceinline__ void store1(float* p, float x) { *p = x; }
 __device__ __forceinline__ void store1(uint16_t* p, float x) { *p = f32_to_bf16(x); }
 
-__device__ __forceinline__ Part better(const Part& a, const Part& b)
-{
-    return b.top > a.top || (b.top == a.top && b.at >= 0 && (a.at < 0 || b.at < a.at)) ? b : a;
-}
-
 __device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * 1.4426950408889634f); }
+
+// What a sum by `top` counts in one by `all`. (One of nothing is 0, or a NaN that stays one.)
+__device__ __forceinline__ float weight(float top, float all) { return top == -INFINITY ? 0.0f : exp_of(top - all); }
+
+// The parts of a wave's lanes as one, in all of them: the largest top, its lowest index, the sums
+// by it. (~at orders indexes the other way round, -1 last; equal tops are compared as numbers, so
+// that 0 is -0's equal.)
+__device__ __forceinline__ Part join_lanes(const Part& p)
+{
+    Part r;
+    r.top = wave_fold_max64(p.top);
+    r.at = (int)~lanes_max_u<64>(p.top == r.top ? ~(uint32_t)p.at : 0u);
+    r.pad = 0;
+    r.sum = wave_fold_sum64(p.sum * weight(p.top, r.top));
+    return r;
+}
 
 // l after its penalties and bias; every operation rounded by itself, as they are stated (a fused
 // product and sum would round once).
@@ -83,141 +92,66 @@ __device__ __forceinline__ float ruled(float l, uint32_t w, float repetition, fl
     return l;
 }
 
-template <class T>
-__global__ __launch_bounds__(kThreads) void pick_kernel(PickArgs a)
-{
-    __shared__ __attribute__((aligned(16))) uint32_t words[kTile];
-    __shared__ Part best[kThreads / 64];
-    __shared__ float sums[kThreads / 64];
-    const int tid = threadIdx.x, row = blockIdx.x / a.tiles, tile = blockIdx.x % a.tiles;
-    const int base = tile * kTile, n = min(kTile, a.vocab - base);
-    const T* in = static_cast<const T*>(a.logits) + (int64_t)row * a.logits_stride + base;
-    f32x4 x[kVecs];
-#pragma unroll
-    for (int k = 0; k < kVecs; ++k) {
-        const int i = (k * kThreads + tid) * 4;
-        x[k] = f32x4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-        if (i + 4 <= n) x[k] = load4(in + i);
-        else
-            for (int e = 0; e < 3; ++e)
-                if (i + e < n) x[k][e] = load1(in + i + e);
-    }
-    const heph_token_rules& r = a.rules;
-    const int slot = a.slots ? a.slots[row] : -1;
-    const bool has_rules = a.slots && slot >= 0 && slot < r.n_slots;
-    float repetition = 1.0f, presence = 0.0f, frequency = 0.0f;
-    int n_seen = 0, n_bias = 0, n_prompt = 0;
-    if (has_rules) {
-        const float* p = r.penalties + (size_t)slot * 3;
-        repetition = p[0];
-        presence = p[1];
-        frequency = p[2];
-        if (repetition != 1.0f || presence != 0.0f || frequency != 0.0f) {
-            n_seen = min(max(r.length[slot], 0), r.max_tokens);
-            n_prompt = r.n_prompt[slot];
-        }
-        if (r.max_bias > 0) n_bias = min(max(r.n_bias[slot], 0), r.max_bias);
-    }
-    const float* bias = r.bias + (size_t)(has_rules ? slot : 0) * r.max_bias;
-    if (n_seen > 0 || n_bias > 0) {
-        for (int i = tid; i < kTile / 4; i += kThreads) reinterpret_cast<uint4*>(words)[i] = make_uint4(0, 0, 0, 0);
-        __syncthreads();
-        const int32_t* history = r.history + (size_t)slot * r.max_tokens;
-        for (int i = tid; i < n_seen; i += kThreads) {
-            const unsigned at = (unsigned)history[i] - (unsigned)base;
-            if (at >= (unsigned)n) continue;
-            if (i < n_prompt) atomicOr(&words[at], kPrompt);
-            else atomicAdd(&words[at], 1u);
-        }
-        __syncthreads();
-        const int32_t* ids = r.bias_ids + (size_t)slot * r.max_bias;
-        for (int i = tid; i < n_bias; i += kThreads) {
-            const unsigned at = (unsigned)ids[i] - (unsigned)base;
-            // (what is below the entry's number stays as it is from here on)
-            if (at < (unsigned)n) atomicMax(&words[at], (words[at] & kSeen) | (uint32_t)(i + 1) << kBiasShift);
-        }
-        __syncthreads();
-#pragma unroll
-        for (int k = 0; k < kVecs; ++k) {
-            const uint4 w4 = reinterpret_cast<const uint4*>(words)[k * kThreads + tid];
-            if ((w4.x | w4.y | w4.z | w4.w) == 0) continue;
-            const uint32_t ws[4] = {w4.x, w4.y, w4.z, w4.w};
-#pragma unroll
-            for (int e = 0; e < 4; ++e) x[k][e] = ruled(x[k][e], ws[e], repetition, presence, frequency, bias);
-        }
-    }
-    const int mask = a.masks && a.mask_ids ? a.mask_ids[row] : -1;
-    if (mask >= 0 && mask < a.n_masks) {
-        const uint32_t* bits = a.masks + (size_t)mask * ((a.vocab + 31) / 32) + base / 32;
-#pragma unroll
-        for (int k = 0; k < kVecs; ++k) {
-            const int i = (k * kThreads + tid) * 4;
-            if (i >= n) continue;
-            const uint32_t b = bits[i / 32] >> (i % 32);
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (!(b >> e & 1)) x[k][e] = -INFINITY;
-        }
-    }
-    if (a.out) {
-        T* out = static_cast<T*>(a.out) + (int64_t)row * a.out_stride + base;
-#pragma unroll
-        for (int k = 0; k < kVecs; ++k) {
-            const int i = (k * kThreads + tid) * 4;
-            if (i + 4 <= n) store4(out + i, x[k]);
-            else
-                for (int e = 0; e < 3; ++e)
-                    if (i + e < n) store1(out + i + e, x[k][e]);
-        }
-    }
-    Part p{-INFINITY, 0.0f, -1, 0};
-#pragma unroll
-    for (int k = 0; k < kVecs; ++k)
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (x[k][e] > p.top) {
-                p.top = x[k][e];
-                p.at = base + (k * kThreads + tid) * 4 + e;
-            }
-    for (int m = 32; m; m >>= 1) {
-        const Part o{__shfl_xor(p.top, m), 0.0f, __shfl_xor(p.at, m), 0};
-        p = better(p, o);
-    }
-    if ((tid & 63) == 0) best[tid / 64] = p;
-    __syncthreads();
-    for (int i = 0; i < kThreads / 64; ++i) p = better(p, best[i]);
-    const float top = p.top == -INFINITY ? 0.0f : p.top;
-    float sum = 0.0f;
-#pragma unroll
-    for (int k = 0; k < kVecs; ++k)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) sum += exp_of(x[k][e] - top);
-    sum = wave_fold_sum64(sum);
-    if ((tid & 63) == 0) sums[tid / 64] = sum;
-    __syncthreads();
-    if (tid == 0) {
-        p.sum = 0.0f;
-        for (int i = 0; i < kThreads / 64; ++i) p.sum += sums[i];
-        a.parts[blockIdx.x] = p;
-    }
-}
+// A thread holds V vectors of four logits: a workgroup's tile is 2048 * V of them.
+constexpr int kThreads = 512;
+constexpr int tile_of(int V) { return kThreads * V * 4; }
 
-// One wave a row joins its tiles' parts.
-__global__ __launch_bounds__(64) void join_kernel(PickArgs a)
+// Sixteen tokens of a history in each thread, loaded at once; -1 behind its end.
+constexpr int kBatchVecs = 4, kBatch = kBatchVecs * kThreads * 4;
+struct Tokens {
+    int t[kBatchVecs][4];
+
+    static __device__ __forceinline__ int at(int u) { return (u * kThreads + (int)threadIdx.x) * 4; }
+    __device__ __forceinline__ void load(int u, const int32_t* history, int first, int end)
+    {
+        const int i = first + at(u);
+        if (i + 4 <= end) {
+            const i32x4_a4 w = *reinterpret_cast<const i32x4_a4*>(history + i);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) t[u][e] = w[e];
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) t[u][e] = i + e < end ? history[i + e] : -1;
+        }
+    }
+    // Counted in the words of the tile of n tokens from base on, those from number n_prompt of the
+    // history on as answered. A token of another tile goes to a word of its lane's behind the
+    // tile's, which costs less than to leave it out.
+    __device__ __forceinline__ void count(uint32_t* words, int spare, int first, int end, int n_prompt, int base,
+                                          int n) const
+    {
+#pragma unroll
+        for (int u = 0; u < kBatchVecs; ++u) {
+            const int i = first + at(u), low = __builtin_amdgcn_readfirstlane(i);     // the wave's first of 256
+            if (low >= end) break;
+            uint32_t* word[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const unsigned place = (unsigned)t[u][e] - (unsigned)base;
+                word[e] = words + (place < (unsigned)n ? place : (unsigned)spare + (threadIdx.x & 63));
+            }
+            if (low >= n_prompt) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) atomicAdd(word[e], 1u);
+            } else if (low + 256 <= n_prompt) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) atomicOr(word[e], kPrompt);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    if (i + e < n_prompt) atomicOr(word[e], kPrompt);
+                    else atomicAdd(word[e], 1u);
+                }
+            }
+        }
+    }
+};
+
+__device__ __forceinline__ void finish(const PickArgs& a, int row, const Part& p)
 {
-    const int row = blockIdx.x, l = threadIdx.x;
-    const Part* parts = a.parts + (size_t)row * a.tiles;
-    Part p{-INFINITY, 0.0f, -1, 0};
-    for (int i = l; i < a.tiles; i += 64) p = better(p, parts[i]);
-    for (int m = 32; m; m >>= 1) p = better(p, Part{__shfl_xor(p.top, m), 0.0f, __shfl_xor(p.at, m), 0});
-    const float top = p.top == -INFINITY ? 0.0f : p.top;
-    float sum = 0.0f;
-    for (int i = l; i < a.tiles; i += 64) sum = __builtin_fmaf(parts[i].sum, exp_of(parts[i].top - top), sum);
-    sum = wave_fold_sum64(sum);
-    if (l != 0) return;
     if (a.tokens) a.tokens[row] = p.at;
     // (no token: the sum is zero, or NaN where there is one)
-    if (a.logprob) a.logprob[row] = p.at < 0 && sum == 0.0f ? -INFINITY : -logf(sum);
+    if (a.logprob) a.logprob[row] = p.at < 0 && p.sum == 0.0f ? -INFINITY : -logf(p.sum);
     if (a.append && p.at >= 0 && a.slots) {
         const int slot = a.slots[row];
         if (slot < 0 || slot >= a.rules.n_slots) return;
@@ -228,8 +162,172 @@ __global__ __launch_bounds__(64) void join_kernel(PickArgs a)
     }
 }
 
+template <class T, int V>
+__global__ __launch_bounds__(kThreads) void pick_kernel(PickArgs a)
+{
+    constexpr int kTile = tile_of(V);
+    __shared__ __attribute__((aligned(16))) uint32_t words[kTile + 64];
+    __shared__ Part waves[kThreads / 64];
+    const int tid = threadIdx.x, row = blockIdx.x / a.tiles, base = blockIdx.x % a.tiles * kTile;
+    const int n = min(kTile, a.vocab - base);
+    // The start is a chain of loads: slot and mask, then what they have, the first tokens of the
+    // history (whatever its length) among it; the logits are on their way beside it.
+    const int slot = a.slots ? a.slots[row] : -1;
+    const int mask_id = a.masks && a.mask_ids ? a.mask_ids[row] : -1;
+    const T* in = static_cast<const T*>(a.logits) + (int64_t)row * a.logits_stride + base;
+    float x[V][4];
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+        const int i = (k * kThreads + tid) * 4;
+        if (i + 4 <= n) {
+            const f32x4 w = load4(in + i);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[k][e] = w[e];
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[k][e] = i + e < n ? load1(in + i + e) : -INFINITY;
+        }
+    }
+    const bool masked = mask_id >= 0 && mask_id < a.n_masks;
+    uint32_t bits[V];
+    if (masked) {
+        const uint32_t* m = a.masks + (size_t)mask_id * ((a.vocab + 31) / 32) + base / 32;
+#pragma unroll
+        for (int k = 0; k < V; ++k) bits[k] = m[min((k * kThreads + tid) * 4, n - 1) / 32];
+    }
+    const heph_token_rules& r = a.rules;
+    if (slot >= 0 && slot < r.n_slots) {
+        const float* p = r.penalties + (size_t)slot * 3;
+        const int32_t* history = r.history + (size_t)slot * r.max_tokens;
+        const float repetition = p[0], presence = p[1], frequency = p[2];
+        const int n_prompt = r.n_prompt[slot], length = r.length[slot];
+        const int n_bias = r.max_bias > 0 ? min(max(r.n_bias[slot], 0), r.max_bias) : 0;
+        Tokens batch;
+        batch.load(0, history, 0, r.max_tokens);
+        const bool neutral = repetition == 1.0f && presence == 0.0f && frequency == 0.0f;
+        const int n_seen = neutral ? 0 : min(max(length, 0), r.max_tokens);
+        const float* bias = r.bias + (size_t)slot * r.max_bias;
+        if (n_seen > 0 || n_bias > 0) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (batch.at(0) + e >= n_seen) batch.t[0][e] = -1;
+#pragma unroll
+            for (int u = 1; u < kBatchVecs; ++u) batch.load(u, history, 0, n_seen);
+            for (int i = tid; i < (n + 3) / 4; i += kThreads)
+                reinterpret_cast<uint4*>(words)[i] = make_uint4(0, 0, 0, 0);
+            lds_barrier();
+            for (int first = 0; first < n_seen; first += kBatch) {
+                if (first > 0)
+#pragma unroll
+                    for (int u = 0; u < kBatchVecs; ++u) batch.load(u, history, first, n_seen);
+                batch.count(words, kTile, first, n_seen, n_prompt, base, n);
+            }
+            lds_barrier();
+            if (n_bias > 0) {
+                const int32_t* ids = r.bias_ids + (size_t)slot * r.max_bias;
+                for (int i = tid; i < n_bias; i += kThreads) {
+                    const unsigned at = (unsigned)ids[i] - (unsigned)base;
+                    // (what is below the entry's number stays as it is from here on)
+                    if (at < (unsigned)n) atomicMax(&words[at], (words[at] & kSeen) | (uint32_t)(i + 1) << kBiasShift);
+                }
+                lds_barrier();
+            }
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
+                const int i = (k * kThreads + tid) * 4;
+                const uint4 w = reinterpret_cast<const uint4*>(words)[i / 4];
+                if (i >= n || (w.x | w.y | w.z | w.w) == 0) continue;
+                const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[k][e] = ruled(x[k][e], ws[e], repetition, presence, frequency, bias);
+            }
+        }
+    }
+    if (masked) {
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            const uint32_t b = bits[k] >> (tid * 4 % 32);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (!(b >> e & 1)) x[k][e] = -INFINITY;
+        }
+    }
+    if (a.out) {
+        T* out = static_cast<T*>(a.out) + (int64_t)row * a.out_stride + base;
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            const int i = (k * kThreads + tid) * 4;
+            if (i + 4 <= n) store4(out + i, f32x4{x[k][0], x[k][1], x[k][2], x[k][3]});
+            else
+#pragma unroll
+                for (int e = 0; e < 3; ++e)
+                    if (i + e < n) store1(out + i + e, x[k][e]);
+        }
+    }
+    Part p{-INFINITY, 0.0f, -1, 0};
+#pragma unroll
+    for (int k = 0; k < V; ++k)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (x[k][e] > p.top) {
+                p.top = x[k][e];
+                p.at = base + (k * kThreads + tid) * 4 + e;
+            }
+    if (a.logprob) {
+        const float by = p.top == -INFINITY ? 0.0f : p.top;
+#pragma unroll
+        for (int k = 0; k < V; ++k)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) p.sum += exp_of(x[k][e] - by);
+    }
+    p = join_lanes(p);
+    if ((tid & 63) == 0) waves[tid / 64] = p;
+    lds_barrier();
+    if (tid >= 64) return;
+    p = join_lanes(tid < kThreads / 64 ? waves[tid] : Part{-INFINITY, 0.0f, -1, 0});
+    if (tid != 0) return;
+    if (a.tiles == 1) finish(a, row, p);
+    else a.parts[blockIdx.x] = p;
+}
+
+// One wave a row joins its tiles' parts.
+__global__ __launch_bounds__(64) void join_kernel(PickArgs a)
+{
+    const int row = blockIdx.x, l = threadIdx.x;
+    const Part* parts = a.parts + (size_t)row * a.tiles;
+    Part p{-INFINITY, 0.0f, -1, 0};
+    for (int i = l; i < a.tiles; i += 64) {
+        // (in order of their indexes: of equal tops the first is kept)
+        const Part o = parts[i];
+        const float top = fmaxf(p.top, o.top), sum = p.sum * weight(p.top, top) + o.sum * weight(o.top, top);
+        if (o.top > p.top) p.at = o.at;
+        p.top = top;
+        p.sum = sum;
+    }
+    p = join_lanes(p);
+    if (l == 0) finish(a, row, p);
+}
+
 bool sizes_ok(int rows, int vocab) { return rows >= 1 && rows <= (1 << 20) && vocab >= 1 && vocab <= (1 << 24); }
-int tiles_of(int vocab) { return (vocab + kTile - 1) / kTile; }
+int tiles_of(int vocab, int V) { return (vocab + tile_of(V) - 1) / tile_of(V); }
+
+// The longest tile that still gives every CU two workgroups: each of a row's reads its whole history.
+int vecs_of(int rows, int vocab)
+{
+    int V = 4;
+    while (V > 1 && (int64_t)rows * tiles_of(vocab, V) < 512) V /= 2;
+    return V;
+}
+
+template <class T>
+void launch(const PickArgs& a, int V, hipStream_t s)
+{
+    const unsigned blocks = (unsigned)(a.rows * (int64_t)a.tiles);
+    if (V == 4) pick_kernel<T, 4><<<blocks, kThreads, 0, s>>>(a);
+    else if (V == 2) pick_kernel<T, 2><<<blocks, kThreads, 0, s>>>(a);
+    else pick_kernel<T, 1><<<blocks, kThreads, 0, s>>>(a);
+    if (a.tiles > 1) join_kernel<<<a.rows, 64, 0, s>>>(a);
+}
 
 }  // namespace
 }  // namespace heph
@@ -240,7 +338,7 @@ extern "C" {
 
 size_t heph_pick_ws_bytes(int rows, int vocab)
 {
-    return sizes_ok(rows, vocab) ? sizeof(Part) * (size_t)rows * tiles_of(vocab) : 0;
+    return sizes_ok(rows, vocab) ? sizeof(Part) * (size_t)rows * tiles_of(vocab, vecs_of(rows, vocab)) : 0;
 }
 
 int heph_pick_tokens(int32_t* tokens, float* logprob, void* out, int64_t out_stride,
@@ -266,8 +364,8 @@ int heph_pick_tokens(int32_t* tokens, float* logprob, void* out, int64_t out_str
     const size_t element = dtype == HEPH_DTYPE_F32 ? 4 : 2;
     if (!aligned(logits, element) || !aligned(out, element) || !aligned(ws, 16)) return HEPH_ERR_ALIGN;
     if (ws_bytes < heph_pick_ws_bytes(rows, vocab)) return HEPH_ERR_WORKSPACE;
-    const int64_t blocks = (int64_t)rows * tiles_of(vocab);
-    if (blocks > UINT32_MAX / kThreads) return HEPH_ERR_UNSUPPORTED;     // (a launch's most threads)
+    const int V = vecs_of(rows, vocab);
+    if (rows * (int64_t)tiles_of(vocab, V) > UINT32_MAX / kThreads) return HEPH_ERR_UNSUPPORTED;     // (a launch's most threads)
     if (int st = check_device()) return st;
     PickArgs a{};
     a.tokens = tokens;
@@ -283,13 +381,12 @@ int heph_pick_tokens(int32_t* tokens, float* logprob, void* out, int64_t out_str
     if (rules) a.rules = *rules;
     a.rows = rows;
     a.vocab = vocab;
-    a.tiles = tiles_of(vocab);
+    a.tiles = tiles_of(vocab, V);
     a.n_masks = n_masks;
     a.append = append;
     hipStream_t s = static_cast<hipStream_t>(stream);
-    if (dtype == HEPH_DTYPE_F32) pick_kernel<float><<<(unsigned)blocks, kThreads, 0, s>>>(a);
-    else pick_kernel<uint16_t><<<(unsigned)blocks, kThreads, 0, s>>>(a);
-    join_kernel<<<rows, 64, 0, s>>>(a);
+    if (dtype == HEPH_DTYPE_F32) launch<float>(a, V, s);
+    else launch<uint16_t>(a, V, s);
     return status_of(hipGetLastError());
 }
 
