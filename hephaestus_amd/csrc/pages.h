@@ -21,6 +21,14 @@ __host__ __device__ __forceinline__ int v_place(int j)
 __host__ __device__ __forceinline__ int k_byte(int j, int d) { return d / 64 * 4096 + j * 64 + d % 64; }
 __host__ __device__ __forceinline__ int v_byte(int j, int d) { return d * 64 + v_place(j); }
 
+// s_waitcnt: at most N of this wave's vector memory operations and no LDS one left.
+template <int N>
+__device__ __forceinline__ void wait_vm()
+{
+    __builtin_amdgcn_s_waitcnt(0x0070 | (N & 15) | (N >> 4) << 14);
+    asm volatile("" ::: "memory");
+}
+
 // LDS accesses of the workgroup before and behind it are ordered; loads from
 // memory stay in flight (__syncthreads would wait for them).
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }

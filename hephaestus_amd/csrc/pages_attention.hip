@@ -835,14 +835,6 @@ __device__ __forceinline__ int page_ids(const AttnArgs& a, const Unit& u, int p)
     return n < a.table_pages ? a.table[(size_t)u.seq * a.table_pages + n] : -1;
 }
 
-// s_waitcnt: at most N of this wave's vector memory operations and no LDS one left.
-template <int N>
-__device__ __forceinline__ void wait_vm()
-{
-    __builtin_amdgcn_s_waitcnt(0x0070 | (N & 15) | (N >> 4) << 14);
-    asm volatile("" ::: "memory");
-}
-
 // Up to 64 rows: a wave takes 16 of them and, where that leaves waves, every
 // KW-th page of the run. Bound by the stream of K and V: the next page's 16 KB
 // a wave are on their way into registers while one is worked on. (64 sequences, each

@@ -35,8 +35,13 @@ __device__ __forceinline__ void norm_rope(float (&lo)[8], float (&hi)[8], const 
     float ss = 0.0f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) ss = __builtin_fmaf(lo[i], lo[i], __builtin_fmaf(hi[i], hi[i], ss));
-#pragma unroll
-    for (int m = 1; m < 8; m <<= 1) ss += __shfl_xor(ss, m);
+    // over the eight lanes: the neighbour, the other pair, the other quad (whose lanes are equal by then)
+    auto other = [](float x, auto ctrl) {
+        return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), decltype(ctrl)::value, 0xf, 0xf, false));
+    };
+    ss += other(ss, std::integral_constant<int, 0xB1>{});
+    ss += other(ss, std::integral_constant<int, 0x4E>{});
+    ss += other(ss, std::integral_constant<int, 0x141>{});
     const float r = 1.0f / __fsqrt_rn(ss * (1.0f / kHeadDim) + eps);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {

@@ -29,19 +29,21 @@ __device__ __forceinline__ int exp_in(float scale)
     return min(max(e, kMinExp), kMaxExp);
 }
 
-// x * 2^-e as an E4M3 value; what is no number in E4M3 (NaN, infinities) is NaN.
-__device__ __forceinline__ float in_block(float x, int e)
+// Codes of eight values times f = 2^-e; what is no number in E4M3 (NaN, infinities) is NaN.
+__device__ __forceinline__ float in_block(float x, float f)
 {
-    const float y = __builtin_amdgcn_ldexpf(x, -e);
-    const float c = fminf(fmaxf(y, -kE4M3Max), kE4M3Max);
-    return __builtin_fabsf(x) <= 3.4028234663852886e38f ? c : __uint_as_float(0x7FC00000u);
+    const float y = __builtin_amdgcn_fmed3f(x * f, -kE4M3Max, kE4M3Max);
+    return __builtin_fabsf(x) <= 3.4028234663852886e38f ? y : __uint_as_float(0x7FC00000u);
 }
 
-__device__ __forceinline__ uint2 block_codes8(const float* f, int e)
+__device__ __forceinline__ uint2 block_codes8(const float* x, float f)
 {
-    return make_uint2(pack4_e4m3(in_block(f[0], e), in_block(f[1], e), in_block(f[2], e), in_block(f[3], e)),
-                      pack4_e4m3(in_block(f[4], e), in_block(f[5], e), in_block(f[6], e), in_block(f[7], e)));
+    return make_uint2(pack4_e4m3(in_block(x[0], f), in_block(x[1], f), in_block(x[2], f), in_block(x[3], f)),
+                      pack4_e4m3(in_block(x[4], f), in_block(x[5], f), in_block(x[6], f), in_block(x[7], f)));
 }
+
+// 2^-e of a block's e: a normal float.
+__device__ __forceinline__ float inverse(int e) { return __uint_as_float((uint32_t)(127 - e) << 23); }
 
 // Largest finite |f|.
 __device__ __forceinline__ float finite_max8(const float* f, float m)
@@ -85,177 +87,288 @@ struct WriteArgs {
     float eps;
 };
 
-// A wave takes eight query heads of one token.
+// A wave takes 8 * B query heads of one token: their loads are all on their way at once, which
+// keeps memory busy with the few waves that the blocks' registers leave.
+template <int B>
 __device__ __forceinline__ void q_heads(const WriteArgs& a, long unit)
 {
-    const int blocks = (a.n_heads + 7) / 8, lane = threadIdx.x & 63, c = lane & 7;
-    const int t = (int)(unit / blocks), h = (int)(unit % blocks) * 8 + lane / 8;
-    if (t >= a.n_tok || h >= a.n_heads) return;        // (whole heads: eight lanes at a time)
+    const int groups = (a.n_heads + 8 * B - 1) / (8 * B), lane = threadIdx.x & 63, c = lane & 7;
+    const int t = (int)(unit / groups), first = (int)(unit % groups) * 8 * B + lane / 8;
+    if (t >= a.n_tok) return;
     const int pos = a.positions[t];
-    const uint16_t* row = a.qkv + t * a.qkv_stride + (size_t)h * kHeadDim + 8 * c;
-    const uint4 x_lo = ldg16u(row), x_hi = ldg16u(row + 64);
+    const uint16_t* row = a.qkv + t * a.qkv_stride + 8 * c;
+    uint4 x_lo[B], x_hi[B];
+#pragma unroll
+    for (int i = 0; i < B; ++i) {
+        const uint16_t* p = row + (size_t)min(first + 8 * i, a.n_heads - 1) * kHeadDim;
+        x_lo[i] = ldg16u(p);
+        x_hi[i] = ldg16u(p + 64);
+    }
     const uint4 y_lo = ldg16u(a.q_gamma + 8 * c), y_hi = ldg16u(a.q_gamma + 64 + 8 * c);
     if (pos < 0 || pos >= a.n_rope) return;
     const float4* cs = reinterpret_cast<const float4*>(a.rope + (size_t)pos * kHeadDim + 16 * c);
     const float4 w[4] = {cs[0], cs[1], cs[2], cs[3]};
-    float lo[8], hi[8];
-    norm_rope(lo, hi, x_lo, x_hi, y_lo, y_hi, w, a.eps);
-    store_head(a.q_out + t * a.q_stride + (size_t)h * kHeadDim + 8 * c, lo, hi);
+#pragma unroll
+    for (int i = 0; i < B; ++i) {
+        const int h = first + 8 * i;
+        if (h >= a.n_heads) return;                // (whole heads: eight lanes at a time)
+        float lo[8], hi[8];
+        norm_rope(lo, hi, x_lo[i], x_hi[i], y_lo, y_hi, w, a.eps);
+        store_head(a.q_out + t * a.q_stride + (size_t)h * kHeadDim + 8 * c, lo, hi);
+    }
 }
 
-// A workgroup takes the runs of tokens of one page that start among its W tokens, one kv head.
+// One thread's part of a token: sixteen values of k (normalized and rotated), dims 8c .. and
+// 64+8c .., or of v. K and V of a block have nothing to do with each other: different waves and
+// workgroups take them.
+template <bool V>
+struct Values {
+    float lo[8], hi[8];
+    uint4 w_lo, w_hi;              // v as it came
+
+    // Token t's, and the largest finite magnitude.
+    __device__ __forceinline__ float load(const WriteArgs& a, int h, int64_t t, int pos, int c)
+    {
+        const uint16_t* p = a.qkv + t * a.qkv_stride + (size_t)(a.n_heads + (V ? a.n_kv : 0) + h) * kHeadDim + 8 * c;
+        w_lo = ldg16u(p);
+        w_hi = ldg16u(p + 64);
+        if constexpr (V) {
+            unpack8(w_lo, lo);
+            unpack8(w_hi, hi);
+        } else {
+            const float4* cs = reinterpret_cast<const float4*>(a.rope + (size_t)pos * kHeadDim + 16 * c);
+            const float4 w[4] = {cs[0], cs[1], cs[2], cs[3]};
+            const uint4 y_lo = ldg16u(a.k_gamma + 8 * c), y_hi = ldg16u(a.k_gamma + 64 + 8 * c);
+            norm_rope(lo, hi, w_lo, w_hi, y_lo, y_hi, w, a.eps);
+        }
+        return finite_max8(hi, finite_max8(lo, 0.0f));
+    }
+    // Codes of the two eights under 2^e.
+    __device__ __forceinline__ void codes(uint2 (&w)[2], int e)
+    {
+        if constexpr (V) {         // (unpacked again: fewer registers while the block's scale is found)
+            unpack8(w_lo, lo);
+            unpack8(w_hi, hi);
+        }
+        w[0] = block_codes8(lo, inverse(e));
+        w[1] = block_codes8(hi, inverse(e));
+    }
+};
+
+// A block: its codes, its scale, and the exponent that the scale had.
+template <bool V>
+struct Block {
+    uint8_t* codes;
+    float* scale;
+    int was;
+
+    __device__ __forceinline__ Block(const WriteArgs& a, int page, int h)
+        : codes((V ? a.v_pages : a.k_pages) + ((size_t)page * a.n_kv + h) * kPageBytes),
+          scale(a.scale + (size_t)page * 2 * a.n_kv + (V ? a.n_kv : 0) + h), was(exp_in(*scale))
+    {
+    }
+    // Its exponent with new values up to top.
+    __device__ __forceinline__ int grow(float top, bool fresh) const
+    {
+        const int e = exp_of(top);
+        return fresh ? e : max(e, was);
+    }
+    // The codes that are there divided by 2^(e - was), by THREADS threads.
+    template <int THREADS>
+    __device__ __forceinline__ void rescale(int e, int tid) const
+    {
+        const float f = __builtin_amdgcn_ldexpf(1.0f, was - e);
+        uint4* w = reinterpret_cast<uint4*>(codes) + tid;
+#pragma unroll 1
+        for (int i = 0; i < kPageBytes / 16; i += THREADS) {
+            const uint4 x = w[i];
+            w[i] = make_uint4(rescale4(x.x, f), rescale4(x.y, f), rescale4(x.z, f), rescale4(x.w, f));
+        }
+    }
+    __device__ __forceinline__ void store_scale(int e) const { *scale = __builtin_amdgcn_ldexpf(1.0f, e); }
+    __device__ __forceinline__ void store_k(int key, int c, const uint2 (&w)[2]) const
+    {
+        *reinterpret_cast<uint2*>(codes + k_byte(key, 8 * c)) = w[0];
+        *reinterpret_cast<uint2*>(codes + k_byte(key, 64 + 8 * c)) = w[1];
+    }
+};
+
 constexpr int kPitch = kHeadDim + 4;               // bytes of a token's codes in LDS
 struct WriteLds {
     uint32_t v[kPage * kPitch / 4];
-    float amax[2][4];
+    float top[8];
     int has[kPage];
 };
 
-// n <= 64 tokens from t0 on, all of page `page`: lane i's slot and position are token t0 + i's.
-__device__ __forceinline__ void write_block(const WriteArgs& a, WriteLds& lds, int h, int t0, int n, int page,
-                                            int slot, int pos)
+// n <= 8 tokens from t0 on, all of page `page`, by one wave: slot and pos are those of this lane's
+// token, t0 + l/8; fresh: key 0 is among them. V's codes leave as single bytes.
+template <bool V>
+__device__ __forceinline__ void write_few(const WriteArgs& a, int h, int t0, int n, int page, bool fresh, int slot,
+                                          int pos)
 {
-    const int tid = threadIdx.x, l = tid & 63, c = tid & 7;
-    const size_t at = (size_t)page * a.n_kv + h;
-    float* scale = a.scale + (size_t)page * 2 * a.n_kv + h;
-    const float old_k = scale[0], old_v = scale[a.n_kv];
-    const uint16_t* gamma = a.k_gamma + 8 * c;
-    const uint4 y_lo = ldg16u(gamma), y_hi = ldg16u(gamma + 64);
-    const int key = slot & (kPage - 1);
-    const bool fresh = __ballot(l < n && key == 0) != 0;
-    // thread: dims 8c .., 64+8c .. of tokens tid/8 and 32 + tid/8
-    float lo[2][8], hi[2][8];
-    uint4 v_lo[2], v_hi[2];
-    int my_key[2];
-    float top_k = 0.0f, top_v = 0.0f;
+    const int l = threadIdx.x & 63, c = l & 7, i = l / 8, key = slot & (kPage - 1);
+    const Block<V> block(a, page, h);
+    Values<V> x;
+    float top = 0.0f;
+    if (i < n) top = x.load(a, h, t0 + i, pos, c);
+    const int e = block.grow(wave_fold_max64(top), fresh);
+    if (!fresh && e > block.was) {
+        block.template rescale<64>(e, l);
+        wait_vm<0>();                              // (the new codes come behind)
+    }
+    if (l == 0) block.store_scale(e);
+    if (i >= n) return;
+    uint2 w[2];
+    x.codes(w, e);
+    if constexpr (V) {
+        uint8_t* to = block.codes + v_byte(key, 8 * c);
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-        const int i = r * 32 + tid / 8;
+        for (int half = 0; half < 2; ++half)
+#pragma unroll
+            for (int d = 0; d < 8; ++d)
+                to[half * 4096 + d * 64] = (uint8_t)((d < 4 ? w[half].x : w[half].y) >> (d % 4 * 8));
+    } else {
+        block.store_k(key, c, w);
+    }
+}
+
+// The same for n <= 64 by the workgroup; lane i's slot and position are token t0 + i's.
+template <int THREADS, bool V>
+__device__ __forceinline__ void write_block(const WriteArgs& a, WriteLds& lds, int h, int t0, int n, int page,
+                                            bool fresh, int slot, int pos)
+{
+    constexpr int R = 512 / THREADS;               // a thread's tokens: tid/8, and every THREADS/8-th
+    const int tid = threadIdx.x, l = tid & 63, c = tid & 7, key = slot & (kPage - 1);
+    const Block<V> block(a, page, h);
+    Values<V> x[R];
+    int my_key[R];
+    float top = 0.0f;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const int i = r * (THREADS / 8) + tid / 8;
         my_key[r] = __shfl(key, i);
         const int p = __shfl(pos, i);
-        if (i >= n) continue;
-        const uint16_t* row = a.qkv + (int64_t)(t0 + i) * a.qkv_stride + (size_t)(a.n_heads + h) * kHeadDim + 8 * c;
-        const uint16_t* v = row + (size_t)a.n_kv * kHeadDim;
-        const uint4 x_lo = ldg16u(row), x_hi = ldg16u(row + 64);
-        v_lo[r] = ldg16u(v);
-        v_hi[r] = ldg16u(v + 64);
-        const float4* cs = reinterpret_cast<const float4*>(a.rope + (size_t)p * kHeadDim + 16 * c);
-        const float4 w[4] = {cs[0], cs[1], cs[2], cs[3]};
-        norm_rope(lo[r], hi[r], x_lo, x_hi, y_lo, y_hi, w, a.eps);
-        top_k = finite_max8(hi[r], finite_max8(lo[r], top_k));
-        float f[8];
-        unpack8(v_lo[r], f);
-        top_v = finite_max8(f, top_v);
-        unpack8(v_hi[r], f);
-        top_v = finite_max8(f, top_v);
+        if (i < n) top = fmaxf(top, x[r].load(a, h, t0 + i, p, c));
     }
-    top_k = wave_fold_max64(top_k);
-    top_v = wave_fold_max64(top_v);
-    if (l == 0) {
-        lds.amax[0][tid / 64] = top_k;
-        lds.amax[1][tid / 64] = top_v;
-    }
+    top = wave_fold_max64(top);
     if (tid < kPage) lds.has[tid] = 0;
+    if (l == 0) lds.top[tid / 64] = top;
     __syncthreads();
     if (tid < n) lds.has[key] = 1;
-    auto all = [&](const float (&m)[4]) { return fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])); };
-    int ek = exp_of(all(lds.amax[0])), ev = exp_of(all(lds.amax[1]));
-    uint8_t* kp = a.k_pages + at * kPageBytes;
-    uint8_t* vp = a.v_pages + at * kPageBytes;
-    if (!fresh) {
-        const int was_k = exp_in(old_k), was_v = exp_in(old_v);
-        ek = max(ek, was_k);
-        ev = max(ev, was_v);
-        auto rescale = [&](uint8_t* p, int by) {
-            const float f = __builtin_amdgcn_ldexpf(1.0f, by);
-            uint4* w = reinterpret_cast<uint4*>(p) + tid;
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const uint4 x = w[i * 256];
-                w[i * 256] = make_uint4(rescale4(x.x, f), rescale4(x.y, f), rescale4(x.z, f), rescale4(x.w, f));
-            }
-        };
-        if (ek > was_k) rescale(kp, was_k - ek);
-        if (ev > was_v) rescale(vp, was_v - ev);
-    }
-    if (tid == 0) {
-        scale[0] = __builtin_amdgcn_ldexpf(1.0f, ek);
-        scale[a.n_kv] = __builtin_amdgcn_ldexpf(1.0f, ev);
+    for (int i = 0; i < THREADS / 64; ++i) top = fmaxf(top, lds.top[i]);
+    const int e = block.grow(top, fresh);
+    if (!fresh && e > block.was) {                 // (the same in all threads)
+        block.template rescale<THREADS>(e, tid);
+        __syncthreads();                           // (the new codes come behind)
     }
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-        if (r * 32 + tid / 8 >= n) continue;
-        float f[8];
-        uint32_t* to = lds.v + my_key[r] * (kPitch / 4) + 2 * c;
-        unpack8(v_lo[r], f);
-        uint2 w = block_codes8(f, ev);
-        to[0] = w.x;
-        to[1] = w.y;
-        unpack8(v_hi[r], f);
-        w = block_codes8(f, ev);
-        to[16] = w.x;
-        to[17] = w.y;
-    }
-    __syncthreads();                               // (the old codes are written too)
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-        if (r * 32 + tid / 8 >= n) continue;
-        *reinterpret_cast<uint2*>(kp + k_byte(my_key[r], 8 * c)) = block_codes8(lo[r], ek);
-        *reinterpret_cast<uint2*>(kp + k_byte(my_key[r], 64 + 8 * c)) = block_codes8(hi[r], ek);
-    }
-    // V lies key-minor: dims 4g .. 4g+3 of four keys at a time
-    const uint8_t* bytes = reinterpret_cast<const uint8_t*>(lds.v);
-    for (int i = tid; i < 16 * 32; i += 256) {
-        const int j = i % 16 * 4, g = i / 16;
-        const int has = lds.has[j] | lds.has[j + 1] << 1 | lds.has[j + 2] << 2 | lds.has[j + 3] << 3;
-        if (has == 15) {
-            uint32_t k[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) k[e] = lds.v[(j + e) * (kPitch / 4) + g];
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                *reinterpret_cast<uint32_t*>(vp + v_byte(j, 4 * g + e)) = column(k, e);
-        } else if (has) {
-            for (int e = 0; e < 4; ++e)
-                if (has >> e & 1)
-                    for (int d = 4 * g; d < 4 * g + 4; ++d) vp[v_byte(j + e, d)] = bytes[(j + e) * kPitch + d];
+    for (int r = 0; r < R; ++r) {
+        if (r * (THREADS / 8) + tid / 8 >= n) continue;
+        uint2 w[2];
+        x[r].codes(w, e);
+        if constexpr (V) {
+            uint32_t* to = lds.v + my_key[r] * (kPitch / 4) + 2 * c;
+            to[0] = w[0].x;
+            to[1] = w[0].y;
+            to[16] = w[1].x;
+            to[17] = w[1].y;
+        } else {
+            block.store_k(my_key[r], c, w);
         }
     }
-    __syncthreads();                               // (LDS is used again)
-}
-
-template <int W>
-__device__ __forceinline__ void write_window(const WriteArgs& a, long unit)
-{
-    __shared__ WriteLds lds;
-    const int h = (int)(unit % a.n_kv), t0 = (int)(unit / a.n_kv) * W, l = threadIdx.x & 63;
-    // lane i: tokens t0 + i and t0 + 64 + i; a token that is not cached has no slot
-    auto slot_of = [&](int t, int& pos) {
-        if (t < 0 || t >= a.n_tok) return -1;
-        const int s = a.slots[t];
-        pos = a.positions[t];
-        return pos >= 0 && pos < a.n_rope && s >= 0 && s < a.n_slots ? s : -1;
-    };
-    int pos0 = 0, pos1 = 0, none = 0;
-    const int s0 = slot_of(t0 + l, pos0), s1 = slot_of(t0 + 64 + l, pos1);
-    const int p0 = s0 >> 6, p1 = s1 >> 6;          // (no slot: -1)
-    const int before = slot_of(t0 - 1, none) >> 6, shifted = __shfl_up(p0, 1);
-    const int prev = l ? shifted : before;
-    for (unsigned long long starts = __ballot(l < W && p0 >= 0 && p0 != prev); starts; starts &= starts - 1) {
-        const int s = __ffsll((long long)starts) - 1, page = __builtin_amdgcn_readlane(p0, s);
-        const unsigned long long same = __ballot(p0 == page) >> s |
-                                        (s ? __ballot(p1 == page) << (64 - s) : 0ull);
-        const int n = ~same ? __ffsll((long long)~same) - 1 : 64, i = (l + s) & 63;
-        const int a0 = __shfl(s0, i), a1 = __shfl(s1, i), b0 = __shfl(pos0, i), b1 = __shfl(pos1, i);
-        write_block(a, lds, h, t0 + s, n, page, l + s < 64 ? a0 : a1, l + s < 64 ? b0 : b1);
+    __syncthreads();                               // (the scale is read by all)
+    if (tid == 0) block.store_scale(e);
+    if constexpr (V) {
+        // V lies key-minor: dims 4g .. 4g+3 of four keys at a time
+        const uint8_t* bytes = reinterpret_cast<const uint8_t*>(lds.v);
+#pragma unroll
+        for (int i = tid; i < 16 * 32; i += THREADS) {
+            const int j = i % 16 * 4, g = i / 16;
+            const int has = lds.has[j] | lds.has[j + 1] << 1 | lds.has[j + 2] << 2 | lds.has[j + 3] << 3;
+            if (has == 15) {
+                uint32_t k[4];
+#pragma unroll
+                for (int d = 0; d < 4; ++d) k[d] = lds.v[(j + d) * (kPitch / 4) + g];
+#pragma unroll
+                for (int d = 0; d < 4; ++d)
+                    *reinterpret_cast<uint32_t*>(block.codes + v_byte(j, 4 * g + d)) = column(k, d);
+            } else if (has) {
+#pragma unroll 1
+                for (int k = 0; k < 4; ++k)
+                    if (has >> k & 1)
+#pragma unroll
+                        for (int d = 0; d < 4; ++d)
+                            block.codes[v_byte(j + k, 4 * g + d)] = bytes[(j + k) * kPitch + 4 * g + d];
+            }
+        }
+        __syncthreads();                           // (LDS is used again)
     }
 }
 
-template <int W>
-__global__ __launch_bounds__(256) void write_kernel(WriteArgs a, long page_blocks)
+// A workgroup takes K or V of one kv head of the runs of tokens of one page that start among its W
+// tokens: each run of up to eight by a wave, then the longer ones by all of them.
+template <int THREADS, int W, bool V>
+__device__ __forceinline__ void write_window(const WriteArgs& a, WriteLds& lds, int h, int t0)
 {
-    if ((long)blockIdx.x < page_blocks) write_window<W>(a, blockIdx.x);
-    else q_heads(a, ((long)blockIdx.x - page_blocks) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6));
+    const int l = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    // lane i: tokens t0 + i and t0 + 64 + i (all loads at once); a token that is not cached has no slot
+    const int u0 = t0 + l, u1 = u0 + 64, ub = t0 - 1, last = a.n_tok - 1;
+    int s0 = a.slots[min(u0, last)], s1 = a.slots[min(u1, last)], sb = a.slots[max(ub, 0)];
+    const int pos0 = a.positions[min(u0, last)], pos1 = a.positions[min(u1, last)], posb = a.positions[max(ub, 0)];
+    auto cached = [&](int t, int s, int pos) {
+        return (t >= 0) & (t <= last) & (pos >= 0) & (pos < a.n_rope) & (s >= 0) & (s < a.n_slots);
+    };
+    s0 = cached(u0, s0, pos0) ? s0 : -1;
+    s1 = cached(u1, s1, pos1) ? s1 : -1;
+    sb = cached(ub, sb, posb) ? sb : -1;
+    const int p0 = s0 >> 6, p1 = s1 >> 6;          // (no slot: -1)
+    const int shifted = __builtin_amdgcn_update_dpp(sb >> 6, p0, 0x138, 0xF, 0xF, false);     // the lane below's
+    unsigned long long starts = __ballot(l < W && p0 >= 0 && p0 != shifted), more = 0;
+    // The run that starts at lane s: its page and tokens, and lane i's slot and position of its i-th.
+    auto page_of = [&](int s) { return __builtin_amdgcn_readlane(p0, s); };
+    auto from = [](int s, unsigned long long m0, unsigned long long m1) { return m0 >> s | (s ? m1 << (64 - s) : 0ull); };
+    auto length = [&](int s) {
+        const int page = page_of(s);
+        const unsigned long long same = from(s, __ballot(p0 == page), __ballot(p1 == page));
+        return ~same ? __ffsll((long long)~same) - 1 : 64;
+    };
+    const unsigned long long first0 = __ballot((s0 & (kPage - 1)) == 0), first1 = __ballot((s1 & (kPage - 1)) == 0);
+    auto fresh = [&](int s, int n) { return (from(s, first0, first1) << (64 - n)) != 0; };
+    // token i of the run's value
+    auto of_run = [&](int s, int i, int v0, int v1) {
+        const int a0 = __shfl(v0, (i + s) & 63);
+        const int a1 = __shfl(v1, (i + s) & 63);
+        return i + s < 64 ? a0 : a1;
+    };
+    for (int k = 0; starts; starts &= starts - 1) {
+        const int s = __ffsll((long long)starts) - 1, n = length(s);
+        if (n > 8) more |= 1ull << s;
+        else if (k++ % (THREADS / 64) == wave)
+            write_few<V>(a, h, t0 + s, n, page_of(s), fresh(s, n), of_run(s, l / 8, s0, s1), of_run(s, l / 8, pos0, pos1));
+    }
+    for (; more; more &= more - 1) {
+        const int s = __ffsll((long long)more) - 1, n = length(s);
+        write_block<THREADS, V>(a, lds, h, t0 + s, n, page_of(s), fresh(s, n), of_run(s, l, s0, s1), of_run(s, l, pos0, pos1));
+    }
+}
+
+// Every q_every-th workgroup takes query heads, the others windows of tokens, until either are done.
+template <int THREADS, int W, int B>
+__global__ __launch_bounds__(THREADS) void write_kernel(WriteArgs a, int q_every, int page_blocks)
+{
+    const int b = blockIdx.x, turn = b / q_every;
+    const bool is_q = b % q_every == 0;
+    if (!is_q) {
+        __shared__ WriteLds lds;
+        const int unit = b - turn - 1, index = unit % (2 * a.n_kv), t0 = unit / (2 * a.n_kv) * W;
+        if (unit >= page_blocks) return;
+        if (index < a.n_kv) write_window<THREADS, W, false>(a, lds, index, t0);
+        else write_window<THREADS, W, true>(a, lds, index - a.n_kv, t0);
+    } else {
+        q_heads<B>(a, (long)turn * (THREADS / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6));
+    }
 }
 
 // ------------------------------------------------------------------- read ----
@@ -365,10 +478,13 @@ int heph_qk_norm_rope_pages_scaled(void* q_out_bf16, int64_t q_stride, const voi
     // in place only with the rows where they are: another stride would let one wave overwrite
     // what the next one reads
     if (q_out_bf16 == qkv_bf16 && q_stride != qkv_stride) return HEPH_ERR_SHAPE;
-    const int W = n_tok > 512 ? 16 : 1;
-    const int64_t page_blocks = ((int64_t)n_tok + W - 1) / W * n_kv_heads;
-    const int64_t blocks = page_blocks + ((int64_t)n_tok * ((n_heads + 7) / 8) + 3) / 4;
-    if (blocks > UINT32_MAX / 256) return HEPH_ERR_UNSUPPORTED;          // (a launch's most threads)
+    const bool many = n_tok > 1024;
+    const int W = many ? 64 : 4, waves = many ? 8 : 4, heads_a_wave = many ? 32 : 8;
+    const int64_t page_blocks = ((int64_t)n_tok + W - 1) / W * 2 * n_kv_heads;
+    const int64_t q_blocks = ((int64_t)n_tok * ((n_heads + heads_a_wave - 1) / heads_a_wave) + waves - 1) / waves;
+    // one q block and then q_every - 1 of pages, in turn
+    const int64_t q_every = 1 + (page_blocks + q_blocks - 1) / q_blocks, blocks = q_blocks * q_every;
+    if (blocks > UINT32_MAX / 512) return HEPH_ERR_UNSUPPORTED;          // (a launch's most threads)
     if (int st = check_device()) return st;
     WriteArgs a;
     a.q_out = static_cast<uint16_t*>(q_out_bf16);
@@ -390,8 +506,8 @@ int heph_qk_norm_rope_pages_scaled(void* q_out_bf16, int64_t q_stride, const voi
     a.n_kv = n_kv_heads;
     a.eps = eps;
     hipStream_t s = static_cast<hipStream_t>(stream);
-    if (W == 16) write_kernel<16><<<(unsigned)blocks, 256, 0, s>>>(a, page_blocks);
-    else write_kernel<1><<<(unsigned)blocks, 256, 0, s>>>(a, page_blocks);
+    if (many) write_kernel<512, 64, 4><<<(unsigned)blocks, 512, 0, s>>>(a, (int)q_every, (int)page_blocks);
+    else write_kernel<256, 4, 1><<<(unsigned)blocks, 256, 0, s>>>(a, (int)q_every, (int)page_blocks);
     return status_of(hipGetLastError());
 }
 
