@@ -1064,39 +1064,40 @@ __device__ __forceinline__ void merge_row(const AttnArgs& a, const Token& tk, lo
                                            : tk.own + (k - tk.n_prefix) * tk.own_step) + h % G;
         return (size_t)(h / G) * max_parts + ((unsigned long)part < (unsigned long)max_parts ? part : 0);
     };
-    float2 ml[2];
-    float top = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        ml[i] = i * 64 + l < n ? a.part_ml[slot(i * 64 + l)] : make_float2(-INFINITY, 0.0f);
-        top = fmaxf(top, ml[i].x);
-    }
-    top = wave_fold_max64(top);
-    const float f0 = weight(ml[0].x, top), f1 = weight(ml[1].x, top);
-    const float sum = wave_fold_sum64(__builtin_fmaf(ml[0].y, f0, ml[1].y * f1));
     const float2* part = reinterpret_cast<const float2*>(a.part_o) + l;
-    float x = 0.0f, y = 0.0f;
-    auto add = [&](auto parts, int k) {
+    float x = 0.0f, y = 0.0f, top = -INFINITY, sum;
+    // P of the parts on their way at a time, the first ones beside the maxima and sums
+    auto join = [&](auto parts) {
         constexpr int P = decltype(parts)::value;
-        float2 o[P];
+        float2 ml[2], o[P];
+        auto load = [&](int k) {
 #pragma unroll
-        for (int i = 0; i < P; ++i) o[i] = part[slot(min(k + i, n - 1)) * (kHeadDim / 2)];
+            for (int i = 0; i < P; ++i) o[i] = part[slot(min(k + i, n - 1)) * (kHeadDim / 2)];
+        };
 #pragma unroll
-        for (int i = 0; i < P; ++i) {
-            const float f = __int_as_float(__builtin_amdgcn_readlane(
-                __float_as_int(k + i < 64 ? f0 : f1), (k + i) & 63));
-            if (k + i < n) {
-                x = __builtin_fmaf(o[i].x, f, x);
-                y = __builtin_fmaf(o[i].y, f, y);
+        for (int i = 0; i < 2; ++i)
+            ml[i] = i * 64 + l < n ? a.part_ml[slot(i * 64 + l)] : make_float2(-INFINITY, 0.0f);
+        load(0);
+        top = wave_fold_max64(fmaxf(ml[0].x, ml[1].x));
+        const float f0 = weight(ml[0].x, top), f1 = weight(ml[1].x, top);
+        sum = wave_fold_sum64(__builtin_fmaf(ml[0].y, f0, ml[1].y * f1));
+        for (int k = 0; k < n; k += P) {
+            if (k > 0) load(k);
+#pragma unroll
+            for (int i = 0; i < P; ++i) {
+                const float f = lane_of(k + i < 64 ? f0 : f1, (k + i) & 63);
+                if (k + i < n) {
+                    x = __builtin_fmaf(o[i].x, f, x);
+                    y = __builtin_fmaf(o[i].y, f, y);
+                }
             }
         }
     };
-    // (as many loads on their way as there are parts, up to 16: one sequence of 32768 keys
-    // 24.3 us, 25.7 with eight always; four tokens behind 512 keys, four layers, 42.0 and 42.6)
-    if (n <= 4) add(std::integral_constant<int, 4>{}, 0);
-    else if (n <= 8) add(std::integral_constant<int, 8>{}, 0);
-    else
-        for (int k = 0; k < n; k += 16) add(std::integral_constant<int, 16>{}, k);
+    // (as many as there are, up to 16: 32 take registers that many rows' waves need, 15.3 us for 12.5 where
+    // six prompts of 700 tokens are joined)
+    if (n <= 4) join(std::integral_constant<int, 4>{});
+    else if (n <= 8) join(std::integral_constant<int, 8>{});
+    else join(std::integral_constant<int, 16>{});
     const float f = sum == 0.0f && top == -INFINITY ? 0.0f : out_scale<BLOCK>(a, h / G) / sum;
     *reinterpret_cast<uint32_t*>(a.out + row * kHeadDim + 2 * l) =
         (uint32_t)f32_to_bf16(x * f) | (uint32_t)f32_to_bf16(y * f) << 16;

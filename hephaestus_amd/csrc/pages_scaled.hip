@@ -479,7 +479,7 @@ int heph_qk_norm_rope_pages_scaled(void* q_out_bf16, int64_t q_stride, const voi
     // what the next one reads
     if (q_out_bf16 == qkv_bf16 && q_stride != qkv_stride) return HEPH_ERR_SHAPE;
     const bool many = n_tok > 1024;
-    const int W = many ? 64 : 4, waves = many ? 8 : 4, heads_a_wave = many ? 32 : 8;
+    const int W = many ? 64 : 4, waves = many ? 8 : 4, heads_a_wave = many ? 16 : 8;
     const int64_t page_blocks = ((int64_t)n_tok + W - 1) / W * 2 * n_kv_heads;
     const int64_t q_blocks = ((int64_t)n_tok * ((n_heads + heads_a_wave - 1) / heads_a_wave) + waves - 1) / waves;
     // one q block and then q_every - 1 of pages, in turn
@@ -506,7 +506,7 @@ int heph_qk_norm_rope_pages_scaled(void* q_out_bf16, int64_t q_stride, const voi
     a.n_kv = n_kv_heads;
     a.eps = eps;
     hipStream_t s = static_cast<hipStream_t>(stream);
-    if (many) write_kernel<512, 64, 4><<<(unsigned)blocks, 512, 0, s>>>(a, (int)q_every, (int)page_blocks);
+    if (many) write_kernel<512, 64, 2><<<(unsigned)blocks, 512, 0, s>>>(a, (int)q_every, (int)page_blocks);
     else write_kernel<256, 4, 1><<<(unsigned)blocks, 256, 0, s>>>(a, (int)q_every, (int)page_blocks);
     return status_of(hipGetLastError());
 }
