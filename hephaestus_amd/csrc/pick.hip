@@ -312,11 +312,19 @@ bool sizes_ok(int rows, int vocab) { return rows >= 1 && rows <= (1 << 20) && vo
 int tiles_of(int vocab, int V) { return (vocab + tile_of(V) - 1) / tile_of(V); }
 
 // The longest tile that still gives every CU two workgroups: each of a row's reads its whole history.
+constexpr int kMostVecs = 4, kEnough = 512;
 int vecs_of(int rows, int vocab)
 {
-    int V = 4;
-    while (V > 1 && (int64_t)rows * tiles_of(vocab, V) < 512) V /= 2;
+    int V = kMostVecs;
+    while (V > 1 && (int64_t)rows * tiles_of(vocab, V) < kEnough) V /= 2;
     return V;
+}
+
+// Parts of as many rows or fewer, of a vocabulary as large or smaller: where a tile is halved, there
+// were less than kEnough of the longer ones.
+int64_t most_parts(int rows, int vocab)
+{
+    return std::max<int64_t>((int64_t)rows * tiles_of(vocab, kMostVecs), 2 * kEnough);
 }
 
 template <class T>
@@ -338,7 +346,7 @@ extern "C" {
 
 size_t heph_pick_ws_bytes(int rows, int vocab)
 {
-    return sizes_ok(rows, vocab) ? sizeof(Part) * (size_t)rows * tiles_of(vocab, vecs_of(rows, vocab)) : 0;
+    return sizes_ok(rows, vocab) ? sizeof(Part) * (size_t)most_parts(rows, vocab) : 0;
 }
 
 int heph_pick_tokens(int32_t* tokens, float* logprob, void* out, int64_t out_stride,

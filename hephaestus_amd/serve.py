@@ -416,7 +416,7 @@ class TokenRules:
 
 
 def pick_ws(rows: int, vocab: int, device="cuda") -> torch.Tensor:
-    """Scratch for pick_tokens over [rows, vocab] logits."""
+    """Scratch for pick_tokens over [rows, vocab] logits, or fewer of either."""
     nb = L.lib().heph_pick_ws_bytes(rows, vocab)
     if nb == 0:
         raise HephError(L.HEPH_ERR_SHAPE, "pick_ws")
@@ -739,10 +739,7 @@ class Qwen3BatchDecoder:
         try:
             return self._run(tokens, seqs, adapters)
         except BaseException:
-            for s, length, pages in before:
-                for p in s.pages[pages:]:
-                    kv._drop(p)
-                s.length, s.pages = length, s.pages[:pages]
+            self._undo(before)
             raise
 
     def next_tokens(self, tokens: list[list[int]], seqs: list[Sequence], adapters: list[int] | None = None,
@@ -750,28 +747,41 @@ class Qwen3BatchDecoder:
                     mask_ids: list[int] | None = None) -> tuple[torch.Tensor, torch.Tensor]:
         """step(), and the pick of each sequence's next token from its logits (pick_tokens: rules
         of slots[i] and mask mask_ids[i], -1: none) as int32 [len(seqs)], with their
-        log-probabilities, both in device memory. The tokens are written behind their histories."""
+        log-probabilities, both in device memory. The tokens are written behind their histories.
+        A call that raises leaves the sequences as they were."""
         S, dev = len(seqs), self.w.embed.w.device
+        vocab = self.w.cfg.vocab
         if (rules is None) != (slots is None) or (masks is None) != (mask_ids is None):
             raise ValueError("rules come with slots, masks with mask_ids")
-        if slots is not None:
+        if rules is not None:
             used = [s for s in slots if s >= 0]
             if len(slots) != S or len(set(used)) != len(used) or any(s >= rules.n_slots for s in used):
                 raise ValueError(f"slots {slots} are not one of {rules.n_slots} for each of {S} sequences")
-            if rules.vocab != self.w.cfg.vocab:
-                raise ValueError(f"rules of {rules.vocab} tokens, {self.w.cfg.vocab} in the model")
-        if mask_ids is not None:
+            if rules.vocab != vocab or rules._dev != self.w.embed.w.get_device():
+                raise ValueError(f"rules of {rules.vocab} tokens on device {rules._dev} for a model of {vocab} on {dev}")
+        if masks is not None:
             if len(mask_ids) != S or any(m >= masks.shape[0] for m in mask_ids):
                 raise ValueError(f"mask_ids {mask_ids} are not one of {masks.shape[0]} for each of {S} sequences")
-            if masks.shape[1:] != ((self.w.cfg.vocab + 31) // 32,) or masks.dtype != torch.int32:
-                raise ValueError(f"masks {tuple(masks.shape)} for a vocabulary of {self.w.cfg.vocab}")
+            _matrix(masks, "masks", _I32, masks.shape[0], (vocab + 31) // 32, self.w.embed.w.get_device())
         ids = [None if x is None else torch.tensor(array("i", x), dtype=torch.int32, device=dev)
                for x in (slots, mask_ids)]
+        before = [(s, s.length, len(s.pages)) for s in seqs]
         logits = self.step(tokens, seqs, adapters)
-        picked = torch.empty(S, dtype=torch.int32, device=dev)
-        logprob = torch.empty(S, dtype=torch.float32, device=dev)
-        pick_tokens(picked, logits, rules, ids[0], masks, ids[1], logprob=logprob, append=rules is not None)
+        try:
+            picked = torch.empty(S, dtype=torch.int32, device=dev)
+            logprob = torch.empty(S, dtype=torch.float32, device=dev)
+            pick_tokens(picked, logits, rules, ids[0], masks, ids[1], logprob=logprob, append=rules is not None)
+        except BaseException:
+            self._undo(before)
+            raise
         return picked, logprob
+
+    def _undo(self, before) -> None:
+        """The sequences as they were: (sequence, length, pages) each."""
+        for s, length, pages in before:
+            for p in s.pages[pages:]:
+                self.kv._drop(p)
+            s.length, s.pages = length, s.pages[:pages]
 
     def _layout(self, tokens, seqs, adapters) -> list:
         """The sequences take their tokens; the int32 values that the step's ops read: tokens,

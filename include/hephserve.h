@@ -261,8 +261,9 @@ int heph_lora_add(void* c, int c_dtype, const void* base, const uint16_t* x_bf16
  * with max_bias 0), masks [n_masks][(vocab + 31) / 32]. max_tokens up to
  * 262144, max_bias up to HEPH_PICK_MAX_BIAS. Lengths are clamped to their
  * buffers on the device, ids outside the vocabulary are passed over.
- * ws: heph_pick_ws_bytes(rows, vocab) bytes, 16-byte aligned; calls that share it are
- * ordered by the caller.
+ * ws: heph_pick_ws_bytes(rows, vocab) bytes (which are enough for fewer rows and
+ * smaller vocabularies too), 16-byte aligned; calls that share it are ordered by
+ * the caller.
  * Replaces, for a batch with rules, argmax (src/hephaestus/kernels.mojo:1376-1433),
  * which rounds logits to bf16 first.
  */

@@ -262,6 +262,16 @@ def test_pick_appends_to_the_histories():
     assert np.array_equal(r.history.cpu().numpy(), want) and np.array_equal(r.length.cpu().numpy(), length)
 
 
+def test_pick_scratch_of_a_larger_batch_serves_smaller_ones():
+    ws = S.pick_ws(40, 151936)
+    for rows, vocab in ((40, 151936), (27, 151936), (26, 151936), (13, 151936), (1, 151936), (14, 50000), (3, 9)):
+        c = dict(case(rows, vocab, seed=rows), rules=None, slots=None)
+        tokens = i32([0] * rows)
+        S.pick_tokens(tokens, c["logits"], ws=ws)
+        assert torch.equal(tokens.long(), c["logits"].argmax(1))
+        assert S.pick_ws(rows, vocab).numel() <= ws.numel()
+
+
 def test_pick_repeats_bit_for_bit():
     c = case(40, 30000, 3000, 50, 4, seed=12)
     first = pick(c, out=True)
@@ -385,10 +395,12 @@ def test_next_tokens_follow_the_logits():
     before = [s.length for s in seqs]
     for kw in (dict(rules=rules), dict(rules=rules, slots=[0, 1]), dict(rules=rules, slots=[1, 1, 0]),
                dict(rules=rules, slots=[0, 1, 4]), dict(masks=masks), dict(masks=masks, mask_ids=[0, 0, 1]),
-               dict(masks=masks[:, :3], mask_ids=[0, 0, 0]),
+               dict(masks=masks[:, :3], mask_ids=[0, 0, 0]), dict(masks=masks.cpu(), mask_ids=[0, 0, 0]),
                dict(rules=S.TokenRules(4, 100, 3), slots=[0, 1, 2])):
         with pytest.raises(ValueError):
             a.next_tokens(new, seqs, **kw)
+    with pytest.raises(TypeError):
+        a.next_tokens(new, seqs, masks=masks.long(), mask_ids=[0, 0, 0])
     assert [s.length for s in seqs] == before
 
 

@@ -206,3 +206,34 @@ def test_fork_and_compaction_take_the_scales_with_them(monkeypatch):
     c.compact()
     assert (c.page_scale[:, b.pages[0]] == 0).all() and (c.page_scale[:, b.pages[1]] == 1).all()
     assert b.pages == [0, 1]
+
+
+def test_next_tokens_that_fail_leave_the_sequences(monkeypatch):
+    from types import SimpleNamespace
+    c = S.PagedKVCache(CFG, 12, device="cpu", page_scales=True)
+    w = SimpleNamespace(cfg=CFG, embed=SimpleNamespace(block=True, w=torch.zeros(1)), layers=[None] * CFG.n_layers)
+    monkeypatch.setattr(S, "rope_table_f32", lambda n, theta, device: torch.zeros(n, 64, 2))
+    d = S.Qwen3BatchDecoder(w, c, n_pos=300)
+    a, b = c.new(), c.new()
+    c.extend(a, 60)
+
+    def run(tokens, seqs, adapters):
+        d._layout(tokens, seqs, adapters)
+        return torch.zeros(len(seqs), CFG.vocab)
+    monkeypatch.setattr(d, "_run", run)
+
+    def fails(*args, **kw):
+        raise S.HephError(L.HEPH_ERR_LAUNCH, "heph_pick_tokens")
+    monkeypatch.setattr(S, "pick_tokens", fails)
+    with pytest.raises(S.HephError):
+        d.next_tokens([[1] * 70, [2]], [a, b])
+    assert (a.length, len(a.pages), b.length, b.pages) == (60, 1, 0, []) and c.free_pages == 11
+    rules = S.TokenRules(2, CFG.vocab, 5, device="cpu")
+    words = torch.zeros(1, CFG.vocab // 32, dtype=torch.int32)
+    for kw in (dict(rules=rules), dict(slots=[0, 1]), dict(rules=rules, slots=[0]), dict(rules=rules, slots=[1, 1]),
+               dict(rules=rules, slots=[0, 2]), dict(masks=words), dict(masks=words, mask_ids=[0]),
+               dict(masks=words, mask_ids=[0, 1]), dict(masks=words[:, 1:], mask_ids=[0, 0]),
+               dict(rules=S.TokenRules(2, 7, 5, device="cpu"), slots=[0, 1])):
+        with pytest.raises(ValueError):
+            d.next_tokens([[1], [2]], [a, b], **kw)
+    assert (a.length, b.length, c.free_pages) == (60, 0, 11)
