@@ -92,14 +92,15 @@ def _matrix(t, name: str, dtypes, m: int, n: int, dev: int) -> int:
 
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_raw_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def _at(ctx) -> tuple[int, int]:
     """The current device and the stream of a call: ctx, or its current one."""
-    dev = torch.cuda.current_device()
     if ctx is None and _raw_stream is not None:
+        dev = _raw_device()
         return dev, _raw_stream(dev)
-    return dev, HK._stream(ctx)
+    return torch.cuda.current_device(), HK._stream(ctx)
 
 
 def _call(name: str, *args) -> None:
