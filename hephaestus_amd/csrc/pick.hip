@@ -36,7 +36,7 @@ struct PickArgs {
     const int32_t* mask_ids;
     int64_t out_stride, logits_stride;
     heph_token_rules rules;
-    int rows, vocab, tiles, n_masks, append;
+    int rows, vocab, tiles, n_masks, append, by_xcd;
 };
 
 typedef int i32x4_a4 __attribute__((ext_vector_type(4), aligned(4)));
@@ -168,7 +168,11 @@ __global__ __launch_bounds__(kThreads) void pick_kernel(PickArgs a)
     constexpr int kTile = tile_of(V);
     __shared__ __attribute__((aligned(16))) uint32_t words[kTile + 64];
     __shared__ Part waves[kThreads / 64];
-    const int tid = threadIdx.x, row = blockIdx.x / a.tiles, base = blockIdx.x % a.tiles * kTile;
+    // (workgroups go round the eight XCDs)
+    const int tid = threadIdx.x, block = a.by_xcd ? blockIdx.x / 8 : blockIdx.x;
+    const int row = a.by_xcd ? block / a.tiles * 8 + (int)(blockIdx.x % 8) : block / a.tiles;
+    const int tile = block % a.tiles, base = tile * kTile;
+    if (row >= a.rows) return;
     const int n = min(kTile, a.vocab - base);
     // The start is a chain of loads: slot and mask, then what they have, the first tokens of the
     // history (whatever its length) among it; the logits are on their way beside it.
@@ -287,7 +291,7 @@ __global__ __launch_bounds__(kThreads) void pick_kernel(PickArgs a)
     p = join_lanes(tid < kThreads / 64 ? waves[tid] : Part{-INFINITY, 0.0f, -1, 0});
     if (tid != 0) return;
     if (a.tiles == 1) finish(a, row, p);
-    else a.parts[blockIdx.x] = p;
+    else a.parts[(size_t)row * a.tiles + tile] = p;
 }
 
 // One wave a row joins its tiles' parts.
@@ -327,10 +331,14 @@ int64_t most_parts(int rows, int vocab)
     return std::max<int64_t>((int64_t)rows * tiles_of(vocab, kMostVecs), 2 * kEnough);
 }
 
+// With so many rows a row's tiles lie on one XCD, whose L2 then holds its history for all of them.
+constexpr int kRowsByXcd = 64;
+int64_t blocks_of(int rows, int tiles) { return (int64_t)(rows >= kRowsByXcd ? (rows + 7) / 8 * 8 : rows) * tiles; }
+
 template <class T>
 void launch(const PickArgs& a, int V, hipStream_t s)
 {
-    const unsigned blocks = (unsigned)(a.rows * (int64_t)a.tiles);
+    const unsigned blocks = (unsigned)blocks_of(a.rows, a.tiles);
     if (V == 4) pick_kernel<T, 4><<<blocks, kThreads, 0, s>>>(a);
     else if (V == 2) pick_kernel<T, 2><<<blocks, kThreads, 0, s>>>(a);
     else pick_kernel<T, 1><<<blocks, kThreads, 0, s>>>(a);
@@ -373,7 +381,7 @@ int heph_pick_tokens(int32_t* tokens, float* logprob, void* out, int64_t out_str
     if (!aligned(logits, element) || !aligned(out, element) || !aligned(ws, 16)) return HEPH_ERR_ALIGN;
     if (ws_bytes < heph_pick_ws_bytes(rows, vocab)) return HEPH_ERR_WORKSPACE;
     const int V = vecs_of(rows, vocab);
-    if (rows * (int64_t)tiles_of(vocab, V) > UINT32_MAX / kThreads) return HEPH_ERR_UNSUPPORTED;     // (a launch's most threads)
+    if (blocks_of(rows, tiles_of(vocab, V)) > UINT32_MAX / kThreads) return HEPH_ERR_UNSUPPORTED;     // (a launch's most threads)
     if (int st = check_device()) return st;
     PickArgs a{};
     a.tokens = tokens;
@@ -392,6 +400,7 @@ int heph_pick_tokens(int32_t* tokens, float* logprob, void* out, int64_t out_str
     a.tiles = tiles_of(vocab, V);
     a.n_masks = n_masks;
     a.append = append;
+    a.by_xcd = rows >= kRowsByXcd;
     hipStream_t s = static_cast<hipStream_t>(stream);
     if (dtype == HEPH_DTYPE_F32) launch<float>(a, V, s);
     else launch<uint16_t>(a, V, s);
