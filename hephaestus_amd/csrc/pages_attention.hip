@@ -22,6 +22,11 @@
 // units out from the lengths in device memory; units of the same row meet in
 // the workspace and merge_kernel joins them.
 //
+// The cache has one scale for a layer's kv head, or one for each page of it (BLOCK), a power of
+// two by which the conversion of codes to bf16 multiplies in passing: nothing is rescaled page by
+// page, and the times are the same within 2 % (96 sequences of 2048 shared and up to 1500 own keys,
+// three layers 147 and 145 us).
+//
 // Measured (8 kv heads, 32 heads, graph replays): 64 sequences x 4096 keys of their
 // own 102 us, 5.3 TB/s of K and V; 16 prompts of 128 tokens behind 20000 keys 706 us,
 // 948 TFLOP/s (a library product of 8192^3 in bf16 reaches 1240); one sequence of
@@ -1094,7 +1099,7 @@ __device__ __forceinline__ void merge_row(const AttnArgs& a, const Token& tk, lo
         }
     };
     // (as many as there are, up to 16: 32 take registers that many rows' waves need, 15.3 us for 12.5 where
-    // six prompts of 700 tokens are joined)
+    // six prompts of 700 tokens are joined, and gain nothing where one row of 64 parts is)
     if (n <= 4) join(std::integral_constant<int, 4>{});
     else if (n <= 8) join(std::integral_constant<int, 8>{});
     else join(std::integral_constant<int, 16>{});

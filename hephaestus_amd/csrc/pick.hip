@@ -6,6 +6,14 @@
 // with integer atomics (the same in any order), and the biases. The logits are in registers
 // meanwhile; each is read once, and log-sum-exp's pieces (maximum, sum) of a row's tiles join
 // exactly in a second, small launch.
+//
+// Measured (vocabulary of 151936 in f32, replayed): bound by memory without rules (256 rows 29.5 us,
+// 5.3 TB/s; 64 rows 11.5, with the logits after the rules written 20.9, 3.7 TB/s), by a chain of
+// launches and loads for few (three rows 4.8 us, with rules 6.5). Rules add the chain slot, history,
+// words: 64 rows with histories of 600 tokens 16.3 us, 256 rows 39.6; histories of 20000, of which
+// every tile takes its own tokens, 61, the atomics in LDS. Longer tiles (16384 logits: a row's
+// history is read half as often) leave fewer workgroups to hide that chain: 256 rows of 600 tokens
+// 48 us, of 20000 75; a workgroup of 1024 threads that loads the next tile ahead 69 and 102.
 #include <algorithm>
 
 #include "pages.h"
@@ -116,7 +124,7 @@ struct Tokens {
     }
     // Counted in the words of the tile of n tokens from base on, those from number n_prompt of the
     // history on as answered. A token of another tile goes to a word of its lane's behind the
-    // tile's, which costs less than to leave it out.
+    // tile's, which costs less than to leave it out (256 rows of 20000 tokens 64 us instead of 74).
     __device__ __forceinline__ void count(uint32_t* words, int spare, int first, int end, int n_prompt, int base,
                                           int n) const
     {
@@ -316,6 +324,8 @@ bool sizes_ok(int rows, int vocab) { return rows >= 1 && rows <= (1 << 20) && vo
 int tiles_of(int vocab, int V) { return (vocab + tile_of(V) - 1) / tile_of(V); }
 
 // The longest tile that still gives every CU two workgroups: each of a row's reads its whole history.
+// Tiles of 2048, 4096 and 8192, histories of 600 tokens, us: 3 rows 6.4, 6.7, 7.5; 16 rows 10.5, 8.9,
+// 9.3; 64 rows 23.2, 17.8, 16.1.
 constexpr int kMostVecs = 4, kEnough = 512;
 int vecs_of(int rows, int vocab)
 {
@@ -331,7 +341,8 @@ int64_t most_parts(int rows, int vocab)
     return std::max<int64_t>((int64_t)rows * tiles_of(vocab, kMostVecs), 2 * kEnough);
 }
 
-// With so many rows a row's tiles lie on one XCD, whose L2 then holds its history for all of them.
+// With so many rows a row's tiles lie on one XCD, whose L2 then holds its history for all of them
+// (histories of 20000 tokens: 64 rows 24.8 -> 23.0 us, 256 rows 64.3 -> 60.9; of 600: the same).
 constexpr int kRowsByXcd = 64;
 int64_t blocks_of(int rows, int tiles) { return (int64_t)(rows >= kRowsByXcd ? (rows + 7) / 8 * 8 : rows) * tiles; }
 
