@@ -24,8 +24,8 @@
 //
 // The cache has one scale for a layer's kv head, or one for each page of it (BLOCK), a power of
 // two by which the conversion of codes to bf16 multiplies in passing: nothing is rescaled page by
-// page, and the times are the same within 2 % (96 sequences of 2048 shared and up to 1500 own keys,
-// three layers 147 and 145 us).
+// page, and the times are the same within 1 % (96 sequences of 2048 shared and up to 1500 own keys,
+// three layers 146 and 145 us).
 //
 // Measured (8 kv heads, 32 heads, graph replays): 64 sequences x 4096 keys of their
 // own 102 us, 5.3 TB/s of K and V; 16 prompts of 128 tokens behind 20000 keys 706 us,
@@ -862,18 +862,15 @@ __device__ __forceinline__ void attend_narrow(const AttnArgs& a, const Unit& u, 
     };
     struct Page {
         i32x4 k[8], v[8];
-        int id;
-        float sk, sv;
+        int id, lane;
     } p0, p1;
     int ids = 0, first = 0, last = 0;
     float sk = 1.0f, sv = 1.0f;            // of the pages of ids, one a lane
     // (past the run its last page again: a load that is left out on some path would make
     // the waits for the page before count without it, and hold up the one behind)
     auto load = [&](Page& p, int n) {
-        const int i = min(n, last - 1) - first;
-        p.id = __builtin_amdgcn_readlane(ids, i);
-        p.sk = BLOCK ? lane_of(sk, i) : 1.0f;
-        p.sv = BLOCK ? lane_of(sv, i) : 1.0f;
+        p.lane = min(n, last - 1) - first;
+        p.id = __builtin_amdgcn_readlane(ids, p.lane);
         const size_t o = place(p.id);
 #pragma unroll
         for (int i = 0; i < 8; ++i) p.k[i] = ldg16(a.k_pages + o + i * 1024);
@@ -882,6 +879,7 @@ __device__ __forceinline__ void attend_narrow(const AttnArgs& a, const Unit& u, 
     };
     auto work = [&](Page& p, int n) {
         if (p.id < 0 || p.id >= a.n_pages) return;
+        const float k_scale = BLOCK ? lane_of(sk, p.lane) : 1.0f, v_scale = BLOCK ? lane_of(sv, p.lane) : 1.0f;
         auto half = [](const i32x4& w, int h, float s) { return bf16_of_codes(w[2 * h], w[2 * h + 1], s); };
         auto clear = [&] {
             bool any = false;
@@ -889,18 +887,18 @@ __device__ __forceinline__ void attend_narrow(const AttnArgs& a, const Unit& u, 
             for (int i = 0; i < 8; ++i) any |= clear_nan(p.v[i]);
             return __any(any);
         };
-        x.template page<false>(n, sc, [&](int i, int h) { return half(p.k[i], h, p.sk); },
-                      [&](int i, int h) { return half(p.v[i], h, p.sv); }, clear,
+        x.template page<false>(n, sc, [&](int i, int h) { return half(p.k[i], h, k_scale); },
+                      [&](int i, int h) { return half(p.v[i], h, v_scale); }, clear,
                       a.v_pages + place(p.id));
     };
     for (first = u.page0; first < end; first += 64) {
         last = min(first + 64, end);
         ids = first == u.page0 ? ids0 : page_ids(a, u, first);
+        wait_vm<0>();           // (nothing but pages, and their scales before them, on its way below)
         if constexpr (BLOCK) {
             sk = page_scale(a, ids, head);
             sv = page_scale(a, ids, n_kv + head);
         }
-        wait_vm<0>();           // (nothing but pages on its way below)
         int n = first + kw;
         load(p0, n);
         while (n < last) {
@@ -981,8 +979,8 @@ __device__ __forceinline__ void attend_wide(const AttnArgs& a, const Unit& u, in
     const uint8_t* pool = (wave < 2 ? a.k_pages : a.v_pages) + (wave & 1) * 4096 + c * 64 + g4 * 16;
     for (int first = u.page0; first < end; first += 64) {
         const int last = min(first + 64, end), ids = first == u.page0 ? ids0 : page_ids(a, u, first);
+        wait_vm<0>();           // (nothing but pages, and their scales before them, on its way below)
         const float scales = BLOCK ? page_scale(a, ids, (wave < 2 ? 0 : n_kv) + head) : 1.0f;
-        wait_vm<0>();           // (nothing but pages on its way below)
         auto id_of = [&](int n) { return __builtin_amdgcn_readlane(ids, n - first); };
         struct Codes {
             i32x4 w[4];
