@@ -278,8 +278,8 @@ __device__ int scan_block(int& g, int& s, int2* red)
     return all_g + all_s;
 }
 
-// One thread a sequence and a group. Every workgroup repeats that and writes a share
-// of the tokens; the first one also writes the units and the header.
+// One thread a sequence and a group. Every workgroup repeats that; the first half of them write the
+// units (the first one also the header), the others the tokens: both at once are a longer chain.
 constexpr int kPlanTokens = 64;
 __global__ __launch_bounds__(kMaxSeqs) void plan_kernel(PlanArgs a)
 {
@@ -408,7 +408,8 @@ __global__ __launch_bounds__(kMaxSeqs) void plan_kernel(PlanArgs a)
         *a.plan = PlanHeader{kMagic, a.s.n_tok, a.s.n_seqs, a.s.n_groups, a.table_pages, a.s.n_heads,
                              a.s.n_kv, n_units, merges, {}};
     // Units: a source's tiles from its last on, each one's runs in order.
-    for (int u = blockIdx.x * nt + t; u < n_units; u += gridDim.x * nt) {
+    const int half = gridDim.x / 2;
+    for (int u = blockIdx.x * nt + t; (int)blockIdx.x < half && u < n_units; u += half * nt) {
         auto source = [&](int i) -> const Source& {
             return i < a.s.n_groups ? groups[i] : seqs[i - a.s.n_groups].x;
         };
@@ -431,7 +432,9 @@ __global__ __launch_bounds__(kMaxSeqs) void plan_kernel(PlanArgs a)
         }
         units[u] = unit;
     }
-    for (int i = blockIdx.x * kPlanTokens + t; i < min(a.s.n_tok, ((int)blockIdx.x + 1) * kPlanTokens); i += nt) {
+    if ((int)blockIdx.x < half) return;
+    const int tokens0 = ((int)blockIdx.x - half) * kPlanTokens;
+    for (int i = tokens0 + t; i < min(a.s.n_tok, tokens0 + kPlanTokens); i += nt) {
         int lo = 0, hi = a.s.n_seqs;              // the last sequence that starts at i or before
         while (lo < hi) {
             const int mid = (lo + hi) / 2;
@@ -1225,7 +1228,7 @@ int heph_pages_attention_plan(void* plan, size_t plan_bytes, const int32_t* q_st
     const PlanArgs a{static_cast<PlanHeader*>(plan), q_start, kv_len, group_start, shared_pages,
                      Sizes{n_tok, n_seqs, n_groups, n_heads, n_kv_heads}, table_pages};
     const int threads = (n_seqs + 63) / 64 * 64;
-    plan_kernel<<<(n_tok + kPlanTokens - 1) / kPlanTokens, threads, 0, static_cast<hipStream_t>(stream)>>>(a);
+    plan_kernel<<<2 * ((n_tok + kPlanTokens - 1) / kPlanTokens), threads, 0, static_cast<hipStream_t>(stream)>>>(a);
     return status_of(hipGetLastError());
 }
 
