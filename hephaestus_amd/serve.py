@@ -43,9 +43,12 @@ _I32, _BF16, _F32 = (torch.int32,), (torch.bfloat16,), (torch.float32,)
 # The checks run before every call of a decode step: one look at each property, and the
 # words of a refusal only where there is one.
 
+_Tensor = torch.Tensor
+
+
 def _dev(t, name: str, dtypes, numel: int, dev: int) -> int:
     """Pointer of a contiguous tensor on device dev with at least numel elements."""
-    if isinstance(t, torch.Tensor) and t.dtype in dtypes and t.get_device() == dev and \
+    if isinstance(t, _Tensor) and t.dtype in dtypes and t.get_device() == dev and \
             t.is_contiguous() and t.numel() >= numel:
         return t.data_ptr()
     HK._dev(t, name, dtypes)
@@ -103,9 +106,15 @@ def _at(ctx) -> tuple[int, int]:
     return torch.cuda.current_device(), HK._stream(ctx)
 
 
+_functions: dict = {}          # of the library, by name
+
+
 def _call(name: str, *args) -> None:
-    status = getattr(L.lib(), name)(*args)
-    if status != L.HEPH_OK:
+    f = _functions.get(name)
+    if f is None:
+        f = _functions[name] = getattr(L.lib(), name)
+    status = f(*args)
+    if status != 0:
         raise HephError(status, name)
 
 
@@ -125,9 +134,12 @@ def rope_table_f32(n_pos: int, theta: float = 1e6, device="cuda", ctx=None) -> t
     return t
 
 
+_K_PAGE, _V_PAGE = (2, PAGE, 64), (128, PAGE)
+
+
 def _pools(k_pages, v_pages, lead: tuple, dev: int) -> tuple[int, int]:
     """Pointers of the K and V pools [*lead, ...], lead ending with n_pages and n_kv."""
-    if k_pages.shape != lead + (2, PAGE, 64) or v_pages.shape != lead + (128, PAGE):
+    if k_pages.shape != lead + _K_PAGE or v_pages.shape != lead + _V_PAGE:
         raise ValueError(f"pools of shapes {tuple(k_pages.shape)} and {tuple(v_pages.shape)} are "
                          f"not {list(lead)} pages and heads of [2, 64, 64] and [128, 64]")
     return _dev(k_pages, "k_pages", _U8, 0, dev), _dev(v_pages, "v_pages", _U8, 0, dev)
@@ -135,8 +147,8 @@ def _pools(k_pages, v_pages, lead: tuple, dev: int) -> tuple[int, int]:
 
 def _page_scale(t, lead: tuple, n_kv: int, dev: int) -> int:
     """Pointer of the pages' scales [*lead, 2 n_kv], lead ending with n_pages."""
-    if t.shape != lead + (2 * n_kv,):
-        raise ValueError(f"page_scale of shape {tuple(t.shape)} is not {list(lead + (2 * n_kv,))}")
+    if not isinstance(t, _Tensor) or t.shape != (*lead, 2 * n_kv):
+        raise ValueError(f"page_scale of shape {tuple(getattr(t, 'shape', ()))} is not {[*lead, 2 * n_kv]}")
     return _dev(t, "page_scale", _F32, 0, dev)
 
 
@@ -260,16 +272,22 @@ class AttentionPlan:
               stream)
 
 
-def _attention(name: str, out, q, k_pages, v_pages, scale, page_table, p, dev, stream) -> None:
-    n_pages = k_pages.shape[0]
-    kp, vp = _pools(k_pages, v_pages, (n_pages, p.n_kv), dev)
-    if page_table.shape != (p.n_seqs, p.table_pages):
+def _attention(name: str, out, q, k_pages, v_pages, kv_scale, page_scale, page_table, p, ctx) -> None:
+    dev, stream = _at(ctx)
+    n_kv = p.n_kv
+    n_pages, n_tok, n_heads, table_pages = k_pages.shape[0], p.n_tok, p.n_heads, p.table_pages
+    kp, vp = _pools(k_pages, v_pages, (n_pages, n_kv), dev)
+    if page_table.shape != (p.n_seqs, table_pages):
         raise ValueError(f"page_table of shape {tuple(page_table.shape)} is not "
                          f"[{p.n_seqs}, {p.table_pages}] as planned")
-    qp, qs = _rows(q, "q", p.n_tok, p.n_heads * 128, dev)
-    _call(name, _dev(out, "out", _BF16, p.n_tok * p.n_heads * 128, dev), qp, qs, kp, vp, n_pages,
-          scale(n_pages), _dev(page_table, "page_table", _I32, 0, dev), p.table_pages,
-          *_bound(p, dev), p.n_tok, p.n_seqs, p.n_groups, p.n_heads, p.n_kv, 128, stream)
+    qp, qs = _rows(q, "q", n_tok, n_heads * 128, dev)
+    if kv_scale is not None:
+        scale = _dev(kv_scale, "kv_scale", _F32, 2 * n_kv, dev)
+    else:
+        scale = _page_scale(page_scale, (n_pages,), n_kv, dev)
+    _call(name, _dev(out, "out", _BF16, n_tok * n_heads * 128, dev), qp, qs, kp, vp, n_pages, scale,
+          _dev(page_table, "page_table", _I32, 0, dev), table_pages, *_bound(p, dev), n_tok, p.n_seqs,
+          p.n_groups, n_heads, n_kv, 128, stream)
 
 
 def attention_pages(out, q, k_pages, v_pages, kv_scale, page_table, plan: AttentionPlan,
@@ -278,17 +296,15 @@ def attention_pages(out, q, k_pages, v_pages, kv_scale, page_table, plan: Attent
     laid out by plan (updated with this step's lengths). q [n_tok, n_heads,
     128] (rows may lie apart), out contiguous; page_table int32 [n_seqs,
     table_pages]."""
-    dev, stream = _at(ctx)
-    _attention("heph_pages_attention", out, q, k_pages, v_pages,
-               lambda n: _dev(kv_scale, "kv_scale", _F32, 2 * plan.n_kv, dev), page_table, plan, dev, stream)
+    if kv_scale is None:
+        raise TypeError("kv_scale must be a torch tensor")
+    _attention("heph_pages_attention", out, q, k_pages, v_pages, kv_scale, None, page_table, plan, ctx)
 
 
 def attention_pages_scaled(out, q, k_pages, v_pages, page_scale, page_table, plan: AttentionPlan,
                            ctx=None) -> None:
     """attention_pages over pages with scales of their own, page_scale [n_pages, 2 n_kv]."""
-    dev, stream = _at(ctx)
-    _attention("heph_pages_attention_scaled", out, q, k_pages, v_pages,
-               lambda n: _page_scale(page_scale, (n,), plan.n_kv, dev), page_table, plan, dev, stream)
+    _attention("heph_pages_attention_scaled", out, q, k_pages, v_pages, None, page_scale, page_table, plan, ctx)
 
 
 def copy_pages(k_pools, v_pools, src, dst, ctx=None, page_scale=None) -> None:
