@@ -11,6 +11,8 @@
 // copy of 1 GiB reaches 5.2), with one scale for all pages 18.7; 128 tokens of as many sequences 6.1
 // (4.8), three 4.1 (2.9): there a chain of three loads, the scale's rounds among the lanes and V's
 // single bytes count. 65001 rows read back (399 MB) in 86 us, 4.6 TB/s.
+#include <algorithm>
+
 #include "pages_norm.h"
 
 namespace heph {
@@ -496,7 +498,8 @@ int heph_qk_norm_rope_pages_scaled(void* q_out_bf16, int64_t q_stride, const voi
     const int64_t page_blocks = ((int64_t)n_tok + W - 1) / W * 2 * n_kv_heads;
     const int64_t q_blocks = ((int64_t)n_tok * ((n_heads + heads_a_wave - 1) / heads_a_wave) + waves - 1) / waves;
     // one q block and then q_every - 1 of pages, in turn
-    const int64_t q_every = 1 + (page_blocks + q_blocks - 1) / q_blocks, blocks = q_blocks * q_every;
+    const int64_t pages_a_turn = std::max<int64_t>((page_blocks + q_blocks / 2) / q_blocks, 1), q_every = 1 + pages_a_turn;
+    const int64_t turns = std::max(q_blocks, (page_blocks + pages_a_turn - 1) / pages_a_turn), blocks = turns * q_every;
     if (blocks > UINT32_MAX / 512) return HEPH_ERR_UNSUPPORTED;          // (a launch's most threads)
     if (int st = check_device()) return st;
     WriteArgs a;

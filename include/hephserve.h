@@ -160,7 +160,8 @@ int heph_copy_pages(uint8_t* k_pages, uint8_t* v_pages, int n_layers, int n_page
  * range, which are rounded to its subnormal ones); new codes are
  * e4m3(x * 2^-e), and a NaN or an infinity, which E4M3 has not, is the code of
  * NaN. A scale outside the range (memory that was never written) counts as the
- * nearest one in it.
+ * nearest one in it; a page that begins behind its key 0 has its scales set to
+ * 0 first.
  * The tokens of a page are neighbours among the call's rows, as a sequence's
  * newest tokens are, and a page belongs to one sequence while it is written; a
  * page whose tokens lie apart gets codes of more than one scale.

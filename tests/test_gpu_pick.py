@@ -262,6 +262,13 @@ def test_pick_appends_to_the_histories():
     assert np.array_equal(r.history.cpu().numpy(), want) and np.array_equal(r.length.cpu().numpy(), length)
 
 
+def test_pick_rows_that_share_a_request():
+    # several rows of one slot (samples of one request) and one mask; nothing is appended
+    c = case(6, 9001, 300, 5, 2, seed=17)
+    c["slots"], c["mask_ids"] = i32([2, 2, 2, 0, 2, 0]), i32([1, 1, 1, 1, 0, 1])
+    check(c)
+
+
 def test_pick_scratch_of_a_larger_batch_serves_smaller_ones():
     ws = S.pick_ws(40, 151936)
     for rows, vocab in ((40, 151936), (27, 151936), (26, 151936), (13, 151936), (1, 151936), (14, 50000), (3, 9)):

@@ -152,6 +152,19 @@ def test_write_over_scales_that_were_never_written(value):
     check_write(c)
 
 
+def test_write_a_page_that_begins_behind_its_key_0():
+    # its scale set to 0 first: the new values' own, as where key 0 is among them
+    for T in (3, 40):
+        c, d = write_case([(10, T)], seed=18), write_case([(0, T)], seed=18)
+        for x in (c, d):
+            x["qkv"][:, x["H"] + x["KV"]:] *= 2.0 ** -20
+        c["scale"].zero_()
+        check_write(c)
+        write(d)
+        page = [int(x["slot"][0]) // PAGE for x in (c, d)]
+        assert torch.equal(c["scale"][page[0], c["KV"]:], d["scale"][page[1], d["KV"]:])
+
+
 def test_write_slots_of_a_run_in_any_order():
     c = write_case([(0, 64), (70, 40)], seed=4)
     order = torch.cat([torch.randperm(64), 64 + torch.randperm(40).flip(0)]).cuda()
