@@ -56,13 +56,27 @@ __device__ __forceinline__ void norm_rope(float (&lo)[8], float (&hi)[8], const 
     }
 }
 
-// Such a lane's values to its head at out, as bf16.
+// A store that leaves no line in the caches: for what is more than these hold.
+__device__ __forceinline__ void store_past(uint16_t* p, const uint4& x)
+{
+    __builtin_nontemporal_store(i32x4{(int)x.x, (int)x.y, (int)x.z, (int)x.w}, reinterpret_cast<i32x4*>(p));
+}
+
+// Such a lane's values to its head at out, as bf16; PAST: past the caches.
+template <bool PAST = false>
 __device__ __forceinline__ void store_head(uint16_t* out, const float (&lo)[8], const float (&hi)[8])
 {
-    *reinterpret_cast<uint4*>(out) = make_uint4(pack2_bf16(lo[0], lo[1]), pack2_bf16(lo[2], lo[3]),
-                                                pack2_bf16(lo[4], lo[5]), pack2_bf16(lo[6], lo[7]));
-    *reinterpret_cast<uint4*>(out + 64) = make_uint4(pack2_bf16(hi[0], hi[1]), pack2_bf16(hi[2], hi[3]),
-                                                     pack2_bf16(hi[4], hi[5]), pack2_bf16(hi[6], hi[7]));
+    const uint4 a = make_uint4(pack2_bf16(lo[0], lo[1]), pack2_bf16(lo[2], lo[3]), pack2_bf16(lo[4], lo[5]),
+                               pack2_bf16(lo[6], lo[7]));
+    const uint4 b = make_uint4(pack2_bf16(hi[0], hi[1]), pack2_bf16(hi[2], hi[3]), pack2_bf16(hi[4], hi[5]),
+                               pack2_bf16(hi[6], hi[7]));
+    if constexpr (PAST) {
+        store_past(out, a);
+        store_past(out + 64, b);
+    } else {
+        *reinterpret_cast<uint4*>(out) = a;
+        *reinterpret_cast<uint4*>(out + 64) = b;
+    }
 }
 
 }  // namespace heph

@@ -96,7 +96,7 @@ struct WriteArgs {
 
 // A wave takes 8 * B query heads of one token: their loads are all on their way at once, which
 // keeps memory busy with the few waves that the blocks' registers leave (4090 tokens, 32 heads:
-// B = 1 24.6 us, 2 22.0, 4 23.0).
+// B = 1 24.6 us, 2 22.0, 4 23.0). A long batch's q (B > 1) goes past the caches: 24.0 us, 19.4.
 template <int B>
 __device__ __forceinline__ void q_heads(const WriteArgs& a, long unit)
 {
@@ -122,7 +122,7 @@ __device__ __forceinline__ void q_heads(const WriteArgs& a, long unit)
         if (h >= a.n_heads) return;                // (whole heads: eight lanes at a time)
         float lo[8], hi[8];
         norm_rope(lo, hi, x_lo[i], x_hi[i], y_lo, y_hi, w, a.eps);
-        store_head(a.q_out + t * a.q_stride + (size_t)h * kHeadDim + 8 * c, lo, hi);
+        store_head<(B > 1)>(a.q_out + t * a.q_stride + (size_t)h * kHeadDim + 8 * c, lo, hi);
     }
 }
 
@@ -412,7 +412,8 @@ __device__ __forceinline__ uint4 bf16_of8(uint2 w, float s)
 }
 
 // A workgroup takes the runs of consecutive slots of a page that start among its W rows, one kv
-// head: V's codes meet in LDS and leave key by key. Bound by the rows' 16-bit stores.
+// head: V's codes meet in LDS and leave key by key. Bound by the rows' 16-bit stores, which go past
+// the caches (65001 rows 79 us instead of 87).
 template <int W>
 __global__ __launch_bounds__(256) void read_kernel(ReadArgs a)
 {
@@ -439,6 +440,14 @@ __global__ __launch_bounds__(256) void read_kernel(ReadArgs a)
         const uint8_t* kp = a.k_pages + at * kPageBytes;
         const uint8_t* vp = a.v_pages + at * kPageBytes;
         const size_t out = ((size_t)(t0 + s) * a.n_kv + h) * kHeadDim;
+        // (all of the block's loads at once; past the run its last piece again, not used)
+        uint2 k_codes[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int i = min(tid + u * 256, n * 16 - 1);
+            k_codes[u] = *reinterpret_cast<const uint2*>(kp + k_byte(key0 + i / 16, i % 16 * 8));
+        }
+#pragma unroll
         for (int i = tid; i < 16 * 32; i += 256) {
             const int j = i % 16 * 4, g = i / 16;
             if (j + 3 < key0 || j >= key0 + n) continue;
@@ -449,13 +458,14 @@ __global__ __launch_bounds__(256) void read_kernel(ReadArgs a)
             for (int e = 0; e < 4; ++e) lds[(j + e) * (kPitch / 4) + g] = column(k, e);
         }
         __syncthreads();
-        for (int i = tid; i < n * 16; i += 256) {
-            const int r = i / 16, d = i % 16 * 8;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int i = tid + u * 256, r = i / 16, d = i % 16 * 8;
+            if (r >= n) break;
             const size_t o = out + (size_t)r * a.n_kv * kHeadDim + d;
-            *reinterpret_cast<uint4*>(a.k_out + o) =
-                bf16_of8(*reinterpret_cast<const uint2*>(kp + k_byte(key0 + r, d)), sk);
+            store_past(a.k_out + o, bf16_of8(k_codes[u], sk));
             const uint32_t* v = lds + (key0 + r) * (kPitch / 4) + d / 4;
-            *reinterpret_cast<uint4*>(a.v_out + o) = bf16_of8(make_uint2(v[0], v[1]), sv);
+            store_past(a.v_out + o, bf16_of8(make_uint2(v[0], v[1]), sv));
         }
         __syncthreads();
     }

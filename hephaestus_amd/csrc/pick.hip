@@ -59,10 +59,15 @@ __device__ __forceinline__ f32x4 load4(const uint16_t* p)
 }
 __device__ __forceinline__ float load1(const float* p) { return *p; }
 __device__ __forceinline__ float load1(const uint16_t* p) { return bf16_bits_f32(*p); }
-__device__ __forceinline__ void store4(float* p, const f32x4& x) { *reinterpret_cast<f32x4_row*>(p) = x; }
+// (past the caches: 64 rows of logits are more than these hold; with ordinary stores 20.9 us, so 17.1)
+__device__ __forceinline__ void store4(float* p, const f32x4& x)
+{
+    __builtin_nontemporal_store(x, reinterpret_cast<f32x4_row*>(p));
+}
 __device__ __forceinline__ void store4(uint16_t* p, const f32x4& x)
 {
-    *reinterpret_cast<u16x4_row*>(p) = u16x4_row{f32_to_bf16(x[0]), f32_to_bf16(x[1]), f32_to_bf16(x[2]), f32_to_bf16(x[3])};
+    const u16x4_row w = {f32_to_bf16(x[0]), f32_to_bf16(x[1]), f32_to_bf16(x[2]), f32_to_bf16(x[3])};
+    __builtin_nontemporal_store(w, reinterpret_cast<u16x4_row*>(p));
 }
 __device__ __forceinline__ void store1(float* p, float x) { *p = x; }
 __device__ __forceinline__ void store1(uint16_t* p, float x) { *p = f32_to_bf16(x); }
