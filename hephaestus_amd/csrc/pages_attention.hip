@@ -25,12 +25,12 @@
 // The cache has one scale for a layer's kv head, or one for each page of it (BLOCK), a power of
 // two by which the conversion of codes to bf16 multiplies in passing: nothing is rescaled page by
 // page, and the times are the same within 1 % (96 sequences of 2048 shared and up to 1500 own keys,
-// three layers 146 and 145 us).
+// three layers 131 and 130 us).
 //
 // Measured (8 kv heads, 32 heads, graph replays): 64 sequences x 4096 keys of their
-// own 102 us, 5.3 TB/s of K and V; 16 prompts of 128 tokens behind 20000 keys 706 us,
+// own 86 us, 6.3 TB/s of K and V; 16 prompts of 128 tokens behind 20000 keys 706 us,
 // 948 TFLOP/s (a library product of 8192^3 in bf16 reaches 1240); one sequence of
-// 32768 keys 24.3 us.
+// 32768 keys 24.1 us.
 #include <algorithm>
 #include <type_traits>
 
@@ -846,14 +846,17 @@ __device__ __forceinline__ int page_ids(const AttnArgs& a, const Unit& u, int p)
 // Up to 64 rows: a wave takes 16 of them and, where that leaves waves, every
 // KW-th page of the run. Bound by the stream of K and V: the next page's 16 KB
 // a wave are on their way into registers while one is worked on. (64 sequences, each
-// 1024 keys 27 us, 4.9 TB/s; 64 keys 8.3 us, where a chain of four loads counts: unit,
-// limits and page ids, q, pages.)
-template <bool BLOCK>
+// 1024 keys 24.2 us, 5.5 TB/s; 64 keys 6.9 us, where a chain of four loads counts: unit,
+// limits and page ids, q, pages.) ONCE, up to 16 rows: one wave alone reads a page, and
+// the page goes past the caches (96 sequences, three layers 131 us instead of 145; one
+// sequence of 131000 keys, two layers 108 instead of 121). With more rows the other waves
+// find it there (64 sequences of 16 tokens 68 us, past the caches 84).
+template <bool BLOCK, bool ONCE>
 __device__ __forceinline__ void attend_narrow(const AttnArgs& a, const Unit& u, int head, int ids0, uint8_t* lds)
 {
     const int l = threadIdx.x & 63, c = l & 15, g4 = l >> 4, n_kv = a.s.n_kv;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int KW = u.rows <= 16 ? 4 : u.rows <= 32 ? 2 : 1, kw = wave % KW;
+    const int KW = ONCE ? 4 : u.rows <= 32 ? 2 : 1, kw = wave % KW;
     Rows<1> x;
     x.init(a, u, head, wave / KW * 16);
     const int end = min(u.page0 + u.pages, (x.hi + kPage - 1) / kPage);
@@ -867,6 +870,9 @@ __device__ __forceinline__ void attend_narrow(const AttnArgs& a, const Unit& u, 
         i32x4 k[8], v[8];
         int id, lane;
     } p0, p1;
+    auto codes = [](const uint8_t* p) {
+        return ONCE ? __builtin_nontemporal_load(reinterpret_cast<const i32x4*>(p)) : ldg16(p);
+    };
     int ids = 0, first = 0, last = 0;
     float sk = 1.0f, sv = 1.0f;            // of the pages of ids, one a lane
     // (past the run its last page again: a load that is left out on some path would make
@@ -876,9 +882,9 @@ __device__ __forceinline__ void attend_narrow(const AttnArgs& a, const Unit& u, 
         p.id = __builtin_amdgcn_readlane(ids, p.lane);
         const size_t o = place(p.id);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) p.k[i] = ldg16(a.k_pages + o + i * 1024);
+        for (int i = 0; i < 8; ++i) p.k[i] = codes(a.k_pages + o + i * 1024);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) p.v[i] = ldg16(a.v_pages + o + i * 1024);
+        for (int i = 0; i < 8; ++i) p.v[i] = codes(a.v_pages + o + i * 1024);
     };
     auto work = [&](Page& p, int n) {
         if (p.id < 0 || p.id >= a.n_pages) return;
@@ -1054,7 +1060,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     const Unit u = plan_units(a.plan, a.s.n_tok)[unit];        // (the plan has room for all of the grid's)
     if (!plan_fits(h, a) || unit >= h.n_units) return;
     const int ids = page_ids(a, u, u.page0);        // (on its way while the rows are looked at)
-    if (u.rows <= kNarrow) attend_narrow<BLOCK>(a, u, head, ids, lds);
+    if (u.rows <= 16) attend_narrow<BLOCK, true>(a, u, head, ids, lds);
+    else if (u.rows <= kNarrow) attend_narrow<BLOCK, false>(a, u, head, ids, lds);
     else attend_wide<BLOCK>(a, u, head, ids, lds);
 }
 
