@@ -7,10 +7,10 @@
 // 2^-6, off by at most half of the smallest one's step), and lets the attention's conversions
 // multiply by it in passing.
 //
-// Measured (32 + 8 heads, graph replays): 4090 tokens of prompts (94 MB with q) 22.0 us, 4.3 TB/s (a
-// copy of 1 GiB reaches 5.2), with one scale for all pages 18.7; 128 tokens of as many sequences 6.1
+// Measured (32 + 8 heads, graph replays): 4090 tokens of prompts (94 MB with q) 19.8 us, 4.7 TB/s (a
+// copy of 1 GiB reaches 5.2), with one scale for all pages 18.9; 128 tokens of as many sequences 6.1
 // (4.8), three 4.1 (2.9): there a chain of three loads, the scale's rounds among the lanes and V's
-// single bytes count. 65001 rows read back (399 MB) in 86 us, 4.6 TB/s.
+// single bytes count. 65001 rows read back (399 MB) in 79 us, 5.0 TB/s.
 #include <algorithm>
 
 #include "pages_norm.h"
@@ -96,7 +96,8 @@ struct WriteArgs {
 
 // A wave takes 8 * B query heads of one token: their loads are all on their way at once, which
 // keeps memory busy with the few waves that the blocks' registers leave (4090 tokens, 32 heads:
-// B = 1 24.6 us, 2 22.0, 4 23.0). A long batch's q (B > 1) goes past the caches: 24.0 us, 19.4.
+// B = 1 24.6 us, 2 22.0, 4 23.0, with ordinary stores). A long batch's q (B > 1) goes past the
+// caches: 19.4 us where ordinary stores took 24.0.
 template <int B>
 __device__ __forceinline__ void q_heads(const WriteArgs& a, long unit)
 {
@@ -501,8 +502,8 @@ int heph_qk_norm_rope_pages_scaled(void* q_out_bf16, int64_t q_stride, const voi
     if (q_out_bf16 == qkv_bf16 && q_stride != qkv_stride) return HEPH_ERR_SHAPE;
     // A long batch takes windows of 64 tokens, a prompt's page to a workgroup of 512 threads; a
     // shorter one windows of 4, more workgroups. Windows of 4 and of 64, us: 512 tokens of as many
-    // sequences 13.8, 23.5, in runs 8.7, 7.2; 1024 scattered 28, 39, in runs 12.9, 10.3; 2048 scattered
-    // 76, 81, in runs 20, 14.5; 4090 in runs 40, 22.
+    // sequences 13.7, 23.6, in runs 8.8, 7.2; 1024 scattered 28, 38, in runs 12.9, 10.4; 2048 scattered
+    // 76, 80, in runs 20.6, 12.7; 4090 in runs 39, 19.0.
     const bool many = n_tok > 1024;
     const int W = many ? 64 : 4, waves = many ? 8 : 4, heads_a_wave = many ? 16 : 8;
     const int64_t page_blocks = ((int64_t)n_tok + W - 1) / W * 2 * n_kv_heads;
@@ -550,8 +551,8 @@ int heph_read_pages(void* k_out_bf16, void* v_out_bf16, const uint8_t* k_pages,
     if (!aligned(k_out_bf16, 16) || !aligned(v_out_bf16, 16) || !aligned(k_pages, 16) ||
         !aligned(v_pages, 16))
         return HEPH_ERR_ALIGN;
-    // Windows of 16 rows and of 64, us: 100 rows 4.0, 5.4; 1000 5.5, 6.2; 2000 6.4, 6.4, scattered 27,
-    // 63; 4000 10.7, 9.9; 65001 194, 87.
+    // Windows of 16 rows and of 64, us: 100 rows 4.0, 5.3; 1000 5.4, 6.1; 2000 5.8, 5.7, scattered 26,
+    // 59; 4000 8.8, 8.0; 65001 168, 77.
     const int W = n_rows > 2048 ? 64 : 16;
     const int64_t blocks = ((int64_t)n_rows + W - 1) / W * n_kv_heads;
     if (blocks > UINT32_MAX / 256) return HEPH_ERR_UNSUPPORTED;          // (a launch's most threads)

@@ -8,7 +8,7 @@
 // exactly in a second, small launch.
 //
 // Measured (vocabulary of 151936 in f32, replayed): bound by memory without rules (256 rows 29.5 us,
-// 5.3 TB/s; 64 rows 11.5, with the logits after the rules written 20.9, 3.7 TB/s), by a chain of
+// 5.3 TB/s; 64 rows 11.1, with the logits after the rules written 17.0, 4.6 TB/s), by a chain of
 // launches and loads for few (three rows 4.8 us, with rules 6.5). Rules add the chain slot, history,
 // words: 64 rows with histories of 600 tokens 16.3 us, 256 rows 39.6; histories of 20000, of which
 // every tile takes its own tokens, 61, the atomics in LDS. Longer tiles (16384 logits: a row's
