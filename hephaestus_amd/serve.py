@@ -24,6 +24,7 @@ from __future__ import annotations
 
 import heapq
 from array import array
+from contextlib import nullcontext
 from itertools import accumulate
 
 import numpy as np
@@ -104,6 +105,16 @@ def _at(ctx) -> tuple[int, int]:
         dev = _raw_device()
         return dev, _raw_stream(dev)
     return torch.cuda.current_device(), HK._stream(ctx)
+
+
+def _on(ctx):
+    """What a call itself allocates and uploads is done on its stream: in another stream's
+    memory, given back when the call returns, it could be overwritten before the kernel reads it."""
+    if ctx is None:
+        return nullcontext()
+    if not isinstance(ctx, torch.cuda.Stream):
+        ctx = torch.cuda.ExternalStream(int(ctx)) if int(ctx) else torch.cuda.default_stream()
+    return torch.cuda.stream(ctx)
 
 
 _functions: dict = {}          # of the library, by name
@@ -469,7 +480,8 @@ def pick_tokens(tokens, logits, rules: TokenRules | None = None, slots=None, mas
         n_masks = masks.shape[0]
         mp = _matrix(masks, "masks", _I32, n_masks, (vocab + 31) // 32, dev)
     if ws is None:
-        ws = pick_ws(rows, vocab, logits.device)
+        with _on(ctx):
+            ws = pick_ws(rows, vocab, logits.device)
     _call("heph_pick_tokens", None if tokens is None else _dev(tokens, "tokens", _I32, rows, dev),
           None if logprob is None else _dev(logprob, "logprob", _F32, rows, dev), op, os_, lp, ls,
           HK._OUT[logits.dtype], rows, vocab, None if rules is None else rules._args,
@@ -591,7 +603,7 @@ class PagedKVCache:
 
     def read(self, seq: Sequence, layer: int, first: int = 0, n: int | None = None, ctx=None):
         """Keys first .. first+n-1 (n None: to the end) of one layer as bf16 rows, (k, v) of
-        [n, n_kv, 128]."""
+        [n, n_kv, 128], on the current stream or ctx: the rows belong to that stream."""
         self._own(seq)
         n = seq.length - first if n is None else n
         if not 0 <= first <= first + n <= seq.length:
@@ -599,9 +611,10 @@ class PagedKVCache:
         if not 0 <= layer < self.cfg.n_layers:
             raise ValueError(f"layer {layer} of {self.cfg.n_layers}")
         dev = self.k.device
-        slots = torch.tensor([seq.pages[j // PAGE] * PAGE + j % PAGE for j in range(first, first + n)],
-                             dtype=torch.int32, device=dev)
-        k, v = (torch.empty(n, self.cfg.n_kv_heads, 128, dtype=torch.bfloat16, device=dev) for _ in range(2))
+        with _on(ctx):
+            slots = torch.tensor([seq.pages[j // PAGE] * PAGE + j % PAGE for j in range(first, first + n)],
+                                 dtype=torch.int32, device=dev)
+            k, v = (torch.empty(n, self.cfg.n_kv_heads, 128, dtype=torch.bfloat16, device=dev) for _ in range(2))
         if self.page_scale is None:
             read_pages(k, v, self.k[layer], self.v[layer], slots, kv_scale=self.scale[layer], ctx=ctx)
         else:

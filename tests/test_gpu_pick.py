@@ -343,6 +343,34 @@ def test_pick_on_two_streams_at_once():
         assert torch.equal(w[2], o[2])
 
 
+def test_pick_scratch_on_another_stream():
+    """A call on another stream than the current one, whose scratch it allocates itself: what the
+    current stream allocates and writes behind the call is other memory."""
+    c = case(300, 20000, 100, seed=31)
+    want, lp = torch.empty(2, 300, device="cuda").unbind()
+    want = want.int()
+    S.pick_tokens(want, c["logits"], c["rules"], c["slots"], logprob=lp)
+    tokens, logprob = torch.zeros(300, dtype=torch.int32, device="cuda"), torch.zeros(300, device="cuda")
+    s, busy = torch.cuda.Stream(), torch.randn(4096, 4096, device="cuda")
+    torch.cuda.synchronize()
+    for ctx in (s, s.cuda_stream):
+        with torch.cuda.stream(s):
+            for _ in range(10):
+                busy = torch.mm(busy, busy).mul_(2.0 ** -12)
+        S.pick_tokens(tokens, c["logits"], c["rules"], c["slots"], logprob=logprob, ctx=ctx)
+        nb = S.pick_ws(300, 20000).numel()
+        full = [torch.full((nb,), 0x41, dtype=torch.uint8, device="cuda") for _ in range(8)]
+        torch.cuda.synchronize()
+        assert torch.equal(tokens, want) and torch.equal(logprob, lp)
+        assert all((f == 0x41).all() for f in full)
+        tokens.zero_()
+        logprob.zero_()
+        torch.cuda.synchronize()
+    S.pick_tokens(tokens, c["logits"], c["rules"], c["slots"], logprob=logprob, ctx=0)
+    torch.cuda.synchronize()
+    assert torch.equal(tokens, want) and torch.equal(logprob, lp)
+
+
 def test_pick_rows_past_32_bits():
     # logits of 8.6 GB: the last rows equal the same rows alone
     rows, vocab = 14200, 151936

@@ -637,6 +637,29 @@ def test_cache_reads_what_the_decoder_wrote():
                 d.kv.read(*args)
 
 
+def test_cache_reads_on_another_stream():
+    """Reads of two sequences on a stream that is busy, while the current one allocates and writes."""
+    for page_scales in (True, False):
+        d = decoder(seed=5, page_scales=page_scales)
+        a, b = d.kv.new(), d.kv.new()
+        rng = np.random.default_rng(5)
+        d.step([rng.integers(0, CFG.vocab, n).tolist() for n in (200, 200)], [a, b])
+        want = [d.kv.read(q, 1) for q in (a, b)]
+        s, busy = torch.cuda.Stream(), torch.randn(4096, 4096, device="cuda")
+        torch.cuda.synchronize()
+        for ctx in (s, s.cuda_stream, 0):
+            if ctx != 0:
+                with torch.cuda.stream(s):
+                    for _ in range(10):
+                        busy = torch.mm(busy, busy).mul_(2.0 ** -12)
+            got = [d.kv.read(q, 1, ctx=ctx) for q in (a, b)]
+            full = [torch.full((n,), -1, dtype=torch.int32, device="cuda") for n in (200, 200, 200 * 128, 200 * 128)]
+            torch.cuda.synchronize()
+            for g, w in zip(got, want):
+                assert torch.equal(g[0], w[0]) and torch.equal(g[1], w[1])
+            del full
+
+
 def test_captured_step_of_write_attend_read():
     # the run of them as a serving step makes it, captured and replayed over growing sequences
     # (a page filled, one begun, a padding row), against the same run made eagerly

@@ -237,3 +237,44 @@ def test_next_tokens_that_fail_leave_the_sequences(monkeypatch):
         with pytest.raises(ValueError):
             d.next_tokens([[1], [2]], [a, b], **kw)
     assert (a.length, b.length, c.free_pages) == (60, 0, 11)
+
+
+def test_what_a_call_allocates_is_its_streams(monkeypatch):
+    """Scratch, slots and rows of a call with ctx are allocated and uploaded on that stream."""
+    on = []
+
+    class On:
+        def __init__(self, stream):
+            self.stream = stream
+
+        def __enter__(self):
+            on.append(self.stream)
+
+        def __exit__(self, *exc):
+            on.pop()
+    monkeypatch.setattr(torch.cuda, "stream", On)
+    monkeypatch.setattr(torch.cuda, "ExternalStream", lambda handle: handle)
+    monkeypatch.setattr(torch.cuda, "default_stream", lambda: 0)
+    monkeypatch.setattr(S, "_at", lambda ctx: (0, ctx))
+    made = []
+
+    def watched(f):
+        def make(*args, **kw):
+            made.append(list(on))
+            return f(*args, **kw)
+        return make
+    for name in ("empty", "tensor"):
+        monkeypatch.setattr(torch, name, watched(getattr(torch, name)))
+    c = S.PagedKVCache(CFG, 4, device="cpu")
+    seq = c.new()
+    c.extend(seq, 70)
+    for ctx, want in ((77, [77]), (0, [0]), (None, [])):
+        with pytest.raises(ValueError):                # (host tensors: refused behind the allocations)
+            c.read(seq, 0, ctx=ctx)
+        assert made == [want] * 3
+        made.clear()
+        monkeypatch.setattr(S, "_rows", lambda t, *args: (FAKE, 512))
+        with pytest.raises(ValueError):
+            S.pick_tokens(torch.zeros(2, dtype=torch.int32), torch.zeros(2, 512), ctx=ctx)
+        assert made == [want]
+        made.clear()
