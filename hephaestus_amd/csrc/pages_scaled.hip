@@ -209,17 +209,29 @@ struct WriteLds {
     int has[kPage];
 };
 
-// n <= 8 tokens from t0 on, all of page `page`, by one wave: slot and pos are those of this lane's
-// token, t0 + l/8; fresh: key 0 is among them. V's codes leave as single bytes.
+// The n <= 64 tokens of a page that a workgroup takes together: lane i has the i-th one's row of the
+// call, slot and position.
+struct Run {
+    int page, n, row, slot, pos;
+
+    // Key 0 is among them.
+    __device__ __forceinline__ bool fresh() const
+    {
+        return __ballot((int)(threadIdx.x & 63) < n && (slot & (kPage - 1)) == 0) != 0;
+    }
+};
+
+// A run of n <= 8 by one wave: this lane's token is number l/8. V's codes leave as single bytes.
 template <bool V>
-__device__ __forceinline__ void write_few(const WriteArgs& a, int h, int t0, int n, int page, bool fresh, int slot,
-                                          int pos)
+__device__ __forceinline__ void write_few(const WriteArgs& a, int h, const Run& run)
 {
-    const int l = threadIdx.x & 63, c = l & 7, i = l / 8, key = slot & (kPage - 1);
-    const Block<V> block(a, page, h);
+    const int l = threadIdx.x & 63, c = l & 7, i = l / 8, n = run.n;
+    const int key = __shfl(run.slot, i) & (kPage - 1), row = __shfl(run.row, i), pos = __shfl(run.pos, i);
+    const bool fresh = run.fresh();
+    const Block<V> block(a, run.page, h);
     Values<V> x;
     float top = 0.0f;
-    if (i < n) top = x.load(a, h, t0 + i, pos, c);
+    if (i < n) top = x.load(a, h, row, pos, c);
     const int e = block.grow(wave_fold_max64(top), fresh);
     if (!fresh && e > block.was) {
         block.template rescale<64>(e, l);
@@ -241,14 +253,14 @@ __device__ __forceinline__ void write_few(const WriteArgs& a, int h, int t0, int
     }
 }
 
-// The same for n <= 64 by the workgroup; lane i's slot and position are token t0 + i's.
+// Any run by the workgroup.
 template <int THREADS, bool V>
-__device__ __forceinline__ void write_block(const WriteArgs& a, WriteLds& lds, int h, int t0, int n, int page,
-                                            bool fresh, int slot, int pos)
+__device__ __forceinline__ void write_block(const WriteArgs& a, WriteLds& lds, int h, const Run& run)
 {
     constexpr int R = 512 / THREADS;               // a thread's tokens: tid/8, and every THREADS/8-th
-    const int tid = threadIdx.x, l = tid & 63, c = tid & 7, key = slot & (kPage - 1);
-    const Block<V> block(a, page, h);
+    const int tid = threadIdx.x, l = tid & 63, c = tid & 7, n = run.n, key = run.slot & (kPage - 1);
+    const bool fresh = run.fresh();
+    const Block<V> block(a, run.page, h);
     Values<V> x[R];
     int my_key[R];
     float top = 0.0f;
@@ -256,8 +268,8 @@ __device__ __forceinline__ void write_block(const WriteArgs& a, WriteLds& lds, i
     for (int r = 0; r < R; ++r) {
         const int i = r * (THREADS / 8) + tid / 8;
         my_key[r] = __shfl(key, i);
-        const int p = __shfl(pos, i);
-        if (i < n) top = fmaxf(top, x[r].load(a, h, t0 + i, p, c));
+        const int p = __shfl(run.pos, i), row = __shfl(run.row, i);
+        if (i < n) top = fmaxf(top, x[r].load(a, h, row, p, c));
     }
     top = wave_fold_max64(top);
     if (tid < kPage) lds.has[tid] = 0;
@@ -315,53 +327,102 @@ __device__ __forceinline__ void write_block(const WriteArgs& a, WriteLds& lds, i
     }
 }
 
+// Token t's slot; -1: it is not cached, or not there.
+__device__ __forceinline__ int slot_of(const WriteArgs& a, int64_t t, int& pos)
+{
+    const int64_t at = min(max(t, (int64_t)0), (int64_t)a.n_tok - 1);      // (no branch: all loads at once)
+    const int s = a.slots[at];
+    pos = a.positions[at];
+    return (t >= 0) & (t < a.n_tok) & (pos >= 0) & (pos < a.n_rope) & (s >= 0) & (s < a.n_slots) ? s : -1;
+}
+
+// The page of the last cached token before token t, -1: there is none.
+__device__ __forceinline__ int page_before(const WriteArgs& a, int t)
+{
+    for (int64_t end = t; end > 0; end -= 64) {
+        int pos;
+        const int s = slot_of(a, end - 64 + (threadIdx.x & 63), pos);
+        const unsigned long long there = __ballot(s >= 0);
+        if (there) return __builtin_amdgcn_readlane(s >> 6, 63 - __clzll((long long)there));
+    }
+    return -1;
+}
+
+// A run from token t on among whose rows are tokens that are not cached.
+__device__ __forceinline__ Run sparse_run(const WriteArgs& a, int t, int page)
+{
+    const int l = threadIdx.x & 63;
+    Run run{page, 0, 0, 0, 0};
+    for (int64_t first = t; first < a.n_tok && run.n < kPage; first += 64) {
+        int pos;
+        const int s = slot_of(a, first + l, pos);
+        const unsigned long long other = __ballot(s >= 0 && s >> 6 != page);
+        const unsigned long long mine = __ballot(s >= 0 && s >> 6 == page) & (other ? (other & -other) - 1 : ~0ull);
+        // lane n + k takes what the k-th of these lanes has
+        unsigned long long m = mine;
+        for (int k = run.n; k < l; ++k) m &= m - 1;
+        const int from = m ? __ffsll((long long)m) - 1 : 0;
+        const int row = __shfl((int)first + l, from), slot = __shfl(s, from), p = __shfl(pos, from);
+        const bool takes = l >= run.n && m;
+        run.row = takes ? row : run.row;
+        run.slot = takes ? slot : run.slot;
+        run.pos = takes ? p : run.pos;
+        run.n = min(run.n + __popcll(mine), kPage);
+        if (other) break;
+    }
+    return run;
+}
+
 // A workgroup takes K or V of one kv head of the runs of tokens of one page that start among its W
-// tokens: each run of up to eight by a wave, then the longer ones by all of them. No other one
-// touches those blocks, so that a scale and the codes under it change without an atomic.
+// tokens: each run of up to eight by a wave, then the longer ones by all of them. Tokens that are not
+// cached neither end a run nor belong to one. No other workgroup touches those blocks, so that a scale
+// and the codes under it change without an atomic.
 template <int THREADS, int W, bool V>
 __device__ __forceinline__ void write_window(const WriteArgs& a, WriteLds& lds, int h, int t0)
 {
     const int l = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    // lane i: tokens t0 + i and t0 + 64 + i (all loads at once); a token that is not cached has no slot
-    const int u0 = t0 + l, u1 = u0 + 64, ub = t0 - 1, last = a.n_tok - 1;
-    int s0 = a.slots[min(u0, last)], s1 = a.slots[min(u1, last)], sb = a.slots[max(ub, 0)];
-    const int pos0 = a.positions[min(u0, last)], pos1 = a.positions[min(u1, last)], posb = a.positions[max(ub, 0)];
-    auto cached = [&](int t, int s, int pos) {
-        return (t >= 0) & (t <= last) & (pos >= 0) & (pos < a.n_rope) & (s >= 0) & (s < a.n_slots);
-    };
-    s0 = cached(u0, s0, pos0) ? s0 : -1;
-    s1 = cached(u1, s1, pos1) ? s1 : -1;
-    sb = cached(ub, sb, posb) ? sb : -1;
+    // lane i: tokens t0 + i and t0 + 64 + i, and the one before (all loads at once)
+    int pos0, pos1, posb;
+    const int s0 = slot_of(a, (int64_t)t0 + l, pos0), s1 = slot_of(a, (int64_t)t0 + 64 + l, pos1);
+    const int sb = slot_of(a, (int64_t)t0 - 1, posb);
     const int p0 = s0 >> 6, p1 = s1 >> 6;          // (no slot: -1)
-    const int shifted = __builtin_amdgcn_update_dpp(sb >> 6, p0, 0x138, 0xF, 0xF, false);     // the lane below's
-    unsigned long long starts = __ballot(l < W && p0 >= 0 && p0 != shifted), more = 0;
-    // The run that starts at lane s: its page and tokens, and lane i's slot and position of its i-th.
-    auto page_of = [&](int s) { return __builtin_amdgcn_readlane(p0, s); };
+    const unsigned long long there0 = __ballot(p0 >= 0), there1 = __ballot(p1 >= 0);
+    // the page of the last cached token before the lane's
+    const int first = there0 ? __ffsll((long long)there0) - 1 : 64;
+    if (first >= W) return;                        // (the same in all of the workgroup)
+    const unsigned long long below = there0 & ((1ull << l) - 1);
+    int before = __builtin_amdgcn_readfirstlane(sb >> 6);
+    if (before < 0 && t0 > 1) before = page_before(a, t0 - 1);
+    const int lower = __shfl(p0, below ? 63 - __clzll((long long)below) : 0);
+    unsigned long long starts = __ballot(l < W && p0 >= 0 && p0 != (below ? lower : before)), more = 0;
     auto from = [](int s, unsigned long long m0, unsigned long long m1) { return m0 >> s | (s ? m1 << (64 - s) : 0ull); };
-    auto length = [&](int s) {
-        const int page = page_of(s);
-        const unsigned long long same = from(s, __ballot(p0 == page), __ballot(p1 == page));
-        return ~same ? __ffsll((long long)~same) - 1 : 64;
+    // token l of the run's value
+    auto of_run = [&](int s, int v0, int v1) {
+        const int a0 = __shfl(v0, (l + s) & 63);
+        const int a1 = __shfl(v1, (l + s) & 63);
+        return l + s < 64 ? a0 : a1;
     };
-    const unsigned long long first0 = __ballot((s0 & (kPage - 1)) == 0), first1 = __ballot((s1 & (kPage - 1)) == 0);
-    auto fresh = [&](int s, int n) { return (from(s, first0, first1) << (64 - n)) != 0; };
-    // token i of the run's value
-    auto of_run = [&](int s, int i, int v0, int v1) {
-        const int a0 = __shfl(v0, (i + s) & 63);
-        const int a1 = __shfl(v1, (i + s) & 63);
-        return i + s < 64 ? a0 : a1;
+    // The run that starts at lane s.
+    auto run_at = [&](int s) {
+        const int page = __builtin_amdgcn_readlane(p0, s);
+        const unsigned long long same = from(s, __ballot(p0 == page), __ballot(p1 == page));
+        const int n = ~same ? __ffsll((long long)~same) - 1 : 64;
+        if (n < 64) {                              // does the next cached token belong to it too?
+            const unsigned long long next = from(s, there0, there1) >> n;
+            if (next ? (next & -next & same >> n) != 0 : (int64_t)t0 + s + 64 < a.n_tok)
+                return sparse_run(a, t0 + s, page);
+        }
+        return Run{page, n, t0 + s + l, of_run(s, s0, s1), of_run(s, pos0, pos1)};
     };
     for (int k = 0; starts; starts &= starts - 1) {
-        const int s = __ffsll((long long)starts) - 1, n = length(s);
-        if (n > 8) more |= 1ull << s;
+        const int s = __ffsll((long long)starts) - 1;
+        const Run run = run_at(s);
+        if (run.n > 8) more |= 1ull << s;
         else if (k++ % (THREADS / 64) == wave)
-            write_few<V>(a, h, t0 + s, n, page_of(s), fresh(s, n), of_run(s, l / 8, s0, s1), of_run(s, l / 8, pos0, pos1));
+            write_few<V>(a, h, run);
     }
-    for (; more; more &= more - 1) {
-        const int s = __ffsll((long long)more) - 1, n = length(s);
-        write_block<THREADS, V>(a, lds, h, t0 + s, n, page_of(s), fresh(s, n), of_run(s, l, s0, s1), of_run(s, l, pos0, pos1));
-    }
+    for (; more; more &= more - 1) write_block<THREADS, V>(a, lds, h, run_at(__ffsll((long long)more) - 1));
 }
 
 // Every q_every-th workgroup takes query heads, the others windows of tokens, until either are done:

@@ -205,7 +205,8 @@ def qk_norm_rope_pages_scaled(q_out, qkv, q_gamma, k_gamma, k_pages, v_pages, pa
     """qk_norm_rope_pages into pages with scales of their own, page_scale [n_pages, 2 n_kv]
     (powers of two, updated): the least one that holds a block's new values and is no less
     than the block's so far, whose codes are rescaled where it grows. Tokens that bring a
-    page's key 0 begin it anew. A page's tokens are neighbours among the rows."""
+    page's key 0 begin it anew. A page's tokens are neighbours among the rows; skipped ones may
+    stand between them."""
     _qk("heph_qk_norm_rope_pages_scaled", q_out, qkv, q_gamma, k_gamma, k_pages, v_pages, "page_scale",
         page_scale, rope, positions, slots, eps, ctx)
 

@@ -163,9 +163,11 @@ int heph_copy_pages(uint8_t* k_pages, uint8_t* v_pages, int n_layers, int n_page
  * nearest one in it; a page that begins behind its key 0 has its scales set to
  * 0 first.
  * The tokens of a page are neighbours among the call's rows, as a sequence's
- * newest tokens are, no two of them with one slot, and a page belongs to one
- * sequence while it is written; a page whose tokens lie apart gets codes of more
- * than one scale, and of two tokens for one slot either may be left out.
+ * newest tokens are (tokens that are skipped, for their position or their slot, may
+ * stand between them), no two of them with one slot, and a page belongs to one
+ * sequence while it is written; a page among whose tokens one of another page
+ * stands gets codes of more than one scale, and of two tokens for one slot either
+ * may be left out.
  * Writes no page and no scale without a token of the call.
  *
  * heph_pages_attention_scaled takes a plan of heph_pages_attention_plan and the

@@ -189,6 +189,49 @@ def test_write_padding_rows_and_bad_slots(T):
     check_write(c)
 
 
+@pytest.mark.parametrize("T", [3, 70, 130, 600, 1100])
+@pytest.mark.parametrize("first", [0, 5])
+@pytest.mark.parametrize("holes", ["one", "third", "most", "edges", "long"])
+def test_write_skipped_tokens_inside_pages(T, first, holes):
+    """Tokens without a position or a slot among those of a page, also more of them than a window
+    or two hold: the page's other tokens are still written as one."""
+    c = write_case([(first, T)], seed=14)
+    t = torch.arange(T)
+    skip = {"one": t % 64 == 30, "third": t % 3 == 1, "most": t % 20 != 7, "edges": (t % 4 == 3) | (t % 64 == 0),
+            "long": (t % 64 == 1) | (t % 64 == 40)}[holes]
+    if holes == "long":                                        # 150 skipped ones in one place of each page
+        n = 1 + 149 * skip.long()
+        idx = torch.repeat_interleave(t, n).cuda()
+        skip = torch.repeat_interleave(skip, n)
+        for f in ("pos", "slot"):
+            c[f] = c[f][idx].contiguous()
+        c["qkv"], c["q"] = c["qkv"][idx].contiguous(), c["q"][idx].contiguous()
+    bad = torch.nonzero(skip).flatten()
+    for i, b in enumerate(bad.tolist()):
+        if i % 3 == 0:
+            c["pos"][b] = -1
+        else:
+            c["slot"][b] = (-1, c["k"].shape[0] * PAGE)[i % 2]
+    check_write(c)
+
+
+@pytest.mark.parametrize("T", [3, 600, 1100])
+def test_write_skipped_tokens_between_sequences(T):
+    # a padded batch: each sequence's rows are followed by rows of none
+    runs = [(i * 5, 1 + i % 3) for i in range(T // 3 + 1)]
+    c = write_case(runs, seed=15)
+    idx, keep, at = [], [], 0
+    for _, n in runs:
+        idx += [*range(at, at + n), *[at] * (4 - n)]
+        keep += [True] * n + [False] * (4 - n)
+        at += n
+    idx, off = torch.tensor(idx).cuda(), ~torch.tensor(keep).cuda()
+    for f in ("pos", "slot", "qkv", "q"):
+        c[f] = c[f][idx].contiguous()
+    c["pos"][off] = -1
+    check_write(c)
+
+
 @pytest.mark.parametrize("T", [70, 600])
 def test_write_nan_infinities_and_extremes(T):
     c = write_case([(5, T)], seed=8)
