@@ -24,8 +24,8 @@
 //
 // The cache has one scale for a layer's kv head, or one for each page of it (BLOCK), a power of
 // two by which the conversion of codes to bf16 multiplies in passing: nothing is rescaled page by
-// page, and the times are the same within 1 % (96 sequences of 2048 shared and up to 1500 own keys,
-// three layers 131 and 130 us).
+// page, and the times are the same within 1.5 % (96 sequences of 2048 shared and up to 1500 own keys,
+// three layers 132 and 130 us).
 //
 // Measured (8 kv heads, 32 heads, graph replays): 64 sequences x 4096 keys of their
 // own 86 us, 6.3 TB/s of K and V; 16 prompts of 128 tokens behind 20000 keys 706 us,
@@ -587,6 +587,12 @@ __device__ __forceinline__ float lane_of(float v, int lane)
     return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), lane));
 }
 
+// Values of pages with scales of their own reach 2^128, and their sums with probabilities below
+// 2^8 over up to 2^18 keys would leave f32's range where the mean does not: V enters times 2^-up,
+// up by how much the largest scale is past 2^kTopExp (sums stay below 2^125). For the rest of its
+// way that is part of the maximum: o of weight 2^m and scale 2^up counts as o of weight 2^(m + up).
+constexpr int kTopExp = 90, kMaxExp = 119;
+
 // One wave's query rows: RT tiles of 16, column c of each in lane c, c+16, c+32, c+48.
 template <int RT>
 struct Rows {
@@ -596,6 +602,7 @@ struct Rows {
     f32x4 o[8][RT];
     float m[RT];
     f32x4 sum[RT];           // four times the same value
+    int up = 0;              // wave-uniform
 
     __device__ __forceinline__ void init(const AttnArgs& a, const Unit& u, int head, int wave_rows)
     {
@@ -630,6 +637,34 @@ struct Rows {
         }
         lo = __builtin_amdgcn_readfirstlane(lo);
         hi = __builtin_amdgcn_readfirstlane(hi);
+    }
+
+    // Scales of V as the next pages enter, one a lane; used: the lane has one of them.
+    __device__ __forceinline__ float enter(float scale, bool used)
+    {
+        const int e = (int)(__float_as_uint(scale) >> 23 & 0xFF) - 127;
+        if (up == 0 && !__any(used && e > kTopExp)) return scale;
+        const float top = wave_fold_max64(used ? (float)min(e, kMaxExp) : 0.0f);
+        const int to = __builtin_amdgcn_readfirstlane(max((int)top - kTopExp, up));
+        if (to > up) {
+#pragma unroll
+            for (int d = 0; d < 8; ++d)
+#pragma unroll
+                for (int r = 0; r < RT; ++r) o[d][r] *= __builtin_amdgcn_ldexpf(1.0f, up - to);
+            up = to;
+        }
+        return __builtin_amdgcn_ldexpf(scale, -to);
+    }
+
+    // Behind the last page.
+    __device__ __forceinline__ void leave()
+    {
+        if (up == 0) return;
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+            m[r] += (float)up;
+            sum[r] *= __builtin_amdgcn_ldexpf(1.0f, -up);
+        }
     }
 
     // The keys of one page. k(i, h) and v(i, h) give this lane's operands from the
@@ -724,7 +759,7 @@ struct Rows {
             top[r] = rows4_max(x * sc);
             moves |= top[r] > m[r] + 8.0f;
         }
-        // The maximum moves only by 2^8 or more: probabilities stay below 2^8, sums
+        // The maximum moves only by 2^8 or more: probabilities stay below 2^8, their sums
         // far from f32's range, and most pages scale nothing.
         if (__any(moves)) {
 #pragma unroll
@@ -910,6 +945,7 @@ __device__ __forceinline__ void attend_narrow(const AttnArgs& a, const Unit& u, 
         }
         int n = first + kw;
         load(p0, n);
+        if constexpr (BLOCK) sv = x.enter(sv, l < last - first && ids >= 0 && ids < a.n_pages);
         while (n < last) {
             load(p1, n + KW);
             work(p0, n);
@@ -921,6 +957,7 @@ __device__ __forceinline__ void attend_narrow(const AttnArgs& a, const Unit& u, 
         }
     }
 
+    if constexpr (BLOCK) x.leave();
     // Waves on the same rows join: each takes 8 / KW of the dim tiles.
     int d0 = 0, nd = 8;
     if (KW > 1) {
@@ -989,7 +1026,11 @@ __device__ __forceinline__ void attend_wide(const AttnArgs& a, const Unit& u, in
     for (int first = u.page0; first < end; first += 64) {
         const int last = min(first + 64, end), ids = first == u.page0 ? ids0 : page_ids(a, u, first);
         wait_vm<0>();           // (nothing but pages, and their scales before them, on its way below)
-        const float scales = BLOCK ? page_scale(a, ids, (wave < 2 ? 0 : n_kv) + head) : 1.0f;
+        float scales = 1.0f, values = 1.0f;
+        if constexpr (BLOCK) {
+            values = page_scale(a, ids, n_kv + head);
+            scales = page_scale(a, ids, head);
+        }
         auto id_of = [&](int n) { return __builtin_amdgcn_readlane(ids, n - first); };
         struct Codes {
             i32x4 w[4];
@@ -1036,6 +1077,10 @@ __device__ __forceinline__ void attend_wide(const AttnArgs& a, const Unit& u, in
         load(c0, first);
         if (threadIdx.x < 2) nan_page[threadIdx.x] = -1;
         lds_barrier();          // (the last block's pages are read)
+        if constexpr (BLOCK) {
+            values = x.enter(values, l < last - first && ids >= 0 && ids < a.n_pages);
+            if (wave >= 2) scales = values;
+        }
         convert(c0, first);
         load(c0, first + 1);
         load(c1, first + 2);
@@ -1046,6 +1091,7 @@ __device__ __forceinline__ void attend_wide(const AttnArgs& a, const Unit& u, in
             step(c1, n + 1);
         }
     }
+    if constexpr (BLOCK) x.leave();
     x.template store<BLOCK>(a, u, head, 0, 8);
 }
 

@@ -172,7 +172,9 @@ int heph_copy_pages(uint8_t* k_pages, uint8_t* v_pages, int n_layers, int n_page
  *
  * heph_pages_attention_scaled takes a plan of heph_pages_attention_plan and the
  * workspace of heph_pages_attention_ws_bytes. Of a page_scale only the exponent
- * is used.
+ * is used. V's scales may lie anywhere in the range above: sums are kept relative to
+ * the largest one (values 2^200 times smaller than a run's largest may be lost
+ * beside it). Scores q . k are f32 numbers, and have to be finite as such.
  *
  * heph_copy_pages_scaled copies the pages' scales with them (page_scale
  * [n_layers][n_pages][2 * n_kv_heads]).

@@ -468,6 +468,35 @@ def test_attention_scales_far_apart():
         check_attention(b, attend(b))
 
 
+@pytest.mark.parametrize("lo,hi", [(105, 119), (60, 119), (-117, -100), (-117, -60), (-117, 119)])
+def test_attention_values_at_the_ends_of_their_range(lo, hi):
+    """Values up to 448 * 2^119, whose sums leave f32's range though their mean does not, and down to
+    the smallest normal ones; in one unit, in parts that are merged, behind a prefix, wide and narrow."""
+    for i, (new, own, shared, group_start) in enumerate([
+            ([1], [300], (), ()), ([1], [64 * 70 + 3], (), ()), ([5, 40], [30, 200], (), ()), ([150], [700], (), ()),
+            ([1] * 9, [10, 20, 30, 40, 50, 60, 70, 80, 90], [2, 7, 1], [0, 4, 5, 9]),
+            ([1, 100, 1, 1], [3, 120, 70, 5], [25], [0, 4])]):
+        b = with_scales(batch(new, own, shared, group_start, seed=50 + i), seed=50 + i)
+        g = torch.Generator().manual_seed(i)
+        scale = torch.randint(lo, hi + 1, (b["k"].shape[0], b["KV"]), generator=g).double().exp2()
+        b["page_scale"][:, b["KV"]:] = scale.float().cuda()
+        check_attention(b, attend(b))
+
+
+@pytest.mark.parametrize("new", [1, 20])
+def test_attention_values_grow_along_a_long_run(new):
+    # more than 64 pages of one unit (as many sequences as there are places), the later ones' values
+    # larger or smaller than the first ones'
+    n, pages = 70, 70
+    b = with_scales(batch([new] * n, [64 * pages - 5] * n, seed=60, H=8 if new == 1 else 32, garbage=False), seed=60)
+    first = torch.zeros(b["k"].shape[0], dtype=torch.bool)
+    first[b["table"][:, :64].flatten().cpu().long()] = True
+    for early, late in ((110, 119), (119, 110), (-117, -85), (-90, -117), (0, 100), (0, 0)):
+        e = torch.where(first, early, late).float()
+        b["page_scale"][:, b["KV"]:] = e.exp2()[:, None].cuda()
+        check_attention(b, attend(b), tokens=[0, 5 * new + new // 2, n * new - 1])
+
+
 def test_attention_one_scale_equals_the_static_op():
     # with one power of two everywhere the codes enter as multiples of it: the products are the
     # same but for the order of the exact scaling, out to the last bit where nothing is rounded twice
