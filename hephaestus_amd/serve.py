@@ -743,7 +743,10 @@ class Qwen3BatchDecoder:
         """tokens[i] (one or more) enter sequence seqs[i], with adapter
         adapters[i] (-1: none). Returns the f32 logits [len(seqs), vocab] after
         each sequence's last token. A step that raises leaves the sequences as
-        they were."""
+        they were: what it may refuse or find no memory for comes before the first
+        key is written. (Interrupted behind that, a cache with page scales may keep
+        the keys of a sequence's last page at a larger scale, as a step that ends
+        would have left them.)"""
         cfg, kv = self.w.cfg, self.kv
         if len(tokens) != len(seqs) or not seqs or any(len(t) < 1 for t in tokens):
             raise ValueError("every sequence brings one token or more")
@@ -791,17 +794,19 @@ class Qwen3BatchDecoder:
             if rules.vocab != vocab or rules._dev != self.w.embed.w.get_device():
                 raise ValueError(f"rules of {rules.vocab} tokens on device {rules._dev} for a model of {vocab} on {dev}")
         if masks is not None:
-            if len(mask_ids) != S or any(m >= masks.shape[0] for m in mask_ids):
+            if masks.shape[0] < 1 or len(mask_ids) != S or any(m >= masks.shape[0] for m in mask_ids):
                 raise ValueError(f"mask_ids {mask_ids} are not one of {masks.shape[0]} for each of {S} sequences")
             _matrix(masks, "masks", _I32, masks.shape[0], (vocab + 31) // 32, self.w.embed.w.get_device())
         ids = [None if x is None else torch.tensor(array("i", x), dtype=torch.int32, device=dev)
                for x in (slots, mask_ids)]
+        # (no memory: said before the step writes keys)
+        picked = torch.empty(S, dtype=torch.int32, device=dev)
+        logprob = torch.empty(S, dtype=torch.float32, device=dev)
+        ws = pick_ws(max(S, 1), vocab, dev)
         before = [(s, s.length, len(s.pages)) for s in seqs]
         logits = self.step(tokens, seqs, adapters)
         try:
-            picked = torch.empty(S, dtype=torch.int32, device=dev)
-            logprob = torch.empty(S, dtype=torch.float32, device=dev)
-            pick_tokens(picked, logits, rules, ids[0], masks, ids[1], logprob=logprob, append=rules is not None)
+            pick_tokens(picked, logits, rules, ids[0], masks, ids[1], logprob=logprob, append=rules is not None, ws=ws)
         except BaseException:
             self._undo(before)
             raise
@@ -845,6 +850,8 @@ class Qwen3BatchDecoder:
         x, xn = torch.empty(T, H, **bf), torch.empty(T, H, **bf)
         qkv, att = torch.empty(T, Q + 2 * KV, **bf), torch.empty(T, Q, **bf)
         gu, act = torch.empty(T, 2 * I, **bf), torch.empty(T, I, **bf)
+        ends, last = q_start[1:].long() - 1, torch.empty(S, H, **bf)
+        logits = torch.empty(S, cfg.vocab, dtype=torch.float32, device=dev)
         q_bytes = max(L.lib().heph_fp8_linear_ws_bytes(T, n, k) for n, k in
                       ((Q + 2 * KV, H), (H, Q), (2 * I, H), (H, I)))
         ws = (torch.empty(q_bytes, dtype=torch.uint8, device=dev),
@@ -856,6 +863,8 @@ class Qwen3BatchDecoder:
         if lora is not None:
             lplan = LoraPlan(T, lora.n_adapters, lora.max_rank, lora.max_k, device=dev)
             lplan.update(ids)
+            # (silu_mul takes gate and up each in one piece)
+            halves = torch.empty(2, T, I, **bf) if any("down" in d for d in lora.layers) else None
 
         def adapt(li, op, c, a):
             if lora is not None and op in lora.layers[li]:
@@ -888,15 +897,14 @@ class Qwen3BatchDecoder:
             adapt(li, "o", x, att)
             norm_linear(li, "gate_up", gu, lw.ffn_norm, lw.gate_up)
             if lora is not None and "down" in lora.layers[li]:
-                # (the op takes gate and up each in one piece)
-                DEC.silu_mul(act, gu[:, :I].contiguous(), gu[:, I:].contiguous(), T * I)
+                halves.copy_(gu.view(T, 2, I).transpose(0, 1))
+                DEC.silu_mul(act, halves[0], halves[1], T * I)
                 self._linear(x, act, lw.down, I, ws, residual=True)
                 adapt(li, "down", x, act)
             else:
                 HK.silu_mul_quant_fp8(ws[0], ws[1], gu, gu[:, I:], T, I, 2 * I)
                 self._linear(x, None, lw.down, I, ws, residual=True, quantized=True)
-        last = x[q_start[1:].long() - 1]
-        logits = torch.empty(S, cfg.vocab, dtype=torch.float32, device=dev)
+        torch.index_select(x, 0, ends, out=last)
         HK.rmsnorm_quant_fp8(ws[0], ws[1], last, w.final_norm, S, H, cfg.eps)
         self._linear(logits, None, w.embed, H, ws, quantized=True)
         return logits

@@ -709,6 +709,45 @@ def test_cache_reads_what_the_decoder_wrote():
                 d.kv.read(*args)
 
 
+@pytest.mark.parametrize("fails", ["logits", "tokens", "scratch", "no masks"])
+def test_a_step_without_memory_writes_no_keys(monkeypatch, fails):
+    """A step that finds no memory for its logits, or for the pick behind them, has not touched the
+    older keys of a partly filled page, whose scales and codes it would change."""
+    d = decoder(seed=6, page_scales=True)
+    seq = d.kv.new()
+    rng = np.random.default_rng(6)
+    d.step([rng.integers(0, CFG.vocab, 70).tolist()], [seq])
+    kv, more = d.kv, rng.integers(0, CFG.vocab, 50).tolist()
+
+    def state():
+        return [t.clone() for t in (kv.k, kv.v, kv.page_scale)], seq.length, list(seq.pages), kv.free_pages
+    before = state()
+    empty, shape = torch.empty, {"logits": (1, CFG.vocab), "tokens": (1,)}.get(fails)
+
+    def full(*args, **kw):
+        if args == shape:
+            raise torch.OutOfMemoryError("no memory")
+        return empty(*args, **kw)
+
+    def scratch(*args):
+        raise torch.OutOfMemoryError("no memory")
+    with monkeypatch.context() as m:
+        m.setattr(torch, "empty", full)
+        if fails == "scratch":
+            m.setattr(S, "pick_ws", scratch)
+        with pytest.raises(ValueError if fails == "no masks" else torch.OutOfMemoryError):
+            if fails == "logits":
+                d.step([more], [seq])
+            elif fails == "no masks":
+                d.next_tokens([more], [seq], masks=torch.zeros(0, -(-CFG.vocab // 32), **I32), mask_ids=[-1])
+            else:
+                d.next_tokens([more], [seq])
+    after = state()
+    assert after[1:] == before[1:] and all(torch.equal(a, b) for a, b in zip(after[0], before[0]))
+    d.step([more], [seq])
+    assert not torch.equal(kv.page_scale[:, before[2][1]], before[0][2][:, before[2][1]])
+
+
 def test_cache_reads_on_another_stream():
     """Reads of two sequences on a stream that is busy, while the current one allocates and writes."""
     for page_scales in (True, False):
