@@ -426,17 +426,18 @@ class TokenRules:
                              f"{self.max_tokens} and {self.max_bias}")
         if any(not 0 <= t < self.vocab for t in (*tokens, *bias)):
             raise ValueError(f"a token outside the vocabulary of {self.vocab}")
-        penalties = [float(repetition), float(presence), float(frequency)]
-        if not all(np.isfinite(penalties)) or not repetition > 0:
-            raise ValueError(f"penalties {penalties}")
-        if any(not float(b) < np.inf for b in bias.values()):
+        # (checked as the f32 numbers that the pick takes)
+        values = torch.tensor([float(x) for x in (repetition, presence, frequency, *bias.values())],
+                              dtype=torch.float32)
+        if not values[:3].isfinite().all() or not values[0] > 0:
+            raise ValueError(f"penalties {[repetition, presence, frequency]}")
+        if not (values[3:] < np.inf).all():
             raise ValueError("a bias that is NaN or +inf")
         # (array: what is no whole number is refused, not rounded)
         ids = torch.from_numpy(np.frombuffer(array("i", [*tokens, *bias, len(tokens), len(prompt), len(bias)]),
                                              dtype=np.int32).copy()).to(self.history.device)
         n, m = len(tokens), len(bias)
-        values = torch.tensor(penalties + [float(b) for b in bias.values()], dtype=torch.float32,
-                              device=self.history.device)
+        values = values.to(self.history.device)
         self.history[slot, :n] = ids[:n]
         self.bias_ids[slot, :m] = ids[n:n + m]
         self.length[slot], self.n_prompt[slot], self.n_bias[slot] = ids[n + m:].unbind()

@@ -278,3 +278,15 @@ def test_what_a_call_allocates_is_its_streams(monkeypatch):
             S.pick_tokens(torch.zeros(2, dtype=torch.int32), torch.zeros(2, 512), ctx=ctx)
         assert made == [want]
         made.clear()
+
+
+def test_rules_refuse_what_f32_does_not_hold():
+    r = S.TokenRules(1, 50, 4, 2, device="cpu")
+    for kw in (dict(repetition=1e-50), dict(repetition=1e39), dict(presence=1e39), dict(frequency=-1e39),
+               dict(bias={3: 1e39}), dict(bias={3: 1.0, 4: 3.5e38})):
+        with pytest.raises(ValueError):
+            r.set(0, [1], **kw)
+    assert (r.length == 0).all() and (r.penalties == torch.tensor([1.0, 0, 0])).all()
+    r.set(0, [1], repetition=1e-38, presence=3e38, bias={3: -1e39, 4: 1e-50})
+    assert r.penalties.tolist() == [[float(np.float32(1e-38)), float(np.float32(3e38)), 0.0]]
+    assert r.bias.tolist() == [[-float("inf"), 0.0]]
