@@ -214,7 +214,7 @@ def qk_norm_rope_pages_scaled(q_out, qkv, q_gamma, k_gamma, k_pages, v_pages, pa
 def read_pages(k_out, v_out, k_pages, v_pages, slots, kv_scale=None, page_scale=None,
                ctx=None) -> None:
     """Row t of k_out and v_out (bf16 [n, n_kv, 128]): the key and value of slots[t], code times
-    scale. One of kv_scale [2 n_kv] (of all pages) and page_scale [n_pages, 2 n_kv]. A slot
+    scale in f32, rounded to bf16. One of kv_scale [2 n_kv] (of all pages) and page_scale [n_pages, 2 n_kv]. A slot
     outside the pools leaves its row as it was."""
     if (kv_scale is None) == (page_scale is None):
         raise ValueError("read_pages takes one of kv_scale and page_scale")

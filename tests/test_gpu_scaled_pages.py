@@ -373,6 +373,31 @@ def test_read_heads(KV):
     check_read(list(range(60, 200)), KV=KV, seed=KV, nan=KV > 1)
 
 
+def test_read_rounds_the_product_in_f32_and_then_to_bf16():
+    # with one scale for all pages: scales whose product with 1.875 (code 0x3F) is, rounded to f32,
+    # just between two bf16 values, while the exact product is not
+    x = (np.arange(1, 4000, 4, dtype=np.uint32) << 16 | 0x3F808000).view(np.float32)     # halfway, odd above
+    x = x[x < 4]
+    s = (x.astype(np.float64) / 1.875).astype(np.float32)
+    exact = s.astype(np.float64) * 1.875
+    twice = (s * np.float32(1.875) == x) & (exact != x)
+    s, exact = s[twice][:8], exact[twice][:8]
+    assert len(s) == 8
+    KV = 4
+    k = torch.full((1, KV, 2, PAGE, 64), 0x3F, dtype=torch.uint8, device="cuda")
+    v = torch.full((1, KV, D, PAGE), 0x3F, dtype=torch.uint8, device="cuda")
+    out = [torch.zeros(3, KV, D, dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+    S.read_pages(*out, k, v, i32([0, 1, 63]), kv_scale=torch.from_numpy(s).cuda())
+    want = torch.from_numpy(s * np.float32(1.875)).to(torch.bfloat16)
+    once = torch.from_numpy(exact).to(torch.float64)
+    got = torch.cat([out[0][0, :, 0], out[1][0, :, 0]]).cpu()
+    assert torch.equal(got, want)
+    # one step off the nearest at most: half a step of bf16 and half of one of f32
+    assert ((got.double() - once).abs() <= (2.0 ** -8 + 2.0 ** -24) * once).all()
+    for o in out:
+        assert (o == o[:1, :, :1]).all()
+
+
 def test_read_any_slots():
     rng = np.random.default_rng(0)
     check_read(rng.integers(0, 9 * PAGE, 500).tolist(), seed=1)                      # scattered, repeated
