@@ -150,6 +150,14 @@ def test_pick_counts_past_sixteen_bits():
     check(c)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_pick_repetition_below_one(dtype):
+    # what was seen is preferred: positive logits grow, negative ones shrink towards 0
+    c = case(6, 7001, 900, 20, 2, seed=17, dtype=dtype)
+    c["rules"].penalties[:, 0] = torch.tensor([0.3, 0.5, 0.75, 0.999, 2.0 ** -20, 1e-30, 1.0, 0.1]).cuda()
+    check(c)
+
+
 def test_pick_without_rules_or_masks():
     for seed, kw in enumerate((dict(rules=None, slots=None), dict())):
         c = dict(case(5, 7001, 100, 3, 0, seed=seed), **kw)
