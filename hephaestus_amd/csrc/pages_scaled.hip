@@ -7,9 +7,9 @@
 // 2^-6, off by at most half of the smallest one's step), and lets the attention's conversions
 // multiply by it in passing.
 //
-// Measured (32 + 8 heads, graph replays): 4090 tokens of prompts (94 MB with q) 19.8 us, 4.7 TB/s (a
-// copy of 1 GiB reaches 5.2), with one scale for all pages 18.9; 128 tokens of as many sequences 6.1
-// (4.8), three 4.1 (2.9): there a chain of three loads, the scale's rounds among the lanes and V's
+// Measured (32 + 8 heads, graph replays): 4090 tokens of prompts (94 MB with q) 20.8 us, 4.5 TB/s (a
+// copy of 1 GiB reaches 5.2), with one scale for all pages 18.9; 128 tokens of as many sequences 6.3
+// (4.8), three 4.3 (2.9): there a chain of three loads, the scale's rounds among the lanes and V's
 // single bytes count. 65001 rows read back (399 MB) in 79 us, 5.0 TB/s.
 #include <algorithm>
 
@@ -209,29 +209,17 @@ struct WriteLds {
     int has[kPage];
 };
 
-// The n <= 64 tokens of a page that a workgroup takes together: lane i has the i-th one's row of the
-// call, slot and position.
-struct Run {
-    int page, n, row, slot, pos;
-
-    // Key 0 is among them.
-    __device__ __forceinline__ bool fresh() const
-    {
-        return __ballot((int)(threadIdx.x & 63) < n && (slot & (kPage - 1)) == 0) != 0;
-    }
-};
-
-// A run of n <= 8 by one wave: this lane's token is number l/8. V's codes leave as single bytes.
+// n <= 8 tokens from t0 on, all of page `page`, by one wave: slot and pos are those of this lane's
+// token, t0 + l/8; fresh: key 0 is among them. V's codes leave as single bytes.
 template <bool V>
-__device__ __forceinline__ void write_few(const WriteArgs& a, int h, const Run& run)
+__device__ __forceinline__ void write_few(const WriteArgs& a, int h, int t0, int n, int page, bool fresh, int slot,
+                                          int pos)
 {
-    const int l = threadIdx.x & 63, c = l & 7, i = l / 8, n = run.n;
-    const int key = __shfl(run.slot, i) & (kPage - 1), row = __shfl(run.row, i), pos = __shfl(run.pos, i);
-    const bool fresh = run.fresh();
-    const Block<V> block(a, run.page, h);
+    const int l = threadIdx.x & 63, c = l & 7, i = l / 8, key = slot & (kPage - 1);
+    const Block<V> block(a, page, h);
     Values<V> x;
     float top = 0.0f;
-    if (i < n) top = x.load(a, h, row, pos, c);
+    if (i < n) top = x.load(a, h, t0 + i, pos, c);
     const int e = block.grow(wave_fold_max64(top), fresh);
     if (!fresh && e > block.was) {
         block.template rescale<64>(e, l);
@@ -253,14 +241,14 @@ __device__ __forceinline__ void write_few(const WriteArgs& a, int h, const Run& 
     }
 }
 
-// Any run by the workgroup.
-template <int THREADS, bool V>
-__device__ __forceinline__ void write_block(const WriteArgs& a, WriteLds& lds, int h, const Run& run)
+// The same for n <= 64 by the workgroup: token i is row row_of(i), lane i has its slot and position.
+template <int THREADS, bool V, class Row>
+__device__ __forceinline__ void write_block(const WriteArgs& a, WriteLds& lds, int h, Row row_of, int n, int page,
+                                            bool fresh, int slot, int pos)
 {
     constexpr int R = 512 / THREADS;               // a thread's tokens: tid/8, and every THREADS/8-th
-    const int tid = threadIdx.x, l = tid & 63, c = tid & 7, n = run.n, key = run.slot & (kPage - 1);
-    const bool fresh = run.fresh();
-    const Block<V> block(a, run.page, h);
+    const int tid = threadIdx.x, l = tid & 63, c = tid & 7, key = slot & (kPage - 1);
+    const Block<V> block(a, page, h);
     Values<V> x[R];
     int my_key[R];
     float top = 0.0f;
@@ -268,8 +256,8 @@ __device__ __forceinline__ void write_block(const WriteArgs& a, WriteLds& lds, i
     for (int r = 0; r < R; ++r) {
         const int i = r * (THREADS / 8) + tid / 8;
         my_key[r] = __shfl(key, i);
-        const int p = __shfl(run.pos, i), row = __shfl(run.row, i);
-        if (i < n) top = fmaxf(top, x[r].load(a, h, row, p, c));
+        const int p = __shfl(pos, i), t = row_of(i);
+        if (i < n) top = fmaxf(top, x[r].load(a, h, t, p, c));
     }
     top = wave_fold_max64(top);
     if (tid < kPage) lds.has[tid] = 0;
@@ -330,106 +318,140 @@ __device__ __forceinline__ void write_block(const WriteArgs& a, WriteLds& lds, i
 // Token t's slot; -1: it is not cached, or not there.
 __device__ __forceinline__ int slot_of(const WriteArgs& a, int64_t t, int& pos)
 {
-    const int64_t at = min(max(t, (int64_t)0), (int64_t)a.n_tok - 1);      // (no branch: all loads at once)
+    const int64_t at = min(max(t, (int64_t)0), (int64_t)a.n_tok - 1);
     const int s = a.slots[at];
     pos = a.positions[at];
     return (t >= 0) & (t < a.n_tok) & (pos >= 0) & (pos < a.n_rope) & (s >= 0) & (s < a.n_slots) ? s : -1;
 }
 
-// The page of the last cached token before token t, -1: there is none.
-__device__ __forceinline__ int page_before(const WriteArgs& a, int t)
+// The page of the nearest cached token from token t on, upwards (step 1) or downwards (-1); -1: none.
+// (512 tokens' loads at once: the padding behind a batch may be long.)
+__device__ __forceinline__ int page_near(const WriteArgs& a, int64_t t, int step)
 {
-    for (int64_t end = t; end > 0; end -= 64) {
-        int pos;
-        const int s = slot_of(a, end - 64 + (threadIdx.x & 63), pos);
-        const unsigned long long there = __ballot(s >= 0);
-        if (there) return __builtin_amdgcn_readlane(s >> 6, 63 - __clzll((long long)there));
+    constexpr int K = 8;
+    for (; t >= 0 && t < a.n_tok; t += 64 * K * step) {
+        int slot[K], pos;
+#pragma unroll
+        for (int k = 0; k < K; ++k) slot[k] = slot_of(a, t + step * (64 * k + (int)(threadIdx.x & 63)), pos);
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            const unsigned long long there = __ballot(slot[k] >= 0);
+            if (there) return __builtin_amdgcn_readlane(slot[k] >> 6, __ffsll((long long)there) - 1);
+        }
     }
     return -1;
 }
 
-// A run from token t on among whose rows are tokens that are not cached.
-__device__ __forceinline__ Run sparse_run(const WriteArgs& a, int t, int page)
+// The tokens of a page from token t on with others among them that are not cached: how many, and
+// lane i's row, slot and position of the i-th.
+__device__ __forceinline__ int sparse_run(const WriteArgs& a, int t, int page, int& row, int& slot, int& pos)
 {
     const int l = threadIdx.x & 63;
-    Run run{page, 0, 0, 0, 0};
-    for (int64_t first = t; first < a.n_tok && run.n < kPage; first += 64) {
-        int pos;
-        const int s = slot_of(a, first + l, pos);
+    int n = 0;
+    for (int64_t first = t; first < a.n_tok && n < kPage; first += 64) {
+        int p;
+        const int s = slot_of(a, first + l, p);
         const unsigned long long other = __ballot(s >= 0 && s >> 6 != page);
         const unsigned long long mine = __ballot(s >= 0 && s >> 6 == page) & (other ? (other & -other) - 1 : ~0ull);
         // lane n + k takes what the k-th of these lanes has
         unsigned long long m = mine;
-        for (int k = run.n; k < l; ++k) m &= m - 1;
-        const int from = m ? __ffsll((long long)m) - 1 : 0;
-        const int row = __shfl((int)first + l, from), slot = __shfl(s, from), p = __shfl(pos, from);
-        const bool takes = l >= run.n && m;
-        run.row = takes ? row : run.row;
-        run.slot = takes ? slot : run.slot;
-        run.pos = takes ? p : run.pos;
-        run.n = min(run.n + __popcll(mine), kPage);
+#pragma unroll 1
+        for (int k = n; k < l; ++k) m &= m - 1;
+        const int from = m ? __ffsll((long long)m) - 1 : 0, from_slot = __shfl(s, from), from_pos = __shfl(p, from);
+        if (l >= n && m) {
+            row = (int)first + from;
+            slot = from_slot;
+            pos = from_pos;
+        }
+        n = min(n + __popcll(mine), kPage);
         if (other) break;
     }
-    return run;
+    return n;
 }
 
 // A workgroup takes K or V of one kv head of the runs of tokens of one page that start among its W
-// tokens: each run of up to eight by a wave, then the longer ones by all of them. Tokens that are not
-// cached neither end a run nor belong to one. No other workgroup touches those blocks, so that a scale
-// and the codes under it change without an atomic.
+// tokens: each run of up to eight by a wave, then the longer ones by all of them. No other one
+// touches those blocks, so that a scale and the codes under it change without an atomic. Tokens that
+// are not cached neither end a run nor belong to one: a window with such among a run's is written
+// run by run (512 tokens of a prompt 8.9 us, with every eighth skipped 13.6). To look for them costs
+// batches without any nothing or little (4090 tokens 20.8 us instead of 20.2).
 template <int THREADS, int W, bool V>
 __device__ __forceinline__ void write_window(const WriteArgs& a, WriteLds& lds, int h, int t0)
 {
     const int l = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    // lane i: tokens t0 + i and t0 + 64 + i, and the one before (all loads at once)
-    int pos0, pos1, posb;
-    const int s0 = slot_of(a, (int64_t)t0 + l, pos0), s1 = slot_of(a, (int64_t)t0 + 64 + l, pos1);
-    const int sb = slot_of(a, (int64_t)t0 - 1, posb);
-    const int p0 = s0 >> 6, p1 = s1 >> 6;          // (no slot: -1)
-    const unsigned long long there0 = __ballot(p0 >= 0), there1 = __ballot(p1 >= 0);
-    // the page of the last cached token before the lane's
-    const int first = there0 ? __ffsll((long long)there0) - 1 : 64;
-    if (first >= W) return;                        // (the same in all of the workgroup)
-    const unsigned long long below = there0 & ((1ull << l) - 1);
-    int before = __builtin_amdgcn_readfirstlane(sb >> 6);
-    if (before < 0 && t0 > 1) before = page_before(a, t0 - 1);
-    const int lower = __shfl(p0, below ? 63 - __clzll((long long)below) : 0);
-    unsigned long long starts = __ballot(l < W && p0 >= 0 && p0 != (below ? lower : before)), more = 0;
-    auto from = [](int s, unsigned long long m0, unsigned long long m1) { return m0 >> s | (s ? m1 << (64 - s) : 0ull); };
-    // token l of the run's value
-    auto of_run = [&](int s, int v0, int v1) {
-        const int a0 = __shfl(v0, (l + s) & 63);
-        const int a1 = __shfl(v1, (l + s) & 63);
-        return l + s < 64 ? a0 : a1;
+    // lane i: tokens t0 + i and t0 + 64 + i (all loads at once); a token that is not cached has no slot
+    const int u0 = t0 + l, u1 = u0 + 64, ub = t0 - 1, last = a.n_tok - 1;
+    int s0 = a.slots[min(u0, last)], s1 = a.slots[min(u1, last)], sb = a.slots[max(ub, 0)];
+    const int pos0 = a.positions[min(u0, last)], pos1 = a.positions[min(u1, last)], posb = a.positions[max(ub, 0)];
+    auto cached = [&](int t, int s, int pos) {
+        return (t >= 0) & (t <= last) & (pos >= 0) & (pos < a.n_rope) & (s >= 0) & (s < a.n_slots);
     };
-    // The run that starts at lane s.
-    auto run_at = [&](int s) {
-        const int page = __builtin_amdgcn_readlane(p0, s);
-        const unsigned long long same = from(s, __ballot(p0 == page), __ballot(p1 == page));
-        const int n = ~same ? __ffsll((long long)~same) - 1 : 64;
-        if (n < 64) {                              // does the next cached token belong to it too?
-            const unsigned long long next = from(s, there0, there1) >> n;
-            if (next ? (next & -next & same >> n) != 0 : (int64_t)t0 + s + 64 < a.n_tok)
-                return sparse_run(a, t0 + s, page);
+    s0 = cached(u0, s0, pos0) ? s0 : -1;
+    s1 = cached(u1, s1, pos1) ? s1 : -1;
+    sb = cached(ub, sb, posb) ? sb : -1;
+    const int p0 = s0 >> 6, p1 = s1 >> 6;          // (no slot: -1)
+    if (__builtin_expect(__any((p0 < 0 && u0 <= last) || (p1 < 0 && u1 <= last) || (sb < 0 && t0 > 0)), 0)) {
+        const unsigned long long there0 = __ballot(p0 >= 0), there1 = __ballot(p1 >= 0);
+        if (!(there0 << (64 - W))) return;         // (none starts here)
+        const int before = sb >= 0 ? sb >> 6 : page_near(a, (int64_t)t0 - 2, -1);
+        const unsigned long long below0 = there0 & ((1ull << l) - 1), below1 = there1 & ((1ull << l) - 1);
+        // the page of the last cached token before the lane's two
+        const int in0 = __shfl(p0, 63 - __clzll((long long)(below0 | 1))), end0 = __shfl(p0, 63 - __clzll((long long)(there0 | 1)));
+        const int in1 = __shfl(p1, 63 - __clzll((long long)(below1 | 1)));
+        const int prev0 = below0 ? in0 : before, prev1 = below1 ? in1 : there0 ? end0 : before;
+        // behind these 128 tokens, is there more of a run that starts here?
+        const int end = there1 ? __shfl(p1, 63 - __clzll((long long)there1)) : end0;
+        const bool open = !(there1 >> 63) && __any(l < W && p0 == end) && page_near(a, (int64_t)t0 + 128, 1) == end;
+        const bool gap0 = p0 >= 0 && p0 == prev0 && (l ? !(there0 >> (l - 1) & 1) : sb < 0);
+        const bool gap1 = p1 >= 0 && p1 == prev1 && (l ? !(there1 >> (l - 1) & 1) : !(there0 >> 63));
+        if (__any(gap0 | gap1 | open)) {
+            for (unsigned long long starts = __ballot(l < W && p0 >= 0 && p0 != prev0); starts; starts &= starts - 1) {
+                const int s = __ffsll((long long)starts) - 1, page = __builtin_amdgcn_readlane(p0, s);
+                int row = 0, slot = 0, pos = 0;
+                const int n = sparse_run(a, t0 + s, page, row, slot, pos);
+                const bool begins = __any(l < n && (slot & (kPage - 1)) == 0);
+                write_block<THREADS, V>(a, lds, h, [&](int i) { return __shfl(row, i); }, n, page, begins, slot, pos);
+            }
+            return;
         }
-        return Run{page, n, t0 + s + l, of_run(s, s0, s1), of_run(s, pos0, pos1)};
+    }
+    const int shifted = __builtin_amdgcn_update_dpp(sb >> 6, p0, 0x138, 0xF, 0xF, false);     // the lane below's
+    unsigned long long starts = __ballot(l < W && p0 >= 0 && p0 != shifted), more = 0;
+    // The run that starts at lane s: its page and tokens, and lane i's slot and position of its i-th.
+    auto page_of = [&](int s) { return __builtin_amdgcn_readlane(p0, s); };
+    auto from = [](int s, unsigned long long m0, unsigned long long m1) { return m0 >> s | (s ? m1 << (64 - s) : 0ull); };
+    auto length = [&](int s) {
+        const int page = page_of(s);
+        const unsigned long long same = from(s, __ballot(p0 == page), __ballot(p1 == page));
+        return ~same ? __ffsll((long long)~same) - 1 : 64;
+    };
+    const unsigned long long first0 = __ballot((s0 & (kPage - 1)) == 0), first1 = __ballot((s1 & (kPage - 1)) == 0);
+    auto fresh = [&](int s, int n) { return (from(s, first0, first1) << (64 - n)) != 0; };
+    // token i of the run's value
+    auto of_run = [&](int s, int i, int v0, int v1) {
+        const int a0 = __shfl(v0, (i + s) & 63);
+        const int a1 = __shfl(v1, (i + s) & 63);
+        return i + s < 64 ? a0 : a1;
     };
     for (int k = 0; starts; starts &= starts - 1) {
-        const int s = __ffsll((long long)starts) - 1;
-        const Run run = run_at(s);
-        if (run.n > 8) more |= 1ull << s;
+        const int s = __ffsll((long long)starts) - 1, n = length(s);
+        if (n > 8) more |= 1ull << s;
         else if (k++ % (THREADS / 64) == wave)
-            write_few<V>(a, h, run);
+            write_few<V>(a, h, t0 + s, n, page_of(s), fresh(s, n), of_run(s, l / 8, s0, s1), of_run(s, l / 8, pos0, pos1));
     }
-    for (; more; more &= more - 1) write_block<THREADS, V>(a, lds, h, run_at(__ffsll((long long)more) - 1));
+    for (; more; more &= more - 1) {
+        const int s = __ffsll((long long)more) - 1, n = length(s);
+        write_block<THREADS, V>(a, lds, h, [&](int i) { return t0 + s + i; }, n, page_of(s), fresh(s, n), of_run(s, l, s0, s1), of_run(s, l, pos0, pos1));
+    }
 }
 
 // Every q_every-th workgroup takes query heads, the others windows of tokens, until either are done:
 // the blocks wait for their loads while q streams (4090 tokens, all windows first 43 us, all q
-// first 41, in turn 31, each with windows of 16 and 32 heads a wave).
+// first 41, in turn 31, each with windows of 16 and 32 heads a wave). Three workgroups of 512 threads
+// a CU: they leave 80 registers, with two the same 4090 tokens take 22.4 us instead of 20.2.
 template <int THREADS, int W, int B>
-__global__ __launch_bounds__(THREADS) void write_kernel(WriteArgs a, int q_every, int page_blocks)
+__global__ __launch_bounds__(THREADS, THREADS == 512 ? 6 : 4) void write_kernel(WriteArgs a, int q_every, int page_blocks)
 {
     const int b = blockIdx.x, turn = b / q_every;
     const bool is_q = b % q_every == 0;
