@@ -59,15 +59,21 @@ __device__ __forceinline__ f32x4 load4(const uint16_t* p)
 }
 __device__ __forceinline__ float load1(const float* p) { return *p; }
 __device__ __forceinline__ float load1(const uint16_t* p) { return bf16_bits_f32(*p); }
-// (past the caches: 64 rows of logits are more than these hold; with ordinary stores 20.9 us, so 17.1)
+// Four logits; PAST: past the caches.
+template <bool PAST>
 __device__ __forceinline__ void store4(float* p, const f32x4& x)
 {
-    __builtin_nontemporal_store(x, reinterpret_cast<f32x4_row*>(p));
+    auto* to = reinterpret_cast<f32x4_row*>(p);
+    if constexpr (PAST) __builtin_nontemporal_store(x, to);
+    else *to = x;
 }
+template <bool PAST>
 __device__ __forceinline__ void store4(uint16_t* p, const f32x4& x)
 {
     const u16x4_row w = {f32_to_bf16(x[0]), f32_to_bf16(x[1]), f32_to_bf16(x[2]), f32_to_bf16(x[3])};
-    __builtin_nontemporal_store(w, reinterpret_cast<u16x4_row*>(p));
+    auto* to = reinterpret_cast<u16x4_row*>(p);
+    if constexpr (PAST) __builtin_nontemporal_store(w, to);
+    else *to = w;
 }
 __device__ __forceinline__ void store1(float* p, float x) { *p = x; }
 __device__ __forceinline__ void store1(uint16_t* p, float x) { *p = f32_to_bf16(x); }
@@ -175,7 +181,7 @@ __device__ __forceinline__ void finish(const PickArgs& a, int row, const Part& p
     }
 }
 
-template <class T, int V>
+template <class T, int V, bool PAST>
 __global__ __launch_bounds__(kThreads) void pick_kernel(PickArgs a)
 {
     constexpr int kTile = tile_of(V);
@@ -274,7 +280,7 @@ __global__ __launch_bounds__(kThreads) void pick_kernel(PickArgs a)
 #pragma unroll
         for (int k = 0; k < V; ++k) {
             const int i = (k * kThreads + tid) * 4;
-            if (i + 4 <= n) store4(out + i, f32x4{x[k][0], x[k][1], x[k][2], x[k][3]});
+            if (i + 4 <= n) store4<PAST>(out + i, f32x4{x[k][0], x[k][1], x[k][2], x[k][3]});
             else
 #pragma unroll
                 for (int e = 0; e < 3; ++e)
@@ -351,13 +357,19 @@ int64_t most_parts(int rows, int vocab)
 constexpr int kRowsByXcd = 64;
 int64_t blocks_of(int rows, int tiles) { return (int64_t)(rows >= kRowsByXcd ? (rows + 7) / 8 * 8 : rows) * tiles; }
 
-template <class T>
+// Logits after the rules that the L2s do not hold go past the caches; the others are there for whoever
+// reads them next. Ordinary stores and past, us, alone and with a softmax behind them (f32): one row 5.2
+// and 5.2, 56 and 68; 16 rows 9.0 and 8.4, 63 and 75; 64 21.2 and 17.0, 102 and 116; 256 63 and 57, 216
+// and 184.
+constexpr int64_t kL2Bytes = 8 * 4 << 20;
+
+template <class T, bool PAST>
 void launch(const PickArgs& a, int V, hipStream_t s)
 {
     const unsigned blocks = (unsigned)blocks_of(a.rows, a.tiles);
-    if (V == 4) pick_kernel<T, 4><<<blocks, kThreads, 0, s>>>(a);
-    else if (V == 2) pick_kernel<T, 2><<<blocks, kThreads, 0, s>>>(a);
-    else pick_kernel<T, 1><<<blocks, kThreads, 0, s>>>(a);
+    if (V == 4) pick_kernel<T, 4, PAST><<<blocks, kThreads, 0, s>>>(a);
+    else if (V == 2) pick_kernel<T, 2, PAST><<<blocks, kThreads, 0, s>>>(a);
+    else pick_kernel<T, 1, PAST><<<blocks, kThreads, 0, s>>>(a);
     if (a.tiles > 1) join_kernel<<<a.rows, 64, 0, s>>>(a);
 }
 
@@ -418,8 +430,9 @@ int heph_pick_tokens(int32_t* tokens, float* logprob, void* out, int64_t out_str
     a.append = append;
     a.by_xcd = rows >= kRowsByXcd;
     hipStream_t s = static_cast<hipStream_t>(stream);
-    if (dtype == HEPH_DTYPE_F32) launch<float>(a, V, s);
-    else launch<uint16_t>(a, V, s);
+    const bool past = !out || (int64_t)rows * vocab * (int64_t)element > kL2Bytes;
+    if (dtype == HEPH_DTYPE_F32) past ? launch<float, true>(a, V, s) : launch<float, false>(a, V, s);
+    else past ? launch<uint16_t, true>(a, V, s) : launch<uint16_t, false>(a, V, s);
     return status_of(hipGetLastError());
 }
 

@@ -379,6 +379,12 @@ def test_pick_scratch_on_another_stream():
     assert torch.equal(tokens, want) and torch.equal(logprob, lp)
 
 
+@pytest.mark.parametrize("dtype,rows", [(torch.float32, 55), (torch.float32, 56), (torch.bfloat16, 111)])
+def test_pick_logits_that_the_caches_hold_and_more(dtype, rows):
+    # 32 MiB of logits after the rules are the border
+    check(case(rows, 151937, 300, 20, 3, seed=rows, dtype=dtype))
+
+
 def test_pick_rows_past_32_bits():
     # logits of 8.6 GB: the last rows equal the same rows alone
     rows, vocab = 14200, 151936
