@@ -56,7 +56,7 @@ __device__ __forceinline__ void norm_rope(float (&lo)[8], float (&hi)[8], const 
     }
 }
 
-// A store that leaves no line in the caches: for what is more than these hold.
+// A store past the caches (nontemporal): for long streams.
 __device__ __forceinline__ void store_past(uint16_t* p, const uint4& x)
 {
     __builtin_nontemporal_store(i32x4{(int)x.x, (int)x.y, (int)x.z, (int)x.w}, reinterpret_cast<i32x4*>(p));

@@ -95,9 +95,10 @@ struct WriteArgs {
 };
 
 // A wave takes 8 * B query heads of one token: their loads are all on their way at once, which
-// keeps memory busy with the few waves that the blocks' registers leave (4090 tokens, 32 heads:
-// B = 1 24.6 us, 2 22.0, 4 23.0, with ordinary stores). A long batch's q (B > 1) goes past the
-// caches: 19.4 us where ordinary stores took 24.0.
+// keeps memory busy with the few waves that the blocks' registers leave (4090 tokens, 32 heads, with
+// ordinary stores: B = 1 27.0 us, 2 24.7, 4 24.3). A long batch's q (B > 1) goes past the caches: 20.5 us
+// (B = 4 21.0; 2048 scattered tokens 78 and 84). With the attention behind the write both take
+// the same (8 prompts of 512 tokens 75.0 us, 74.4 with ordinary stores; 16 of 1024 296, 297).
 template <int B>
 __device__ __forceinline__ void q_heads(const WriteArgs& a, long unit)
 {
@@ -497,7 +498,8 @@ __device__ __forceinline__ uint4 bf16_of8(uint2 w, float s)
 
 // A workgroup takes the runs of consecutive slots of a page that start among its W rows, one kv
 // head: V's codes meet in LDS and leave key by key. Bound by the rows' 16-bit stores, which go past
-// the caches (65001 rows 79 us instead of 87).
+// the caches (65001 rows 79 us instead of 85, and 146 instead of 151 with an addition of k and v behind
+// them; 100 and 1000 rows the same, alone and with it).
 template <int W>
 __global__ __launch_bounds__(256) void read_kernel(ReadArgs a)
 {
