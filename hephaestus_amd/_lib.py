@@ -131,7 +131,6 @@ SIGNATURES = {
 ATTN_MAX_KEYS = 262144
 PAGE_KEYS = 64
 PAGES_MAX_SEQS = 1024
-PAGES_RECUR = 0x40000000
 # HEPH_ABI_VERSION of include/hephfp8.h that these signatures follow
 ABI_VERSION = 6
 

@@ -50,10 +50,9 @@ struct PlanHeader {
 // Rows row0 .. row0+rows-1 (row = token * G + head of the group, from token
 // tok0 on) over pages page0 .. page0+pages-1 of table row seq. part: the
 // unit's number among those of its rows, counted within the prefix (prefix
-// != 0) or behind the row's prefix units. alone: no other unit reads its pages.
+// != 0) or behind the row's prefix units.
 struct Unit {
-    int seq;                // and alone << 16
-    int tok0, row0, rows, page0, pages, part, prefix;
+    int seq, tok0, row0, rows, page0, pages, part, prefix;
 };
 // Per token: keys it attends to (-1: no sequence), how many prefix and own units hold
 // any of them, and where its first row's partial results lie among a kv head's: those of
@@ -132,8 +131,7 @@ struct PlanLds {
 // sequence's on its own. Tiles are numbered over all sources from `base` on, a
 // sequence's last (longest) tile first.
 struct Source {
-    int seq, alone;                             // alone: no other source has its pages
-    int tok0, n_tok, page0, pages, kv;          // kv: 0 for a group
+    int seq, tok0, n_tok, page0, pages, kv;     // kv: 0 for a group
     int tile, tiles, base;
     int chunks;                                 // a tile's units before the last round
     int parts, units;                           // where its partial results and units start
@@ -166,26 +164,19 @@ __device__ __forceinline__ void set_tiles(Source& x, int G)
 // again is 16 MB or more (100 own keys each; 64 of 16 tokens, 32 + 8 heads: 256 pages
 // 479 us -> 288, 64 pages 135 -> 98, but 16 pages 47 -> 56; 16 of one token, 64 + 1 heads:
 // 256 pages 39 -> 35; four of them 22 -> 27).
-// alone: the group says that no other pages of its sequences recur, and those that it shares are
-// worked on as such. (A sequence in no group has said nothing.)
 constexpr int kLongPrefix = 32;
 __device__ Source group_source(const PlanLds& in, const PlanArgs& a, int g)
 {
     const int s0 = clampi(in.group_start[g], 0, a.s.n_seqs);
     const int s1 = clampi(in.group_start[g + 1], s0, a.s.n_seqs);
     const int t0 = clampi(in.q_start[s0], 0, a.s.n_tok), t1 = clampi(in.q_start[s1], t0, a.s.n_tok);
-    const int shared = max(in.shared[g], 0);
-    int pages = min(shared & ~HEPH_PAGES_RECUR, a.table_pages);
-    bool alone = !(shared & HEPH_PAGES_RECUR);
+    int pages = clampi(in.shared[g], 0, a.table_pages);
     const int counts = in.few[s1] - in.few[s0], full = counts >> 16;
     const bool again = pages >= kLongPrefix && (long)(full - 1) * pages * a.s.n_kv >= 1024;
     const int few = (counts & 0xFFFF) + (again ? full : 0);
     const long many_rows = (long)(t1 - t0 - (in.few_tokens[s1] - in.few_tokens[s0])) * a.s.group();
-    if (few < 2 || many_rows > 10L * (few - 1) * pages) {
-        alone &= pages == 0 || s1 - s0 < 2;
-        pages = 0;
-    }
-    Source x{s0, alone, t0, t1 - t0, 0, pages, 0};
+    if (few < 2 || many_rows > 10L * (few - 1) * pages) pages = 0;
+    Source x{s0, t0, t1 - t0, 0, pages, 0};
     set_tiles(x, a.s.group());
     return x;
 }
@@ -201,9 +192,8 @@ __device__ Source seq_source(const PlanLds& in, const PlanArgs& a, int s, int& g
         else hi = mid;
     }
     group = lo > 0 && s < in.group_start[lo] ? lo - 1 : -1;
-    const Source shared = group >= 0 ? group_source(in, a, group) : Source{};
-    const int page0 = shared.pages;
-    Source x{s, shared.alone | (a.s.n_seqs == 1), t0, t1 - t0, page0, max((kv + kPage - 1) / kPage - page0, 0), kv};
+    const int page0 = group >= 0 ? group_source(in, a, group).pages : 0;
+    Source x{s, t0, t1 - t0, page0, max((kv + kPage - 1) / kPage - page0, 0), kv};
     set_tiles(x, a.s.group());
     return x;
 }
@@ -432,12 +422,12 @@ __global__ __launch_bounds__(kMaxSeqs) void plan_kernel(PlanArgs a)
         const Source x = source(max(lo - 1, 0));
         const int at = u - x.units, last = last_round(x, rounds), whole = (x.tiles - last) * x.chunks;
         // (none of the source's where the counts wrapped: q_start falls)
-        Unit unit{};
+        Unit unit{0, 0, 0, 0, 0, 0, 0, 0};
         if ((unsigned)at < (unsigned)count(x)) {
             const int in_last = max(at - whole, 0), k = at < whole ? at % x.chunks : in_last % rounds.chunks;
             const int r = at < whole ? x.tiles - 1 - at / x.chunks : last - 1 - in_last / rounds.chunks;
             const int per = cut_tile(x, rounds, G, r).per;
-            unit = Unit{x.seq | x.alone << 16, x.tok0, r * x.tile, rows_in(x, r), x.page0 + k * per,
+            unit = Unit{x.seq, x.tok0, r * x.tile, rows_in(x, r), x.page0 + k * per,
                         min(per, x.pages - k * per), k, lo <= a.s.n_groups};
         }
         units[u] = unit;
@@ -885,25 +875,23 @@ struct Rows {
 __device__ __forceinline__ int page_ids(const AttnArgs& a, const Unit& u, int p)
 {
     const int n = p + (threadIdx.x & 63);
-    return n < a.table_pages ? a.table[(size_t)(u.seq & 0xFFFF) * a.table_pages + n] : -1;
+    return n < a.table_pages ? a.table[(size_t)u.seq * a.table_pages + n] : -1;
 }
 
 // Up to 64 rows: a wave takes 16 of them and, where that leaves waves, every
 // KW-th page of the run. Bound by the stream of K and V: the next page's 16 KB
 // a wave are on their way into registers while one is worked on. (64 sequences, each
 // 1024 keys 24.2 us, 5.5 TB/s; 64 keys 6.9 us, where a chain of four loads counts: unit,
-// limits and page ids, q, pages.) FEW: up to 16 rows. ONCE: of a unit that is alone with its pages:
-// one wave alone reads a page, and the page goes past the caches (96 sequences, three layers 132 us
-// instead of 145; one sequence of 131000 keys, two layers 108 instead of 121). With more rows the
-// other waves find it there (64 sequences of 16 tokens 68 us, past the caches 84), and so do
-// sequences whose common pages are not declared (256 of them, eight prefixes of 1024 keys in turn,
-// 53 us a layer, past the caches 62; 32, two of 16384, 75 and 89).
-template <bool BLOCK, bool FEW, bool ONCE>
+// limits and page ids, q, pages.) ONCE, up to 16 rows: one wave alone reads a page, and
+// the page goes past the caches (96 sequences, three layers 131 us instead of 145; one
+// sequence of 131000 keys, two layers 108 instead of 121). With more rows the other waves
+// find it there (64 sequences of 16 tokens 68 us, past the caches 84).
+template <bool BLOCK, bool ONCE>
 __device__ __forceinline__ void attend_narrow(const AttnArgs& a, const Unit& u, int head, int ids0, uint8_t* lds)
 {
     const int l = threadIdx.x & 63, c = l & 15, g4 = l >> 4, n_kv = a.s.n_kv;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int KW = FEW ? 4 : u.rows <= 32 ? 2 : 1, kw = wave % KW;
+    const int KW = ONCE ? 4 : u.rows <= 32 ? 2 : 1, kw = wave % KW;
     Rows<1> x;
     x.init(a, u, head, wave / KW * 16);
     const int end = min(u.page0 + u.pages, (x.hi + kPage - 1) / kPage);
@@ -1118,9 +1106,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     const Unit u = plan_units(a.plan, a.s.n_tok)[unit];        // (the plan has room for all of the grid's)
     if (!plan_fits(h, a) || unit >= h.n_units) return;
     const int ids = page_ids(a, u, u.page0);        // (on its way while the rows are looked at)
-    if (u.rows <= 16 && u.seq >> 16) attend_narrow<BLOCK, true, true>(a, u, head, ids, lds);
-    else if (u.rows <= 16) attend_narrow<BLOCK, true, false>(a, u, head, ids, lds);
-    else if (u.rows <= kNarrow) attend_narrow<BLOCK, false, false>(a, u, head, ids, lds);
+    if (u.rows <= 16) attend_narrow<BLOCK, true>(a, u, head, ids, lds);
+    else if (u.rows <= kNarrow) attend_narrow<BLOCK, false>(a, u, head, ids, lds);
     else attend_wide<BLOCK>(a, u, head, ids, lds);
 }
 

@@ -24,7 +24,6 @@ from __future__ import annotations
 
 import heapq
 from array import array
-from collections import Counter
 from contextlib import nullcontext
 from itertools import accumulate
 
@@ -37,7 +36,7 @@ from . import kernels as HK
 from .kernels import HephError
 from .loader import Fp8Weight, Qwen3Config, Qwen3Fp8Weights
 
-PAGE, PAGES_RECUR = L.PAGE_KEYS, L.PAGES_RECUR
+PAGE = L.PAGE_KEYS
 _U8 = (torch.uint8, torch.float8_e4m3fn)
 _I32, _BF16, _F32 = (torch.int32,), (torch.bfloat16,), (torch.float32,)
 
@@ -269,8 +268,7 @@ class AttentionPlan:
 
     def update(self, q_start, kv_len, group_start=None, shared_pages=None, ctx=None) -> None:
         """q_start int32 [n_seqs + 1], kv_len int32 [n_seqs]; with groups
-        group_start int32 [n_groups + 1], shared_pages int32 [n_groups] (with PAGES_RECUR
-        added where a group's pages recur elsewhere: faster, the same answer)."""
+        group_start int32 [n_groups + 1], shared_pages int32 [n_groups]."""
         g = self.n_groups > 0
         if g != (group_start is not None) or g != (shared_pages is not None):
             raise ValueError(f"a plan of {self.n_groups} groups "
@@ -715,18 +713,6 @@ def _groups(seqs: list[Sequence]) -> tuple[list[int], list[int]]:
     return start, shared
 
 
-def _recurring(seqs: list[Sequence], start: list[int], shared: list[int]) -> list[int]:
-    """shared_pages of _groups with PAGES_RECUR where pages are shared that they do not cover:
-    sequences that share any pages share their first ones."""
-    heads = Counter(seqs[a].pages[0] for a in start[:-1] if seqs[a].pages)
-    marked = []
-    for a, b, n in zip(start, start[1:], shared):
-        behind = [s.pages[n] for s in seqs[a:b] if len(s.pages) > n]
-        recur = len(set(behind)) < len(behind) or (seqs[a].pages and heads[seqs[a].pages[0]] > 1)
-        marked.append(n + PAGES_RECUR if recur else n)
-    return marked
-
-
 class Qwen3BatchDecoder:
     """A step of many sequences: prompts or single tokens, behind whatever
     their caches hold."""
@@ -846,9 +832,7 @@ class Qwen3BatchDecoder:
         table = np.full((len(seqs), max(len(s.pages) for s in seqs)), -1, dtype=np.int32)
         for row, s in zip(table, seqs):
             row[:len(s.pages)] = s.pages
-        start, shared = _groups(seqs)
-        rows = [flat, positions, slots, q_start, [s.length for s in seqs], start,
-                _recurring(seqs, start, shared), ids]
+        rows = [flat, positions, slots, q_start, [s.length for s in seqs], *_groups(seqs), ids]
         # (array: what is no whole number is refused, not rounded)
         return [np.frombuffer(array("i", r), dtype=np.int32) for r in rows] + [table]
 

@@ -40,9 +40,6 @@ extern "C" {
 #define HEPH_PAGE_KEYS 64
 /* Most sequences of one attention call. */
 #define HEPH_PAGES_MAX_SEQS 1024
-/* In shared_pages: the group's pages recur in other groups' page tables, or further ones among its
- * own sequences'. */
-#define HEPH_PAGES_RECUR 0x40000000
 
 /*
  * Rotation table: table[pos][p] = (cos, sin) of pair p < head_dim/2 at
@@ -100,10 +97,7 @@ int heph_qk_norm_rope_pages(void* q_out_bf16, int64_t q_stride, const void* qkv_
  * prompts' rows would not pay more for it than that saves; else for each sequence
  * from its own table row, with the same answer up to the order of sums. Sequences in no
  * group, or n_groups = 0 with both NULL: nothing shared. A shared_pages beyond a
- * sequence's own keys is allowed, a negative one is 0. What a group declares tells, too,
- * which pages are read once in all, and need no place in the caches: where pages
- * recur that its number does not cover, HEPH_PAGES_RECUR is added to it (the answer
- * is the same without it, and slower).
+ * sequence's own keys is allowed.
  *
  * heph_pages_attention_plan (one small launch) lays out a step's work from
  * the lengths in device memory; one plan serves the attention of every layer

@@ -377,53 +377,6 @@ def test_attention_sequences_of_64_rows_share_a_long_prefix(n, new, H, KV, share
     check_attention(b, run_attention(b, plan), tokens=set(rng.integers(0, b["T"], 25).tolist()))
 
 
-def alone_units(plan):
-    """Which of the plan's units have their pages to themselves: (prefix ones, others)."""
-    words = plan.plan.cpu().numpy().view(np.int32)
-    first = 12 + 8 * plan.n_tok
-    units = words[first:first + 8 * int(words[7])].reshape(-1, 8)
-    return [set((units[(units[:, 7] != 0) == p, 0] >> 16).tolist()) for p in (True, False)]
-
-
-@pytest.mark.parametrize("scaled", [False, True])
-def test_attention_pages_that_recur(scaled):
-    """Sequences that share pages without saying so, or with a mark: the same bits, read through
-    the caches; pages that a group declares its sequences' own go past them."""
-    n = 12
-    b = batch([1] * n, [150] * n, [5], [0, n], seed=70)
-    b["page_scale"] = torch.full((b["k"].shape[0], 2 * b["KV"]), 2.0 ** -7, device="cuda")
-
-    def attend(plan):
-        out = torch.zeros(b["T"], b["H"], D, dtype=torch.bfloat16, device="cuda")
-        if scaled:
-            S.attention_pages_scaled(out, b["q"], b["k"], b["v"], b["page_scale"], b["table"], plan)
-        else:
-            S.attention_pages(out, b["q"], b["k"], b["v"], b["scale"], b["table"], plan)
-        return out
-    plans, outs = [], []
-    start, one = list(range(n + 1)), [0] * n
-    for group_start, shared in (([0, n], [5]), ([0, n], [5 + S.PAGES_RECUR]), (None, None), (start, one),
-                                (start, [S.PAGES_RECUR] * n), (start, [-7] * n)):
-        b["group_start"], b["shared"] = (None if x is None else torch.tensor(x, dtype=torch.int32).cuda()
-                                         for x in (group_start, shared))
-        plans.append(make_plan(b))
-        outs.append(attend(plans[-1]))
-    assert [alone_units(p) for p in plans] == [[{1}, {1}], [{0}, {0}], [set(), {0}], [set(), {1}], [set(), {0}],
-                                                   [set(), {1}]]
-    assert torch.equal(outs[0], outs[1]) and all(torch.equal(outs[2], o) for o in outs[3:])
-    if not scaled:
-        for o in (outs[0], outs[2]):
-            check_attention(b, o)
-    # a group whose prefix is not worth sharing: each reads it from its own table
-    b = batch([17] * 30, [17] * 30, [40], [0, 30], seed=71, H=16, KV=4)
-    assert prefix_rows(make_plan(b)) == 0 and alone_units(make_plan(b)) == [set(), {0}]
-    # a group of one sequence, and one sequence in none
-    b = batch([1, 1], [500, 100], [3, 2], [0, 1, 2], seed=72)
-    assert alone_units(make_plan(b)) == [set(), {1}]
-    b = batch([1], [500], seed=72)
-    assert alone_units(make_plan(b)) == [set(), {1}]
-
-
 def test_attention_shared_equals_unshared():
     # what is shared changes where keys are summed, not what is summed
     b = batch([1] * 12, [30 * i + 1 for i in range(12)], [9], [0, 12], seed=77)

@@ -290,23 +290,3 @@ def test_rules_refuse_what_f32_does_not_hold():
     r.set(0, [1], repetition=1e-38, presence=3e38, bias={3: -1e39, 4: 1e-50})
     assert r.penalties.tolist() == [[float(np.float32(1e-38)), float(np.float32(3e38)), 0.0]]
     assert r.bias.tolist() == [[-float("inf"), 0.0]]
-
-
-def test_groups_say_where_pages_recur():
-    def groups(*pages):
-        seqs = []
-        for p in pages:
-            seqs.append(S.Sequence())
-            seqs[-1].pages = list(p)
-        start, shared = S._groups(seqs)
-        got = S._recurring(seqs, start, shared)
-        assert [n & ~S.PAGES_RECUR for n in got] == shared
-        return start, shared, [n >= S.PAGES_RECUR for n in got]
-    assert groups([1, 2], [3]) == ([0, 1, 2], [0, 0], [False] * 2)
-    assert groups([1, 2], [1, 3], [4], []) == ([0, 2, 3, 4], [1, 0, 0], [False] * 3)
-    # two prefixes in turn
-    assert groups([1, 5], [2, 6], [1, 7], [2, 8]) == ([0, 1, 2, 3, 4], [0] * 4, [True] * 4)
-    assert groups([1, 5], [1, 6], [3], [1, 7], [1, 8]) == ([0, 2, 3, 5], [1, 0, 1], [True, False, True])
-    # two share more than the group does
-    assert groups([1, 2, 3, 9], [1, 2, 3, 8], [1, 2, 7]) == ([0, 3], [2], [True])
-    assert groups([1, 2, 3], [1, 2, 3]) == ([0, 2], [3], [False])
