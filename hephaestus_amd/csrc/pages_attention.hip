@@ -882,18 +882,36 @@ __device__ __forceinline__ int page_ids(const AttnArgs& a, const Unit& u, int p)
 // KW-th page of the run. Bound by the stream of K and V: the next page's 16 KB
 // a wave are on their way into registers while one is worked on. (64 sequences, each
 // 1024 keys 24.2 us, 5.5 TB/s; 64 keys 6.9 us, where a chain of four loads counts: unit,
-// limits and page ids, q, pages.) ONCE, up to 16 rows: one wave alone reads a page, and
-// the page goes past the caches (96 sequences, three layers 131 us instead of 145; one
-// sequence of 131000 keys, two layers 108 instead of 121). With more rows the other waves
-// find it there (64 sequences of 16 tokens 68 us, past the caches 84).
-template <bool BLOCK, bool ONCE>
+// limits and page ids, q, pages.) FEW, up to 16 rows: one wave alone reads a page, and
+// the page goes past the caches (96 sequences, three layers 132 us instead of 145; one
+// sequence of 131000 keys, two layers 108 instead of 121) unless another sequence has it
+// too. Sequences that share a page share those before it, so the run's first one tells;
+// each wave looks for it in a quarter of the page tables. (256 sequences, eight prefixes of
+// 1024 keys in turn that no group declares, 53 us a layer, past the caches 62; 32, two of
+// 16384, 75 and 89.) With more rows the other waves find the page in the caches (64
+// sequences of 16 tokens 68 us, past them 84).
+template <bool BLOCK, bool FEW>
 __device__ __forceinline__ void attend_narrow(const AttnArgs& a, const Unit& u, int head, int ids0, uint8_t* lds)
 {
     const int l = threadIdx.x & 63, c = l & 15, g4 = l >> 4, n_kv = a.s.n_kv;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int KW = ONCE ? 4 : u.rows <= 32 ? 2 : 1, kw = wave % KW;
+    const int KW = FEW ? 4 : u.rows <= 32 ? 2 : 1, kw = wave % KW;
+    // the page tables' entries of the run's first page, on their way with the rows' limits and q
+    const int quarter = (a.s.n_seqs + 3) / 4, s0 = wave * quarter + l, s1 = min((wave + 1) * quarter, a.s.n_seqs);
+    const int32_t* column = a.table + min(u.page0, a.table_pages - 1);
+    auto entry = [&](int s) { return column[(size_t)min(s, a.s.n_seqs - 1) * a.table_pages]; };
+    int beside = -1;
+    if (FEW && !u.prefix) beside = entry(s0);
     Rows<1> x;
     x.init(a, u, head, wave / KW * 16);
+    bool alone = FEW;
+    if (FEW && !u.prefix) {
+        const int mine = __builtin_amdgcn_readlane(ids0, 0);
+        bool recurs = s0 < s1 && beside == mine && s0 != u.seq;
+        if (__builtin_expect(quarter > 64, 0))
+            for (int s = s0 + 64; s < s1; s += 64) recurs |= entry(s) == mine && s != u.seq;
+        alone = !__any(recurs);
+    }
     const int end = min(u.page0 + u.pages, (x.hi + kPage - 1) / kPage);
     const float sc = score_scale<BLOCK>(a, head);
     auto place = [&](int id) {
@@ -905,14 +923,15 @@ __device__ __forceinline__ void attend_narrow(const AttnArgs& a, const Unit& u, 
         i32x4 k[8], v[8];
         int id, lane;
     } p0, p1;
-    auto codes = [](const uint8_t* p) {
-        return ONCE ? __builtin_nontemporal_load(reinterpret_cast<const i32x4*>(p)) : ldg16(p);
-    };
     int ids = 0, first = 0, last = 0;
     float sk = 1.0f, sv = 1.0f;            // of the pages of ids, one a lane
     // (past the run its last page again: a load that is left out on some path would make
     // the waits for the page before count without it, and hold up the one behind)
-    auto load = [&](Page& p, int n) {
+    auto load = [&](Page& p, int n, auto past) {
+        auto codes = [](const uint8_t* c) {
+            if constexpr (decltype(past)::value) return __builtin_nontemporal_load(reinterpret_cast<const i32x4*>(c));
+            else return ldg16(c);
+        };
         p.lane = min(n, last - 1) - first;
         p.id = __builtin_amdgcn_readlane(ids, p.lane);
         const size_t o = place(p.id);
@@ -935,27 +954,33 @@ __device__ __forceinline__ void attend_narrow(const AttnArgs& a, const Unit& u, 
                       [&](int i, int h) { return half(p.v[i], h, v_scale); }, clear,
                       a.v_pages + place(p.id));
     };
-    for (first = u.page0; first < end; first += 64) {
-        last = min(first + 64, end);
-        ids = first == u.page0 ? ids0 : page_ids(a, u, first);
-        wait_vm<0>();           // (nothing but pages, and their scales before them, on its way below)
-        if constexpr (BLOCK) {
-            sk = page_scale(a, ids, head);
-            sv = page_scale(a, ids, n_kv + head);
+    auto run = [&](auto past) {
+        for (first = u.page0; first < end; first += 64) {
+            last = min(first + 64, end);
+            ids = first == u.page0 ? ids0 : page_ids(a, u, first);
+            wait_vm<0>();           // (nothing but pages, and their scales before them, on its way below)
+            if constexpr (BLOCK) {
+                sk = page_scale(a, ids, head);
+                sv = page_scale(a, ids, n_kv + head);
+            }
+            int n = first + kw;
+            load(p0, n, past);
+            if constexpr (BLOCK) sv = x.enter(sv, l < last - first && ids >= 0 && ids < a.n_pages);
+            while (n < last) {
+                load(p1, n + KW, past);
+                work(p0, n);
+                n += KW;
+                if (n >= last) break;
+                load(p0, n + KW, past);
+                work(p1, n);
+                n += KW;
+            }
         }
-        int n = first + kw;
-        load(p0, n);
-        if constexpr (BLOCK) sv = x.enter(sv, l < last - first && ids >= 0 && ids < a.n_pages);
-        while (n < last) {
-            load(p1, n + KW);
-            work(p0, n);
-            n += KW;
-            if (n >= last) break;
-            load(p0, n + KW);
-            work(p1, n);
-            n += KW;
-        }
-    }
+    };
+    // (where it is expected the scaled form is 1 % faster; the other one would spill registers)
+    if constexpr (!FEW) run(std::false_type{});
+    else if (BLOCK ? __builtin_expect(alone, 1) : alone) run(std::true_type{});
+    else run(std::false_type{});
 
     if constexpr (BLOCK) x.leave();
     // Waves on the same rows join: each takes 8 / KW of the dim tiles.

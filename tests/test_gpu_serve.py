@@ -377,6 +377,33 @@ def test_attention_sequences_of_64_rows_share_a_long_prefix(n, new, H, KV, share
     check_attention(b, run_attention(b, plan), tokens=set(rng.integers(0, b["T"], 25).tolist()))
 
 
+@pytest.mark.parametrize("scaled", [False, True])
+@pytest.mark.parametrize("n,prefixes,H,KV", [(12, 1, 32, 8), (13, 2, 32, 8), (3, 1, 8, 8), (700, 3, 4, 1), (1024, 1, 4, 1)])
+def test_attention_pages_that_recur(scaled, n, prefixes, H, KV):
+    """Sequences that share their first pages without saying so read them through the caches, and
+    those with copies of their own past them: the same bits."""
+    b = batch([1] * n, [130 + i % 70 for i in range(n)], seed=n, H=H, KV=KV, garbage=False)
+    shared = b["table"].clone()
+    for s in range(n):
+        shared[s, :2] = b["table"][s % prefixes, :2]
+    ids = shared[:, :2].flatten().long()
+    own = b["table"][:, :2].flatten().long()
+    b["page_scale"] = torch.full((b["k"].shape[0], 2 * KV), 2.0 ** -7, device="cuda")
+    for t in ("k", "v"):
+        b[t][own] = b[t][ids]
+    outs = []
+    for table in (b["table"], shared):
+        out = torch.zeros(b["T"], H, D, dtype=torch.bfloat16, device="cuda")
+        if scaled:
+            S.attention_pages_scaled(out, b["q"], b["k"], b["v"], b["page_scale"], table, make_plan(b))
+        else:
+            S.attention_pages(out, b["q"], b["k"], b["v"], b["scale"], table, make_plan(b))
+        outs.append(out)
+    assert torch.equal(*outs)
+    if not scaled:
+        check_attention(b, outs[0], tokens=set(range(0, n, max(n // 10, 1))))
+
+
 def test_attention_shared_equals_unshared():
     # what is shared changes where keys are summed, not what is summed
     b = batch([1] * 12, [30 * i + 1 for i in range(12)], [9], [0, 12], seed=77)
