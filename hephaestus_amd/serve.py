@@ -138,8 +138,9 @@ def v_place(j: int) -> int:
 
 def rope_table_f32(n_pos: int, theta: float = 1e6, device="cuda", ctx=None) -> torch.Tensor:
     """(cos, sin) in f32 of the 64 pairs of a 128-wide head at positions
-    0..n_pos-1, [n_pos, 64, 2], the angles in double."""
-    t = torch.empty(n_pos, 64, 2, dtype=torch.float32, device=device)
+    0..n_pos-1, [n_pos, 64, 2], the angles in double; on ctx the table is that stream's."""
+    with _on(ctx):
+        t = torch.empty(n_pos, 64, 2, dtype=torch.float32, device=device)
     dev, stream = _at(ctx)
     _call("heph_rope_table_f32", _dev(t, "table", _F32, 0, dev), n_pos, 128, theta, stream)
     return t

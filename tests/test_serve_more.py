@@ -273,6 +273,10 @@ def test_what_a_call_allocates_is_its_streams(monkeypatch):
             c.read(seq, 0, ctx=ctx)
         assert made == [want] * 3
         made.clear()
+        with pytest.raises(ValueError):
+            S.rope_table_f32(10, device="cpu", ctx=ctx)
+        assert made == [want]
+        made.clear()
         monkeypatch.setattr(S, "_rows", lambda t, *args: (FAKE, 512))
         with pytest.raises(ValueError):
             S.pick_tokens(torch.zeros(2, dtype=torch.int32), torch.zeros(2, 512), ctx=ctx)
