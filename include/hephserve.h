@@ -200,10 +200,11 @@ int heph_copy_pages_scaled(uint8_t* k_pages, uint8_t* v_pages, float* page_scale
 /*
  * Keys read back: row t < n_rows of k_out and v_out ([n_rows, n_kv_heads, 128]
  * bf16) gets the key and value of slots[t]: code * scale in f32, rounded to bf16
- * (both exact with page_scale, two roundings with kv_scale). One of kv_scale (2 * n_kv_heads, of all pages) and
- * page_scale is given, the other NULL. Rows of a slot outside
- * [0, 64 * n_pages) are left as they were; n_pages < 2^25. Slots may repeat and come
- * in any order; consecutive ones are read together. k_out and v_out do not overlap.
+ * (both exact with page_scale, two roundings with kv_scale). One of kv_scale
+ * (2 * n_kv_heads, of all pages) and page_scale is given, the other NULL. Rows of a
+ * slot outside [0, 64 * n_pages) are left as they were; n_pages < 2^25. Slots may
+ * repeat and come in any order; consecutive ones are read together. k_out and v_out
+ * do not overlap.
  */
 int heph_read_pages(void* k_out_bf16, void* v_out_bf16, const uint8_t* k_pages,
                     const uint8_t* v_pages, int n_pages, const float* kv_scale,
